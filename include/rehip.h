@@ -305,6 +305,113 @@ size_t re_ffn_block_work_bytes(const re_ffn *f, const re_qmat *down, size_t rows
 int re_ffn_block_dev(re_ffn *f, re_qmat *down, const float *d_x, size_t rows, const float *d_add, float *d_y,
                      float *d_work, size_t work_bytes, int mode, void *stream);
 
+/* ---- batched serving over a paged int8 K/V cache ------------------------------------------
+ * No counterpart on the reference's forward path, which holds one sequence's f32 K and V
+ * (forward.rs:347-363); the reference's own page table over requests is infer.rs:328-527. Device
+ * pointers, enqueued on `stream`; nothing is allocated and no value is read back, so every call may
+ * be captured into a graph (with buffers of its own, or replayed one after the other). The stream's
+ * device is the current one, and all buffers are on it.
+ *
+ * A ragged batch: request b's rows are row_start[b] .. row_start[b] + row_count[b] - 1 of the row
+ * arrays (q, k, v, ctx, positions), ranges ascending and disjoint, row_start[b + 1] >= row_start[b] +
+ * row_count[b]; rows between and behind them are left as they were. kv_len[b] counts the request's
+ * tokens, its new rows included: row i stands at position kv_len[b] - row_count[b] + i. Token t of
+ * it lies in page d_table[b * table_ld + t / page] at place t % page; an entry outside 0 .. n_pages - 1
+ * holds no page. A page that is being appended to belongs to one request; full pages may be shared.
+ *
+ * The cache: d_kcodes and d_vcodes hold n_pages x n_kv_heads x page x head_dim int8 codes (page and
+ * head_dim multiples of 32 up to 256; 16-byte aligned), d_kscale and d_vscale n_pages x n_kv_heads f32
+ * scales; a code c stands for c * scale. The codes of one page and head are blocks of 32 tokens x 32
+ * dimensions, 1 KiB each, [page / 32][head_dim / 32], with token t and dimension d of a block at byte
+ *   K: 256 (d / 8) + 16 (t % 16) + 8 (t / 16) + d % 8
+ *   V: 256 (t / 4 % 4) + 16 (d % 16) + 8 (d / 16) + 4 (t / 16) + t % 4
+ * (the order in which a wave's lanes hold matrix operands). A page needs no preparation. */
+
+/* The plan of a step from the requests' lengths. Request b holds d_kv_len[b] tokens and brings
+ * d_new_len[b] more (0: none this time; up to 262144); -1 ends it: its pages go back to the pool,
+ * request after request, and its length becomes 0. d_free is a stack of free pages, n_pages entries of
+ * which the first *d_n_free are set; the step's new pages are taken from its top in request order and
+ * written to d_table (other entries are left). A request whose pages, with those of the requests
+ * before it, exceed the free ones, or whose tokens exceed table_ld * page, is refused: row_count 0,
+ * length and pages unchanged. Outputs: d_kv_len_out and d_n_free_out (may be d_kv_len and d_n_free);
+ * d_row_start (rows packed in request order, refused ones included, as the caller packed them from
+ * new_len) and d_row_count; for rows 0 .. row_cap - 1 the request, the position and the slot
+ * (page * page size + place), -1 for rows of refused requests and behind the last; d_status[0] refused
+ * requests, d_status[1] rows. Up to 4096 requests. */
+int re_kv_plan_dev(size_t requests, size_t page, const int *d_new_len, const int *d_kv_len, int *d_table,
+                   size_t table_ld, int *d_free, size_t n_pages, const int *d_n_free, int *d_kv_len_out,
+                   int *d_n_free_out, int *d_row_start, int *d_row_count, size_t row_cap, int *d_row_seq,
+                   int *d_row_pos, int *d_row_slot, int *d_status, void *stream);
+
+/* Rotary frequencies on the host: freqs[i] radians per position of pair i < rot_dim / 2, theta^(-2i/rot_dim)
+ * scaled for contexts longer than the trained ones, and the factor of the rotated vectors in *mscale
+ * (1 except for RE_ROPE_YARN):
+ *   RE_ROPE_LINEAR  all divided by factor;
+ *   RE_ROPE_NTK     theta * factor^(d / (d - 2)) in theta's place, d = rot_dim;
+ *   RE_ROPE_YARN    pairs from the one that makes p0 turns over trained_len positions (fast, e.g. 32)
+ *                   to the one that makes p1 (slow, e.g. 1) move from theirs to theirs / factor along a
+ *                   ramp; mscale = 0.1 ln(factor) + 1;
+ *   RE_ROPE_BANDS   pairs of up to p0 turns over trained_len are divided by factor, of p1 or more kept,
+ *                   between them mixed linearly in the number of turns (p0 < p1, e.g. 1 and 4). */
+#define RE_ROPE_NONE 0
+#define RE_ROPE_LINEAR 1
+#define RE_ROPE_NTK 2
+#define RE_ROPE_YARN 3
+#define RE_ROPE_BANDS 4
+int re_rope_freqs(double theta, size_t rot_dim, int scaling, double factor, double trained_len, double p0, double p1,
+                  double *freqs, float *mscale);
+/* Rotary positions of rows x heads x head_dim (row strides ldx and ldo floats): the first rot_dim
+ * dimensions of each head of row r turn by d_pos[r] * d_freqs[i] (angles in 64 bits, so far positions
+ * keep theirs) and are scaled by mscale, pair i being (x[i], x[i + rot_dim / 2]) (RE_ROPE_HALF, as
+ * infer.rs:90-139) or (x[2i], x[2i + 1]) (RE_ROPE_INTERLEAVED); the other dimensions are copied. d_out
+ * may be d_x (with ldo = ldx), and then holds q and k of a fused projection rotated in one call; other
+ * overlaps are not allowed. Rows at negative positions are left as they were. d_freqs: rot_dim / 2 doubles. */
+#define RE_ROPE_HALF 0
+#define RE_ROPE_INTERLEAVED 1
+int re_rope_rows_dev(const float *d_x, size_t ldx, size_t rows, size_t heads, size_t head_dim, size_t rot_dim,
+                     int layout, const double *d_freqs, float mscale, const int *d_pos, float *d_out, size_t ldo,
+                     void *stream);
+
+/* Append the batch's K and V rows (strides ldk, ldv floats, multiples of 4; 16-byte aligned) to the cache.
+ * A page and head's scale is the largest finite magnitude of what it holds / 127 (0 where that is below the
+ * smallest normal float), a code round(x / scale), ties to even; +-inf are stored as +-127 and NaN as 0.
+ * Rows that raise the scale of a page with earlier rows of the request in it round those rows' codes
+ * to the new one, round(c * (old / new)); a page that the new rows begin starts a scale of its own. A
+ * request's kv_len may have been set back before: the codes behind it are overwritten, the scale of a
+ * page that keeps rows is kept. Requests with kv_len < row_count or beyond the table are skipped. */
+int re_kv8_append_dev(const float *d_k, size_t ldk, const float *d_v, size_t ldv, size_t rows, size_t requests,
+                      const int *d_row_start, const int *d_row_count, const int *d_kv_len, const int *d_table,
+                      size_t table_ld, size_t page, size_t n_pages, int8_t *d_kcodes, int8_t *d_vcodes,
+                      float *d_kscale, float *d_vscale, size_t n_kv_heads, size_t head_dim, void *stream);
+
+/* Causal GQA attention of the batch's q rows (stride ldq floats, a multiple of 4; after their k and v are
+ * appended): row at position p sees the tokens max(0, p - window + 1) .. p (window 0: all up to p) that lie
+ * in a page, ctx = softmax(scale * q . k) v, rows x n_heads x head_dim; a row that sees nothing gets zeros.
+ * Products and sums are f32-accurate (the codes are exact in f16; q and the probabilities are split into two
+ * f16 parts of 22 bits). max_rows: no request has more rows (rows past it are left). max_len: the largest
+ * kv_len to plan for (longer ones are computed too, only slower). d_work: re_attention_kv8_work_bytes bytes,
+ * 16-byte aligned (NULL where that is 0); calls that may run at the same time, replays of captured graphs
+ * among them, each need their own. */
+size_t re_attention_kv8_work_bytes(size_t rows, size_t requests, size_t max_rows, size_t max_len, size_t n_heads,
+                                   size_t n_kv_heads, size_t head_dim);
+int re_attention_kv8_dev(const float *d_q, size_t ldq, size_t rows, size_t requests, const int *d_row_start,
+                         const int *d_row_count, const int *d_kv_len, const int *d_table, size_t table_ld, size_t page,
+                         size_t n_pages, const int8_t *d_kcodes, const int8_t *d_vcodes, const float *d_kscale,
+                         const float *d_vscale, size_t max_rows, size_t max_len, size_t n_heads, size_t n_kv_heads,
+                         size_t head_dim, float scale, size_t window, float *d_ctx, void *d_work, size_t work_bytes,
+                         void *stream);
+
+/* Of rows x vocab logits (row stride ld): d_logprob[r] = log softmax of logit d_targets[r] (a target outside
+ * 0 .. vocab - 1: 0, so that a sum over rows skips it), d_entropy[r] in nats, and the top_k (up to 64)
+ * largest logits' ids and log probabilities in descending order, ties to the lower id; rows x top_k. d_logprob
+ * (with d_targets) and d_entropy may be NULL, top_k 0. A logit of -inf has probability 0 and adds nothing to the
+ * entropy. A row with NaN or +inf among its logits, or with nothing above -inf, has no distribution: its log
+ * probabilities and entropy are NaN; ids rank NaN as -inf. d_work: re_logprobs_work_bytes bytes, as above. */
+size_t re_logprobs_work_bytes(size_t rows, size_t vocab, size_t top_k);
+int re_logprobs_dev(const float *d_logits, size_t ld, size_t rows, size_t vocab, const int *d_targets, size_t top_k,
+                    float *d_logprob, float *d_entropy, int *d_top_ids, float *d_top_logprobs, void *d_work,
+                    size_t work_bytes, void *stream);
+
 /* ---- int8 activations (src/kernel.rs:70-166) ------------------------------------------
  * re_quantize_q8_act[_dev]: Q8Activation::from_f32 (kernel.rs:88-105) of `rows` activation rows
  * of n values (n a multiple of 32): scales rows x n/32 f32 (d = max|x|/127 per block) and qs

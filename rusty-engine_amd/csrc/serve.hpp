@@ -1,0 +1,112 @@
+// Argument blocks and host-side launchers of the batched serving step (serve.hip, kv8.hip), shared with
+// their C ABI (serve_api.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <cstddef>
+#include <cstdint>
+
+namespace rehip {
+
+// A ragged batch over pages: request b's rows are start[b] .. start[b] + count[b] - 1 of the row arrays
+// (start ascending, ranges disjoint), its last row is position len[b] - 1, and token t of it lies in page
+// table[b * table_ld + t / page] at place t % page. Entries outside 0 .. n_pages - 1 hold no page.
+struct PagedBatch {
+  const int* start;
+  const int* count;
+  const int* len;
+  const int* table;
+  int requests, rows, table_ld, page, n_pages;
+};
+
+// The int8 pages and their scales (n_pages x kv_heads each): codes of one page and head are
+// [page / 32][hd / 32] blocks of 1 KiB in fragment order (kv8.hip).
+struct Kv8Cache {
+  int8_t* k;
+  int8_t* v;
+  float* ks;
+  float* vs;
+  int kv_heads, hd;
+};
+
+struct PlanArgs {
+  const int* new_len;
+  const int* len;
+  int* table;
+  int* free_pages;
+  const int* n_free;
+  int* len_out;
+  int* n_free_out;
+  int* start;
+  int* count;
+  int* seq;
+  int* pos;
+  int* slot;
+  int* status;
+  int requests, page, table_ld, n_pages, cap;
+};
+
+constexpr int kPlanMaxRequests = 4096;
+constexpr int kPlanMaxNew = 1 << 18;       // new tokens of one request (the sum over all stays below 2^31)
+
+struct RopeArgs {
+  const float* x;
+  float* out;
+  const double* freqs;
+  const int* pos;
+  size_t ldx, ldo;
+  float mscale;
+  int rows, heads, hd, rot, interleaved;
+};
+
+struct LogprobArgs {
+  const float* x;
+  const int* targets;
+  float* logprob;
+  float* entropy;
+  int* ids;
+  float* top;
+  float* work;
+  size_t ld;
+  int rows, vocab, k;
+};
+
+constexpr int kLogprobsMaxTop = 64;
+
+struct Attn8Args {
+  const float* q;
+  float* ctx;
+  float* work;
+  size_t ldq;
+  float scale;
+  int window, heads, max_rows, max_len;
+};
+
+hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
+hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s);
+size_t logprobs_work_floats(int rows, int vocab, int k);
+hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s);
+hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, size_t ldk, const float* v,
+                             size_t ldv, hipStream_t s);
+size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd);
+hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s);
+
+// Request of unit u, where request b owns the units from start[b] / div + mult * b on: the number of requests
+// whose first unit is at most u, less one (-1: none). Every thread of a workgroup of THREADS calls it.
+template <int THREADS>
+__device__ __forceinline__ int request_of_unit(int u, const int* __restrict__ start, int requests, int rows, int div,
+                                               int mult) {
+  __shared__ int part[THREADS / 64];
+  int n = 0;
+  for (int b = threadIdx.x; b < requests; b += THREADS) n += min(max(start[b], 0), rows) / div + mult * b <= u;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
+  __syncthreads();
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) n += part[w];
+  return n - 1;
+}
+
+}  // namespace rehip

@@ -53,7 +53,9 @@ EXPORTS = ("re_init", "re_last_error", "re_version", "re_row_bytes", "re_tiled_b
            "re_gguf_find_tensor", "re_gguf_tensor_data", "re_qmat_from_gguf", "re_moe_from_gguf",
            "re_quantize_q8_act", "re_quantize_q8_act_dev", "re_qmat_matmul_i8", "re_qmat_matmul_i8_dev",
            "re_attention_decode_dev", "re_qmat_gemv_plan", "re_qmat_matmul_noalloc_dev", "re_moe_set_shared",
-           "re_rope_table_dev", "re_moe_route_group_dev", "re_moe_layer_group_dev")
+           "re_rope_table_dev", "re_moe_route_group_dev", "re_moe_layer_group_dev",
+           "re_kv_plan_dev", "re_rope_freqs", "re_rope_rows_dev", "re_kv8_append_dev", "re_attention_kv8_work_bytes",
+           "re_attention_kv8_dev", "re_logprobs_work_bytes", "re_logprobs_dev")
 GEMV_KERNELS = {0: "split", 1: "rows", 2: "tile", 3: "dense"}
 
 
@@ -162,6 +164,17 @@ def lib() -> C.CDLL:
         L.re_moe_from_gguf.argtypes = [_vp, C.c_char_p, C.c_char_p, C.c_char_p, _sz, _sz, _sz, C.POINTER(_vp)]
         L.re_qmat_gemv_plan.argtypes = [_vp, _sz] + [C.POINTER(C.c_int)] * 4
         L.re_qmat_matmul_noalloc_dev.argtypes = [_vp, _vp, _sz, _vp, C.c_int, _vp]
+        L.re_kv_plan_dev.argtypes = [_sz, _sz, _vp, _vp, _vp, _sz, _vp, _sz] + [_vp] * 5 + [_sz] + [_vp] * 5
+        L.re_rope_freqs.argtypes = [C.c_double, _sz, C.c_int] + [C.c_double] * 4 + [_vp, C.POINTER(C.c_float)]
+        L.re_rope_rows_dev.argtypes = [_vp, _sz, _sz, _sz, _sz, _sz, C.c_int, _vp, C.c_float, _vp, _vp, _sz, _vp]
+        batch = [_sz, _sz] + [_vp] * 4 + [_sz] * 3 + [_vp] * 4        # rows .. scales, as the two calls share them
+        L.re_kv8_append_dev.argtypes = [_vp, _sz, _vp, _sz] + batch + [_sz, _sz, _vp]
+        L.re_attention_kv8_work_bytes.argtypes = [_sz] * 7
+        L.re_attention_kv8_work_bytes.restype = _sz
+        L.re_attention_kv8_dev.argtypes = [_vp, _sz] + batch + [_sz] * 5 + [C.c_float, _sz, _vp, _vp, _sz, _vp]
+        L.re_logprobs_work_bytes.argtypes = [_sz] * 3
+        L.re_logprobs_work_bytes.restype = _sz
+        L.re_logprobs_dev.argtypes = [_vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp]
         _lib = L
     return _lib
 
@@ -571,6 +584,71 @@ class MoeExperts:
             self.close()
         except Exception:
             pass
+
+
+# ---- batched serving over a paged int8 K/V cache ------------------------------------------------
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = range(5)
+
+
+def kv_plan_dev(requests, page, new_len, kv_len, table, table_ld, free, n_pages, n_free, kv_len_out, n_free_out,
+                row_start, row_count, row_cap, row_seq, row_pos, row_slot, status, stream=None):
+    """Pages, block table entries and row maps of a step from the requests' lengths (re_kv_plan_dev): new_len -1
+    ends a request; kv_len_out / n_free_out may be kv_len / n_free."""
+    _check(lib().re_kv_plan_dev(requests, page, _p(new_len), _p(kv_len), _p(table), table_ld, _p(free), n_pages,
+                                _p(n_free), _p(kv_len_out), _p(n_free_out), _p(row_start), _p(row_count), row_cap,
+                                _p(row_seq), _p(row_pos), _p(row_slot), _p(status), _stream_ptr(stream)))
+
+
+def rope_freqs(theta, rot_dim, scaling=ROPE_NONE, factor=1.0, trained_len=0.0, p0=None, p1=None):
+    """(radians per position of each pair as float64, factor of the rotated vectors): re_rope_freqs. p0 and p1
+    are turns over the trained positions: 32 and 1 for ROPE_YARN, 1 and 4 for ROPE_BANDS unless given."""
+    usual = (1.0, 4.0) if scaling == ROPE_BANDS else (32.0, 1.0)
+    out, m = np.empty(max(rot_dim // 2, 1), np.float64), C.c_float()
+    _check(lib().re_rope_freqs(theta, rot_dim, scaling, factor, trained_len, usual[0] if p0 is None else p0,
+                               usual[1] if p1 is None else p1, out.ctypes.data, C.byref(m)))
+    return out, m.value
+
+
+def rope_rows_dev(x, ldx, rows, heads, head_dim, rot_dim, layout, freqs, mscale, pos, out, ldo, stream=None):
+    """Rotary positions of a batch's rows, row r at pos[r]; `freqs`: the float64 frequencies on the device; `out`
+    may be `x` (re_rope_rows_dev)."""
+    _check(lib().re_rope_rows_dev(_p(x), ldx, rows, heads, head_dim, rot_dim, layout, _p(freqs), mscale, _p(pos),
+                                  _p(out), ldo, _stream_ptr(stream)))
+
+
+def kv8_append_dev(k, ldk, v, ldv, rows, requests, row_start, row_count, kv_len, table, table_ld, page, n_pages,
+                   kcodes, vcodes, kscale, vscale, n_kv_heads, head_dim, stream=None):
+    """K and V rows of a ragged batch into int8 pages with a scale for each page and head (re_kv8_append_dev)."""
+    _check(lib().re_kv8_append_dev(_p(k), ldk, _p(v), ldv, rows, requests, _p(row_start), _p(row_count), _p(kv_len),
+                                   _p(table), table_ld, page, n_pages, _p(kcodes), _p(vcodes), _p(kscale), _p(vscale),
+                                   n_kv_heads, head_dim, _stream_ptr(stream)))
+
+
+def attention_kv8_work_bytes(rows, requests, max_rows, max_len, n_heads, n_kv_heads, head_dim) -> int:
+    return int(lib().re_attention_kv8_work_bytes(rows, requests, max_rows, max_len, n_heads, n_kv_heads, head_dim))
+
+
+def attention_kv8_dev(q, ldq, rows, requests, row_start, row_count, kv_len, table, table_ld, page, n_pages, kcodes,
+                      vcodes, kscale, vscale, max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window, ctx,
+                      work=None, work_bytes=0, stream=None):
+    """Causal GQA attention of a ragged batch over int8 pages (re_attention_kv8_dev)."""
+    _check(lib().re_attention_kv8_dev(_p(q), ldq, rows, requests, _p(row_start), _p(row_count), _p(kv_len), _p(table),
+                                      table_ld, page, n_pages, _p(kcodes), _p(vcodes), _p(kscale), _p(vscale),
+                                      max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window, _p(ctx),
+                                      _p(work), work_bytes, _stream_ptr(stream)))
+
+
+def logprobs_work_bytes(rows, vocab, top_k) -> int:
+    return int(lib().re_logprobs_work_bytes(rows, vocab, top_k))
+
+
+def logprobs_dev(logits, ld, rows, vocab, targets, top_k, logprob, entropy, top_ids, top_logprobs, work=None,
+                 work_bytes=0, stream=None):
+    """Log probabilities of given tokens, entropy and top_k alternatives of logit rows (re_logprobs_dev); targets
+    with logprob, and entropy, may be None."""
+    _check(lib().re_logprobs_dev(_p(logits), ld, rows, vocab, _p(targets), top_k, _p(logprob), _p(entropy),
+                                 _p(top_ids), _p(top_logprobs), _p(work), work_bytes, _stream_ptr(stream)))
 
 
 # ---- int8 activations (src/kernel.rs:70-166) ---------------------------------------------------
