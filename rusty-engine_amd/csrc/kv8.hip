@@ -87,82 +87,363 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 // ---- attention -----------------------------------------------------------------------------------
 // Row i of request r stands at position p = len - count + i and sees the keys max(0, p - window + 1) .. p that lie
 // in a page: softmax over scale * q . k, then the weighted values. A row that sees no key gets zeros.
-// One workgroup per (row, head): 256 keys at a time, a key per thread for the scores, a dimension per thread for the
-// values.
-__global__ __launch_bounds__(256) void attention_kv8_rows_kernel(PagedBatch b, Kv8Cache c, Attn8Args a) {
-  __shared__ float qs[256], ps[256], red[4];
-  __shared__ int pages[256];
-  const int u = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, hd = c.hd;
-  const int r = request_of_unit<256>(u, b.start, b.requests, b.rows, 1, 1);
-  if (r < 0) return;
-  const int row0 = min(max(b.start[r], 0), b.rows);
-  const int n = min(max(b.count[r], 0), min(b.rows - row0, a.max_rows));
-  const int i = u - (row0 + r);
-  if (i < 0 || i >= n) return;
-  const int len = min(max(b.len[r], 0), b.table_ld * b.page);
-  const int p = len - min(max(b.count[r], 0), b.rows - row0) + i;
-  const int head = h / (a.heads / c.kv_heads);
-  if (tid < hd) qs[tid] = a.q[(size_t)(row0 + i) * a.ldq + (size_t)h * hd + tid];
-  float m = -INFINITY, l = 0.0f, o = 0.0f;
-  const int first = a.window > 0 ? max(0, p - a.window + 1) : 0;
-  for (int j0 = first; j0 <= p; j0 += 256) {
-    const int j = j0 + tid;
-    int pid = -1;
-    if (j <= p) pid = b.table[(size_t)r * b.table_ld + j / b.page];
-    if (pid < 0 || pid >= b.n_pages) pid = -1;
-    __syncthreads();
-    pages[tid] = pid;
-    float s = -INFINITY;
-    if (pid >= 0) {
-      const int tok = j % b.page;
-      const int8_t* kc = c.k + ((size_t)pid * c.kv_heads + head) * b.page * hd + (size_t)(tok >> 5) * (hd >> 5) * 1024;
-      s = 0.0f;
-      for (int d = 0; d < hd; ++d) s += qs[d] * (float)kc[(d >> 5) * 1024 + k_byte(tok & 31, d & 31)];
-      s *= c.ks[(size_t)pid * c.kv_heads + head] * a.scale;
-    }
-    float mx = s;
+//
+// All products run on v_mfma_f32_16x16x32_f16: an int8 code is exact in f16, and the f32 operands (q, the
+// probabilities) are split into two f16 parts, hi + lo, good to 2^-22 of the largest: two instructions per product,
+// f32 sums. q is first scaled by the power of two that takes its vector's largest element to 2^13 .. 2^14, so no part
+// falls out of f16's range; the terms exp(s - max), at most 1, are taken times 2^14, which cancels in the division by
+// their sum. Each step's products with V's codes are summed from zero and scaled by the page's scale in f32 (scales
+// taken into the f16 weights cost a row that sees only pages of small scale its precision).
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// eight codes as f16: 0x6400 + u is the f16 value 1024 + u for a byte u = c + 128, less 1152 is c
+__device__ __forceinline__ h8 codes8(unsigned a, unsigned b) {
+  union { unsigned u[4]; h2 h[4]; h8 v; } r;
+  a ^= 0x80808080u;
+  b ^= 0x80808080u;
+  r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+  r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+  r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+  r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+  const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const float y = __shfl_xor(mx, off, 64);
-      mx = y > mx || y != y ? y : mx;
-    }
-    if ((tid & 63) == 0) red[tid >> 6] = mx;
-    __syncthreads();
-    float mn = m;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mn = red[w] > mn || red[w] != red[w] ? red[w] : mn;
-    const float alpha = m == mn ? 1.0f : expf(m - mn);
-    const float e = pid < 0 ? 0.0f : expf(s - mn);
-    ps[tid] = e;
-    float sum = e;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = sum;
-    __syncthreads();
-    l = l * alpha + ((red[0] + red[1]) + (red[2] + red[3]));
-    m = mn;
-    o *= alpha;
-    if (tid < hd) {
-      const int d = tid;
-      for (int t = 0; t < 256 && j0 + t <= p; ++t) {
-        const int pg = pages[t];
-        if (pg < 0) continue;
-        const int tok = (j0 + t) % b.page;
-        const int8_t* vc = c.v + ((size_t)pg * c.kv_heads + head) * b.page * hd;
-        const float x = (float)vc[(size_t)((tok >> 5) * (hd >> 5) + (d >> 5)) * 1024 + v_byte(tok & 31, d & 31)];
-        o += ps[t] * (x * c.vs[(size_t)pg * c.kv_heads + head]);
-      }
-    }
-  }
-  if (tid < hd) a.ctx[((size_t)(row0 + i) * a.heads + h) * hd + tid] = l == 0.0f ? 0.0f : o / l;
+  for (int i = 0; i < 4; ++i) r.h[i] += off;
+  return r.v;
 }
 
-size_t attention_kv8_work_floats(int, int, int, int, int, int, int) { return 0; }
+// x = hi + lo, each rounded to the nearest f16
+__device__ __forceinline__ void split8(const float (&x)[8], h8& hi, h8& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const h2 h = {(_Float16)x[i], (_Float16)x[i + 1]};
+    const h2 l = {(_Float16)(x[i] - (float)h[0]), (_Float16)(x[i + 1] - (float)h[1])};
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    lo[i] = l[0];
+    lo[i + 1] = l[1];
+  }
+}
+
+// the largest / the sum over the four lanes that share a column of the 16 x 16 layouts (lanes l, l ^ 16, l ^ 32, ..)
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// How a launch cuts the batch: a tile holds up to 16 query vectors of one request and KV head, rows_per rows of its
+// grp heads (grp <= 16), or 16 of the grp heads of one row (group_tiles of them); with `direct` unit u is request u,
+// which has one tile at most.
+struct AttnTiles {
+  int grp, rows_per, group_tiles, units, direct, splits;
+};
+
+// A tile's place: request, rows, and the 32-key steps it has to walk, and their cut into splits.
+struct AttnTile {
+  int row0, n, i0, i1;       // first row of the request, its rows, the tile's rows i0 .. i1 - 1 of them
+  int p0;                    // position of the request's row 0 (may be below 0)
+  int len;                   // tokens that the table can hold
+  int first, steps, per;     // first step, number of steps, steps per split
+  int req;
+};
+
+constexpr int kAttnMinSteps = 16;     // steps of a split, at least (four waves take turns)
+
+template <int THREADS>
+__device__ __forceinline__ bool find_tile(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, AttnTile& o) {
+  const int u = blockIdx.x;
+  const int r = t.direct ? u : request_of_unit<THREADS>(u, b.start, b.requests, b.rows, t.rows_per, 1);
+  if (r < 0) return false;
+  o.req = r;
+  o.row0 = min(max(b.start[r], 0), b.rows);
+  const int count = min(max(b.count[r], 0), b.rows - o.row0);
+  o.len = min(max(b.len[r], 0), b.table_ld * b.page);
+  o.n = min(count, a.max_rows);
+  o.p0 = o.len - count;
+  o.i0 = t.direct ? 0 : (u - (o.row0 / t.rows_per + r)) * t.rows_per;
+  if (o.i0 < 0 || o.i0 >= o.n) return false;
+  o.i1 = min(o.i0 + t.rows_per, o.n);
+  const int last = o.p0 + o.i1 - 1;
+  const int lo = a.window > 0 ? max(0, o.p0 + o.i0 - a.window + 1) : 0;
+  o.first = lo >> 5;
+  o.steps = last < 0 ? 0 : (last >> 5) - o.first + 1;
+  o.per = max(kAttnMinSteps, ((o.steps + t.splits - 1) / t.splits + 3) & ~3);
+  return true;
+}
+
+// The workspace holds (m, l) of every row, head and split, then their sums from this float on (16-byte aligned).
+__host__ __device__ inline size_t split_pairs(size_t rows, size_t heads, size_t splits) {
+  return (rows * heads * splits * 2 + 3) & ~(size_t)3;
+}
+__device__ __forceinline__ size_t sums_at(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t) {
+  return split_pairs(b.rows, a.heads, t.splits);
+}
+
+constexpr int kAttnPages = 512;       // pages whose numbers and scales are staged at a time
+
+// One workgroup of four waves per (tile, KV head, split of the keys). A wave takes every fourth step of 32 keys:
+//   S^T = K Q^T (two 16-key tiles; lane l has keys 4 (l / 16) + i of each for vector l % 16), the running maximum
+//   and sum, and O^T += V^T P^T, whose operand P^T is what the lane holds of S^T.
+// Codes go from memory to registers in fragment order: 16 bytes per lane and 1 KiB per load, no LDS. The next K block
+// loads while the softmax and V's products run, the next V block while K's do.
+template <int NB>
+__global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
+  constexpr int HD = 32 * NB, LD = HD + 4;
+  __shared__ int ids[kAttnPages];
+  __shared__ float kss[kAttnPages], vss[kAttnPages];
+  __shared__ float Ms[4][16], Ls[4][16];
+  __shared__ __attribute__((aligned(16))) float Os[4][16][LD];
+  AttnTile tile;
+  if (!find_tile<256>(b, a, t, tile)) return;
+  const int sp = blockIdx.z;
+  const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * 16;
+  if (sp > 0 && sp * tile.per >= tile.steps) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int s0 = tile.first + sp * tile.per, s1 = min(s0 + tile.per, tile.first + tile.steps);
+  // this lane's query vector
+  const int vi = t.grp <= 16 ? tile.i0 + col / t.grp : tile.i0;
+  const int vh = t.grp <= 16 ? col % t.grp : g0 + col;
+  const bool live = vi < tile.i1 && vh < t.grp;
+  const int pos = live ? tile.p0 + vi : -1;                       // sees keys low .. pos
+  const int low = a.window > 0 ? pos - a.window + 1 : 0;
+  h8 qh[NB], ql[NB];
+  float qs;
+  {
+    const float* q = a.q + (size_t)(tile.row0 + (live ? vi : tile.i0)) * a.ldq +
+                     (size_t)(head * t.grp + (live ? vh : 0)) * HD + 8 * g;
+    float x[NB][8];
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      *reinterpret_cast<float4*>(&x[k][0]) = *reinterpret_cast<const float4*>(q + 32 * k);
+      *reinterpret_cast<float4*>(&x[k][4]) = *reinterpret_cast<const float4*>(q + 32 * k + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
+    }
+    top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+    top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+    const int e = (int)(top >> 23);                               // 2^13 <= largest * 2^(f - 127) < 2^14
+    const int f = e == 255 ? 127 : min(267 - e, 253);
+    const float up = __uint_as_float((unsigned)f << 23);
+    qs = __uint_as_float((unsigned)(254 - f) << 23) * (a.scale * 1.4426950408889634f);
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[k][j] *= up;
+      split8(x[k], qh[k], ql[k]);
+    }
+  }
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o[NB][2];
+#pragma unroll
+  for (int k = 0; k < NB; ++k) o[k][0] = o[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const size_t head_bytes = (size_t)b.page * HD;
+  const int page_steps = b.page >> 5;
+  for (int pg0 = s0 / page_steps; pg0 * page_steps < s1; pg0 += kAttnPages) {
+    // the pages of these steps: their numbers and scales
+    const int npg = min(kAttnPages, (s1 - 1) / page_steps - pg0 + 1);
+    if (pg0 != s0 / page_steps) __syncthreads();
+    for (int i = tid; i < npg; i += 256) {
+      int pid = b.table[(size_t)tile.req * b.table_ld + pg0 + i];
+      const bool have = pid >= 0 && pid < b.n_pages;
+      const size_t at = (size_t)(have ? pid : 0) * c.kv_heads + head;
+      ids[i] = have ? pid : -1;
+      kss[i] = have ? c.ks[at] : 0.0f;
+      vss[i] = have ? c.vs[at] : 0.0f;
+    }
+    __syncthreads();
+    const int e0 = max(s0, pg0 * page_steps), e1 = min(s1, (pg0 + npg) * page_steps);
+    u32x4 kf[NB], vf[NB];
+    auto block = [&](const int8_t* base, int s) {
+      const int pi = s / page_steps - pg0;
+      const int pid = __builtin_amdgcn_readfirstlane(max(ids[pi], 0));
+      return base + ((size_t)pid * c.kv_heads + head) * head_bytes + (size_t)(s % page_steps) * (NB * 1024);
+    };
+    auto load = [&](const int8_t* p, u32x4 (&x)[NB]) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+        x[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 1024 * k + 16 * lane));
+    };
+    int s = e0 + w;
+    if (s < e1) {
+      load(block(c.k, s), kf);
+      load(block(c.v, s), vf);
+    }
+    for (; s < e1; s += 4) {
+      const int next = min(s + 4, e1 - 1);
+      const int pi = s / page_steps - pg0;
+      const bool have = ids[pi] >= 0;
+      const float ks = kss[pi] * qs, vs = vss[pi];
+      f32x4 st[2] = {};
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const h8 k0 = codes8(kf[k][0], kf[k][1]), k1 = codes8(kf[k][2], kf[k][3]);
+        st[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[k], st[0], 0, 0, 0);
+        st[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[k], st[1], 0, 0, 0);
+        st[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[k], st[0], 0, 0, 0);
+        st[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[k], st[1], 0, 0, 0);
+      }
+      load(block(c.k, next), kf);
+      float x[8], mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
+        x[e] = have && j <= pos && j >= low ? st[e >> 2][e & 3] * ks : -INFINITY;
+        mx = fmaxf(mx, x[e]);
+      }
+      mx = fmaxf(m, column_max(mx));
+      const float mref = mx == -INFINITY ? 0.0f : mx;
+      if (__ballot(mx > m) != 0) {
+        const float alpha = exp2f(m - mref);
+        l *= alpha;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) { o[k][0] *= alpha; o[k][1] *= alpha; }
+        m = mx;
+      }
+      float ps = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = exp2f(x[e] - (mref - 14.0f));
+        ps += x[e];
+      }
+      l += ps;
+      h8 ph, pl;
+      split8(x, ph, pl);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const h8 v0 = codes8(vf[k][0], vf[k][1]), v1 = codes8(vf[k][2], vf[k][3]);
+        f32x4 y0 = {}, y1 = {};
+        y0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, y0, 0, 0, 0);
+        y1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, y1, 0, 0, 0);
+        y0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, y0, 0, 0, 0);
+        y1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, y1, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[k][0][i] = __builtin_fmaf(y0[i], vs, o[k][0][i]);
+          o[k][1][i] = __builtin_fmaf(y1[i], vs, o[k][1][i]);
+        }
+      }
+      load(block(c.v, next), vf);
+    }
+  }
+  // the four waves' (m, l, O) joined in wave order
+  l = column_sum(l);
+#pragma unroll
+  for (int k = 0; k < NB; ++k)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<float4*>(&Os[w][col][32 * k + 16 * h + 4 * g]) =
+          make_float4(o[k][h][0], o[k][h][1], o[k][h][2], o[k][h][3]);
+  if (g == 0) { Ms[w][col] = m; Ls[w][col] = l; }
+  __syncthreads();
+  const int vec = tid >> 4;
+  const int oi = t.grp <= 16 ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= 16 ? vec % t.grp : g0 + vec;
+  if (oi >= tile.i1 || oh >= t.grp) return;
+  const float M = fmaxf(fmaxf(Ms[0][vec], Ms[1][vec]), fmaxf(Ms[2][vec], Ms[3][vec]));
+  float f[4], L = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    // (a wave that saw nothing: m = -inf, l = 0 and O = 0, unless the vector holds NaN)
+    f[k] = Ms[k][vec] == M ? 1.0f : exp2f(Ms[k][vec] - M);
+    L = __builtin_fmaf(Ls[k][vec], f[k], L);
+  }
+  const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
+  const bool whole = tile.steps <= tile.per;                      // one split: nothing to join
+  const float inv = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
+  float* out = whole ? a.ctx + at * HD : a.work + sums_at(b, a, t) + (at * t.splits + sp) * HD;
+  for (int d = 4 * (tid & 15); d < HD; d += 64) {
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(&Os[k][vec][d]);
+      y.x = __builtin_fmaf(x.x, f[k], y.x);
+      y.y = __builtin_fmaf(x.y, f[k], y.y);
+      y.z = __builtin_fmaf(x.z, f[k], y.z);
+      y.w = __builtin_fmaf(x.w, f[k], y.w);
+    }
+    *reinterpret_cast<float4*>(out + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+  }
+  if (!whole && (tid & 15) == 0) {
+    float* ml = a.work + (at * t.splits + sp) * 2;
+    ml[0] = M;
+    ml[1] = L;
+  }
+}
+
+// Joins a tile's splits in split order: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M).
+__global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
+  AttnTile tile;
+  if (!find_tile<256>(b, a, t, tile) || tile.steps <= tile.per) return;
+  const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * 16;
+  const int vec = threadIdx.x >> 4, hd = c.hd, n = (tile.steps + tile.per - 1) / tile.per;
+  const int oi = t.grp <= 16 ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= 16 ? vec % t.grp : g0 + vec;
+  if (oi >= tile.i1 || oh >= t.grp) return;
+  const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
+  const float* ml = a.work + at * t.splits * 2;
+  const float* os = a.work + sums_at(b, a, t) + at * t.splits * hd;
+  float M = -INFINITY;
+  for (int s = 0; s < n; ++s) M = fmaxf(M, ml[2 * s]);
+  float L = 0.0f;
+  for (int s = 0; s < n; ++s) L = __builtin_fmaf(ml[2 * s + 1], ml[2 * s] == M ? 1.0f : exp2f(ml[2 * s] - M), L);
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  for (int d = 4 * (threadIdx.x & 15); d < hd; d += 64) {
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < n; ++s) {
+      const float f = ml[2 * s] == M ? 1.0f : exp2f(ml[2 * s] - M);
+      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * hd + d);
+      y.x = __builtin_fmaf(x.x, f, y.x);
+      y.y = __builtin_fmaf(x.y, f, y.y);
+      y.z = __builtin_fmaf(x.z, f, y.z);
+      y.w = __builtin_fmaf(x.w, f, y.w);
+    }
+    *reinterpret_cast<float4*>(a.ctx + at * hd + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+  }
+}
+
+static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads) {
+  AttnTiles t;
+  t.grp = heads / kv_heads;
+  t.rows_per = t.grp <= 16 ? std::min(16 / t.grp, max_rows) : 1;
+  t.group_tiles = t.grp <= 16 ? 1 : (t.grp + 15) / 16;
+  t.direct = max_rows <= t.rows_per;
+  t.units = t.direct ? requests : rows / t.rows_per + requests;
+  const long tiles = (long)t.units * kv_heads * t.group_tiles;
+  const int most = (std::max(max_len, 1) + 32 * kAttnMinSteps - 1) / (32 * kAttnMinSteps);
+  t.splits = (int)std::max(1L, std::min({(long)most, 4096 / std::max(tiles, 1L), 256L}));
+  return t;
+}
+
+size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
+  const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads);
+  return t.splits > 1 ? split_pairs(rows, heads, t.splits) + (size_t)rows * heads * t.splits * hd : 0;
+}
 
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s) {
-  const dim3 grid((unsigned)(b.rows + b.requests), (unsigned)a.heads);
-  hipLaunchKernelGGL(attention_kv8_rows_kernel, grid, dim3(256), 0, s, b, c, a);
+  const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.heads, c.kv_heads);
+  const dim3 grid((unsigned)t.units, (unsigned)(c.kv_heads * t.group_tiles), (unsigned)t.splits);
+  void (*k)(PagedBatch, Kv8Cache, Attn8Args, AttnTiles) = nullptr;
+  switch (c.hd / 32) {
+    case 1: k = attention_kv8_kernel<1>; break;
+    case 2: k = attention_kv8_kernel<2>; break;
+    case 3: k = attention_kv8_kernel<3>; break;
+    case 4: k = attention_kv8_kernel<4>; break;
+    case 5: k = attention_kv8_kernel<5>; break;
+    case 6: k = attention_kv8_kernel<6>; break;
+    case 7: k = attention_kv8_kernel<7>; break;
+    default: k = attention_kv8_kernel<8>; break;
+  }
+  hipLaunchKernelGGL(k, grid, dim3(256), 0, s, b, c, a, t);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || t.splits == 1) return e;
+  hipLaunchKernelGGL(attention_kv8_join_kernel, dim3(grid.x, grid.y), dim3(256), 0, s, b, c, a, t);
   return hipGetLastError();
 }
 
