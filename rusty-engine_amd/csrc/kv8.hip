@@ -139,42 +139,110 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // How a launch cuts the batch: a tile holds up to 16 query vectors of one request and KV head, rows_per rows of its
-// grp heads (grp <= 16), or 16 of the grp heads of one row (group_tiles of them); with `direct` unit u is request u,
-// which has one tile at most.
+// grp heads (grp <= 16), or 16 of the grp heads of one row (group_tiles of them).
+//   direct: no request has more than one tile. Its keys are cut into pieces of about the same size over all requests,
+//     `pieces` of them in all (and one more for each request), of at least kAttnMinSteps steps: a batch of lengths 1 ..
+//     16384 then takes the time of its sum, not of its longest request.
+//   else: unit u is a tile, every tile is cut into `splits` pieces.
 struct AttnTiles {
-  int grp, rows_per, group_tiles, units, direct, splits;
+  int grp, rows_per, group_tiles, units, direct, splits, pieces;
 };
 
 // A tile's place: request, rows, and the 32-key steps it has to walk, and their cut into splits.
 struct AttnTile {
-  int row0, n, i0, i1;       // first row of the request, its rows, the tile's rows i0 .. i1 - 1 of them
+  int req, row0, n, i0, i1;  // request, its first row, its rows, the tile's rows i0 .. i1 - 1 of them
   int p0;                    // position of the request's row 0 (may be below 0)
-  int len;                   // tokens that the table can hold
   int first, steps, per;     // first step, number of steps, steps per split
-  int req;
 };
 
+constexpr int kAttnMaxSplits8 = 256;  // one thread of the join each
 constexpr int kAttnMinSteps = 16;     // steps of a split, at least (four waves take turns)
 
-template <int THREADS>
-__device__ __forceinline__ bool find_tile(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, AttnTile& o) {
-  const int u = blockIdx.x;
-  const int r = t.direct ? u : request_of_unit<THREADS>(u, b.start, b.requests, b.rows, t.rows_per, 1);
-  if (r < 0) return false;
+// rows i0 .. of request r; false if it has none
+__device__ __forceinline__ bool place_tile(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int r, int i0,
+                                           AttnTile& o) {
   o.req = r;
   o.row0 = min(max(b.start[r], 0), b.rows);
   const int count = min(max(b.count[r], 0), b.rows - o.row0);
-  o.len = min(max(b.len[r], 0), b.table_ld * b.page);
+  const int len = min(max(b.len[r], 0), b.table_ld * b.page);
   o.n = min(count, a.max_rows);
-  o.p0 = o.len - count;
-  o.i0 = t.direct ? 0 : (u - (o.row0 / t.rows_per + r)) * t.rows_per;
-  if (o.i0 < 0 || o.i0 >= o.n) return false;
-  o.i1 = min(o.i0 + t.rows_per, o.n);
+  o.p0 = len - count;
+  o.i0 = i0;
+  o.i1 = min(i0 + t.rows_per, o.n);
   const int last = o.p0 + o.i1 - 1;
-  const int lo = a.window > 0 ? max(0, o.p0 + o.i0 - a.window + 1) : 0;
+  const int lo = a.window > 0 ? max(0, o.p0 + i0 - a.window + 1) : 0;
   o.first = lo >> 5;
   o.steps = last < 0 ? 0 : (last >> 5) - o.first + 1;
-  o.per = max(kAttnMinSteps, ((o.steps + t.splits - 1) / t.splits + 3) & ~3);
+  return i0 >= 0 && i0 < o.n;
+}
+__device__ __forceinline__ int steps_per(int steps, int pieces) {
+  return max(kAttnMinSteps, ((steps + pieces - 1) / pieces + 3) & ~3);
+}
+
+// The sum over a workgroup of 256 threads, and in `before` that of the threads below this one.
+__device__ __forceinline__ int scan256(int v, int& before) {
+  __shared__ int part[4];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int inc = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(inc, off, 64);
+    if (lane >= off) inc += y;
+  }
+  if (lane == 63) part[w] = inc;
+  __syncthreads();
+  const int p0 = part[0], p1 = part[1], p2 = part[2], p3 = part[3];
+  __syncthreads();
+  before = inc - v + (w > 0 ? p0 : 0) + (w > 1 ? p1 : 0) + (w > 2 ? p2 : 0);
+  return p0 + p1 + p2 + p3;
+}
+
+// direct: steps of a piece over the whole batch
+__device__ __forceinline__ int piece_steps(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t) {
+  AttnTile o;
+  int sum = 0, before;
+  const int most = (1 << 30) / b.requests;      // (the sum stays an int)
+  for (int r = threadIdx.x; r < b.requests; r += 256) sum += place_tile(b, a, t, r, 0, o) ? min(o.steps, most) : 0;
+  return steps_per(scan256(sum, before), t.pieces);
+}
+__device__ __forceinline__ void cut_tile(const AttnTiles& t, int piece, AttnTile& o) {
+  o.per = max(piece, steps_per(o.steps, t.splits));
+}
+
+// The tile and split of workgroup `u` of a head; false if there is none.
+__device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int u,
+                                           AttnTile& o, int& sp) {
+  if (!t.direct) {
+    sp = u / t.units;
+    u = (u + sp) % t.units;
+    const int r = request_of_unit<256>(u, b.start, b.requests, b.rows, t.rows_per, 1);
+    if (r < 0) return false;
+    if (!place_tile(b, a, t, r, (u - (min(max(b.start[r], 0), b.rows) / t.rows_per + r)) * t.rows_per, o)) return false;
+    o.per = steps_per(o.steps, t.splits);
+    return sp == 0 || sp * o.per < o.steps;
+  }
+  __shared__ int found[2];
+  const int piece = piece_steps(b, a, t), chunk = (b.requests + 255) / 256;
+  auto pieces_of = [&](int r) {
+    if (!place_tile(b, a, t, r, 0, o)) return 0;
+    cut_tile(t, piece, o);
+    return max(1, (o.steps + o.per - 1) / o.per);
+  };
+  const int r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
+  int mine = 0, before;
+  for (int r = r0; r < r1; ++r) mine += pieces_of(r);
+  const int all = scan256(mine, before);
+  if (u >= all) return false;
+  if (u >= before && u < before + mine) {
+    int r = r0, k = u - before;
+    for (int n; k >= (n = pieces_of(r)); ++r) k -= n;
+    found[0] = r;
+    found[1] = k;
+  }
+  __syncthreads();
+  sp = found[1];
+  place_tile(b, a, t, found[0], 0, o);
+  cut_tile(t, piece, o);
   return true;
 }
 
@@ -201,10 +269,10 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   __shared__ float Ms[4][16], Ls[4][16];
   __shared__ __attribute__((aligned(16))) float Os[4][16][LD];
   AttnTile tile;
-  if (!find_tile<256>(b, a, t, tile)) return;
-  const int sp = blockIdx.z;
-  const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * 16;
-  if (sp > 0 && sp * tile.per >= tile.steps) return;
+  const int ht = c.kv_heads * t.group_tiles, yy = blockIdx.x % ht;
+  int sp;
+  if (!find_piece(b, a, t, blockIdx.x / ht, tile, sp)) return;
+  const int head = yy / t.group_tiles, g0 = (yy % t.group_tiles) * 16;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int s0 = tile.first + sp * tile.per, s1 = min(s0 + tile.per, tile.first + tile.steps);
@@ -378,34 +446,69 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   }
 }
 
-// Joins a tile's splits in split order: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M).
+// Joins the splits of one query vector: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). A thread has a
+// split's weight; then 256 / (hd / 4) groups of threads add every so-manieth split, and their sums are added in order.
 __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
+  __shared__ float f[kAttnMaxSplits8], red[2][4];
+  __shared__ float4 part[256];
   AttnTile tile;
-  if (!find_tile<256>(b, a, t, tile) || tile.steps <= tile.per) return;
+  if (t.direct) {
+    const int piece = piece_steps(b, a, t);
+    if (!place_tile(b, a, t, blockIdx.x, 0, tile)) return;
+    cut_tile(t, piece, tile);
+  } else {
+    int sp;
+    if (!find_piece(b, a, t, blockIdx.x, tile, sp)) return;
+  }
+  if (tile.steps <= tile.per) return;
+  const int tid = threadIdx.x, w = tid >> 6, vec = blockIdx.z, hd = c.hd;
   const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * 16;
-  const int vec = threadIdx.x >> 4, hd = c.hd, n = (tile.steps + tile.per - 1) / tile.per;
   const int oi = t.grp <= 16 ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= 16 ? vec % t.grp : g0 + vec;
   if (oi >= tile.i1 || oh >= t.grp) return;
+  const int n = (tile.steps + tile.per - 1) / tile.per;
   const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
   const float* ml = a.work + at * t.splits * 2;
-  const float* os = a.work + sums_at(b, a, t) + at * t.splits * hd;
-  float M = -INFINITY;
-  for (int s = 0; s < n; ++s) M = fmaxf(M, ml[2 * s]);
-  float L = 0.0f;
-  for (int s = 0; s < n; ++s) L = __builtin_fmaf(ml[2 * s + 1], ml[2 * s] == M ? 1.0f : exp2f(ml[2 * s] - M), L);
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  for (int d = 4 * (threadIdx.x & 15); d < hd; d += 64) {
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < n; ++s) {
-      const float f = ml[2 * s] == M ? 1.0f : exp2f(ml[2 * s] - M);
-      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * hd + d);
-      y.x = __builtin_fmaf(x.x, f, y.x);
-      y.y = __builtin_fmaf(x.y, f, y.y);
-      y.z = __builtin_fmaf(x.z, f, y.z);
-      y.w = __builtin_fmaf(x.w, f, y.w);
+  const float m = tid < n ? ml[2 * tid] : -INFINITY;
+  float l = tid < n ? ml[2 * tid + 1] : 0.0f, M = m;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  if ((tid & 63) == 0) red[0][w] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const float fs = m == M ? 1.0f : exp2f(m - M);
+  f[tid] = fs;
+  l *= fs;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+  if ((tid & 63) == 0) red[1][w] = l;
+  __syncthreads();
+  const float L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  const int cols = hd >> 2, groups = 256 / cols;
+  const int col = tid % cols, grp = tid / cols;
+  const float* os = a.work + sums_at(b, a, t) + at * t.splits * hd + 4 * col;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < groups) {
+#pragma unroll 4
+    for (int s = grp; s < n; s += groups) {
+      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * hd);
+      y.x = __builtin_fmaf(x.x, f[s], y.x);
+      y.y = __builtin_fmaf(x.y, f[s], y.y);
+      y.z = __builtin_fmaf(x.z, f[s], y.z);
+      y.w = __builtin_fmaf(x.w, f[s], y.w);
     }
-    *reinterpret_cast<float4*>(a.ctx + at * hd + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
   }
+  part[tid] = y;
+  __syncthreads();
+  if (tid >= cols) return;
+  for (int k = 1; k < groups; ++k) {
+    const float4 x = part[k * cols + tid];
+    y.x += x.x;
+    y.y += x.y;
+    y.z += x.z;
+    y.w += x.w;
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  *reinterpret_cast<float4*>(a.ctx + at * hd + 4 * tid) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
 static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads) {
@@ -415,9 +518,13 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   t.group_tiles = t.grp <= 16 ? 1 : (t.grp + 15) / 16;
   t.direct = max_rows <= t.rows_per;
   t.units = t.direct ? requests : rows / t.rows_per + requests;
-  const long tiles = (long)t.units * kv_heads * t.group_tiles;
+  const long ht = (long)kv_heads * t.group_tiles;
   const int most = (std::max(max_len, 1) + 32 * kAttnMinSteps - 1) / (32 * kAttnMinSteps);
-  t.splits = (int)std::max(1L, std::min({(long)most, 4096 / std::max(tiles, 1L), 256L}));
+  // two workgroups of a piece for each CU (us of 512 / 1024 / 2048 / 8192 workgroups: one request of 131071 tokens, 8
+  // heads of 128, 55.7 / 59.6 / 63.4 / 74; 64 requests of 1 .. 16384, 4 heads, 44.9 / 47.6 / 47.5 / 53.9)
+  t.pieces = (int)std::max(1L, 512 / ht);
+  const long cuts = t.direct ? t.pieces : 1024 / (t.units * ht);
+  t.splits = (int)std::max(1L, std::min({(long)most, cuts, (long)kAttnMaxSplits8}));
   return t;
 }
 
@@ -440,10 +547,13 @@ hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const At
     case 7: k = attention_kv8_kernel<7>; break;
     default: k = attention_kv8_kernel<8>; break;
   }
-  hipLaunchKernelGGL(k, grid, dim3(256), 0, s, b, c, a, t);
+  const unsigned per_head = t.direct ? (unsigned)(t.pieces + b.requests) : grid.x * grid.z;
+  hipLaunchKernelGGL(k, dim3(per_head * grid.y), dim3(256), 0, s, b, c, a, t);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || t.splits == 1) return e;
-  hipLaunchKernelGGL(attention_kv8_join_kernel, dim3(grid.x, grid.y), dim3(256), 0, s, b, c, a, t);
+  const int vecs = t.grp <= 16 ? t.rows_per * t.grp : 16;
+  hipLaunchKernelGGL(attention_kv8_join_kernel, dim3(grid.x, grid.y, (unsigned)vecs), dim3(256), 0, s, b, c,
+                     a, t);
   return hipGetLastError();
 }
 
