@@ -13,13 +13,6 @@
 
 namespace rehip {
 
-__device__ __forceinline__ int k_byte(int token, int dim) {
-  return 16 * (16 * (dim >> 3) + (token & 15)) + 8 * (token >> 4) + (dim & 7);
-}
-__device__ __forceinline__ int v_byte(int token, int dim) {
-  return 16 * (16 * ((token >> 2) & 3) + (dim & 15)) + 8 * (dim >> 4) + 4 * (token >> 4) + (token & 3);
-}
-
 // ---- append --------------------------------------------------------------------------------------
 // A page and head's scale s is the largest finite magnitude of what it holds / 127 (0 below the smallest normal
 // float: such values are stored as 0), a value's code round(x / s), ties to even. Rows that raise the scale of a
@@ -30,7 +23,11 @@ __device__ __forceinline__ int code_of(float x, float s) {
   return x != x || s == 0.0f ? 0 : (int)fminf(fmaxf(r, -127.0f), 127.0f);
 }
 
-// One workgroup per (run of one request's new rows inside one page, head, K or V).
+// One workgroup per (run of one request's new rows inside one page, head, K or V). A thread has U units of 16 codes that
+// lie together in memory (K: 2 tokens x 8 dimensions, V: 8 tokens x 2): it loads their values, and their codes where
+// some token of the unit is not new, all before the largest magnitude is known, so that the chain is one round trip to
+// memory for the request, one for its page and one for all of this. U = 0: the units in turn, their values read twice.
+template <int U>
 __global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache c, const float* __restrict__ k,
                                                          size_t ldk, const float* __restrict__ v, size_t ldv) {
   __shared__ unsigned red[4];
@@ -47,32 +44,115 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache 
   if (lo >= hi) return;
   const int pid = b.table[(size_t)r * b.table_ld + pi];
   if (pid < 0 || pid >= b.n_pages) return;
-  const int o0 = lo - pi * b.page, o1 = hi - pi * b.page, hd = c.hd;
+  const int o0 = lo - pi * b.page, o1 = hi - pi * b.page, hd = c.hd, nb = hd >> 5;
   const size_t ld = is_v ? ldv : ldk;
+  // (the row of token o0; token t's is (t - o0) rows on)
   const float* x = (is_v ? v : k) + (size_t)(row0 + lo - first) * ld + (size_t)head * hd;
   int8_t* codes = (is_v ? c.v : c.k) + ((size_t)pid * c.kv_heads + head) * b.page * hd;
   float* scale = (is_v ? c.vs : c.ks) + (size_t)pid * c.kv_heads + head;
+  const int units = b.page * hd / 16, m = tid & 15, g = (tid >> 4) & 3;
+  // unit q: blocks follow each other 64 units apart, so a thread's place in its blocks is one
+  auto first_token = [&](int q) { return 32 * ((q >> 6) / nb) + (is_v ? 4 * g : m); };
+  auto first_dim = [&](int q) { return 32 * ((q >> 6) % nb) + (is_v ? m : 8 * g); };
+  auto token_of = [&](int t, int e) { return t + (is_v ? 16 * ((e >> 2) & 1) + (e & 3) : 16 * (e >> 3)); };
+  auto load = [&](int q, float (&y)[16]) {
+    const int t = first_token(q), d = first_dim(q);
+    if (is_v) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int tok = token_of(t, e);
+        y[e] = tok >= o0 && tok < o1 ? x[(size_t)(tok - o0) * ld + d + 16 * (e >> 3)] : 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int tok = token_of(t, e);
+        *reinterpret_cast<float4*>(&y[e]) = tok >= o0 && tok < o1
+                                                ? *reinterpret_cast<const float4*>(x + (size_t)(tok - o0) * ld + d + (e & 4))
+                                                : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  };
+  // tokens of a unit: the first, the last, and whether any is new / old / other than new
+  auto news = [&](int t) {
+    return is_v ? (t < o1 && t + 3 >= o0) || (t + 16 < o1 && t + 19 >= o0) : (t < o1 && t >= o0) || (t + 16 < o1 && t + 16 >= o0);
+  };
+  auto whole = [&](int t) { return t >= o0 && t + (is_v ? 20 : 17) <= o1; };
+  auto largest = [&](const float (&y)[16], unsigned top) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const unsigned bits = __float_as_uint(y[e]) & 0x7fffffffu;
+      top = max(top, bits < 0x7f800000u ? bits : 0u);
+    }
+    return top;
+  };
+  float y[U > 0 ? U : 1][16];
+  uint4 old[U > 0 ? U : 1];
   const float s_old = o0 > 0 ? *scale : 0.0f;
-  unsigned a = 0;
-  for (int e = tid; e < (o1 - o0) * hd; e += 256) {
-    const unsigned bits = __float_as_uint(x[(size_t)(e / hd) * ld + e % hd]) & 0x7fffffffu;
-    if (bits < 0x7f800000u) a = max(a, bits);
+  unsigned top = 0;
+  if constexpr (U > 0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int q = tid + 256 * i, t = first_token(q);
+      if (q < units) {
+        load(q, y[i]);
+        if (!whole(t) && (o0 > 0 || news(t))) old[i] = reinterpret_cast<const uint4*>(codes)[q];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (tid + 256 * i < units) top = largest(y[i], top);
+  } else {
+    for (int q = tid; q < units; q += 256) {
+      load(q, y[0]);
+      top = largest(y[0], top);
+    }
   }
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, off, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = a;
+  for (int off = 32; off > 0; off >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, off, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = top;
   __syncthreads();
-  a = max(max(red[0], red[1]), max(red[2], red[3]));
-  float s = __uint_as_float(a) * (1.0f / 127.0f);
+  top = max(max(red[0], red[1]), max(red[2], red[3]));
+  float s = __uint_as_float(top) * (1.0f / 127.0f);
   if (s < 1.17549435e-38f) s = 0.0f;
   s = fmaxf(s, s_old);
-  const float ratio = s > s_old ? s_old / s : 1.0f;
-  const int t0 = ratio != 1.0f ? 0 : o0;       // old codes are touched only if the scale grew
-  for (int e = t0 * hd + tid; e < o1 * hd; e += 256) {
-    const int tok = e / hd, d = e % hd;
-    int8_t* p = codes + (size_t)((tok >> 5) * (hd >> 5) + (d >> 5)) * 1024 +
-                (is_v ? v_byte(tok & 31, d & 31) : k_byte(tok & 31, d & 31));
-    *p = (int8_t)(tok < o0 ? (int)rintf((float)*p * ratio) : code_of(x[(size_t)(tok - o0) * ld + d], s));
+  const bool grown = s > s_old && o0 > 0;
+  const float ratio = grown ? s_old / s : 1.0f;
+  auto store = [&](int q, const float (&z)[16], const uint4& was) {
+    const int t = first_token(q);
+    if (!news(t) && !(grown && t < o0)) return;
+    const unsigned w[4] = {was.x, was.y, was.z, was.w};
+    unsigned out[4];
+    const bool all = whole(t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 4 * i + j, tok = token_of(t, e);
+        int code = code_of(z[e], s);
+        if (!all) {
+          const int held = (int)(int8_t)(w[i] >> (8 * j));
+          if (tok < o0) code = grown ? (int)rintf((float)held * ratio) : held;
+          else if (tok >= o1) code = held;
+        }
+        out[i] |= (unsigned)(code & 0xff) << (8 * j);
+      }
+    }
+    reinterpret_cast<uint4*>(codes)[q] = make_uint4(out[0], out[1], out[2], out[3]);
+  };
+  if constexpr (U > 0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (tid + 256 * i < units) store(tid + 256 * i, y[i], old[i]);
+  } else {
+    for (int q = tid; q < units; q += 256) {
+      const int t = first_token(q);
+      if (!news(t) && !(grown && t < o0)) continue;
+      load(q, y[0]);
+      if (!whole(t)) old[0] = reinterpret_cast<const uint4*>(codes)[q];
+      store(q, y[0], old[0]);
+    }
   }
   if (tid == 0) *scale = s;
 }
@@ -80,7 +160,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache 
 hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, size_t ldk, const float* v,
                              size_t ldv, hipStream_t s) {
   const dim3 grid((unsigned)(b.rows / b.page + 2 * b.requests), (unsigned)c.kv_heads, 2);
-  hipLaunchKernelGGL(kv8_append_kernel, grid, dim3(256), 0, s, b, c, k, ldk, v, ldv);
+  const int units = b.page * c.hd / 16;
+  auto* f = units <= 256 ? kv8_append_kernel<1> : units <= 512 ? kv8_append_kernel<2> : units <= 1024 ? kv8_append_kernel<4>
+                                                                                           : kv8_append_kernel<0>;
+  hipLaunchKernelGGL(f, grid, dim3(256), 0, s, b, c, k, ldk, v, ldv);
   return hipGetLastError();
 }
 
