@@ -200,16 +200,19 @@ __device__ __forceinline__ h8 codes8(unsigned a, unsigned b) {
 
 // x = hi + lo, each rounded to the nearest f16
 __device__ __forceinline__ void split8(const float (&x)[8], h8& hi, h8& lo) {
+  union { h2 h[4]; h8 v; } a, b;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const h2 h = {(_Float16)x[i], (_Float16)x[i + 1]};
-    const h2 l = {(_Float16)(x[i] - (float)h[0]), (_Float16)(x[i + 1] - (float)h[1])};
-    hi[i] = h[0];
-    hi[i + 1] = h[1];
-    lo[i] = l[0];
-    lo[i + 1] = l[1];
+  for (int i = 0; i < 4; ++i) {
+    a.h[i] = __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), h2);
+    const f32x2 r = {__builtin_fmaf((float)a.h[i][0], -1.0f, x[2 * i]), __builtin_fmaf((float)a.h[i][1], -1.0f, x[2 * i + 1])};
+    b.h[i] = __builtin_convertvector(r, h2);
   }
+  hi = a.v;
+  lo = b.v;
 }
+
+// 2^x for x <= 14: what is below the smallest normal float may come out as 0
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // the largest / the sum over the four lanes that share a column of the 16 x 16 layouts (lanes l, l ^ 16, l ^ 32, ..)
 __device__ __forceinline__ float column_max(float v) {
@@ -337,6 +340,12 @@ __device__ __forceinline__ size_t sums_at(const PagedBatch& b, const Attn8Args& 
   return split_pairs(b.rows, a.heads, t.splits);
 }
 
+// the same in every lane, so that what follows from it is scalar
+__device__ __forceinline__ AttnTile uniform(const AttnTile& o) {
+  auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return {u(o.req), u(o.row0), u(o.n), u(o.i0), u(o.i1), u(o.p0), u(o.first), u(o.steps), u(o.per)};
+}
+
 constexpr int kAttnPages = 512;       // pages whose numbers and scales are staged at a time
 
 // One workgroup of four waves per (tile, KV head, split of the keys). A wave takes every fourth step of 32 keys:
@@ -355,6 +364,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   const int ht = c.kv_heads * t.group_tiles, yy = blockIdx.x % ht;
   int sp;
   if (!find_piece(b, a, t, blockIdx.x / ht, tile, sp)) return;
+  tile = uniform(tile);
+  sp = __builtin_amdgcn_readfirstlane(sp);
   const int head = yy / t.group_tiles, g0 = (yy % t.group_tiles) * 16;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -365,6 +376,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   const bool live = vi < tile.i1 && vh < t.grp;
   const int pos = live ? tile.p0 + vi : -1;                       // sees keys low .. pos
   const int low = a.window > 0 ? pos - a.window + 1 : 0;
+  // every vector of the tile sees the keys see_from .. see_all (a place without one may see anything: it is not stored)
+  const int see_all = tile.p0 + tile.i0, see_from = a.window > 0 ? tile.p0 + tile.i1 - a.window : 0;
   h8 qh[NB], ql[NB];
   float qs;
   {
@@ -398,6 +411,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   for (int k = 0; k < NB; ++k) o[k][0] = o[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   const size_t head_bytes = (size_t)b.page * HD;
   const int page_steps = b.page >> 5;
+  const unsigned page_inv = 65536u / page_steps + 1;
   for (int pg0 = s0 / page_steps; pg0 * page_steps < s1; pg0 += kAttnPages) {
     // the pages of these steps: their numbers and scales
     const int npg = min(kAttnPages, (s1 - 1) / page_steps - pg0 + 1);
@@ -411,12 +425,14 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       vss[i] = have ? c.vs[at] : 0.0f;
     }
     __syncthreads();
-    const int e0 = max(s0, pg0 * page_steps), e1 = min(s1, (pg0 + npg) * page_steps);
+    // steps from here on count from page pg0's first (below kAttnPages * 8): the quotient by page_steps is exact
+    const int c0 = pg0 * page_steps, e0 = max(s0 - c0, 0), e1 = min(s1 - c0, npg * page_steps);
+    auto page_of = [&](int s) { return (int)((unsigned)s * page_inv >> 16); };
     u32x4 kf[NB], vf[NB];
     auto block = [&](const int8_t* base, int s) {
-      const int pi = s / page_steps - pg0;
+      const int pi = page_of(s);
       const int pid = __builtin_amdgcn_readfirstlane(max(ids[pi], 0));
-      return base + ((size_t)pid * c.kv_heads + head) * head_bytes + (size_t)(s % page_steps) * (NB * 1024);
+      return base + ((size_t)pid * c.kv_heads + head) * head_bytes + (size_t)(s - pi * page_steps) * (NB * 1024);
     };
     auto load = [&](const int8_t* p, u32x4 (&x)[NB]) {
 #pragma unroll
@@ -430,7 +446,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     }
     for (; s < e1; s += 4) {
       const int next = min(s + 4, e1 - 1);
-      const int pi = s / page_steps - pg0;
+      const int pi = page_of(s), key0 = 32 * (s + c0);
       const bool have = ids[pi] >= 0;
       const float ks = kss[pi] * qs, vs = vss[pi];
       f32x4 st[2] = {};
@@ -445,15 +461,20 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       load(block(c.k, next), kf);
       float x[8], mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
-        x[e] = have && j <= pos && j >= low ? st[e >> 2][e & 3] * ks : -INFINITY;
-        mx = fmaxf(mx, x[e]);
+      for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3] * ks;
+      if (!have || key0 + 31 > see_all || key0 < see_from) {      // some vector does not see some key
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
+          if (!have || j > pos || j < low) x[e] = -INFINITY;
+        }
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
       mx = fmaxf(m, column_max(mx));
       const float mref = mx == -INFINITY ? 0.0f : mx;
       if (__ballot(mx > m) != 0) {
-        const float alpha = exp2f(m - mref);
+        const float alpha = pow2(m - mref);
         l *= alpha;
 #pragma unroll
         for (int k = 0; k < NB; ++k) { o[k][0] *= alpha; o[k][1] *= alpha; }
@@ -462,7 +483,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       float ps = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = exp2f(x[e] - (mref - 14.0f));
+        x[e] = pow2(x[e] - (mref - 14.0f));
         ps += x[e];
       }
       l += ps;
@@ -503,7 +524,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     // (a wave that saw nothing: m = -inf, l = 0 and O = 0, unless the vector holds NaN)
-    f[k] = Ms[k][vec] == M ? 1.0f : exp2f(Ms[k][vec] - M);
+    f[k] = Ms[k][vec] == M ? 1.0f : pow2(Ms[k][vec] - M);
     L = __builtin_fmaf(Ls[k][vec], f[k], L);
   }
   const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
@@ -558,7 +579,7 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
   if ((tid & 63) == 0) red[0][w] = M;
   __syncthreads();
   M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  const float fs = m == M ? 1.0f : exp2f(m - M);
+  const float fs = m == M ? 1.0f : pow2(m - M);
   f[tid] = fs;
   l *= fs;
 #pragma unroll
