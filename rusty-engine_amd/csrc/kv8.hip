@@ -174,13 +174,15 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 // All products run on v_mfma_f32_16x16x32_f16: an int8 code is exact in f16, and the f32 operands (q, the
 // probabilities) are split into two f16 parts, hi + lo, good to 2^-22 of the largest: two instructions per product,
 // f32 sums. q is first scaled by the power of two that takes its vector's largest element to 2^13 .. 2^14, so no part
-// falls out of f16's range; the terms exp(s - max), at most 1, are taken times 2^14, which cancels in the division by
-// their sum. Each step's products with V's codes are summed from zero and scaled by the page's scale in f32 (scales
+// falls out of f16's range; the terms exp(s - m) are taken times 2^kTermBits, which cancels in the division by their
+// sum. m is the vector's largest score so far or up to kSlack (in powers of 2) below it: sums are moved to a new m only
+// when a score passes that, which after the first steps is rare. Each step's products with V's codes are summed from zero and scaled by the page's scale in f32 (scales
 // taken into the f16 weights cost a row that sees only pages of small scale its precision).
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+constexpr float kTermBits = 10.0f, kSlack = 5.0f;     // 2^(10 + 5) stays below f16's 65504
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // eight codes as f16: 0x6400 + u is the f16 value 1024 + u for a byte u = c + 128, less 1152 is c
@@ -198,40 +200,54 @@ __device__ __forceinline__ h8 codes8(unsigned a, unsigned b) {
   return r.v;
 }
 
-// x = hi + lo, each rounded to the nearest f16
-__device__ __forceinline__ void split8(const float (&x)[8], h8& hi, h8& lo) {
+// x = hi + lo, each rounded to the nearest f16. minus_one: -1, but unknown to the compiler, which then subtracts hi in
+// one mixed-precision fma instead of converting it back first
+__device__ __forceinline__ void split8(const float (&x)[8], float minus_one, h8& hi, h8& lo) {
   union { h2 h[4]; h8 v; } a, b;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     a.h[i] = __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), h2);
-    const f32x2 r = {__builtin_fmaf((float)a.h[i][0], -1.0f, x[2 * i]), __builtin_fmaf((float)a.h[i][1], -1.0f, x[2 * i + 1])};
+    const f32x2 r = {__builtin_fmaf((float)a.h[i][0], minus_one, x[2 * i]),
+                     __builtin_fmaf((float)a.h[i][1], minus_one, x[2 * i + 1])};
     b.h[i] = __builtin_convertvector(r, h2);
   }
   hi = a.v;
   lo = b.v;
 }
 
-// 2^x for x <= 14: what is below the smallest normal float may come out as 0
+// 2^x for x <= 16: what is below the smallest normal float may come out as 0
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// the largest / the sum over the four lanes that share a column of the 16 x 16 layouts (lanes l, l ^ 16, l ^ 32, ..)
+// v of lane l ^ 16 / l ^ 32, without LDS: the swaps exchange halves, and a lane keeps the one that was its partner's
+__device__ __forceinline__ float swap16(float v) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 16) ? s[0] : s[1]);
+}
+__device__ __forceinline__ float swap32(float v) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? s[0] : s[1]);
+}
+// the largest over the four lanes that share a column of the 16 x 16 layouts (one of the swapped values is the lane's
+// own, so both may be taken), and the sum
 __device__ __forceinline__ float column_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float column_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  v += swap16(v);
+  return v + swap32(v);
 }
 
-// How a launch cuts the batch: a tile holds up to 16 query vectors of one request and KV head, rows_per rows of its
-// grp heads (grp <= 16), or 16 of the grp heads of one row (group_tiles of them).
+// How a launch cuts the batch: a tile holds up to vecs query vectors of one request and KV head, rows_per rows of its
+// grp heads (grp <= vecs), or vecs of the grp heads of one row (group_tiles of them).
 //   direct: no request has more than one tile. Its keys are cut into pieces of about the same size over all requests,
 //     `pieces` of them in all (and one more for each request), of at least kAttnMinSteps steps: a batch of lengths 1 ..
 //     16384 then takes the time of its sum, not of its longest request.
 //   else: unit u is a tile, every tile is cut into `splits` pieces.
 struct AttnTiles {
-  int grp, rows_per, group_tiles, units, direct, splits, pieces;
+  int vecs, grp, rows_per, group_tiles, units, direct, splits, pieces;
 };
 
 // A tile's place: request, rows, and the 32-key steps it has to walk, and their cut into splits.
@@ -300,7 +316,7 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
                                            AttnTile& o, int& sp) {
   if (!t.direct) {
     sp = u / t.units;
-    u = (u + sp) % t.units;
+    u = t.units - 1 - (u + sp) % t.units;             // (a prompt's last rows see the most keys: first)
     const int r = request_of_unit<256>(u, b.start, b.requests, b.rows, t.rows_per, 1);
     if (r < 0) return false;
     if (!place_tile(b, a, t, r, (u - (min(max(b.start[r], 0), b.rows) / t.rows_per + r)) * t.rows_per, o)) return false;
@@ -348,41 +364,54 @@ __device__ __forceinline__ AttnTile uniform(const AttnTile& o) {
 
 constexpr int kAttnPages = 512;       // pages whose numbers and scales are staged at a time
 
-// One workgroup of four waves per (tile, KV head, split of the keys). A wave takes every fourth step of 32 keys:
+// One workgroup of four waves per (tile, KV head, split of the keys). A wave takes every fourth step of 32 keys, for
+// VT groups of 16 query vectors:
 //   S^T = K Q^T (two 16-key tiles; lane l has keys 4 (l / 16) + i of each for vector l % 16), the running maximum
 //   and sum, and O^T += V^T P^T, whose operand P^T is what the lane holds of S^T.
 // Codes go from memory to registers in fragment order: 16 bytes per lane and 1 KiB per load, no LDS. The next K block
-// loads while the softmax and V's products run, the next V block while K's do.
-template <int NB>
+// loads while the softmax and V's products run, the next V block while K's do. With one group its q stays in
+// registers; with more (prompts) the groups' q lies in LDS, in fragment order too, and every code is converted to f16
+// once for all of them.
+template <int NB, int VT>
 __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
   constexpr int HD = 32 * NB, LD = HD + 4;
   __shared__ int ids[kAttnPages];
   __shared__ float kss[kAttnPages], vss[kAttnPages];
   __shared__ float Ms[4][16], Ls[4][16];
-  __shared__ __attribute__((aligned(16))) float Os[4][16][LD];
+  constexpr size_t kQ = VT > 1 ? (size_t)VT * NB * 2 * 1024 : 0, kO = sizeof(float) * 4 * 16 * LD;
+  __shared__ __attribute__((aligned(16))) char big[kQ > kO ? kQ : kO];    // q, and after the steps the waves' sums
+  float (*Os)[16][LD] = reinterpret_cast<float (*)[16][LD]>(big);
+  h8* const qf = reinterpret_cast<h8*>(big);                              // [VT][NB][hi, lo][lane]
+  __shared__ float qss[VT][16];
   AttnTile tile;
   const int ht = c.kv_heads * t.group_tiles, yy = blockIdx.x % ht;
   int sp;
   if (!find_piece(b, a, t, blockIdx.x / ht, tile, sp)) return;
   tile = uniform(tile);
   sp = __builtin_amdgcn_readfirstlane(sp);
-  const int head = yy / t.group_tiles, g0 = (yy % t.group_tiles) * 16;
+  const int head = yy / t.group_tiles, g0 = (yy % t.group_tiles) * t.vecs;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int s0 = tile.first + sp * tile.per, s1 = min(s0 + tile.per, tile.first + tile.steps);
-  // this lane's query vector
-  const int vi = t.grp <= 16 ? tile.i0 + col / t.grp : tile.i0;
-  const int vh = t.grp <= 16 ? col % t.grp : g0 + col;
-  const bool live = vi < tile.i1 && vh < t.grp;
-  const int pos = live ? tile.p0 + vi : -1;                       // sees keys low .. pos
-  const int low = a.window > 0 ? pos - a.window + 1 : 0;
   // every vector of the tile sees the keys see_from .. see_all (a place without one may see anything: it is not stored)
   const int see_all = tile.p0 + tile.i0, see_from = a.window > 0 ? tile.p0 + tile.i1 - a.window : 0;
+  // vector col of group v: row and head, the last key it sees (-1: no such vector)
+  auto row_of = [&](int vec) { return t.grp <= t.vecs ? tile.i0 + vec / t.grp : tile.i0; };
+  auto head_of = [&](int vec) { return t.grp <= t.vecs ? vec % t.grp : g0 + vec; };
+  int pos[VT];
+#pragma unroll
+  for (int v = 0; v < VT; ++v)
+    pos[v] = row_of(16 * v + col) < tile.i1 && head_of(16 * v + col) < t.grp ? tile.p0 + row_of(16 * v + col) : -1;
+  float minus_one = -1.0f;
+  asm volatile("" : "+v"(minus_one));
   h8 qh[NB], ql[NB];
-  float qs;
-  {
-    const float* q = a.q + (size_t)(tile.row0 + (live ? vi : tile.i0)) * a.ldq +
-                     (size_t)(head * t.grp + (live ? vh : 0)) * HD + 8 * g;
+  float qs = 0.0f;
+#pragma unroll
+  for (int v = 0; v < VT; ++v) {
+    if (VT > 1 && v % 4 != w) continue;                            // (a wave each)
+    const bool live = row_of(16 * v + col) < tile.i1 && head_of(16 * v + col) < t.grp;
+    const float* q = a.q + (size_t)(tile.row0 + (live ? row_of(16 * v + col) : tile.i0)) * a.ldq +
+                     (size_t)(head * t.grp + (live ? head_of(16 * v + col) : 0)) * HD + 8 * g;
     float x[NB][8];
     unsigned top = 0;
 #pragma unroll
@@ -396,19 +425,32 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
     const int e = (int)(top >> 23);                               // 2^13 <= largest * 2^(f - 127) < 2^14
     const int f = e == 255 ? 127 : min(267 - e, 253);
-    const float up = __uint_as_float((unsigned)f << 23);
-    qs = __uint_as_float((unsigned)(254 - f) << 23) * (a.scale * 1.4426950408889634f);
+    const float up = copysignf(__uint_as_float((unsigned)f << 23), a.scale);   // (scores' factor is then positive)
+    qs = __uint_as_float((unsigned)(254 - f) << 23) * (fabsf(a.scale) * 1.4426950408889634f);
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[k][j] *= up;
-      split8(x[k], qh[k], ql[k]);
+      split8(x[k], minus_one, qh[k], ql[k]);
+      if (VT > 1) {
+        qf[((v * NB + k) * 2 + 0) * 64 + lane] = qh[k];
+        qf[((v * NB + k) * 2 + 1) * 64 + lane] = ql[k];
+      }
     }
+    if (VT > 1 && g == 0) qss[v][col] = qs;
   }
-  float m = -INFINITY, l = 0.0f;
-  f32x4 o[NB][2];
+  if (VT > 1) __syncthreads();
+  float qsv[VT], m[VT], l[VT];
+  f32x4 o[VT][NB][2];
 #pragma unroll
-  for (int k = 0; k < NB; ++k) o[k][0] = o[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int v = 0; v < VT; ++v) {
+    qsv[v] = VT > 1 ? qss[v][col] : qs;
+    m[v] = -INFINITY;
+    l[v] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) o[v][k][0] = o[v][k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  bool huge = false;                     // some vector's m is beyond 2^20
   const size_t head_bytes = (size_t)b.page * HD;
   const int page_steps = b.page >> 5;
   const unsigned page_inv = 65536u / page_steps + 1;
@@ -434,10 +476,13 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       const int pid = __builtin_amdgcn_readfirstlane(max(ids[pi], 0));
       return base + ((size_t)pid * c.kv_heads + head) * head_bytes + (size_t)(s - pi * page_steps) * (NB * 1024);
     };
+    // (a decode step reads every code once; prompts' tiles read them again, from L2)
     auto load = [&](const int8_t* p, u32x4 (&x)[NB]) {
 #pragma unroll
-      for (int k = 0; k < NB; ++k)
-        x[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 1024 * k + 16 * lane));
+      for (int k = 0; k < NB; ++k) {
+        const u32x4* at = reinterpret_cast<const u32x4*>(p + 1024 * k + 16 * lane);
+        x[k] = VT > 1 ? *at : __builtin_nontemporal_load(at);
+      }
     };
     int s = e0 + w;
     if (s < e1) {
@@ -448,126 +493,213 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       const int next = min(s + 4, e1 - 1);
       const int pi = page_of(s), key0 = 32 * (s + c0);
       const bool have = ids[pi] >= 0;
-      const float ks = kss[pi] * qs, vs = vss[pi];
-      f32x4 st[2] = {};
+      const float ks = kss[pi], vs = vss[pi];
+      f32x4 st[VT][2] = {};
+      int at = lane;                     // (q is read in every step: held in registers it costs a SIMD its third wave)
+      if (VT > 1) asm volatile("" : "+v"(at));
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         const h8 k0 = codes8(kf[k][0], kf[k][1]), k1 = codes8(kf[k][2], kf[k][3]);
-        st[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[k], st[0], 0, 0, 0);
-        st[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[k], st[1], 0, 0, 0);
-        st[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[k], st[0], 0, 0, 0);
-        st[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[k], st[1], 0, 0, 0);
-      }
-      load(block(c.k, next), kf);
-      float x[8], mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3] * ks;
-      if (!have || key0 + 31 > see_all || key0 < see_from) {      // some vector does not see some key
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
-          if (!have || j > pos || j < low) x[e] = -INFINITY;
+        for (int v = 0; v < VT; ++v) {
+          const h8 hi = VT > 1 ? qf[((v * NB + k) * 2 + 0) * 64 + at] : qh[k];
+          const h8 lo = VT > 1 ? qf[((v * NB + k) * 2 + 1) * 64 + at] : ql[k];
+          st[v][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, hi, st[v][0], 0, 0, 0);
+          st[v][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, hi, st[v][1], 0, 0, 0);
+          st[v][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, lo, st[v][0], 0, 0, 0);
+          st[v][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, lo, st[v][1], 0, 0, 0);
         }
       }
+      load(block(c.k, next), kf);
+      // f > 0, so the largest product is the largest score (0 would make NaN of the hidden ones' -inf)
+      float f[VT], mx[VT];
+      const bool hides = !have || key0 + 31 > see_all || key0 < see_from;      // some vector does not see some key
+      if (hides) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
-      mx = fmaxf(m, column_max(mx));
-      const float mref = mx == -INFINITY ? 0.0f : mx;
-      if (__ballot(mx > m) != 0) {
-        const float alpha = pow2(m - mref);
-        l *= alpha;
+        for (int v = 0; v < VT; ++v) {
+          const int low = a.window > 0 ? pos[v] - a.window + 1 : 0;
 #pragma unroll
-        for (int k = 0; k < NB; ++k) { o[k][0] *= alpha; o[k][1] *= alpha; }
-        m = mx;
+          for (int e = 0; e < 8; ++e) {
+            const int j = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
+            if (!have || j > pos[v] || j < low) st[v][e >> 2][e & 3] = -INFINITY;
+          }
+        }
       }
-      float ps = 0.0f;
+      bool rises = false;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = pow2(x[e] - (mref - 14.0f));
-        ps += x[e];
+      for (int v = 0; v < VT; ++v) {
+        f[v] = fmaxf(ks * qsv[v], 1.17549435e-38f);
+        const f32x4 y = st[v][0], z = st[v][1];
+        mx[v] = column_max(fmaxf(fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(z[0], z[1])), fmaxf(z[2], z[3]))) *
+                f[v];
+        rises |= mx[v] > m[v] + kSlack;
       }
-      l += ps;
-      h8 ph, pl;
-      split8(x, ph, pl);
+      if (__ballot(rises) != 0) {
+        bool far = false;
+#pragma unroll
+        for (int v = 0; v < VT; ++v) {
+          const float mn = fmaxf(m[v], mx[v]);
+          const float alpha = mn == -INFINITY ? 1.0f : pow2(m[v] - mn);
+          l[v] *= alpha;
+#pragma unroll
+          for (int k = 0; k < NB; ++k) { o[v][k][0] *= alpha; o[v][k][1] *= alpha; }
+          m[v] = mn;
+          far |= fabsf(mn) > 1048576.0f && mn != -INFINITY;
+        }
+        huge = __ballot(far) != 0;
+      }
+      if (huge) {                        // m's own rounding would come out of the fma below: products rounded as m was
+#pragma unroll
+        for (int v = 0; v < VT; ++v) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float y = st[v][e >> 2][e & 3] * f[v];
+            asm volatile("" : "+v"(y));
+            st[v][e >> 2][e & 3] = m[v] == -INFINITY ? y : y - m[v];
+          }
+          f[v] = 1.0f;
+        }
+      }
+      h8 ph[VT], pl[VT];
+#pragma unroll
+      for (int v = 0; v < VT; ++v) {
+        const float off = m[v] == -INFINITY || huge ? kTermBits : kTermBits - m[v];
+        float x[8], ps = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = pow2(__builtin_fmaf(st[v][e >> 2][e & 3], f[v], off));
+          ps += x[e];
+        }
+        l[v] += ps;
+        split8(x, minus_one, ph[v], pl[v]);
+      }
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         const h8 v0 = codes8(vf[k][0], vf[k][1]), v1 = codes8(vf[k][2], vf[k][3]);
-        f32x4 y0 = {}, y1 = {};
-        y0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, y0, 0, 0, 0);
-        y1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, y1, 0, 0, 0);
-        y0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, y0, 0, 0, 0);
-        y1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, y1, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[k][0][i] = __builtin_fmaf(y0[i], vs, o[k][0][i]);
-          o[k][1][i] = __builtin_fmaf(y1[i], vs, o[k][1][i]);
+        for (int v = 0; v < VT; ++v) {
+          f32x4 y0 = {}, y1 = {};
+          y0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[v], y0, 0, 0, 0);
+          y1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[v], y1, 0, 0, 0);
+          y0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[v], y0, 0, 0, 0);
+          y1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[v], y1, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[v][k][0][i] = __builtin_fmaf(y0[i], vs, o[v][k][0][i]);
+            o[v][k][1][i] = __builtin_fmaf(y1[i], vs, o[v][k][1][i]);
+          }
         }
       }
       load(block(c.v, next), vf);
     }
   }
-  // the four waves' (m, l, O) joined in wave order
-  l = column_sum(l);
+  // the four waves' (m, l, O) joined in wave order, group after group
+  const bool whole = tile.steps <= tile.per;                      // one split: nothing left to join
 #pragma unroll
-  for (int k = 0; k < NB; ++k)
+  for (int v = 0; v < VT; ++v) {
+    const float lv = column_sum(l[v]);
+    if (VT > 1) __syncthreads();                                   // q, or the group before, has been read
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<float4*>(&Os[w][col][32 * k + 16 * h + 4 * g]) =
-          make_float4(o[k][h][0], o[k][h][1], o[k][h][2], o[k][h][3]);
-  if (g == 0) { Ms[w][col] = m; Ls[w][col] = l; }
-  __syncthreads();
-  const int vec = tid >> 4;
-  const int oi = t.grp <= 16 ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= 16 ? vec % t.grp : g0 + vec;
-  if (oi >= tile.i1 || oh >= t.grp) return;
-  const float M = fmaxf(fmaxf(Ms[0][vec], Ms[1][vec]), fmaxf(Ms[2][vec], Ms[3][vec]));
-  float f[4], L = 0.0f;
+    for (int k = 0; k < NB; ++k)
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    // (a wave that saw nothing: m = -inf, l = 0 and O = 0, unless the vector holds NaN)
-    f[k] = Ms[k][vec] == M ? 1.0f : pow2(Ms[k][vec] - M);
-    L = __builtin_fmaf(Ls[k][vec], f[k], L);
-  }
-  const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
-  const bool whole = tile.steps <= tile.per;                      // one split: nothing to join
-  const float inv = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
-  float* out = whole ? a.ctx + at * HD : a.work + sums_at(b, a, t) + (at * t.splits + sp) * HD;
-  for (int d = 4 * (tid & 15); d < HD; d += 64) {
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float4*>(&Os[w][col][32 * k + 16 * h + 4 * g]) =
+            make_float4(o[v][k][h][0], o[v][k][h][1], o[v][k][h][2], o[v][k][h][3]);
+    if (g == 0) { Ms[w][col] = m[v]; Ls[w][col] = lv; }
+    __syncthreads();
+    const int vec = tid >> 4, oi = row_of(16 * v + vec), oh = head_of(16 * v + vec);
+    if (oi >= tile.i1 || oh >= t.grp) continue;
+    const float M = fmaxf(fmaxf(Ms[0][vec], Ms[1][vec]), fmaxf(Ms[2][vec], Ms[3][vec]));
+    float f[4], L = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float4 x = *reinterpret_cast<const float4*>(&Os[k][vec][d]);
-      y.x = __builtin_fmaf(x.x, f[k], y.x);
-      y.y = __builtin_fmaf(x.y, f[k], y.y);
-      y.z = __builtin_fmaf(x.z, f[k], y.z);
-      y.w = __builtin_fmaf(x.w, f[k], y.w);
+      // (a wave that saw nothing: m = -inf, l = 0 and O = 0, unless the vector holds NaN)
+      f[k] = Ms[k][vec] == M ? 1.0f : pow2(Ms[k][vec] - M);
+      L = __builtin_fmaf(Ls[k][vec], f[k], L);
     }
-    *reinterpret_cast<float4*>(out + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-  }
-  if (!whole && (tid & 15) == 0) {
-    float* ml = a.work + (at * t.splits + sp) * 2;
-    ml[0] = M;
-    ml[1] = L;
+    const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
+    const float inv = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
+    float* out = whole ? a.ctx + at * HD : a.work + sums_at(b, a, t) + (at * t.splits + sp) * HD;
+    for (int d = 4 * (tid & 15); d < HD; d += 64) {
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(&Os[k][vec][d]);
+        y.x = __builtin_fmaf(x.x, f[k], y.x);
+        y.y = __builtin_fmaf(x.y, f[k], y.y);
+        y.z = __builtin_fmaf(x.z, f[k], y.z);
+        y.w = __builtin_fmaf(x.w, f[k], y.w);
+      }
+      *reinterpret_cast<float4*>(out + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    }
+    if (!whole && (tid & 15) == 0) {
+      float* ml = a.work + (at * t.splits + sp) * 2;
+      ml[0] = M;
+      ml[1] = L;
+    }
   }
 }
 
-// Joins the splits of one query vector: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). A thread has a
-// split's weight; then 256 / (hd / 4) groups of threads add every so-manieth split, and their sums are added in order.
+// The tile of workgroup blockIdx.x (.y: head and group of vectors) whose splits are to be joined; false if there are none.
+__device__ __forceinline__ bool find_joint(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, AttnTile& tile) {
+  if (t.direct) {
+    const int piece = piece_steps(b, a, t);
+    if (!place_tile(b, a, t, blockIdx.x, 0, tile)) return false;
+    cut_tile(t, piece, tile);
+  } else {
+    int sp;
+    if (!find_piece(b, a, t, blockIdx.x, tile, sp)) return false;
+  }
+  return tile.steps > tile.per;
+}
+
+// Joins splits: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). Up to kJoinFew splits: one workgroup per tile
+// and head, a thread per vector and four dimensions (a workgroup per vector, as below, cost 502 tiles of 28 vectors and
+// two splits 30 us of 48).
+constexpr int kJoinFew = 32;
+
+__global__ __launch_bounds__(256) void attention_kv8_join_few_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
+  AttnTile tile;
+  if (!find_joint(b, a, t, tile)) return;
+  const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * t.vecs;
+  const int hd = c.hd, cols = hd >> 2, n = (tile.steps + tile.per - 1) / tile.per;
+  const int vecs = t.grp <= t.vecs ? (tile.i1 - tile.i0) * t.grp : min(t.vecs, t.grp - g0);
+  for (int e = threadIdx.x; e < vecs * cols; e += 256) {
+    const int vec = e / cols, col = e - vec * cols;
+    const int oi = t.grp <= t.vecs ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= t.vecs ? vec % t.grp : g0 + vec;
+    const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
+    const float2* ml = reinterpret_cast<const float2*>(a.work) + at * t.splits;
+    const float* os = a.work + sums_at(b, a, t) + at * t.splits * hd + 4 * col;
+    float M = -INFINITY;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) M = fmaxf(M, ml[s].x);
+    float L = 0.0f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float f = ml[s].x == M ? 1.0f : pow2(ml[s].x - M);
+      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * hd);
+      L = __builtin_fmaf(ml[s].y, f, L);
+      y.x = __builtin_fmaf(x.x, f, y.x);
+      y.y = __builtin_fmaf(x.y, f, y.y);
+      y.z = __builtin_fmaf(x.z, f, y.z);
+      y.w = __builtin_fmaf(x.w, f, y.w);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    *reinterpret_cast<float4*>(a.ctx + at * hd + 4 * col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+  }
+}
+
+// More splits (few tiles then): a workgroup per vector, a thread per split for its weight; then 256 / (hd / 4) groups of
+// threads add every so-manieth split, and their sums are added in order.
 __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
   __shared__ float f[kAttnMaxSplits8], red[2][4];
   __shared__ float4 part[256];
   AttnTile tile;
-  if (t.direct) {
-    const int piece = piece_steps(b, a, t);
-    if (!place_tile(b, a, t, blockIdx.x, 0, tile)) return;
-    cut_tile(t, piece, tile);
-  } else {
-    int sp;
-    if (!find_piece(b, a, t, blockIdx.x, tile, sp)) return;
-  }
-  if (tile.steps <= tile.per) return;
+  if (!find_joint(b, a, t, tile)) return;
   const int tid = threadIdx.x, w = tid >> 6, vec = blockIdx.z, hd = c.hd;
-  const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * 16;
-  const int oi = t.grp <= 16 ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= 16 ? vec % t.grp : g0 + vec;
+  const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * t.vecs;
+  const int oi = t.grp <= t.vecs ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= t.vecs ? vec % t.grp : g0 + vec;
   if (oi >= tile.i1 || oh >= t.grp) return;
   const int n = (tile.steps + tile.per - 1) / tile.per;
   const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
@@ -615,13 +747,28 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
   *reinterpret_cast<float4*>(a.ctx + at * hd + 4 * tid) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
-static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads) {
+// the most groups of 16 vectors of a tile: their sums, 64 and 128 registers, leave a SIMD two waves
+constexpr int most_groups(int hd) { return hd <= 128 ? 4 : 2; }
+
+static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
   AttnTiles t;
   t.grp = heads / kv_heads;
-  t.rows_per = t.grp <= 16 ? std::min(16 / t.grp, max_rows) : 1;
-  t.group_tiles = t.grp <= 16 ? 1 : (t.grp + 15) / 16;
-  t.direct = max_rows <= t.rows_per;
-  t.units = t.direct ? requests : rows / t.rows_per + requests;
+  const long vecs = (long)max_rows * t.grp;
+  // Wide tiles convert a code once for all their vectors, but there are fewer of them and each starts and ends later. They
+  // pay where more than half of a tile is filled and
+  //   - tiles stay at four for each CU (us of 16 / 32 / 64 vectors: 2000 rows of 32 heads in 4 of 128 116 / 89 / 92, behind
+  //     20000 tokens 1632 / 1307 / 1191; but 1000 rows of 14 in 2 of 64, 502 tiles of 32, 15.8 / 24.9 / 29.2), or
+  //   - one tile holds all of a request, cut into pieces, and there is work for many of them (4 rows of 8 heads: 64
+  //     requests of up to 4000 tokens 47.8 / 32.3 / 41.4, 8 requests of up to 3000 19.2 / 24.5 / 29.6 for 3 rows).
+  for (int groups = most_groups(hd); groups > 0; groups >>= 1) {
+    t.vecs = 16 * groups;
+    t.rows_per = t.grp <= t.vecs ? std::min(t.vecs / t.grp, max_rows) : 1;
+    t.group_tiles = (t.grp + t.vecs - 1) / t.vecs;
+    t.direct = max_rows <= t.rows_per;
+    t.units = t.direct ? requests : rows / t.rows_per + requests;
+    const long tiles = (long)t.units * kv_heads * t.group_tiles;
+    if (2 * vecs > t.vecs && (t.direct ? (long)requests * kv_heads * (max_len / 32) >= 16384 : tiles >= 1024)) break;
+  }
   const long ht = (long)kv_heads * t.group_tiles;
   const int most = (std::max(max_len, 1) + 32 * kAttnMinSteps - 1) / (32 * kAttnMinSteps);
   // two workgroups of a piece for each CU (us of 512 / 1024 / 2048 / 8192 workgroups: one request of 131071 tokens, 8
@@ -633,31 +780,41 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
 }
 
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
-  const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads);
+  const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd);
   return t.splits > 1 ? split_pairs(rows, heads, t.splits) + (size_t)rows * heads * t.splits * hd : 0;
 }
 
+template <int NB>
+static void launch_attention_hd(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, const AttnTiles& t,
+                                unsigned workgroups, hipStream_t s) {
+  auto* k = t.vecs == 16 ? attention_kv8_kernel<NB, 1> : t.vecs == 32 ? attention_kv8_kernel<NB, 2>
+                                                                      : attention_kv8_kernel<NB, most_groups(32 * NB)>;
+  hipLaunchKernelGGL(k, dim3(workgroups), dim3(256), 0, s, b, c, a, t);
+}
+
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s) {
-  const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.heads, c.kv_heads);
-  const dim3 grid((unsigned)t.units, (unsigned)(c.kv_heads * t.group_tiles), (unsigned)t.splits);
-  void (*k)(PagedBatch, Kv8Cache, Attn8Args, AttnTiles) = nullptr;
+  const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.heads, c.kv_heads, c.hd);
+  const unsigned heads = (unsigned)(c.kv_heads * t.group_tiles);
+  const unsigned n = heads * (t.direct ? (unsigned)(t.pieces + b.requests) : (unsigned)t.units * (unsigned)t.splits);
   switch (c.hd / 32) {
-    case 1: k = attention_kv8_kernel<1>; break;
-    case 2: k = attention_kv8_kernel<2>; break;
-    case 3: k = attention_kv8_kernel<3>; break;
-    case 4: k = attention_kv8_kernel<4>; break;
-    case 5: k = attention_kv8_kernel<5>; break;
-    case 6: k = attention_kv8_kernel<6>; break;
-    case 7: k = attention_kv8_kernel<7>; break;
-    default: k = attention_kv8_kernel<8>; break;
+    case 1: launch_attention_hd<1>(b, c, a, t, n, s); break;
+    case 2: launch_attention_hd<2>(b, c, a, t, n, s); break;
+    case 3: launch_attention_hd<3>(b, c, a, t, n, s); break;
+    case 4: launch_attention_hd<4>(b, c, a, t, n, s); break;
+    case 5: launch_attention_hd<5>(b, c, a, t, n, s); break;
+    case 6: launch_attention_hd<6>(b, c, a, t, n, s); break;
+    case 7: launch_attention_hd<7>(b, c, a, t, n, s); break;
+    default: launch_attention_hd<8>(b, c, a, t, n, s); break;
   }
-  const unsigned per_head = t.direct ? (unsigned)(t.pieces + b.requests) : grid.x * grid.z;
-  hipLaunchKernelGGL(k, dim3(per_head * grid.y), dim3(256), 0, s, b, c, a, t);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || t.splits == 1) return e;
-  const int vecs = t.grp <= 16 ? t.rows_per * t.grp : 16;
-  hipLaunchKernelGGL(attention_kv8_join_kernel, dim3(grid.x, grid.y, (unsigned)vecs), dim3(256), 0, s, b, c,
-                     a, t);
+  if (t.splits <= kJoinFew) {
+    hipLaunchKernelGGL(attention_kv8_join_few_kernel, dim3((unsigned)t.units, heads), dim3(256), 0, s, b, c, a, t);
+    return hipGetLastError();
+  }
+  const int vecs = t.grp <= t.vecs ? t.rows_per * t.grp : t.vecs;
+  hipLaunchKernelGGL(attention_kv8_join_kernel, dim3((unsigned)t.units, heads, (unsigned)vecs), dim3(256), 0, s, b, c, a,
+                     t);
   return hipGetLastError();
 }
 
