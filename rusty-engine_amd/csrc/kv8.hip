@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "serve.hpp"
+#include "wave.hpp"
 
 namespace rehip {
 
@@ -18,147 +19,176 @@ namespace rehip {
 // float: such values are stored as 0), a value's code round(x / s), ties to even. Rows that raise the scale of a
 // page with earlier rows in it round those rows' codes to the new one: round(c * (s_old / s_new)). Infinities
 // are stored as +-127 and NaN as 0, so that one bad value does not reach the page's other tokens.
-__device__ __forceinline__ int code_of(float x, float s) {
-  const float r = rintf(x / s);
-  return x != x || s == 0.0f ? 0 : (int)fminf(fmaxf(r, -127.0f), 127.0f);
+//
+// The quotient is the correctly rounded one: with y = 1 / s rounded, q = x y, then twice q += (x - q s) y in fused
+// multiply-adds, whose remainders are exact (the first leaves q within one unit of the last place, the second rounds it
+// right: Markstein). Below 2^-100 remainders could underflow: there the division itself is used. Of finite values
+// |q| <= 127 (1 + 2^-23), and q + 1.5 2^23 rounds it to an integer, whose low byte is the code.
+constexpr float kCodeMagic = 12582912.0f;
+
+__device__ __forceinline__ unsigned code_of(float x, float s, float y) {
+  float q = x * y;
+  q = __builtin_fmaf(__builtin_fmaf(-q, s, x), y, q);
+  q = __builtin_fmaf(__builtin_fmaf(-q, s, x), y, q);
+  return __float_as_uint(q + kCodeMagic);
+}
+__device__ unsigned code_of_any(float x, float s) {
+  const float q = rintf(x / s);
+  return x != x || s == 0.0f ? 0u : (unsigned)(int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+// the low bytes of four
+__device__ __forceinline__ unsigned bytes4(unsigned a, unsigned b, unsigned c, unsigned d) {
+  const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
-// One workgroup per (run of one request's new rows inside one page, head, K or V). A thread has U units of 16 codes that
-// lie together in memory (K: 2 tokens x 8 dimensions, V: 8 tokens x 2): it loads their values, and their codes where
-// some token of the unit is not new, all before the largest magnitude is known, so that the chain is one round trip to
-// memory for the request, one for its page and one for all of this. U = 0: the units in turn, their values read twice.
-template <int U>
-__global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache c, const float* __restrict__ k,
-                                                         size_t ldk, const float* __restrict__ v, size_t ldv) {
-  __shared__ unsigned red[4];
-  const int u = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
-  const bool is_v = blockIdx.z != 0;
-  const int r = request_of_unit<256>(u, b.start, b.requests, b.rows, b.page, 2);
-  if (r < 0) return;
-  const int row0 = min(max(b.start[r], 0), b.rows);
-  const int n = min(max(b.count[r], 0), b.rows - row0);
-  const int len = b.len[r], first = len - n;
-  if (n == 0 || first < 0 || len > b.table_ld * b.page) return;
-  const int pi = first / b.page + (u - (row0 / b.page + 2 * r));
-  const int lo = max(pi * b.page, first), hi = min((pi + 1) * b.page, len);   // positions
-  if (lo >= hi) return;
-  const int pid = b.table[(size_t)r * b.table_ld + pi];
-  if (pid < 0 || pid >= b.n_pages) return;
-  const int o0 = lo - pi * b.page, o1 = hi - pi * b.page, hd = c.hd, nb = hd >> 5;
-  const size_t ld = is_v ? ldv : ldk;
-  // (the row of token o0; token t's is (t - o0) rows on)
-  const float* x = (is_v ? v : k) + (size_t)(row0 + lo - first) * ld + (size_t)head * hd;
-  int8_t* codes = (is_v ? c.v : c.k) + ((size_t)pid * c.kv_heads + head) * b.page * hd;
-  float* scale = (is_v ? c.vs : c.ks) + (size_t)pid * c.kv_heads + head;
-  const int units = b.page * hd / 16, m = tid & 15, g = (tid >> 4) & 3;
-  // unit q: blocks follow each other 64 units apart, so a thread's place in its blocks is one
-  auto first_token = [&](int q) { return 32 * ((q >> 6) / nb) + (is_v ? 4 * g : m); };
-  auto first_dim = [&](int q) { return 32 * ((q >> 6) % nb) + (is_v ? m : 8 * g); };
-  auto token_of = [&](int t, int e) { return t + (is_v ? 16 * ((e >> 2) & 1) + (e & 3) : 16 * (e >> 3)); };
-  auto load = [&](int q, float (&y)[16]) {
-    const int t = first_token(q), d = first_dim(q);
-    if (is_v) {
+// One page's new tokens o0 .. o1 - 1 of one head: x is token o0's row, codes and scale the page's. A thread has U units of
+// 16 codes that lie together in memory (K: 2 tokens x 8 dimensions, V: 8 tokens x 2), 64 lanes' units a block of 32 x 32:
+// it loads their values, and the codes of a page that is not all new, before the largest magnitude is known, so that all
+// of this is one round trip to memory. Units past the page's (U rounded up) repeat the last and are not stored.
+// U = 0: the units in turn, their values read twice.
+template <bool IS_V, int U>
+__device__ __forceinline__ void append_page(const float* __restrict__ x, int ld, int o0, int o1, int page, int hd,
+                                            int8_t* codes, float* scale, float (*red)[4]) {
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
+  const int nb = hd >> 5, blocks = (page >> 5) * nb;
+  const bool all_new = o0 == 0 && o1 == page;
+  auto first_token = [&](int blk) { return 32 * (blk / nb) + (IS_V ? 4 * g : m); };
+  auto token_of = [&](int t, int e) { return t + (IS_V ? 16 * ((e >> 2) & 1) + (e & 3) : 16 * (e >> 3)); };
+  auto load = [&](int blk, float (&y)[16]) {
+    const int t = first_token(blk), d = 32 * (blk % nb) + (IS_V ? m : 8 * g);
+    // (of a token that is not new, some new one's values: a load under a condition of its lane waits for the one before)
+    auto row = [&](int e) { return x + ((min(max(token_of(t, e), o0), o1 - 1) - o0) * ld + d); };
+    if constexpr (IS_V) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int tok = token_of(t, e);
-        y[e] = tok >= o0 && tok < o1 ? x[(size_t)(tok - o0) * ld + d + 16 * (e >> 3)] : 0.0f;
+      for (int e = 0; e < 8; ++e) {
+        const float* r = row(e);
+        y[e] = r[0];
+        y[e + 8] = r[16];
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int tok = token_of(t, e);
-        *reinterpret_cast<float4*>(&y[e]) = tok >= o0 && tok < o1
-                                                ? *reinterpret_cast<const float4*>(x + (size_t)(tok - o0) * ld + d + (e & 4))
-                                                : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int e = 0; e < 16; e += 8) {
+        const float* r = row(e);
+        *reinterpret_cast<float4*>(&y[e]) = *reinterpret_cast<const float4*>(r);
+        *reinterpret_cast<float4*>(&y[e + 4]) = *reinterpret_cast<const float4*>(r + 4);
       }
     }
   };
-  // tokens of a unit: the first, the last, and whether any is new / old / other than new
-  auto news = [&](int t) {
-    return is_v ? (t < o1 && t + 3 >= o0) || (t + 16 < o1 && t + 19 >= o0) : (t < o1 && t >= o0) || (t + 16 < o1 && t + 16 >= o0);
-  };
-  auto whole = [&](int t) { return t >= o0 && t + (is_v ? 20 : 17) <= o1; };
-  auto largest = [&](const float (&y)[16], unsigned top) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const unsigned bits = __float_as_uint(y[e]) & 0x7fffffffu;
-      top = max(top, bits < 0x7f800000u ? bits : 0u);
-    }
-    return top;
-  };
+  uint4* const units = reinterpret_cast<uint4*>(codes) + lane;    // unit of block blk: units[64 * blk]
   float y[U > 0 ? U : 1][16];
   uint4 old[U > 0 ? U : 1];
-  const float s_old = o0 > 0 ? *scale : 0.0f;
-  unsigned top = 0;
+  float s_old = *scale;
+  float top = 0.0f, odd = 0.0f;            // odd: NaN once an infinity or a NaN was seen
+  auto largest = [&](const float (&z)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      top = fmaxf(top, fabsf(z[e]));
+      odd = __builtin_fmaf(z[e], 0.0f, odd);
+    }
+  };
   if constexpr (U > 0) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int q = tid + 256 * i, t = first_token(q);
-      if (q < units) {
-        load(q, y[i]);
-        if (!whole(t) && (o0 > 0 || news(t))) old[i] = reinterpret_cast<const uint4*>(codes)[q];
-      }
+    for (int i = 0; i < U; ++i) load(min(w + 4 * i, blocks - 1), y[i]);
+    if (!all_new) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) old[i] = units[64 * min(w + 4 * i, blocks - 1)];
     }
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (tid + 256 * i < units) top = largest(y[i], top);
+    for (int i = 0; i < U; ++i) largest(y[i]);
   } else {
-    for (int q = tid; q < units; q += 256) {
-      load(q, y[0]);
-      top = largest(y[0], top);
+    for (int blk = w; blk < blocks; blk += 4) {
+      load(blk, y[0]);
+      largest(y[0]);
     }
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, off, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = top;
+  top = wave_max(top);
+  odd = wave_sum(odd);
+  if (lane == 0) { red[0][w] = top; red[1][w] = odd; }
   __syncthreads();
-  top = max(max(red[0], red[1]), max(red[2], red[3]));
-  float s = __uint_as_float(top) * (1.0f / 127.0f);
-  if (s < 1.17549435e-38f) s = 0.0f;
-  s = fmaxf(s, s_old);
-  const bool grown = s > s_old && o0 > 0;
-  const float ratio = grown ? s_old / s : 1.0f;
-  auto store = [&](int q, const float (&z)[16], const uint4& was) {
-    const int t = first_token(q);
-    if (!news(t) && !(grown && t < o0)) return;
-    const unsigned w[4] = {was.x, was.y, was.z, was.w};
-    unsigned out[4];
-    const bool all = whole(t);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      out[i] = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = 4 * i + j, tok = token_of(t, e);
-        int code = code_of(z[e], s);
-        if (!all) {
-          const int held = (int)(int8_t)(w[i] >> (8 * j));
-          if (tok < o0) code = grown ? (int)rintf((float)held * ratio) : held;
-          else if (tok >= o1) code = held;
-        }
-        out[i] |= (unsigned)(code & 0xff) << (8 * j);
-      }
+  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  odd = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  if (odd != odd) {                        // the finite ones only
+    top = 0.0f;
+    for (int e = tid; e < (o1 - o0) * hd; e += 256) {
+      const float v = fabsf(x[e / hd * ld + e % hd]);
+      if (v < INFINITY) top = fmaxf(top, v);
     }
-    reinterpret_cast<uint4*>(codes)[q] = make_uint4(out[0], out[1], out[2], out[3]);
+    top = wave_max(top);
+    __syncthreads();
+    if (lane == 0) red[0][w] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  }
+  if (o0 == 0) s_old = 0.0f;               // the page is begun: what it held before does not count
+  float s = top * (1.0f / 127.0f);
+  if (s < 1.17549435e-38f) s = 0.0f;
+  s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(s, s_old))));
+  const bool grown = o0 > 0 && s > s_old, plain = s >= 7.8886091e-31f && odd == odd;
+  const float ratio = grown ? s_old / s : 1.0f, inverse = 1.0f / s;
+  auto store = [&](int blk, const float (&z)[16], const uint4& was) {
+    unsigned c[16], out[4];
+    if (plain) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) c[e] = code_of(z[e], s, inverse);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) c[e] = code_of_any(z[e], s);
+    }
+    if (!all_new) {
+      const int t = first_token(blk);
+      bool changes = false;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int tok = token_of(t, e), held = (int)(int8_t)((&was.x)[e >> 2] >> (8 * (e & 3)));
+        if (tok < o0) c[e] = grown ? (unsigned)(int)rintf((float)held * ratio) : (unsigned)held;
+        if (tok >= o1) c[e] = (unsigned)held;
+        changes |= tok < o1 && (tok >= o0 || grown);
+      }
+      if (!changes) return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = bytes4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]);
+    units[64 * blk] = make_uint4(out[0], out[1], out[2], out[3]);
   };
   if constexpr (U > 0) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (tid + 256 * i < units) store(tid + 256 * i, y[i], old[i]);
+      if (w + 4 * i < blocks) store(w + 4 * i, y[i], old[i]);
   } else {
-    for (int q = tid; q < units; q += 256) {
-      const int t = first_token(q);
-      if (!news(t) && !(grown && t < o0)) continue;
-      load(q, y[0]);
-      if (!whole(t)) old[0] = reinterpret_cast<const uint4*>(codes)[q];
-      store(q, y[0], old[0]);
+    for (int blk = w; blk < blocks; blk += 4) {
+      load(blk, y[0]);
+      if (!all_new) old[0] = units[64 * blk];
+      store(blk, y[0], old[0]);
     }
   }
   if (tid == 0) *scale = s;
 }
 
-hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, size_t ldk, const float* v,
-                             size_t ldv, hipStream_t s) {
+// One workgroup per (run of one request's new rows inside one page, head, K or V).
+template <int U>
+__global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache c, const float* __restrict__ k, int ldk,
+                                                         const float* __restrict__ v, int ldv) {
+  __shared__ float red[2][4];
+  const int u = blockIdx.x, head = blockIdx.y;
+  const RequestRows q = request_of_unit(u, b, b.page, 2);
+  const int n = q.count, len = q.len, first = len - n;
+  if (n == 0 || first < 0 || len > b.table_ld * b.page) return;
+  const int pi = first / b.page + (u - (q.row0 / b.page + 2 * q.req));
+  const int lo = max(pi * b.page, first), hi = min((pi + 1) * b.page, len);   // positions
+  if (lo >= hi) return;
+  const int pid = b.table[(size_t)q.req * b.table_ld + pi];
+  if (pid < 0 || pid >= b.n_pages) return;
+  const int o0 = lo - pi * b.page, o1 = hi - pi * b.page;
+  const size_t row = q.row0 + lo - first, at = (size_t)pid * c.kv_heads + head, codes = at * b.page * c.hd;
+  if (blockIdx.z == 0)
+    append_page<false, U>(k + row * ldk + head * c.hd, ldk, o0, o1, b.page, c.hd, c.k + codes, c.ks + at, red);
+  else
+    append_page<true, U>(v + row * ldv + head * c.hd, ldv, o0, o1, b.page, c.hd, c.v + codes, c.vs + at, red);
+}
+
+hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,
+                             hipStream_t s) {
   const dim3 grid((unsigned)(b.rows / b.page + 2 * b.requests), (unsigned)c.kv_heads, 2);
   const int units = b.page * c.hd / 16;
   auto* f = units <= 256 ? kv8_append_kernel<1> : units <= 512 ? kv8_append_kernel<2> : units <= 1024 ? kv8_append_kernel<4>
@@ -218,15 +248,6 @@ __device__ __forceinline__ void split8(const float (&x)[8], float minus_one, h8&
 // 2^x for x <= 16: what is below the smallest normal float may come out as 0
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// v of lane l ^ 16 / l ^ 32, without LDS: the swaps exchange halves, and a lane keeps the one that was its partner's
-__device__ __forceinline__ float swap16(float v) {
-  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float((threadIdx.x & 16) ? s[0] : s[1]);
-}
-__device__ __forceinline__ float swap32(float v) {
-  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float((threadIdx.x & 32) ? s[0] : s[1]);
-}
 // the largest over the four lanes that share a column of the 16 x 16 layouts (one of the swapped values is the lane's
 // own, so both may be taken), and the sum
 __device__ __forceinline__ float column_max(float v) {
@@ -236,8 +257,8 @@ __device__ __forceinline__ float column_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float column_sum(float v) {
-  v += swap16(v);
-  return v + swap32(v);
+  v += lane_xor<16>(v);
+  return v + lane_xor<32>(v);
 }
 
 // How a launch cuts the batch: a tile holds up to vecs query vectors of one request and KV head, rows_per rows of its
@@ -260,15 +281,13 @@ struct AttnTile {
 constexpr int kAttnMaxSplits8 = 256;  // one thread of the join each
 constexpr int kAttnMinSteps = 16;     // steps of a split, at least (four waves take turns)
 
-// rows i0 .. of request r; false if it has none
-__device__ __forceinline__ bool place_tile(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int r, int i0,
-                                           AttnTile& o) {
-  o.req = r;
-  o.row0 = min(max(b.start[r], 0), b.rows);
-  const int count = min(max(b.count[r], 0), b.rows - o.row0);
-  const int len = min(max(b.len[r], 0), b.table_ld * b.page);
-  o.n = min(count, a.max_rows);
-  o.p0 = len - count;
+// rows i0 .. of a request; false if it has none
+__device__ __forceinline__ bool place_tile(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t,
+                                           const RequestRows& q, int i0, AttnTile& o) {
+  o.req = q.req;
+  o.row0 = q.row0;
+  o.n = min(q.count, a.max_rows);
+  o.p0 = min(max(q.len, 0), b.table_ld * b.page) - q.count;
   o.i0 = i0;
   o.i1 = min(i0 + t.rows_per, o.n);
   const int last = o.p0 + o.i1 - 1;
@@ -276,6 +295,10 @@ __device__ __forceinline__ bool place_tile(const PagedBatch& b, const Attn8Args&
   o.first = lo >> 5;
   o.steps = last < 0 ? 0 : (last >> 5) - o.first + 1;
   return i0 >= 0 && i0 < o.n;
+}
+__device__ __forceinline__ bool place_request(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int r,
+                                              AttnTile& o) {
+  return place_tile(b, a, t, request_rows(r, b.start[r], b.count[r], b.len[r], b.rows), 0, o);
 }
 __device__ __forceinline__ int steps_per(int steps, int pieces) {
   return max(kAttnMinSteps, ((steps + pieces - 1) / pieces + 3) & ~3);
@@ -299,56 +322,63 @@ __device__ __forceinline__ int scan256(int v, int& before) {
   return p0 + p1 + p2 + p3;
 }
 
-// direct: steps of a piece over the whole batch
-__device__ __forceinline__ int piece_steps(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t) {
-  AttnTile o;
-  int sum = 0, before;
-  const int most = (1 << 30) / b.requests;      // (the sum stays an int)
-  for (int r = threadIdx.x; r < b.requests; r += 256) sum += place_tile(b, a, t, r, 0, o) ? min(o.steps, most) : 0;
-  return steps_per(scan256(sum, before), t.pieces);
-}
-__device__ __forceinline__ void cut_tile(const AttnTiles& t, int piece, AttnTile& o) {
-  o.per = max(piece, steps_per(o.steps, t.splits));
-}
-
 // The tile and split of workgroup `u` of a head; false if there is none.
 __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int u,
                                            AttnTile& o, int& sp) {
   if (!t.direct) {
     sp = u / t.units;
     u = t.units - 1 - (u + sp) % t.units;             // (a prompt's last rows see the most keys: first)
-    const int r = request_of_unit<256>(u, b.start, b.requests, b.rows, t.rows_per, 1);
-    if (r < 0) return false;
-    if (!place_tile(b, a, t, r, (u - (min(max(b.start[r], 0), b.rows) / t.rows_per + r)) * t.rows_per, o)) return false;
+    const RequestRows q = request_of_unit(u, b, t.rows_per, 1);
+    if (q.req < 0 || !place_tile(b, a, t, q, (u - (q.row0 / t.rows_per + q.req)) * t.rows_per, o)) return false;
     o.per = steps_per(o.steps, t.splits);
     return sp == 0 || sp * o.per < o.steps;
   }
-  __shared__ int found[2];
-  const int piece = piece_steps(b, a, t), chunk = (b.requests + 255) / 256;
-  auto pieces_of = [&](int r) {
-    if (!place_tile(b, a, t, r, 0, o)) return 0;
-    cut_tile(t, piece, o);
-    return max(1, (o.steps + o.per - 1) / o.per);
+  // steps of a piece over the whole batch, then the request that piece u falls into; each thread has some of the
+  // requests, and the one that finds the piece hands its tile on
+  __shared__ AttnTile found;
+  __shared__ int found_sp;
+  const int chunk = (b.requests + 255) / 256, r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
+  const int most = (1 << 30) / b.requests;            // (the sum stays an int)
+  int sum = 0, before;
+  bool has = false;
+  for (int r = r0; r < r1; ++r) {
+    has = place_request(b, a, t, r, o);
+    sum += has ? min(o.steps, most) : 0;
+  }
+  const int piece = steps_per(scan256(sum, before), t.pieces);
+  auto pieces_of = [&] {
+    o.per = max(piece, steps_per(o.steps, t.splits));
+    return has ? max(1, (o.steps + o.per - 1) / o.per) : 0;
   };
-  const int r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
-  int mine = 0, before;
-  for (int r = r0; r < r1; ++r) mine += pieces_of(r);
+  int mine = 0;
+  if (chunk == 1) mine = pieces_of();
+  else
+    for (int r = r0; r < r1; ++r) {
+      has = place_request(b, a, t, r, o);
+      mine += pieces_of();
+    }
   const int all = scan256(mine, before);
   if (u >= all) return false;
   if (u >= before && u < before + mine) {
-    int r = r0, k = u - before;
-    for (int n; k >= (n = pieces_of(r)); ++r) k -= n;
-    found[0] = r;
-    found[1] = k;
+    int k = u - before;
+    if (chunk > 1)
+      for (int r = r0;; ++r) {
+        has = place_request(b, a, t, r, o);
+        const int n = pieces_of();
+        if (k < n) break;
+        k -= n;
+      }
+    found = o;
+    found_sp = k;
   }
   __syncthreads();
-  sp = found[1];
-  place_tile(b, a, t, found[0], 0, o);
-  cut_tile(t, piece, o);
+  o = found;
+  sp = found_sp;
   return true;
 }
 
-// The workspace holds (m, l) of every row, head and split, then their sums from this float on (16-byte aligned).
+// The workspace holds (m, l) of every row, head and split, then from this float on (16-byte aligned) their sums, then
+// every unit's number of splits.
 __host__ __device__ inline size_t split_pairs(size_t rows, size_t heads, size_t splits) {
   return (rows * heads * splits * 2 + 3) & ~(size_t)3;
 }
@@ -362,7 +392,11 @@ __device__ __forceinline__ AttnTile uniform(const AttnTile& o) {
   return {u(o.req), u(o.row0), u(o.n), u(o.i0), u(o.i1), u(o.p0), u(o.first), u(o.steps), u(o.per)};
 }
 
-constexpr int kAttnPages = 512;       // pages whose numbers and scales are staged at a time
+__device__ __forceinline__ int* splits_at(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int hd) {
+  return reinterpret_cast<int*>(a.work + sums_at(b, a, t) + (size_t)b.rows * a.heads * t.splits * hd);
+}
+
+constexpr int kAttnPages = 256;       // pages whose numbers and scales are staged at a time: one per thread
 
 // One workgroup of four waves per (tile, KV head, split of the keys). A wave takes every fourth step of 32 keys, for
 // VT groups of 16 query vectors:
@@ -402,6 +436,35 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
 #pragma unroll
   for (int v = 0; v < VT; ++v)
     pos[v] = row_of(16 * v + col) < tile.i1 && head_of(16 * v + col) < t.grp ? tile.p0 + row_of(16 * v + col) : -1;
+  const size_t head_bytes = (size_t)b.page * HD;
+  const int page_steps = b.page >> 5, page0 = s0 / page_steps, page_last = max(s1 - 1, 0) / page_steps;
+  const unsigned page_inv = 65536u / page_steps + 1;
+  auto entry = [&](int pg) {
+    const int pid = b.table[(size_t)tile.req * b.table_ld + pg];
+    return pid >= 0 && pid < b.n_pages ? pid : -1;
+  };
+  auto block = [&](const int8_t* base, int pid, int in_page) {     // (an absent page: any one, its scores are hidden)
+    return base + ((size_t)__builtin_amdgcn_readfirstlane(max(pid, 0)) * c.kv_heads + head) * head_bytes +
+           (size_t)in_page * (NB * 1024);
+  };
+  // (a decode step reads every code once; prompts' tiles read them again, from L2)
+  auto load = [&](const int8_t* p, u32x4 (&x)[NB]) {
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const u32x4* at = reinterpret_cast<const u32x4*>(p + 1024 * k + 16 * lane);
+      x[k] = VT > 1 ? *at : __builtin_nontemporal_load(at);
+    }
+  };
+  // the wave's first block straight from the table, and the pages this thread stages: on their way while q is split
+  u32x4 kf[NB], vf[NB];
+  const int first = max(min(s0 + w, s1 - 1), 0);
+  int my_page = entry(min(page0 + tid, page_last));
+  {
+    const int pid = entry(first / page_steps), in_page = first - first / page_steps * page_steps;
+    load(block(c.k, pid, in_page), kf);
+    load(block(c.v, pid, in_page), vf);
+  }
+  float my_ks = c.ks[(size_t)max(my_page, 0) * c.kv_heads + head], my_vs = c.vs[(size_t)max(my_page, 0) * c.kv_heads + head];
   float minus_one = -1.0f;
   asm volatile("" : "+v"(minus_one));
   h8 qh[NB], ql[NB];
@@ -451,43 +514,29 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     for (int k = 0; k < NB; ++k) o[v][k][0] = o[v][k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   bool huge = false;                     // some vector's m is beyond 2^20
-  const size_t head_bytes = (size_t)b.page * HD;
-  const int page_steps = b.page >> 5;
-  const unsigned page_inv = 65536u / page_steps + 1;
-  for (int pg0 = s0 / page_steps; pg0 * page_steps < s1; pg0 += kAttnPages) {
+  for (int pg0 = page0; pg0 * page_steps < s1; pg0 += kAttnPages) {
     // the pages of these steps: their numbers and scales
-    const int npg = min(kAttnPages, (s1 - 1) / page_steps - pg0 + 1);
-    if (pg0 != s0 / page_steps) __syncthreads();
-    for (int i = tid; i < npg; i += 256) {
-      int pid = b.table[(size_t)tile.req * b.table_ld + pg0 + i];
-      const bool have = pid >= 0 && pid < b.n_pages;
-      const size_t at = (size_t)(have ? pid : 0) * c.kv_heads + head;
-      ids[i] = have ? pid : -1;
-      kss[i] = have ? c.ks[at] : 0.0f;
-      vss[i] = have ? c.vs[at] : 0.0f;
+    if (pg0 != page0) {
+      my_page = entry(min(pg0 + tid, page_last));
+      my_ks = c.ks[(size_t)max(my_page, 0) * c.kv_heads + head];
+      my_vs = c.vs[(size_t)max(my_page, 0) * c.kv_heads + head];
+      __syncthreads();                   // the pages before have been read
     }
+    ids[tid] = my_page;
+    kss[tid] = my_page >= 0 ? my_ks : 0.0f;
+    vss[tid] = my_page >= 0 ? my_vs : 0.0f;
     __syncthreads();
     // steps from here on count from page pg0's first (below kAttnPages * 8): the quotient by page_steps is exact
-    const int c0 = pg0 * page_steps, e0 = max(s0 - c0, 0), e1 = min(s1 - c0, npg * page_steps);
+    const int c0 = pg0 * page_steps, e0 = max(s0 - c0, 0), e1 = min(s1 - c0, kAttnPages * page_steps);
     auto page_of = [&](int s) { return (int)((unsigned)s * page_inv >> 16); };
-    u32x4 kf[NB], vf[NB];
-    auto block = [&](const int8_t* base, int s) {
+    auto next_block = [&](const int8_t* base, int s) {
       const int pi = page_of(s);
-      const int pid = __builtin_amdgcn_readfirstlane(max(ids[pi], 0));
-      return base + ((size_t)pid * c.kv_heads + head) * head_bytes + (size_t)(s - pi * page_steps) * (NB * 1024);
-    };
-    // (a decode step reads every code once; prompts' tiles read them again, from L2)
-    auto load = [&](const int8_t* p, u32x4 (&x)[NB]) {
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        const u32x4* at = reinterpret_cast<const u32x4*>(p + 1024 * k + 16 * lane);
-        x[k] = VT > 1 ? *at : __builtin_nontemporal_load(at);
-      }
+      return block(base, ids[pi], s - pi * page_steps);
     };
     int s = e0 + w;
-    if (s < e1) {
-      load(block(c.k, s), kf);
-      load(block(c.v, s), vf);
+    if (pg0 != page0 && s < e1) {
+      load(next_block(c.k, s), kf);
+      load(next_block(c.v, s), vf);
     }
     for (; s < e1; s += 4) {
       const int next = min(s + 4, e1 - 1);
@@ -510,7 +559,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
           st[v][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, lo, st[v][1], 0, 0, 0);
         }
       }
-      load(block(c.k, next), kf);
+      load(next_block(c.k, next), kf);
       // f > 0, so the largest product is the largest score (0 would make NaN of the hidden ones' -inf)
       float f[VT], mx[VT];
       const bool hides = !have || key0 + 31 > see_all || key0 < see_from;      // some vector does not see some key
@@ -590,11 +639,14 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
           }
         }
       }
-      load(block(c.v, next), vf);
+      load(next_block(c.v, next), vf);
     }
   }
   // the four waves' (m, l, O) joined in wave order, group after group
   const bool whole = tile.steps <= tile.per;                      // one split: nothing left to join
+  if (t.splits > 1 && sp == 0 && yy == 0 && tid == 0)
+    splits_at(b, a, t, HD)[t.direct ? tile.req : tile.row0 / t.rows_per + tile.req + tile.i0 / t.rows_per] =
+        (tile.steps + tile.per - 1) / tile.per;
 #pragma unroll
   for (int v = 0; v < VT; ++v) {
     const float lv = column_sum(l[v]);
@@ -640,17 +692,14 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   }
 }
 
-// The tile of workgroup blockIdx.x (.y: head and group of vectors) whose splits are to be joined; false if there are none.
-__device__ __forceinline__ bool find_joint(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, AttnTile& tile) {
-  if (t.direct) {
-    const int piece = piece_steps(b, a, t);
-    if (!place_tile(b, a, t, blockIdx.x, 0, tile)) return false;
-    cut_tile(t, piece, tile);
-  } else {
-    int sp;
-    if (!find_piece(b, a, t, blockIdx.x, tile, sp)) return false;
-  }
-  return tile.steps > tile.per;
+// The tile of workgroup blockIdx.x (.y: head and group of vectors) and its number of splits; false if there are none to
+// join.
+__device__ __forceinline__ bool find_joint(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int hd,
+                                           AttnTile& tile, int& n) {
+  n = splits_at(b, a, t, hd)[blockIdx.x];                         // (no tile: not written, and not used)
+  if (t.direct) return place_request(b, a, t, blockIdx.x, tile) && n > 1;
+  const RequestRows q = request_of_unit(blockIdx.x, b, t.rows_per, 1);
+  return q.req >= 0 && place_tile(b, a, t, q, ((int)blockIdx.x - (q.row0 / t.rows_per + q.req)) * t.rows_per, tile) && n > 1;
 }
 
 // Joins splits: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). Up to kJoinFew splits: one workgroup per tile
@@ -660,9 +709,10 @@ constexpr int kJoinFew = 32;
 
 __global__ __launch_bounds__(256) void attention_kv8_join_few_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
   AttnTile tile;
-  if (!find_joint(b, a, t, tile)) return;
+  int n;
+  if (!find_joint(b, a, t, c.hd, tile, n)) return;
   const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * t.vecs;
-  const int hd = c.hd, cols = hd >> 2, n = (tile.steps + tile.per - 1) / tile.per;
+  const int hd = c.hd, cols = hd >> 2;
   const int vecs = t.grp <= t.vecs ? (tile.i1 - tile.i0) * t.grp : min(t.vecs, t.grp - g0);
   for (int e = threadIdx.x; e < vecs * cols; e += 256) {
     const int vec = e / cols, col = e - vec * cols;
@@ -696,26 +746,24 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
   __shared__ float f[kAttnMaxSplits8], red[2][4];
   __shared__ float4 part[256];
   AttnTile tile;
-  if (!find_joint(b, a, t, tile)) return;
+  int n;
+  if (!find_joint(b, a, t, c.hd, tile, n)) return;
   const int tid = threadIdx.x, w = tid >> 6, vec = blockIdx.z, hd = c.hd;
   const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * t.vecs;
   const int oi = t.grp <= t.vecs ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= t.vecs ? vec % t.grp : g0 + vec;
   if (oi >= tile.i1 || oh >= t.grp) return;
-  const int n = (tile.steps + tile.per - 1) / tile.per;
   const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
   const float* ml = a.work + at * t.splits * 2;
   const float m = tid < n ? ml[2 * tid] : -INFINITY;
   float l = tid < n ? ml[2 * tid + 1] : 0.0f, M = m;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  M = wave_max(M);
   if ((tid & 63) == 0) red[0][w] = M;
   __syncthreads();
   M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float fs = m == M ? 1.0f : pow2(m - M);
   f[tid] = fs;
   l *= fs;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+  l = wave_sum(l);
   if ((tid & 63) == 0) red[1][w] = l;
   __syncthreads();
   const float L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
@@ -781,7 +829,7 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
 
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
   const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd);
-  return t.splits > 1 ? split_pairs(rows, heads, t.splits) + (size_t)rows * heads * t.splits * hd : 0;
+  return t.splits > 1 ? split_pairs(rows, heads, t.splits) + (size_t)rows * heads * t.splits * hd + t.units : 0;
 }
 
 template <int NB>

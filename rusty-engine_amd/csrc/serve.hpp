@@ -86,27 +86,44 @@ hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
 hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s);
 size_t logprobs_work_floats(int rows, int vocab, int k);
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s);
-hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, size_t ldk, const float* v,
-                             size_t ldv, hipStream_t s);
+hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,
+                             hipStream_t s);
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd);
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s);
 
-// Request of unit u, where request b owns the units from start[b] / div + mult * b on: the number of requests
-// whose first unit is at most u, less one (-1: none). Every thread of a workgroup of THREADS calls it.
-template <int THREADS>
-__device__ __forceinline__ int request_of_unit(int u, const int* __restrict__ start, int requests, int rows, int div,
-                                               int mult) {
-  __shared__ int part[THREADS / 64];
+// A request's place in the batch, in bounds whatever the arrays hold: rows row0 .. row0 + count - 1, tokens len.
+struct RequestRows {
+  int req, row0, count, len;
+};
+__device__ __forceinline__ RequestRows request_rows(int r, int start, int count, int len, int rows) {
+  const int row0 = min(max(start, 0), rows);
+  return {r, row0, min(max(count, 0), rows - row0), len};
+}
+
+// Request of unit u, where request b owns the units from start[b] / div + mult * b on: the last one whose first unit is
+// at most u (req -1: none, or starts that do not ascend). Every thread of a workgroup of 256 calls it. A thread has read
+// what it hands on, so the search is one round trip to memory.
+__device__ __forceinline__ RequestRows request_of_unit(int u, const PagedBatch& b, int div, int mult) {
+  __shared__ int part[4];
+  __shared__ RequestRows found;
+  RequestRows mine{-1, 0, 0, 0};
   int n = 0;
-  for (int b = threadIdx.x; b < requests; b += THREADS) n += min(max(start[b], 0), rows) / div + mult * b <= u;
+  for (int i = threadIdx.x; i < b.requests; i += 256) {
+    const RequestRows q = request_rows(i, b.start[i], b.count[i], b.len[i], b.rows);
+    if (q.row0 / div + mult * i <= u) {
+      ++n;
+      mine = q;
+    }
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
+  if (threadIdx.x == 0) found = RequestRows{-1, 0, 0, 0};
   __syncthreads();
-  n = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) n += part[w];
-  return n - 1;
+  n = part[0] + part[1] + part[2] + part[3];
+  if (mine.req >= 0 && mine.req == n - 1) found = mine;
+  __syncthreads();
+  return found;
 }
 
 }  // namespace rehip

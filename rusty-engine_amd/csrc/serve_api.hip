@@ -145,16 +145,16 @@ int re_kv8_append_dev(const float* d_k, size_t ldk, const float* d_v, size_t ldv
   int rc = paged_args(rows, requests, d_row_start, d_row_count, d_kv_len, d_table, table_ld, page, n_pages, d_kcodes,
                       d_vcodes, d_kscale, d_vscale, n_kv_heads, head_dim);
   if (rc) return rc;
-  if (ldk < n_kv_heads * head_dim || ldv < n_kv_heads * head_dim || ldk % 4 || ldv % 4 || ldk > (1u << 30) ||
-      ldv > (1u << 30))
-    return report_error(RE_ERR_SIZE, "append strides %zu/%zu (multiples of 4, at least %zu)", ldk, ldv,
+  if (ldk < n_kv_heads * head_dim || ldv < n_kv_heads * head_dim || ldk % 4 || ldv % 4 || ldk > (1u << 22) ||
+      ldv > (1u << 22))
+    return report_error(RE_ERR_SIZE, "append strides %zu/%zu (multiples of 4, %zu .. 4194304)", ldk, ldv,
                         n_kv_heads * head_dim);
   if (!a16(d_k) || !a16(d_v)) return report_error(RE_ERR_ARG, "k and v must be 16-byte aligned");
   if (rows == 0 || requests == 0) return RE_OK;
   const PagedBatch b{d_row_start, d_row_count, d_kv_len, d_table, (int)requests, (int)rows, (int)table_ld, (int)page,
                      (int)n_pages};
   const Kv8Cache c{d_kcodes, d_vcodes, d_kscale, d_vscale, (int)n_kv_heads, (int)head_dim};
-  HIP_TRY(launch_kv8_append(b, c, d_k, ldk, d_v, ldv, (hipStream_t)stream));
+  HIP_TRY(launch_kv8_append(b, c, d_k, (int)ldk, d_v, (int)ldv, (hipStream_t)stream));
   return RE_OK;
 }
 
