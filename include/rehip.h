@@ -372,7 +372,7 @@ int re_rope_rows_dev(const float *d_x, size_t ldx, size_t rows, size_t heads, si
                      int layout, const double *d_freqs, float mscale, const int *d_pos, float *d_out, size_t ldo,
                      void *stream);
 
-/* Append the batch's K and V rows (strides ldk, ldv floats, multiples of 4; 16-byte aligned) to the cache.
+/* Append the batch's K and V rows (strides ldk, ldv floats, multiples of 4 up to 2^22; 16-byte aligned) to the cache.
  * A page and head's scale is the largest finite magnitude of what it holds / 127 (0 where that is below the
  * smallest normal float), a code round(x / scale), ties to even; +-inf are stored as +-127 and NaN as 0.
  * Rows that raise the scale of a page with earlier rows of the request in it round those rows' codes

@@ -827,6 +827,14 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   return t;
 }
 
+static size_t attn_workgroups(const AttnTiles& t, int requests, int kv_heads) {
+  return (size_t)kv_heads * t.group_tiles * (t.direct ? (size_t)t.pieces + requests : (size_t)t.units * t.splits);
+}
+
+size_t attention_kv8_workgroups(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
+  return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd), requests, kv_heads);
+}
+
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
   const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd);
   return t.splits > 1 ? split_pairs(rows, heads, t.splits) + (size_t)rows * heads * t.splits * hd + t.units : 0;
@@ -843,7 +851,7 @@ static void launch_attention_hd(const PagedBatch& b, const Kv8Cache& c, const At
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s) {
   const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.heads, c.kv_heads, c.hd);
   const unsigned heads = (unsigned)(c.kv_heads * t.group_tiles);
-  const unsigned n = heads * (t.direct ? (unsigned)(t.pieces + b.requests) : (unsigned)t.units * (unsigned)t.splits);
+  const unsigned n = (unsigned)attn_workgroups(t, b.requests, c.kv_heads);
   switch (c.hd / 32) {
     case 1: launch_attention_hd<1>(b, c, a, t, n, s); break;
     case 2: launch_attention_hd<2>(b, c, a, t, n, s); break;

@@ -88,6 +88,9 @@ size_t logprobs_work_floats(int rows, int vocab, int k);
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s);
 hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,
                              hipStream_t s);
+// workgroups of the call's first launch: at most kAttnMaxWorkgroups are taken (a launch has fewer than 2^32 threads)
+constexpr size_t kAttnMaxWorkgroups = (size_t)1 << 23;
+size_t attention_kv8_workgroups(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd);
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd);
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s);
 

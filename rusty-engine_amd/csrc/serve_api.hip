@@ -187,6 +187,11 @@ int re_attention_kv8_dev(const float* d_q, size_t ldq, size_t rows, size_t reque
     return report_error(RE_ERR_ARG, "q, ctx and workspace must be 16-byte aligned");
   if (rows == 0 || requests == 0) return RE_OK;
   if (max_rows == 0) return report_error(RE_ERR_SIZE, "max_rows 0 for %zu rows", rows);
+  const size_t ml = max_len < (1u << 30) ? max_len : (1u << 30), mr = max_rows < rows ? max_rows : rows;
+  if (attention_kv8_workgroups((int)rows, (int)requests, (int)mr, (int)ml, (int)n_heads, (int)n_kv_heads,
+                               (int)head_dim) > kAttnMaxWorkgroups)
+    return report_error(RE_ERR_SIZE, "attention of %zu rows and %zu requests with %zu heads is too large for one call",
+                        rows, requests, n_heads);
   const size_t need = re_attention_kv8_work_bytes(rows, requests, max_rows, max_len, n_heads, n_kv_heads, head_dim);
   if (need && !d_work) return report_error(RE_ERR_ARG, "null workspace, need %zu bytes", need);
   if (work_bytes < need) return report_error(RE_ERR_SIZE, "attention workspace of %zu bytes, need %zu", work_bytes, need);
@@ -194,9 +199,8 @@ int re_attention_kv8_dev(const float* d_q, size_t ldq, size_t rows, size_t reque
                      (int)n_pages};
   const Kv8Cache c{const_cast<int8_t*>(d_kcodes), const_cast<int8_t*>(d_vcodes), const_cast<float*>(d_kscale),
                    const_cast<float*>(d_vscale), (int)n_kv_heads, (int)head_dim};
-  const size_t ml = max_len < (1u << 30) ? max_len : (1u << 30);
   const Attn8Args a{d_q, d_ctx, (float*)d_work, ldq, scale, (int)(window < (1u << 30) ? window : (1u << 30)),
-                    (int)n_heads, (int)(max_rows < rows ? max_rows : rows), (int)ml};
+                    (int)n_heads, (int)mr, (int)ml};
   HIP_TRY(launch_attention_kv8(b, c, a, (hipStream_t)stream));
   return RE_OK;
 }

@@ -204,6 +204,71 @@ def test_attention(heads, kv_heads, hd, page, name):
     check_attention(cache, bt, q, hd ** -0.5, ldq=heads * hd + 8)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,page,rows_of,len_of", [
+    (256, 64, 32, 32, [200, 1, 63], [230, 40, 64]),        # 64 vectors a tile: 16 rows of 4 heads
+    (128, 128, 64, 64, [300, 260], [300, 500]),            # .. 64 rows of one
+    (392, 56, 128, 64, [100, 70], [130, 70]),              # .. 9 rows of 7, one place unused
+    (256, 64, 160, 32, [100, 33, 17], [100, 34, 90]),      # 32 vectors: 8 rows of 4
+    (400, 20, 96, 96, [150, 1], [151, 1])])                 # 3 rows of 20 heads: 60 of 64
+@pytest.mark.parametrize("window", [0, 37])
+def test_attention_of_many_tiles(heads, kv_heads, hd, page, rows_of, len_of, window):
+    """Enough tiles for wide ones (32 or 64 query vectors)."""
+    rng = np.random.default_rng(hd)
+    bt, cache, q = make(rng, rows_of, len_of, page, heads, kv_heads, hd, gap=2)
+    check_attention(cache, bt, q, hd ** -0.5, window)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows_of", [(8, 1, 128, [4, 3, 4, 0, 1]), (14, 2, 64, [9, 5, 1, 9, 8]),
+                                                       (20, 1, 256, [1, 1, 1, 0, 1]), (34, 2, 32, [3, 3, 1, 2, 3])])
+def test_attention_of_wide_single_tiles(heads, kv_heads, hd, rows_of):
+    """All rows of a request in one tile of 32 or 64 vectors, cut into pieces (max_len says that there is work for many)."""
+    rng = np.random.default_rng(heads)
+    len_of = [900, 4, 77, 0, 1500]
+    bt, cache, q = make(rng, rows_of, len_of, 64, heads, kv_heads, hd, gap=1)
+    for max_len in (1500, 1 << 20):
+        check_attention(cache, bt, q, hd ** -0.5, max_len=max_len)
+    check_attention(cache, bt, q, hd ** -0.5, 200, max_len=1 << 20)
+
+
+def test_attention_of_many_requests():
+    """More requests than a workgroup has threads, some without rows, in one launch; each wave of lengths 1 .. 60."""
+    rng = np.random.default_rng(21)
+    n = 700
+    rows_of = rng.integers(0, 2, n)
+    len_of = np.maximum(rng.integers(1, 61, n), rows_of)
+    bt, cache, q = make(rng, rows_of, len_of, 32, 2, 1, 32)
+    check_attention(cache, bt, q, 0.3)
+    bt, cache, q = make(rng, rows_of * rng.integers(1, 4, n), len_of + 3, 32, 2, 1, 32, gap=1)
+    check_attention(cache, bt, q, 0.3)
+
+
+def test_append_of_many_requests():
+    rng = np.random.default_rng(22)
+    n = 700
+    rows_of = rng.integers(0, 3, n)
+    bt = Batch(rng, rows_of, rows_of + rng.integers(0, 60, n), 32, gap=1)
+    cache = Cache(rng, bt.n_pages, 1, 32, 32)
+    k, v = (rng.standard_normal((bt.rows, 1, 32)).astype(np.float32) for _ in range(2))
+    append_both(cache, bt, k, v)
+    cache.check()
+
+
+def test_starts_that_do_not_ascend_stay_in_bounds():
+    """Rows of such a batch may be skipped; nothing outside the arrays is touched and other pages keep their codes."""
+    rng = np.random.default_rng(23)
+    bt, cache, q = make(rng, [3, 2, 4, 1], [50, 2, 64, 33], 32, 4, 2, 64)
+    bt.start[:] = [9, -5, 1 << 30, 3]
+    k = rng.standard_normal((bt.rows, 2, 64)).astype(np.float32)
+    other = np.setdiff1d(np.arange(bt.n_pages), bt.table[bt.table >= 0])
+    kc, vc = cache.k.copy(), cache.v.copy()
+    rehip.kv8_append_dev(B.from_array(k), 128, B.from_array(k), 128, *bt.args(), *cache.args(), 2, 64)
+    hip.synchronize()
+    for buf, was, is_v in ((cache.kb, kc, 0), (cache.vb, vc, 1)):
+        got = ref.unpack(buf.download(np.int8, was.size), *cache.shape, is_v)
+        np.testing.assert_array_equal(got[other], was[other])
+    attend(cache, bt, q, 0.1)
+
+
 @pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 1000])
 @pytest.mark.parametrize("heads,kv_heads,hd,page", [(8, 2, 64, 32), (14, 2, 128, 64)])
 def test_attention_window(heads, kv_heads, hd, page, window):

@@ -60,7 +60,8 @@ BAD_BATCH = [
 
 @pytest.mark.parametrize("code,change", BAD_BATCH + [
     (rehip.RE_ERR_ARG, {"k": None}), (rehip.RE_ERR_ARG, {"v": None}), (rehip.RE_ERR_ARG, {"k": A + 4}),
-    (rehip.RE_ERR_SIZE, {"ldk": 124}), (rehip.RE_ERR_SIZE, {"ldv": 130})])
+    (rehip.RE_ERR_SIZE, {"ldk": 124}), (rehip.RE_ERR_SIZE, {"ldv": 130}),
+    (rehip.RE_ERR_SIZE, {"ldv": (1 << 22) + 4})])
 def test_append_refusals(code, change):
     refused(code, rehip.kv8_append_dev, **{**BATCH, "k": A, "v": A, "ldk": 128, "ldv": 128, **change})
 
@@ -73,7 +74,9 @@ ATTN = dict(BATCH, q=A, ldq=512, max_rows=4, max_len=256, n_heads=8, scale=0.125
     *[(rehip.RE_ERR_ARG, c) for c in ({"q": None}, {"ctx": None}, {"q": A + 4}, {"ctx": A + 8}, {"work": A + 4},
                                       {"scale": math.nan}, {"scale": math.inf})],
     *[(rehip.RE_ERR_SIZE, c) for c in ({"n_heads": 0}, {"n_heads": 7}, {"n_heads": 8194}, {"ldq": 508}, {"ldq": 514},
-                                       {"max_rows": 0})]])
+                                       {"max_rows": 0},
+                                      {"rows": 1 << 22, "max_rows": 1 << 22, "n_heads": 1024, "n_kv_heads": 1024,
+                                       "ldq": 65536})]])
 def test_attention_refusals(code, change):
     refused(code, rehip.attention_kv8_dev, **{**ATTN, **change})
 
