@@ -304,16 +304,20 @@ __device__ __forceinline__ int steps_per(int steps, int pieces) {
   return max(kAttnMinSteps, ((steps + pieces - 1) / pieces + 3) & ~3);
 }
 
+// inclusive sums over the lanes of a wave
+__device__ __forceinline__ int wave_scan(int v) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(v, off, 64);
+    if ((int)(threadIdx.x & 63) >= off) v += y;
+  }
+  return v;
+}
+
 // The sum over a workgroup of 256 threads, and in `before` that of the threads below this one.
 __device__ __forceinline__ int scan256(int v, int& before) {
   __shared__ int part[4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int inc = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(inc, off, 64);
-    if (lane >= off) inc += y;
-  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, inc = wave_scan(v);
   if (lane == 63) part[w] = inc;
   __syncthreads();
   const int p0 = part[0], p1 = part[1], p2 = part[2], p3 = part[3];
@@ -333,12 +337,28 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
     o.per = steps_per(o.steps, t.splits);
     return sp == 0 || sp * o.per < o.steps;
   }
-  // steps of a piece over the whole batch, then the request that piece u falls into; each thread has some of the
-  // requests, and the one that finds the piece hands its tile on
+  // steps of a piece over the whole batch, then the request that piece u falls into: up to 64 requests a lane of every
+  // wave each (nothing then goes through LDS), else some for each thread
+  const int most = (1 << 30) / b.requests;            // (the sums stay ints)
+  if (b.requests <= 64) {
+    const int i = threadIdx.x & 63, r = min(i, b.requests - 1);
+    const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
+    const bool has = place_tile(b, a, t, q, 0, o) && i < b.requests;
+    const int sums = wave_scan(has ? min(o.steps, most) : 0);
+    const int piece = steps_per(__builtin_amdgcn_readlane(sums, 63), t.pieces);
+    const int per = max(piece, steps_per(o.steps, t.splits));
+    const int mine = has ? max(1, (o.steps + per - 1) / per) : 0, upto = wave_scan(mine);
+    const unsigned long long at = __ballot(u < upto);
+    if (at == 0) return false;
+    const int l = __ffsll(at) - 1;
+    place_tile(b, a, t, lane_rows(q, l), 0, o);
+    o.per = __builtin_amdgcn_readlane(per, l);
+    sp = u - __builtin_amdgcn_readlane(upto - mine, l);
+    return true;
+  }
   __shared__ AttnTile found;
   __shared__ int found_sp;
   const int chunk = (b.requests + 255) / 256, r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
-  const int most = (1 << 30) / b.requests;            // (the sum stays an int)
   int sum = 0, before;
   bool has = false;
   for (int r = r0; r < r1; ++r) {
@@ -484,8 +504,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
     }
-    top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
-    top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+    top = max(top, lane_xor_u32<16>(top));
+    top = max(top, lane_xor_u32<32>(top));
     const int e = (int)(top >> 23);                               // 2^13 <= largest * 2^(f - 127) < 2^14
     const int f = e == 255 ? 127 : min(267 - e, 253);
     const float up = copysignf(__uint_as_float((unsigned)f << 23), a.scale);   // (scores' factor is then positive)

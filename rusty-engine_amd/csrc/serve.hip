@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "serve.hpp"
+#include "wave.hpp"
 
 namespace rehip {
 
@@ -286,9 +287,10 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
           (fa == 0.0f ? 0.0f : fa * (a.t + da * a.z)) + (fb == 0.0f ? 0.0f : fb * (b.t + db * b.z))};
 }
 __device__ __forceinline__ Stats wave_join(Stats s) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    s = join(s, Stats{__shfl_xor(s.m, off, 64), __shfl_xor(s.z, off, 64), __shfl_xor(s.t, off, 64)});
+  wave_butterfly([&](auto off) {
+    constexpr int X = decltype(off)::value;
+    s = join(s, Stats{lane_xor<X>(s.m), lane_xor<X>(s.z), lane_xor<X>(s.t)});
+  });
   return s;
 }
 
@@ -360,8 +362,7 @@ struct Candidates {
 #pragma unroll 8
     for (int j = 0; j < 64; ++j) rank += (unsigned)__builtin_amdgcn_readlane((int)o, j) > o;
     unsigned low = rank < k ? o : 0xffffffffu;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) low = min(low, (unsigned)__shfl_xor((int)low, off, 64));
+    wave_butterfly([&](auto off) { low = min(low, lane_xor_u32<decltype(off)::value>(low)); });
     low = (unsigned)__builtin_amdgcn_readfirstlane((int)low);
     border = ((key_t64)low << 32) - 1;   // (equal values pass; ordered() is never 0)
     least = value_of((key_t64)low << 32);
@@ -382,23 +383,30 @@ struct Candidates {
   }
 };
 
+// the row's target and its logit, on their way from the start
+struct Target {
+  int id;
+  float x;
+};
+__device__ __forceinline__ Target target_of(const LogprobArgs& a, int r) {
+  const int id = a.logprob ? a.targets[r] : -1;
+  return {id, a.x[(size_t)r * a.ld + min(max(id, 0), a.vocab - 1)]};
+}
+
 // what a finished row gives: the target's log probability, the entropy, the k best of the candidates
-__device__ __forceinline__ void finish_row(const LogprobArgs& a, int r, const Stats& s, const key_t64* list, int n) {
-  const float* x = a.x + (size_t)r * a.ld;
+__device__ __forceinline__ void finish_row(const LogprobArgs& a, int r, const Target& t, const Stats& s,
+                                           const key_t64* list, int n) {
   const float lz = logf(s.z);
   if (threadIdx.x == 0) {
-    if (a.logprob) {
-      const int g = a.targets[r];
-      a.logprob[r] = g >= 0 && g < a.vocab ? (x[g] - s.m) - lz : 0.0f;
-    }
+    if (a.logprob) a.logprob[r] = t.id >= 0 && t.id < a.vocab ? (t.x - s.m) - lz : 0.0f;
     if (a.entropy) a.entropy[r] = lz - s.t / s.z;
   }
   for (int e = threadIdx.x; e < n; e += blockDim.x) {
-    const int rank = rank_in(list, n, list[e]);
+    const key_t64 mine = list[e];
+    const int rank = rank_in(list, n, mine);
     if (rank < a.k) {
-      const int i = index_of(list[e]);
-      a.ids[(size_t)r * a.k + rank] = i;
-      a.top[(size_t)r * a.k + rank] = (x[i] - s.m) - lz;   // (of the logit itself: its key holds NaN as -inf)
+      a.ids[(size_t)r * a.k + rank] = index_of(mine);
+      a.top[(size_t)r * a.k + rank] = (value_of(mine) - s.m) - lz;     // (of a NaN, held as -inf: NaN by ln Z)
     }
   }
 }
@@ -412,6 +420,8 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float* x = a.x + (size_t)r * a.ld;
+  Target target{};
+  if (parts == 1) target = target_of(a, r);
   // parts of whole batches, the last one shorter
   const int batches = (a.vocab + 64 * kLogBatch - 1) / (64 * kLogBatch);
   const int b0 = (int)((long long)batches * part / parts), b1 = (int)((long long)batches * (part + 1) / parts);
@@ -493,7 +503,7 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
     __syncthreads();
   }
   if (parts == 1) {
-    finish_row(a, r, all, lists, n);
+    finish_row(a, r, target, all, lists, n);
     return;
   }
   float* o = a.work + (size_t)blockIdx.x * (4 + 2 * a.k);
@@ -523,6 +533,7 @@ __global__ __launch_bounds__(kLogJoin) void logprobs_join_kernel(LogprobArgs a, 
   __shared__ key_t64 low;
   __shared__ int count;
   const int r = blockIdx.x, tid = threadIdx.x, stride = 4 + 2 * a.k;
+  const Target target = target_of(a, r);
   const float* o = a.work + (size_t)r * parts * stride;
   if (tid < 64) {                          // (a lane per part)
     const bool in = tid < parts;
@@ -531,8 +542,10 @@ __global__ __launch_bounds__(kLogJoin) void logprobs_join_kernel(LogprobArgs a, 
     // a part shorter than q keys: all keys count
     key_t64 least = in && a.k > 0 ? (q <= __float_as_int(p[3]) ? reinterpret_cast<const key_t64*>(p + 4)[q - 1] : 0) : ~0ull;
     const Stats s = wave_join(in ? Stats{p[0], p[1], p[2]} : Stats{-INFINITY, 0.0f, 0.0f});
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) least = min(least, __shfl_xor(least, off, 64));
+    wave_butterfly([&](auto off) {
+      constexpr int X = decltype(off)::value;
+      least = min(least, (key_t64)lane_xor_u32<X>((unsigned)(least >> 32)) << 32 | lane_xor_u32<X>((unsigned)least));
+    });
     if (tid == 0) {
       all = s;
       low = least;
@@ -548,7 +561,7 @@ __global__ __launch_bounds__(kLogJoin) void logprobs_join_kernel(LogprobArgs a, 
     }
   }
   __syncthreads();
-  finish_row(a, r, all, list, count);
+  finish_row(a, r, target, all, list, count);
 }
 
 // About three workgroups for each CU; a part is at least one batch of every wave (64 rows of 151936, top 20: 32.0 / 28.8

@@ -103,10 +103,23 @@ __device__ __forceinline__ RequestRows request_rows(int r, int start, int count,
   return {r, row0, min(max(count, 0), rows - row0), len};
 }
 
+// lane l's of a wave, in every lane (l the same in all of them)
+__device__ __forceinline__ RequestRows lane_rows(const RequestRows& q, int l) {
+  return {__builtin_amdgcn_readlane(q.req, l), __builtin_amdgcn_readlane(q.row0, l), __builtin_amdgcn_readlane(q.count, l),
+          __builtin_amdgcn_readlane(q.len, l)};
+}
+
 // Request of unit u, where request b owns the units from start[b] / div + mult * b on: the last one whose first unit is
 // at most u (req -1: none, or starts that do not ascend). Every thread of a workgroup of 256 calls it. A thread has read
-// what it hands on, so the search is one round trip to memory.
+// what it hands on, so the search is one round trip to memory. Up to 64 requests every wave has them all, a lane each,
+// and nothing goes through LDS.
 __device__ __forceinline__ RequestRows request_of_unit(int u, const PagedBatch& b, int div, int mult) {
+  if (b.requests <= 64) {
+    const int i = threadIdx.x & 63, r = min(i, b.requests - 1);
+    const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
+    const int n = __popcll(__ballot(i < b.requests && q.row0 / div + mult * i <= u));
+    return n == 0 ? RequestRows{-1, 0, 0, 0} : lane_rows(q, n - 1);
+  }
   __shared__ int part[4];
   __shared__ RequestRows found;
   RequestRows mine{-1, 0, 0, 0};

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <type_traits>
 
 namespace rehip {
 
@@ -30,6 +31,20 @@ __device__ __forceinline__ float lane_xor(float v) {
     static_assert(OFF == 1, "lane_xor: OFF is a power of two up to 32");
     return __int_as_float(__builtin_amdgcn_update_dpp(0, u, 0xB1, 0xF, 0xF, false));
   }
+}
+template <int OFF>
+__device__ __forceinline__ unsigned lane_xor_u32(unsigned v) {
+  return __float_as_uint(lane_xor<OFF>(__uint_as_float(v)));
+}
+// f(OFF) for the butterfly's pairs: lanes xor 32, 16, .., 1
+template <class F>
+__device__ __forceinline__ void wave_butterfly(F f) {
+  f(std::integral_constant<int, 32>{});
+  f(std::integral_constant<int, 16>{});
+  f(std::integral_constant<int, 8>{});
+  f(std::integral_constant<int, 4>{});
+  f(std::integral_constant<int, 2>{});
+  f(std::integral_constant<int, 1>{});
 }
 // butterfly max / sum over the wave (every lane ends with the result), pairs xor 32, 16, .., 1
 __device__ __forceinline__ float wave_max(float v) {

@@ -375,7 +375,7 @@ class QMat:
 
 # ---- device-resident transformer steps (src/forward.rs, src/infer.rs) --------------------------
 def _p(b):
-    return _dev_ptr(b) if b is not None else None
+    return b if b is None or b.__class__ is int else _dev_ptr(b)
 
 
 def rmsnorm_dev(x, w, rows, d, eps, out, stream=None):
