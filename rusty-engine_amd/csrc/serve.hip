@@ -294,20 +294,28 @@ __device__ __forceinline__ Stats wave_join(Stats s) {
   return s;
 }
 
-// how many of list[0 .. n) are above `mine`
-__device__ __forceinline__ int rank_in(const key_t64* list, int n, key_t64 mine) {
-  int rank = 0;
-  int e = 0;
-  for (; e + 4 <= n; e += 4)
+// A list of n keys is followed by kPad zeros, so that it is read kPad at a time.
+constexpr int kPad = 8;
+
+// how many of list[0 .. n) are above each of mine
+template <int Q>
+__device__ __forceinline__ void rank_in(const key_t64* list, int n, const key_t64 (&mine)[Q], int (&rank)[Q]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) rank += list[e + q] > mine;
-  for (; e < n; ++e) rank += list[e] > mine;
-  return rank;
+  for (int q = 0; q < Q; ++q) rank[q] = 0;
+  for (int e = 0; e < n; e += kPad) {
+    key_t64 y[kPad];
+#pragma unroll
+    for (int j = 0; j < kPad; ++j) y[j] = list[e + j];
+#pragma unroll
+    for (int j = 0; j < kPad; ++j)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) rank[q] += y[j] > mine[q];
+  }
 }
 
 // A wave's candidates. The members are the same in every lane.
 struct Candidates {
-  key_t64* list;                         // kTopCap of them
+  key_t64* list;                         // kTopCap of them, and the zeros
   int n, k;
   key_t64 border;                        // keys at or below it cannot be among the k best
   float least;                           // .. nor values below this
@@ -318,19 +326,10 @@ struct Candidates {
     key_t64 mine[Q];
     int rank[Q];
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      mine[q] = lane + 64 * q < n ? list[lane + 64 * q] : 0;
-      rank[q] = 0;
-    }
-    int e = 0;
-    for (; e + 4 <= n; e += 4)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int q = 0; q < Q; ++q) rank[q] += list[e + j] > mine[q];
-    for (; e < n; ++e)
-#pragma unroll
-      for (int q = 0; q < Q; ++q) rank[q] += list[e] > mine[q];
+    for (int q = 0; q < Q; ++q) mine[q] = lane + 64 * q < n ? list[lane + 64 * q] : 0;
+    if (lane < kPad) list[n + lane] = 0;
+    __builtin_amdgcn_wave_barrier();
+    rank_in(list, n, mine, rank);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int q = 0; q < Q; ++q)
@@ -374,7 +373,7 @@ struct Candidates {
     if (__ballot(mx >= least) == 0) return;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const bool maybe = !(x[q] < least);
+      const bool maybe = !(x[q] < least);  // (NaN counts as -inf, and so may while the border is)
       if (__ballot(maybe) == 0) continue;
       const key_t64 key = key_of(x[q], at(q));
       push(maybe && at(q) >= 0 && key > border, key);
@@ -402,11 +401,12 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int r, const Ta
     if (a.entropy) a.entropy[r] = lz - s.t / s.z;
   }
   for (int e = threadIdx.x; e < n; e += blockDim.x) {
-    const key_t64 mine = list[e];
-    const int rank = rank_in(list, n, mine);
-    if (rank < a.k) {
-      a.ids[(size_t)r * a.k + rank] = index_of(mine);
-      a.top[(size_t)r * a.k + rank] = (value_of(mine) - s.m) - lz;     // (of a NaN, held as -inf: NaN by ln Z)
+    const key_t64 mine[1] = {list[e]};
+    int rank[1];
+    rank_in(list, n, mine, rank);
+    if (rank[0] < a.k) {
+      a.ids[(size_t)r * a.k + rank[0]] = index_of(mine[0]);
+      a.top[(size_t)r * a.k + rank[0]] = (value_of(mine[0]) - s.m) - lz;   // (of a NaN, held as -inf: NaN by ln Z)
     }
   }
 }
@@ -414,7 +414,7 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int r, const Ta
 // One workgroup per (row, part of it); a part's (m, Z, T) and candidates go to the workspace unless it is the whole row.
 template <bool TOP>
 __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a, int parts) {
-  __shared__ __attribute__((aligned(16))) key_t64 lists[TOP ? kLogWaves * kTopCap : 1];
+  __shared__ __attribute__((aligned(16))) key_t64 lists[TOP ? kLogWaves * (kTopCap + kPad) : 1];
   __shared__ Stats ws[kLogWaves];
   __shared__ int wn[kLogWaves];
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
   // parts of whole batches, the last one shorter
   const int batches = (a.vocab + 64 * kLogBatch - 1) / (64 * kLogBatch);
   const int b0 = (int)((long long)batches * part / parts), b1 = (int)((long long)batches * (part + 1) / parts);
-  Candidates c{lists + (TOP ? w * kTopCap : 0), 0, a.k, 0, -INFINITY};
+  Candidates c{lists + (TOP ? w * (kTopCap + kPad) : 0), 0, a.k, 0, -INFINITY};
   Stats s{-INFINITY, 0.0f, 0.0f};
   bool first = true;
   auto take = [&](const float (&v)[kLogBatch], int base) {
@@ -495,11 +495,12 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
     bool have = false;
     for (int k = 0; k < kLogWaves; ++k) {
       const int e = (int)threadIdx.x - n;
-      if (e >= 0 && e < wn[k]) { y = lists[k * kTopCap + e]; have = true; }
+      if (e >= 0 && e < wn[k]) { y = lists[k * (kTopCap + kPad) + e]; have = true; }
       n += wn[k];
     }
     __syncthreads();
     if (have) lists[threadIdx.x] = y;
+    if (threadIdx.x < kPad) lists[n + threadIdx.x] = 0;
     __syncthreads();
   }
   if (parts == 1) {
@@ -515,9 +516,10 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
   }
   if constexpr (TOP) {
     if ((int)threadIdx.x < n) {
-      const key_t64 mine = lists[threadIdx.x];
-      const int rank = rank_in(lists, n, mine);
-      if (rank < a.k) reinterpret_cast<key_t64*>(o + 4)[rank] = mine;
+      const key_t64 mine[1] = {lists[threadIdx.x]};
+      int rank[1];
+      rank_in(lists, n, mine, rank);
+      if (rank[0] < a.k) reinterpret_cast<key_t64*>(o + 4)[rank[0]] = mine[0];
     }
   }
 }
@@ -528,40 +530,45 @@ constexpr int kLogJoin = 256;
 constexpr int kLogMaxParts = 64;
 
 __global__ __launch_bounds__(kLogJoin) void logprobs_join_kernel(LogprobArgs a, int parts) {
-  __shared__ __attribute__((aligned(16))) key_t64 list[kLogMaxParts * kLogprobsMaxTop];
+  constexpr int kMost = kLogMaxParts * kLogprobsMaxTop;
+  __shared__ __attribute__((aligned(16))) key_t64 every[kMost], list[kMost + kPad];
   __shared__ Stats all;
   __shared__ key_t64 low;
   __shared__ int count;
   const int r = blockIdx.x, tid = threadIdx.x, stride = 4 + 2 * a.k;
   const Target target = target_of(a, r);
   const float* o = a.work + (size_t)r * parts * stride;
+  // the parts' keys, 0 where a part has fewer
+  for (int e = tid; e < parts * a.k; e += kLogJoin) {
+    const float* p = o + e / a.k * stride;
+    const key_t64 key = reinterpret_cast<const key_t64*>(p + 4)[e % a.k];
+    every[e] = e % a.k < __float_as_int(p[3]) ? key : 0;
+  }
+  const float* p = o + min(tid, parts - 1) * stride;
+  const Stats mine = tid < parts ? Stats{p[0], p[1], p[2]} : Stats{-INFINITY, 0.0f, 0.0f};
+  if (tid == 0) count = 0;
+  __syncthreads();
   if (tid < 64) {                          // (a lane per part)
-    const bool in = tid < parts;
-    const float* p = o + (in ? tid : 0) * stride;
-    const int q = (a.k + parts - 1) / parts;
+    const Stats s = wave_join(mine);
     // a part shorter than q keys: all keys count
-    key_t64 least = in && a.k > 0 ? (q <= __float_as_int(p[3]) ? reinterpret_cast<const key_t64*>(p + 4)[q - 1] : 0) : ~0ull;
-    const Stats s = wave_join(in ? Stats{p[0], p[1], p[2]} : Stats{-INFINITY, 0.0f, 0.0f});
+    key_t64 least = a.k > 0 && tid < parts ? every[tid * a.k + (a.k + parts - 1) / parts - 1] : ~0ull;
     wave_butterfly([&](auto off) {
       constexpr int X = decltype(off)::value;
       least = min(least, (key_t64)lane_xor_u32<X>((unsigned)(least >> 32)) << 32 | lane_xor_u32<X>((unsigned)least));
     });
     if (tid == 0) {
       all = s;
-      low = least;
-      count = 0;
+      low = max(least, (key_t64)1);
     }
   }
   __syncthreads();
-  for (int e = tid; e < parts * a.k; e += kLogJoin) {
-    const float* p = o + e / a.k * stride;
-    if (e % a.k < __float_as_int(p[3])) {
-      const key_t64 key = reinterpret_cast<const key_t64*>(p + 4)[e % a.k];
-      if (key >= low) list[atomicAdd(&count, 1)] = key;
-    }
-  }
+  for (int e = tid; e < parts * a.k; e += kLogJoin)
+    if (every[e] >= low) list[atomicAdd(&count, 1)] = every[e];
   __syncthreads();
-  finish_row(a, r, target, all, list, count);
+  const int n = count;
+  if (tid < kPad) list[n + tid] = 0;
+  __syncthreads();
+  finish_row(a, r, target, all, list, n);
 }
 
 // About three workgroups for each CU; a part is at least one batch of every wave (64 rows of 151936, top 20: 32.0 / 28.8
