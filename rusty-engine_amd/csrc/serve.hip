@@ -393,14 +393,15 @@ __device__ __forceinline__ Target target_of(const LogprobArgs& a, int r) {
 }
 
 // what a finished row gives: the target's log probability, the entropy, the k best of the candidates
+// (by `threads` threads, of which this is `tid`)
 __device__ __forceinline__ void finish_row(const LogprobArgs& a, int r, const Target& t, const Stats& s,
-                                           const key_t64* list, int n) {
+                                           const key_t64* list, int n, int tid, int threads) {
   const float lz = logf(s.z);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     if (a.logprob) a.logprob[r] = t.id >= 0 && t.id < a.vocab ? (t.x - s.m) - lz : 0.0f;
     if (a.entropy) a.entropy[r] = lz - s.t / s.z;
   }
-  for (int e = threadIdx.x; e < n; e += blockDim.x) {
+  for (int e = tid; e < n; e += threads) {
     const key_t64 mine[1] = {list[e]};
     int rank[1];
     rank_in(list, n, mine, rank);
@@ -412,13 +413,16 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int r, const Ta
 }
 
 // One workgroup per (row, part of it); a part's (m, Z, T) and candidates go to the workspace unless it is the whole row.
-template <bool TOP>
+// SHORT: a wave per row, four rows per workgroup, and no barrier.
+template <bool TOP, bool SHORT>
 __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a, int parts) {
   __shared__ __attribute__((aligned(16))) key_t64 lists[TOP ? kLogWaves * (kTopCap + kPad) : 1];
   __shared__ Stats ws[kLogWaves];
   __shared__ int wn[kLogWaves];
-  const int r = blockIdx.x / parts, part = blockIdx.x % parts;
+  constexpr int kStep = SHORT ? 1 : kLogWaves;             // batches between two of a wave
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = SHORT ? blockIdx.x * kLogWaves + w : blockIdx.x / parts, part = SHORT ? 0 : blockIdx.x % parts;
+  if (r >= a.rows) return;
   const float* x = a.x + (size_t)r * a.ld;
   Target target{};
   if (parts == 1) target = target_of(a, r);
@@ -461,12 +465,12 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
   };
   // whole batches, the next one loading meanwhile, then the row's last part of one
   const int whole = min(b1, a.vocab / (64 * kLogBatch));
-  int bt = b0 + w;
+  int bt = SHORT ? 0 : b0 + w;
   if (bt < whole) {
     float v[kLogBatch], nx[kLogBatch];
     load(v, bt);
-    for (; bt < whole; bt += kLogWaves) {
-      load(nx, bt + kLogWaves < whole ? bt + kLogWaves : bt);
+    for (; bt < whole; bt += kStep) {
+      load(nx, bt + kStep < whole ? bt + kStep : bt);
       take(v, bt * 64 * kLogBatch + 4 * lane);
 #pragma unroll
       for (int q = 0; q < kLogBatch; ++q) v[q] = nx[q];
@@ -478,13 +482,20 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
 #pragma unroll
     for (int q = 0; q < kLogBatch; ++q) {
       const int at = base + 256 * (q >> 2) + (q & 3);
-      v[q] = at < a.vocab ? x[at] : -INFINITY;
+      const float y = x[min(at, a.vocab - 1)];           // (loaded whatever: a load under a condition is waited for)
+      v[q] = at < a.vocab ? y : -INFINITY;
     }
     take(v, base);
   }
   s = wave_join(s);
   if constexpr (TOP) {
     if (c.n > 64) c.keep_best();           // (k at most 64: a workgroup's lists then have a thread per key)
+  }
+  if constexpr (SHORT) {
+    if (TOP && lane < kPad) c.list[c.n + lane] = 0;
+    __builtin_amdgcn_wave_barrier();
+    finish_row(a, r, target, s, c.list, c.n, lane, 64);
+    return;
   }
   if (lane == 0) { ws[w] = s; wn[w] = TOP ? c.n : 0; }
   __syncthreads();
@@ -504,7 +515,7 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
     __syncthreads();
   }
   if (parts == 1) {
-    finish_row(a, r, target, all, lists, n);
+    finish_row(a, r, target, all, lists, n, threadIdx.x, 64 * kLogWaves);
     return;
   }
   float* o = a.work + (size_t)blockIdx.x * (4 + 2 * a.k);
@@ -568,7 +579,7 @@ __global__ __launch_bounds__(kLogJoin) void logprobs_join_kernel(LogprobArgs a, 
   const int n = count;
   if (tid < kPad) list[n + tid] = 0;
   __syncthreads();
-  finish_row(a, r, target, all, list, n);
+  finish_row(a, r, target, all, list, n, tid, kLogJoin);
 }
 
 // About three workgroups for each CU; a part is at least one batch of every wave (64 rows of 151936, top 20: 32.0 / 28.8
@@ -585,7 +596,14 @@ size_t logprobs_work_floats(int rows, int vocab, int k) {
 
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s) {
   const int parts = logprob_parts(a.rows, a.vocab);
-  auto* k = a.k > 0 ? logprobs_kernel<true> : logprobs_kernel<false>;
+  // a wave per row where one batch is the row, or where rows alone fill the GPU's waves (us of a wave / a workgroup per
+  // row, top 5 or 20: 4000 x 1000 11.8 / 25.8, 2000 x 32000 54 / 67, 8000 x 32000 176 / 238; but 1000 x 16000 31.5 / 26.9)
+  if (a.vocab <= 64 * kLogBatch || a.rows >= 1536) {
+    auto* k = a.k > 0 ? logprobs_kernel<true, true> : logprobs_kernel<false, true>;
+    hipLaunchKernelGGL(k, dim3((unsigned)((a.rows + kLogWaves - 1) / kLogWaves)), dim3(64 * kLogWaves), 0, s, a, 1);
+    return hipGetLastError();
+  }
+  auto* k = a.k > 0 ? logprobs_kernel<true, false> : logprobs_kernel<false, false>;
   hipLaunchKernelGGL(k, dim3((unsigned)(a.rows * parts)), dim3(64 * kLogWaves), 0, s, a, parts);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || parts == 1) return e;

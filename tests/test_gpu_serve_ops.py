@@ -209,7 +209,7 @@ def check_logprobs(x, targets, k, ld=None):
 
 @pytest.mark.parametrize("rows,vocab,k", [(1, 1, 1), (3, 2, 2), (1, 63, 5), (2, 64, 64), (5, 65, 64), (1, 1000, 0),
                                           (7, 1023, 1), (300, 257, 20), (1, 151936, 20), (2, 151935, 64), (3, 32001, 7),
-                                          (40, 32768, 20), (1025, 515, 3)])
+                                          (40, 32768, 20), (1025, 515, 3), (1541, 3000, 20), (1536, 1025, 64)])
 def test_logprobs(rows, vocab, k):
     rng = np.random.default_rng(rows + vocab)
     x = (3 * rng.standard_normal((rows, vocab))).astype(np.float32)
@@ -239,6 +239,8 @@ def test_logprobs_of_hard_rows(vocab):
     assert got[0][8] == 0 and got[1][8] == 0 and got[0][9] == -np.inf
     assert got[2][0].tolist() == list(range(20))
     check_logprobs(x, t, 64)
+    if vocab < 6000:                                        # .. and a wave per row
+        check_logprobs(np.tile(x, (90, 1)), np.tile(t, 90), 20)
 
 
 def test_logprobs_parts_may_be_left_out():
