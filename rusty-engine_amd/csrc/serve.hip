@@ -16,12 +16,11 @@ namespace rehip {
 // it needs none or S_b <= the pages there are, so every thread decides for its own requests after one prefix sum.
 // The accepted and refused alike keep their rows (the caller laid them out from new_len); a refused one gets count 0
 // and keeps its length.
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanPer = kPlanMaxRequests / kPlanThreads;   // requests per thread
 
 // exclusive prefix sums over the workgroup of three numbers per thread; totals in tot
+template <int THREADS>
 __device__ __forceinline__ void scan3(int (&v)[3], int (&tot)[3]) {
-  __shared__ int part[3][kPlanThreads / 64];
+  __shared__ int part[3][THREADS / 64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int inc[3];
 #pragma unroll
@@ -39,7 +38,7 @@ __device__ __forceinline__ void scan3(int (&v)[3], int (&tot)[3]) {
   for (int c = 0; c < 3; ++c) {
     int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kPlanThreads / 64; ++i) {
+    for (int i = 0; i < THREADS / 64; ++i) {
       const int p = part[c][i];
       before += i < w ? p : 0;
       all += p;
@@ -74,18 +73,20 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, const int* start, co
 
 // One workgroup. Pages go back and are taken one per thread, whatever request they are of (a thread that walked its own
 // request's pages waited for memory page after page: 23 -> 8 us for 64 requests, 4 of which end).
-__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a, int rows_here) {
-  __shared__ int start[kPlanMaxRequests], count[kPlanMaxRequests], len[kPlanMaxRequests];
-  __shared__ int back_at[kPlanMaxRequests], need_at[kPlanMaxRequests], held_of[kPlanMaxRequests];
+template <int THREADS, int PER>             // PER requests per thread
+__global__ __launch_bounds__(THREADS) void kv_plan_kernel(PlanArgs a, int rows_here) {
+  constexpr int kMost = THREADS * PER;
+  __shared__ int start[kMost], count[kMost], len[kMost];
+  __shared__ int back_at[kMost], need_at[kMost], held_of[kMost];
   const int tid = threadIdx.x;
-  const int b0 = tid * kPlanPer;
-  int nw[kPlanPer], ln[kPlanPer], need[kPlanPer], back[kPlanPer], held[kPlanPer];
-  bool fits[kPlanPer];
+  const int b0 = tid * PER;
+  int nw[PER], ln[PER], need[PER], back[PER], held[PER];
+  bool fits[PER];
   int sum[3] = {0, 0, 0}, tot[3];
   const int room = a.table_ld * a.page;
   const int free0 = min(max(*a.n_free, 0), a.n_pages);
 #pragma unroll
-  for (int i = 0; i < kPlanPer; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int b = b0 + i;
     const bool in = b < a.requests;
     const int asked = in ? a.new_len[b] : 0;
@@ -100,11 +101,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a, int r
     sum[1] += need[i];
     sum[2] += max(nw[i], 0);
   }
-  scan3(sum, tot);
+  scan3<THREADS>(sum, tot);
   const int have = min(free0 + min(tot[0], a.n_pages), a.n_pages);
   int refused = 0, taken = 0;
 #pragma unroll
-  for (int i = 0; i < kPlanPer; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int b = b0 + i;
     const int n = max(nw[i], 0);
     const bool ok = nw[i] >= 0 && fits[i] && (need[i] == 0 || sum[1] + need[i] <= have);
@@ -123,21 +124,21 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a, int r
     sum[2] += n;
   }
   int fin[3] = {taken, refused, 0}, all[3];
-  scan3(fin, all);                         // (a barrier: the lists are there)
+  scan3<THREADS>(fin, all);                         // (a barrier: the lists are there)
   if (tid == 0) {
     *a.n_free_out = have - all[0];
     a.status[0] = all[1];
     a.status[1] = tot[2];
   }
   // pushes: ended requests' pages behind the free ones; the stack then holds `have`
-  for (int k = tid; k < have - free0; k += kPlanThreads) {
+  for (int k = tid; k < have - free0; k += THREADS) {
     const int b = last_at_most(back_at, a.requests, k);
     a.free_pages[free0 + k] = a.table[(size_t)b * a.table_ld + (k - back_at[b])];
   }
   __threadfence_block();
   __syncthreads();
   // needed page k is the k-th from the top, if its request's last one is there too
-  for (int k = tid; k < min(tot[1], have); k += kPlanThreads) {
+  for (int k = tid; k < min(tot[1], have); k += THREADS) {
     const int b = last_at_most(need_at, a.requests, k);
     const int upto = b + 1 < a.requests ? need_at[b + 1] : tot[1];
     if (upto <= have) a.table[(size_t)b * a.table_ld + held_of[b] + (k - need_at[b])] = a.free_pages[have - 1 - k];
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a, int r
   if (!rows_here) return;
   __threadfence_block();
   __syncthreads();
-  for (int t = tid; t < a.cap; t += kPlanThreads) plan_row(a, start, count, len, t);
+  for (int t = tid; t < a.cap; t += THREADS) plan_row(a, start, count, len, t);
 }
 
 __global__ __launch_bounds__(256) void kv_plan_rows_kernel(PlanArgs a) {
@@ -156,10 +157,18 @@ __global__ __launch_bounds__(256) void kv_plan_rows_kernel(PlanArgs a) {
     plan_row(a, start, a.count, a.len_out, t);
 }
 
+template <int THREADS, int PER>
+static void launch_plan(const PlanArgs& a, bool rows_here, hipStream_t s) {
+  hipLaunchKernelGGL((kv_plan_kernel<THREADS, PER>), dim3(1), dim3(THREADS), 0, s, a, rows_here ? 1 : 0);
+}
+
 hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s) {
+  const bool small = a.requests <= 256;
   // two rows per thread at most; more go to a launch of their own over many workgroups
-  const bool rows_here = a.cap <= 2 * kPlanThreads;
-  hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, rows_here ? 1 : 0);
+  const bool rows_here = a.cap <= (small ? 512 : 2048);
+  if (small) launch_plan<256, 1>(a, rows_here, s);
+  else if (a.requests <= 1024) launch_plan<1024, 1>(a, rows_here, s);
+  else launch_plan<1024, kPlanMaxRequests / 1024>(a, rows_here, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || rows_here) return e;
   hipLaunchKernelGGL(kv_plan_rows_kernel, dim3((unsigned)std::min((a.cap + 255) / 256, 1024)), dim3(256), 0, s, a);
