@@ -501,12 +501,18 @@ class DeviceDecoder:
       token. The host reads back 4 bytes per token (`step`) or nothing until the end (`replay`).
     Prefill (eager): the same with GEMMs over all prompt rows and MFMA flash attention.
 
-    Same computation as `DenseDecoder` (runner.rs:205-282, forward.rs:347-586)."""
+    Same computation as `DenseDecoder` (runner.rs:205-282, forward.rs:347-586). With kv_cache="int8" K and
+    V are kept in int8 pages of 64 tokens with a scale for each page and KV head (a quarter of the f32
+    caches' memory, any max_seq): per layer bias, rotary positions, append and attention over the pages
+    are launches of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32)."""
 
     def __init__(self, mb: ModelBytes, max_seq: int, mode: int = MODE_F32, prefill_rows: int = 1024,
-                 use_graph: bool = True):
+                 use_graph: bool = True, kv_cache: str = "f32"):
         from . import Ffn, attention_work_bytes, hip, rope_table_dev
         self._check_supported(mb)
+        if kv_cache not in ("f32", "int8"):
+            raise ValueError(f"DeviceDecoder: kv_cache {kv_cache!r} (f32 or int8)")
+        self.pages = _Int8Pages(mb, max_seq, prefill_rows) if kv_cache == "int8" else None
         self.mb, self.mode, self.max_seq = mb, mode, max_seq
         self.use_graph = use_graph
         g = self.g = mb.geom
@@ -523,8 +529,12 @@ class DeviceDecoder:
                 up=QMat.from_bytes(mb.ffn_type, b.up, g.d_ff, d),
                 down=QMat.from_bytes(mb.down_type, b.down, d, g.d_ff),
                 attn_norm=B.from_array(b.attn_norm), ffn_norm=B.from_array(b.ffn_norm),
-                q_bias=B.from_array(b.q_bias), k_bias=B.from_array(b.k_bias), v_bias=B.from_array(b.v_bias),
-                kc=B(max_seq * kv * 4), vc=B(max_seq * kv * 4))
+                q_bias=B.from_array(b.q_bias), k_bias=B.from_array(b.k_bias), v_bias=B.from_array(b.v_bias))
+            if self.pages is None:
+                blk.update(kc=B(max_seq * kv * 4), vc=B(max_seq * kv * 4))
+            else:
+                blk.update(bias=B.from_array(np.concatenate([b.q_bias, b.k_bias, b.v_bias]).astype(np.float32)),
+                           cache=self.pages.new_cache())
             # q, k and v share their input: one fused matrix (rows q | k | v) when they share a type
             blk["qkv"] = QMat.from_bytes(mb.attn_type, np.concatenate([b.q, b.k, b.v]), d + 2 * kv, d)
             blk["ffn"] = Ffn(blk["gate"], blk["up"])
@@ -544,7 +554,7 @@ class DeviceDecoder:
         self.ffn_bytes = max(blk["ffn"].block_work_bytes(blk["down"], cap) for blk in self.blocks) if self.blocks else 256
         self.ffn_work = B(self.ffn_bytes)
         self.logits_buf = B(mb.n_vocab * 4)
-        self.work_bytes = attention_work_bytes(8, g.n_heads, hd, max_seq)
+        self.work_bytes = attention_work_bytes(8, g.n_heads, hd, max_seq) if self.pages is None else 16
         self.work = B(self.work_bytes)
         self.pos = B.from_array(np.zeros(1, np.int32))
         self.tok = B.from_array(np.zeros(1, np.int32))
@@ -552,9 +562,10 @@ class DeviceDecoder:
         self.hist = B.from_array(np.zeros(max_seq, np.int32))
         self.toks = B(cap * 4)
         self.stream = hip.Stream()
-        # RoPE (cos, sin) of every position: the decode attention reads them instead of computing
-        self.rope = B(max_seq * hd * 4)
-        rope_table_dev(g.rope_freq_base, hd, max_seq, self.rope, self.stream)
+        if self.pages is None:
+            # RoPE (cos, sin) of every position: the decode attention reads them instead of computing
+            self.rope = B(max_seq * hd * 4)
+            rope_table_dev(g.rope_freq_base, hd, max_seq, self.rope, self.stream)
         self.graph = None
         self.seq_len = 0
 
@@ -609,6 +620,20 @@ class DeviceDecoder:
                       self.pos, self.ctx, work=self.work if rows < 8 else None,
                       work_bytes=self.work_bytes if rows < 8 else 0, stream=self.stream)
 
+    def _paged_attention(self, blk, rows):
+        """int8 pages: bias, rotary positions, append and attention of the rows that the step's plan gave."""
+        from . import ROPE_HALF, add_dev, attention_kv8_dev, kv8_append_dev, rope_rows_dev
+        g, d, kv, p, s = self.g, self.g.d_model, self.kv, self.pages, self.stream
+        ld = d + 2 * kv
+        add_dev(self.qkv, blk["bias"], rows * ld, ld, self.qkv, s)
+        rope_rows_dev(self.qkv, ld, rows, g.n_heads + g.n_kv_heads, g.head_dim, g.head_dim, ROPE_HALF, p.freqs, 1.0,
+                      p.row_pos, self.qkv, ld, s)
+        batch = (rows, 1, p.row_start, p.row_count, p.kv_len, p.table, p.count, p.PAGE, p.count, *blk["cache"])
+        kv8_append_dev(_Offset(self.qkv, 4 * d), ld, _Offset(self.qkv, 4 * (d + kv)), ld, *batch, g.n_kv_heads,
+                       g.head_dim, s)
+        attention_kv8_dev(self.qkv, ld, *batch, rows, self.max_seq, g.n_heads, g.n_kv_heads, g.head_dim,
+                          g.head_dim ** -0.5, 0, self.ctx, p.work, p.work_bytes, s)
+
     def _head_and_advance(self, last_row, delta):
         from . import decode_advance_dev
         self.output.matvec_ex_dev(last_row, self.logits_buf, norm_w=self.output_norm, eps=self.g.rms_eps,
@@ -620,17 +645,22 @@ class DeviceDecoder:
         from . import embed_dev
         g, s, eps = self.g, self.stream, self.g.rms_eps
         embed_dev(self.embed, self.mb.n_vocab, g.d_model, self.tok, 1, self.x, s)
+        if self.pages is not None:
+            self.pages.plan(self.pages.one, 1, s)
         for blk in self.blocks:
             blk["qkv"].matvec_ex_dev(self.x, self.qkv, norm_w=blk["attn_norm"], eps=eps, stream=s)
-            self._decode_attention(blk)
+            if self.pages is None:
+                self._decode_attention(blk)
+            else:
+                self._paged_attention(blk, 1)
             blk["o"].matvec_ex_dev(self.ctx, self.x, add=self.x, stream=s)            # residual
             blk["ffn"].forward_dev(self.x, self.hb, norm_w=blk["ffn_norm"], eps=eps, stream=s)
             blk["down"].matvec_ex_dev(self.hb, self.x, add=self.x, stream=s)          # residual
         self._head_and_advance(self.x, 1)
 
     # -- API -------------------------------------------------------------------------------
-    def prefill(self, prompt) -> int:
-        """Batched prefill of the prompt (runner.rs:236-260); returns the first greedy token."""
+    def _forward_rows(self, prompt) -> int:
+        """The blocks over the prompt's rows, appended behind the sequence; returns their number."""
         from . import add_dev, embed_dev, rmsnorm_dev
         g, s, m = self.g, self.stream, self.mode
         d = g.d_model
@@ -642,20 +672,69 @@ class DeviceDecoder:
             raise ValueError("prompt token outside the vocabulary")
         self.toks.upload(prompt)
         embed_dev(self.embed, self.mb.n_vocab, d, self.toks, rows, self.x, s)
+        if self.pages is not None:
+            if self.seq_len == 0:
+                self.pages.clear()
+            self.pages.new.upload(np.array([rows], np.int32))
+            self.pages.plan(self.pages.new, rows, s)
         for blk in self.blocks:
             rmsnorm_dev(self.x, blk["attn_norm"], rows, d, g.rms_eps, self.n, s)
             blk["qkv"].matmul_dev(self.n, rows, self.qkv, m, stream=s)
-            self._qkv_post(blk, rows)
-            self._attention(blk, rows)
+            if self.pages is None:
+                self._qkv_post(blk, rows)
+                self._attention(blk, rows)
+            else:
+                self._paged_attention(blk, rows)
             blk["o"].matmul_dev(self.ctx, rows, self.ob, m, stream=s)
             add_dev(self.x, self.ob, rows * d, rows * d, self.x, s)
             rmsnorm_dev(self.x, blk["ffn_norm"], rows, d, g.rms_eps, self.n, s)
             blk["ffn"].block_dev(blk["down"], self.n, rows, self.x, self.ffn_work, self.ffn_bytes, m, add=self.x,
                                  stream=s)
-        self._head_and_advance(_Offset(self.x, (rows - 1) * d * 4), rows)
+        return rows
+
+    def prefill(self, prompt) -> int:
+        """Batched prefill of the prompt (runner.rs:236-260); returns the first greedy token."""
+        rows = self._forward_rows(prompt)
+        self._head_and_advance(_Offset(self.x, (rows - 1) * self.g.d_model * 4), rows)
         self.seq_len += rows
         self.stream.synchronize()
         return int(self.tok.download(np.int32, 1)[0])
+
+    SCORE_ROWS = 64                        # rows of logits held at a time
+
+    def score(self, prompt, top_k: int = 0) -> dict:
+        """Prefill of the prompt with, for each of its rows, what the model says of the token that follows:
+        "logprob" of the prompt's own next token (0 for the last row), "entropy" in nats, and the top_k
+        alternatives' "ids" and "top" log probabilities (ties to the lower id). The sequence goes on as after
+        `prefill` (whose greedy token is returned as "next")."""
+        from . import logprobs_dev, logprobs_work_bytes, rmsnorm_dev
+        from .hip import DeviceBuffer as B
+        g, s, d, v = self.g, self.stream, self.g.d_model, self.mb.n_vocab
+        rows = self._forward_rows(prompt)
+        rmsnorm_dev(self.x, self.output_norm, rows, d, g.rms_eps, self.n, s)
+        step = min(rows, self.SCORE_ROWS)
+        targets = B.from_array(np.append(np.asarray(prompt, np.int32)[1:], np.int32(-1)))
+        logits, out = B(step * v * 4), {"logprob": B(rows * 4), "entropy": B(rows * 4)}
+        if top_k:
+            out.update(ids=B(rows * top_k * 4), top=B(rows * top_k * 4))
+        nbytes = max(logprobs_work_bytes(n, v, top_k) for n in {step, rows % step or step})
+        work = B(max(nbytes, 16))
+        at = lambda buf, r: _Offset(buf, 4 * r)   # noqa: E731
+        for r in range(0, rows, step):
+            n = min(step, rows - r)
+            self.output.matmul_dev(at(self.n, r * d), n, logits, self.mode, stream=s)
+            logprobs_dev(logits, v, n, v, at(targets, r), top_k, at(out["logprob"], r), at(out["entropy"], r),
+                         at(out["ids"], r * top_k) if top_k else None, at(out["top"], r * top_k) if top_k else None,
+                         work, nbytes, s)
+        self._head_and_advance(_Offset(self.x, (rows - 1) * d * 4), rows)
+        self.seq_len += rows
+        s.synchronize()
+        got = {k: b.download(np.int32 if k == "ids" else np.float32, rows * (top_k if k in ("ids", "top") else 1))
+               for k, b in out.items()}
+        for k in ("ids", "top"):
+            if top_k:
+                got[k] = got[k].reshape(rows, top_k)
+        return {**got, "next": int(self.tok.download(np.int32, 1)[0])}
 
     def _graph(self):
         from . import hip
@@ -721,6 +800,48 @@ class DeviceDecoder:
                 blk[k].close()
         self.output.close()
         self.stream.destroy()
+
+
+class _Int8Pages:
+    """One sequence's pages of the int8 K/V cache and the plan of its steps, on the device; the layers' codes
+    and scales share the page table."""
+    PAGE = 64
+
+    def __init__(self, mb: ModelBytes, max_seq: int, cap: int):
+        from . import attention_kv8_work_bytes, rope_freqs
+        from .hip import DeviceBuffer as B
+        g = mb.geom
+        if g.head_dim % 32 or g.head_dim > 256:
+            raise ValueError(f"DeviceDecoder: head_dim {g.head_dim}: int8 pages take multiples of 32 up to 256")
+        self.g, self.cap = g, max(1, cap)
+        self.count = -(-max_seq // self.PAGE)
+        i32 = lambda n: B.from_array(np.zeros(n, np.int32))   # noqa: E731
+        self.new, self.kv_len, self.n_free, self.row_start, self.row_count = (i32(1) for _ in range(5))
+        self.one = B.from_array(np.ones(1, np.int32))
+        self.table, self.free, self.status = i32(self.count), i32(self.count), i32(2)
+        self.row_seq, self.row_pos, self.row_slot = (i32(self.cap) for _ in range(3))
+        self.freqs = B.from_array(rope_freqs(g.rope_freq_base, g.head_dim)[0])
+        self.work_bytes = max(attention_kv8_work_bytes(r, 1, r, max_seq, g.n_heads, g.n_kv_heads, g.head_dim)
+                              for r in range(1, self.cap + 1))
+        self.work = B(max(self.work_bytes, 16))
+        self.clear()
+
+    def new_cache(self):
+        """One layer's K codes, V codes and their scales."""
+        from .hip import DeviceBuffer as B
+        n = self.count * self.g.n_kv_heads
+        return tuple(B(n * size) for size in (self.PAGE * self.g.head_dim,) * 2 + (4, 4))
+
+    def clear(self):
+        self.kv_len.upload(np.zeros(1, np.int32))
+        self.free.upload(np.arange(self.count, dtype=np.int32)[::-1])
+        self.n_free.upload(np.array([self.count], np.int32))
+
+    def plan(self, new, rows, stream):
+        from . import kv_plan_dev
+        kv_plan_dev(1, self.PAGE, new, self.kv_len, self.table, self.count, self.free, self.count, self.n_free,
+                    self.kv_len, self.n_free, self.row_start, self.row_count, rows, self.row_seq, self.row_pos,
+                    self.row_slot, self.status, stream)
 
 
 class _Offset:
