@@ -304,6 +304,12 @@ __device__ __forceinline__ int steps_per(int steps, int pieces) {
   return max(kAttnMinSteps, ((steps + pieces - 1) / pieces + 3) & ~3);
 }
 
+// .. of a piece of the whole batch's sum; a float sum is at most 2^-8 too small, and pieces that are too small in all
+// would be more than the launch has workgroups for
+__device__ __forceinline__ int piece_steps(float sum, int pieces) {
+  return max(kAttnMinSteps, ((int)fminf(ceilf(sum * 1.005f / (float)pieces), 1e9f) + 3) & ~3);
+}
+
 // inclusive sums over the lanes of a wave
 __device__ __forceinline__ int wave_scan(int v) {
 #pragma unroll
@@ -339,14 +345,12 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
   }
   // steps of a piece over the whole batch, then the request that piece u falls into: up to 64 requests a lane of every
   // wave each (nothing then goes through LDS), else some for each thread
-  const int most = (1 << 30) / b.requests;            // (the sums stay ints)
   if (b.requests <= 64) {
     const int i = threadIdx.x & 63, r = min(i, b.requests - 1);
     const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
     const bool has = place_tile(b, a, t, q, 0, o) && i < b.requests;
-    const int sums = wave_scan(has ? min(o.steps, most) : 0);
-    const int piece = steps_per(__builtin_amdgcn_readlane(sums, 63), t.pieces);
-    const int per = max(piece, steps_per(o.steps, t.splits));
+    const unsigned sum = (unsigned)__builtin_amdgcn_readlane(wave_scan(has ? o.steps : 0), 63);   // (at most 64 x 2^25)
+    const int per = max(piece_steps((float)sum, t.pieces), steps_per(o.steps, t.splits));
     const int mine = has ? max(1, (o.steps + per - 1) / per) : 0, upto = wave_scan(mine);
     const unsigned long long at = __ballot(u < upto);
     if (at == 0) return false;
@@ -358,14 +362,18 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
   }
   __shared__ AttnTile found;
   __shared__ int found_sp;
+  __shared__ float sums[4];
   const int chunk = (b.requests + 255) / 256, r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
-  int sum = 0, before;
+  float sum = 0.0f;
   bool has = false;
   for (int r = r0; r < r1; ++r) {
     has = place_request(b, a, t, r, o);
-    sum += has ? min(o.steps, most) : 0;
+    sum += has ? (float)o.steps : 0.0f;
   }
-  const int piece = steps_per(scan256(sum, before), t.pieces);
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  const int piece = piece_steps((sums[0] + sums[1]) + (sums[2] + sums[3]), t.pieces);
   auto pieces_of = [&] {
     o.per = max(piece, steps_per(o.steps, t.splits));
     return has ? max(1, (o.steps + o.per - 1) / o.per) : 0;
@@ -377,6 +385,7 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
       has = place_request(b, a, t, r, o);
       mine += pieces_of();
     }
+  int before;
   const int all = scan256(mine, before);
   if (u >= all) return false;
   if (u >= before && u < before + mine) {
