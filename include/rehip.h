@@ -317,7 +317,8 @@ int re_ffn_block_dev(re_ffn *f, re_qmat *down, const float *d_x, size_t rows, co
  * row_count[b]; rows between and behind them are left as they were. kv_len[b] counts the request's
  * tokens, its new rows included: row i stands at position kv_len[b] - row_count[b] + i. Token t of
  * it lies in page d_table[b * table_ld + t / page] at place t % page; an entry outside 0 .. n_pages - 1
- * holds no page. A page that is being appended to belongs to one request; full pages may be shared.
+ * holds no page. A request's pages are distinct, and a page that is being appended to belongs to one
+ * request; full pages may be shared.
  *
  * The cache: d_kcodes and d_vcodes hold n_pages x n_kv_heads x page x head_dim int8 codes (page and
  * head_dim multiples of 32 up to 256; 16-byte aligned), d_kscale and d_vscale n_pages x n_kv_heads f32
@@ -325,11 +326,12 @@ int re_ffn_block_dev(re_ffn *f, re_qmat *down, const float *d_x, size_t rows, co
  * dimensions, 1 KiB each, [page / 32][head_dim / 32], with token t and dimension d of a block at byte
  *   K: 256 (d / 8) + 16 (t % 16) + 8 (t / 16) + d % 8
  *   V: 256 (t / 4 % 4) + 16 (d % 16) + 8 (d / 16) + 4 (t / 16) + t % 4
- * (the order in which a wave's lanes hold matrix operands). A page needs no preparation. */
+ * (the order in which a wave's lanes hold matrix operands). A page needs no preparation; scales that are
+ * written by other means are finite and not negative. */
 
 /* The plan of a step from the requests' lengths. Request b holds d_kv_len[b] tokens and brings
- * d_new_len[b] more (0: none this time; up to 262144); -1 ends it: its pages go back to the pool,
- * request after request, and its length becomes 0. d_free is a stack of free pages, n_pages entries of
+ * d_new_len[b] more (0: none this time; up to 262144); a negative number ends it: its pages go back to
+ * the pool, request after request, and its length becomes 0 (so not a request that shares pages). d_free is a stack of free pages, n_pages entries of
  * which the first *d_n_free are set; the step's new pages are taken from its top in request order and
  * written to d_table (other entries are left). A request whose pages, with those of the requests
  * before it, exceed the free ones, or whose tokens exceed table_ld * page, is refused: row_count 0,
@@ -337,7 +339,7 @@ int re_ffn_block_dev(re_ffn *f, re_qmat *down, const float *d_x, size_t rows, co
  * d_row_start (rows packed in request order, refused ones included, as the caller packed them from
  * new_len) and d_row_count; for rows 0 .. row_cap - 1 the request, the position and the slot
  * (page * page size + place), -1 for rows of refused requests and behind the last; d_status[0] refused
- * requests, d_status[1] rows. Up to 4096 requests. */
+ * requests, d_status[1] rows. Up to 4096 requests, requests * table_ld up to 2^30. */
 int re_kv_plan_dev(size_t requests, size_t page, const int *d_new_len, const int *d_kv_len, int *d_table,
                    size_t table_ld, int *d_free, size_t n_pages, const int *d_n_free, int *d_kv_len_out,
                    int *d_n_free_out, int *d_row_start, int *d_row_count, size_t row_cap, int *d_row_seq,

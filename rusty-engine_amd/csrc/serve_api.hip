@@ -58,6 +58,8 @@ int re_kv_plan_dev(size_t requests, size_t page, const int* d_new_len, const int
       n_pages > (1u << 30) / page)
     return report_error(RE_ERR_SIZE, "table of %zu columns, %zu pages of %zu tokens (tokens up to 2^30)", table_ld,
                         n_pages, page);
+  if (requests * table_ld > (1u << 30))
+    return report_error(RE_ERR_SIZE, "table of %zu x %zu entries (up to 2^30)", requests, table_ld);
   const PlanArgs a{d_new_len,   d_kv_len,  d_table,   d_free,     d_n_free, d_kv_len_out, d_n_free_out,
                    d_row_start, d_row_count, d_row_seq, d_row_pos, d_row_slot, d_status, (int)requests,
                    (int)page,   (int)table_ld, (int)n_pages, (int)row_cap};

@@ -27,7 +27,8 @@ PLAN = dict(requests=4, page=64, new_len=A, kv_len=A, table=A, table_ld=8, free=
                                               "row_slot", "status")],
     *[(rehip.RE_ERR_SIZE, c) for c in ({"requests": 0}, {"requests": 4097}, {"page": 0}, {"page": 65537},
                                        {"table_ld": 0}, {"table_ld": 1 << 25}, {"n_pages": 0}, {"n_pages": 1 << 25},
-                                       {"row_cap": (1 << 22) + 1})]])
+                                       {"row_cap": (1 << 22) + 1},
+                                       {"requests": 4096, "table_ld": (1 << 18) + 1})]])
 def test_plan_refusals(code, change):
     refused(code, rehip.kv_plan_dev, **{**PLAN, **change})
 
