@@ -504,7 +504,8 @@ class DeviceDecoder:
     Same computation as `DenseDecoder` (runner.rs:205-282, forward.rs:347-586). With kv_cache="int8" K and
     V are kept in int8 pages of 64 tokens with a scale for each page and KV head (a quarter of the f32
     caches' memory, any max_seq): per layer bias, rotary positions, append and attention over the pages
-    are launches of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32)."""
+    are launches of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32).
+    A prefill at position 0 (seq_len 0) begins a new sequence."""
 
     def __init__(self, mb: ModelBytes, max_seq: int, mode: int = MODE_F32, prefill_rows: int = 1024,
                  use_graph: bool = True, kv_cache: str = "f32"):
@@ -710,6 +711,8 @@ class DeviceDecoder:
         from . import logprobs_dev, logprobs_work_bytes, rmsnorm_dev
         from .hip import DeviceBuffer as B
         g, s, d, v = self.g, self.stream, self.g.d_model, self.mb.n_vocab
+        if not 0 <= top_k <= min(64, v):
+            raise ValueError(f"score: top {top_k} of {v} tokens (up to 64)")
         rows = self._forward_rows(prompt)
         rmsnorm_dev(self.x, self.output_norm, rows, d, g.rms_eps, self.n, s)
         step = min(rows, self.SCORE_ROWS)

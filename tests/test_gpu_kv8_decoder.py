@@ -94,6 +94,9 @@ def test_score(tiny, kv_cache):
     plain.close()
     only = dd.score(prompt[:7])
     assert set(only) == {"logprob", "entropy", "next"} and only["logprob"][6] == 0
+    for bad in (-1, 65):
+        with pytest.raises(ValueError):
+            dd.score(prompt[:7], bad)
     dd.close()
 
 
