@@ -102,7 +102,7 @@ __global__ __launch_bounds__(THREADS) void kv_plan_kernel(PlanArgs a, int rows_h
     sum[2] += max(nw[i], 0);
   }
   scan3<THREADS>(sum, tot);
-  const int have = min(free0 + min(tot[0], a.n_pages), a.n_pages);
+  const int have = free0 + min(tot[0], a.n_pages - free0);
   int refused = 0, taken = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -337,13 +337,13 @@ struct Candidates {
 #pragma unroll
     for (int q = 0; q < Q; ++q) mine[q] = lane + 64 * q < n ? list[lane + 64 * q] : 0;
     if (lane < kPad) list[n + lane] = 0;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     rank_in(list, n, mine, rank);
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
 #pragma unroll
     for (int q = 0; q < Q; ++q)
       if (lane + 64 * q < n && rank[q] < k) list[rank[q]] = mine[q];
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
   }
   __device__ __forceinline__ void keep_best() {
     if (n <= 64) keep_best_of<1>();
@@ -359,7 +359,7 @@ struct Candidates {
     const unsigned long long who = __ballot(yes);
     if (who == 0) return;
     if (yes) list[n + __popcll(who & ((1ull << (threadIdx.x & 63)) - 1))] = key;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     n += __popcll(who);
     if (n > max(64, 2 * k)) keep_best();
   }
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
   }
   if constexpr (SHORT) {
     if (TOP && lane < kPad) c.list[c.n + lane] = 0;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     finish_row(a, r, target, s, c.list, c.n, lane, 64);
     return;
   }

@@ -64,4 +64,12 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v + lane_xor<1>(v);
 }
 
+// What the wave's lanes wrote to LDS before this, all its lanes read after it. LDS serves a wave in order, so this is
+// no instruction: it keeps the compiler from moving or reusing reads across it.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 }  // namespace rehip
