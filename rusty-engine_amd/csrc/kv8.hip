@@ -267,8 +267,9 @@ __device__ __forceinline__ float column_sum(float v) {
 //     `pieces` of them in all (and one more for each request), of at least kAttnMinSteps steps: a batch of lengths 1 ..
 //     16384 then takes the time of its sum, not of its longest request.
 //   else: unit u is a tile, every tile is cut into `splits` pieces.
+// A head's pieces have `slots` places in the workspace, a tile's one behind the other, each of `used` vectors.
 struct AttnTiles {
-  int vecs, grp, rows_per, group_tiles, units, direct, splits, pieces;
+  int vecs, grp, rows_per, group_tiles, units, direct, splits, pieces, slots, used;
 };
 
 // A tile's place: request, rows, and the 32-key steps it has to walk, and their cut into splits.
@@ -276,6 +277,7 @@ struct AttnTile {
   int req, row0, n, i0, i1;  // request, its first row, its rows, the tile's rows i0 .. i1 - 1 of them
   int p0;                    // position of the request's row 0 (may be below 0)
   int first, steps, per;     // first step, number of steps, steps per split
+  int slot;                  // its first place in the workspace
 };
 
 constexpr int kAttnMaxSplits8 = 256;  // one thread of the join each
@@ -341,6 +343,7 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
     const RequestRows q = request_of_unit(u, b, t.rows_per, 1);
     if (q.req < 0 || !place_tile(b, a, t, q, (u - (q.row0 / t.rows_per + q.req)) * t.rows_per, o)) return false;
     o.per = steps_per(o.steps, t.splits);
+    o.slot = u * t.splits;
     return sp == 0 || sp * o.per < o.steps;
   }
   // steps of a piece over the whole batch, then the request that piece u falls into: up to 64 requests a lane of every
@@ -349,8 +352,7 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
     const int i = threadIdx.x & 63, r = min(i, b.requests - 1);
     const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
     const bool has = place_tile(b, a, t, q, 0, o) && i < b.requests;
-    const unsigned sum = (unsigned)__builtin_amdgcn_readlane(wave_scan(has ? o.steps : 0), 63);   // (at most 64 x 2^25)
-    const int per = max(piece_steps((float)sum, t.pieces), steps_per(o.steps, t.splits));
+    const int per = max(piece_steps(wave_sum(has ? (float)o.steps : 0.0f), t.pieces), steps_per(o.steps, t.splits));
     const int mine = has ? max(1, (o.steps + per - 1) / per) : 0, upto = wave_scan(mine);
     const unsigned long long at = __ballot(u < upto);
     if (at == 0) return false;
@@ -358,6 +360,7 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
     place_tile(b, a, t, lane_rows(q, l), 0, o);
     o.per = __builtin_amdgcn_readlane(per, l);
     sp = u - __builtin_amdgcn_readlane(upto - mine, l);
+    o.slot = u - sp;
     return true;
   }
   __shared__ AttnTile found;
@@ -403,26 +406,30 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
   __syncthreads();
   o = found;
   sp = found_sp;
+  o.slot = u - sp;
   return true;
 }
 
-// The workspace holds (m, l) of every row, head and split, then from this float on (16-byte aligned) their sums, then
-// every unit's number of splits.
-__host__ __device__ inline size_t split_pairs(size_t rows, size_t heads, size_t splits) {
-  return (rows * heads * splits * 2 + 3) & ~(size_t)3;
+// The workspace holds (m, l) of every vector of every piece, then (16-byte aligned) their sums, then every unit's number
+// of splits and first place.
+__host__ __device__ inline size_t piece_vectors(const AttnTiles& t, int kv_heads) {
+  return (size_t)kv_heads * t.group_tiles * t.slots * t.used;
 }
-__device__ __forceinline__ size_t sums_at(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t) {
-  return split_pairs(b.rows, a.heads, t.splits);
+__host__ __device__ inline size_t sums_at(size_t vectors) { return (2 * vectors + 3) & ~(size_t)3; }
+// place of split 0, vector 0 of a tile's head and group yy
+__device__ __forceinline__ size_t place_of(const AttnTiles& t, const AttnTile& tile, int yy) {
+  return ((size_t)yy * t.slots + tile.slot) * t.used;
 }
 
 // the same in every lane, so that what follows from it is scalar
 __device__ __forceinline__ AttnTile uniform(const AttnTile& o) {
   auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  return {u(o.req), u(o.row0), u(o.n), u(o.i0), u(o.i1), u(o.p0), u(o.first), u(o.steps), u(o.per)};
+  return {u(o.req), u(o.row0), u(o.n), u(o.i0), u(o.i1), u(o.p0), u(o.first), u(o.steps), u(o.per), u(o.slot)};
 }
 
-__device__ __forceinline__ int* splits_at(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int hd) {
-  return reinterpret_cast<int*>(a.work + sums_at(b, a, t) + (size_t)b.rows * a.heads * t.splits * hd);
+__device__ __forceinline__ int2* splits_at(const Attn8Args& a, const AttnTiles& t, int kv_heads, int hd) {
+  const size_t n = piece_vectors(t, kv_heads);
+  return reinterpret_cast<int2*>(a.work + sums_at(n) + n * hd);
 }
 
 constexpr int kAttnPages = 256;       // pages whose numbers and scales are staged at a time: one per thread
@@ -674,8 +681,10 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   // the four waves' (m, l, O) joined in wave order, group after group
   const bool whole = tile.steps <= tile.per;                      // one split: nothing left to join
   if (t.splits > 1 && sp == 0 && yy == 0 && tid == 0)
-    splits_at(b, a, t, HD)[t.direct ? tile.req : tile.row0 / t.rows_per + tile.req + tile.i0 / t.rows_per] =
-        (tile.steps + tile.per - 1) / tile.per;
+    splits_at(a, t, c.kv_heads, HD)[t.direct ? tile.req : tile.row0 / t.rows_per + tile.req + tile.i0 / t.rows_per] =
+        make_int2((tile.steps + tile.per - 1) / tile.per, tile.slot);
+  const size_t place = place_of(t, tile, yy) + (size_t)sp * t.used;
+  float* const sums = a.work + sums_at(piece_vectors(t, c.kv_heads));
 #pragma unroll
   for (int v = 0; v < VT; ++v) {
     const float lv = column_sum(l[v]);
@@ -700,7 +709,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     }
     const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
     const float inv = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
-    float* out = whole ? a.ctx + at * HD : a.work + sums_at(b, a, t) + (at * t.splits + sp) * HD;
+    const size_t mine = place + 16 * v + vec;
+    float* out = whole ? a.ctx + at * HD : sums + mine * HD;
     for (int d = 4 * (tid & 15); d < HD; d += 64) {
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -714,21 +724,27 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       *reinterpret_cast<float4*>(out + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
     }
     if (!whole && (tid & 15) == 0) {
-      float* ml = a.work + (at * t.splits + sp) * 2;
-      ml[0] = M;
-      ml[1] = L;
+      a.work[2 * mine] = M;
+      a.work[2 * mine + 1] = L;
     }
   }
 }
 
 // The tile of workgroup blockIdx.x (.y: head and group of vectors) and its number of splits; false if there are none to
 // join.
-__device__ __forceinline__ bool find_joint(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int hd,
+__device__ __forceinline__ bool find_joint(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, const AttnTiles& t,
                                            AttnTile& tile, int& n) {
-  n = splits_at(b, a, t, hd)[blockIdx.x];                         // (no tile: not written, and not used)
-  if (t.direct) return place_request(b, a, t, blockIdx.x, tile) && n > 1;
-  const RequestRows q = request_of_unit(blockIdx.x, b, t.rows_per, 1);
-  return q.req >= 0 && place_tile(b, a, t, q, ((int)blockIdx.x - (q.row0 / t.rows_per + q.req)) * t.rows_per, tile) && n > 1;
+  const int2 at = splits_at(a, t, c.kv_heads, c.hd)[blockIdx.x];  // (no tile: not written, and not used)
+  n = at.x;
+  bool has;
+  if (t.direct) {
+    has = place_request(b, a, t, blockIdx.x, tile);
+  } else {
+    const RequestRows q = request_of_unit(blockIdx.x, b, t.rows_per, 1);
+    has = q.req >= 0 && place_tile(b, a, t, q, ((int)blockIdx.x - (q.row0 / t.rows_per + q.req)) * t.rows_per, tile);
+  }
+  tile.slot = at.y;
+  return has && n > 1;
 }
 
 // Joins splits: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). Up to kJoinFew splits: one workgroup per tile
@@ -739,26 +755,29 @@ constexpr int kJoinFew = 32;
 __global__ __launch_bounds__(256) void attention_kv8_join_few_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
   AttnTile tile;
   int n;
-  if (!find_joint(b, a, t, c.hd, tile, n)) return;
+  if (!find_joint(b, c, a, t, tile, n)) return;
   const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * t.vecs;
   const int hd = c.hd, cols = hd >> 2;
+  const size_t place = place_of(t, tile, blockIdx.y);
+  const float* const sums = a.work + sums_at(piece_vectors(t, c.kv_heads));
   const int vecs = t.grp <= t.vecs ? (tile.i1 - tile.i0) * t.grp : min(t.vecs, t.grp - g0);
   for (int e = threadIdx.x; e < vecs * cols; e += 256) {
     const int vec = e / cols, col = e - vec * cols;
     const int oi = t.grp <= t.vecs ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= t.vecs ? vec % t.grp : g0 + vec;
     const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
-    const float2* ml = reinterpret_cast<const float2*>(a.work) + at * t.splits;
-    const float* os = a.work + sums_at(b, a, t) + at * t.splits * hd + 4 * col;
+    const float2* ml = reinterpret_cast<const float2*>(a.work) + place + vec;
+    const float* os = sums + (place + vec) * hd + 4 * col;
     float M = -INFINITY;
 #pragma unroll 4
-    for (int s = 0; s < n; ++s) M = fmaxf(M, ml[s].x);
+    for (int s = 0; s < n; ++s) M = fmaxf(M, ml[s * t.used].x);
     float L = 0.0f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int s = 0; s < n; ++s) {
-      const float f = ml[s].x == M ? 1.0f : pow2(ml[s].x - M);
-      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * hd);
-      L = __builtin_fmaf(ml[s].y, f, L);
+      const float2 p = ml[s * t.used];
+      const float f = p.x == M ? 1.0f : pow2(p.x - M);
+      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * t.used * hd);
+      L = __builtin_fmaf(p.y, f, L);
       y.x = __builtin_fmaf(x.x, f, y.x);
       y.y = __builtin_fmaf(x.y, f, y.y);
       y.z = __builtin_fmaf(x.z, f, y.z);
@@ -776,15 +795,16 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
   __shared__ float4 part[256];
   AttnTile tile;
   int n;
-  if (!find_joint(b, a, t, c.hd, tile, n)) return;
+  if (!find_joint(b, c, a, t, tile, n)) return;
   const int tid = threadIdx.x, w = tid >> 6, vec = blockIdx.z, hd = c.hd;
   const int head = blockIdx.y / t.group_tiles, g0 = (blockIdx.y % t.group_tiles) * t.vecs;
   const int oi = t.grp <= t.vecs ? tile.i0 + vec / t.grp : tile.i0, oh = t.grp <= t.vecs ? vec % t.grp : g0 + vec;
   if (oi >= tile.i1 || oh >= t.grp) return;
   const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
-  const float* ml = a.work + at * t.splits * 2;
-  const float m = tid < n ? ml[2 * tid] : -INFINITY;
-  float l = tid < n ? ml[2 * tid + 1] : 0.0f, M = m;
+  const size_t place = place_of(t, tile, blockIdx.y) + vec;
+  const float2 mine = reinterpret_cast<const float2*>(a.work)[place + (size_t)min(tid, n - 1) * t.used];
+  const float m = tid < n ? mine.x : -INFINITY;
+  float l = tid < n ? mine.y : 0.0f, M = m;
   M = wave_max(M);
   if ((tid & 63) == 0) red[0][w] = M;
   __syncthreads();
@@ -798,12 +818,12 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
   const float L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   const int cols = hd >> 2, groups = 256 / cols;
   const int col = tid % cols, grp = tid / cols;
-  const float* os = a.work + sums_at(b, a, t) + at * t.splits * hd + 4 * col;
+  const float* os = a.work + sums_at(piece_vectors(t, c.kv_heads)) + place * hd + 4 * col;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   if (grp < groups) {
 #pragma unroll 4
     for (int s = grp; s < n; s += groups) {
-      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * hd);
+      const float4 x = *reinterpret_cast<const float4*>(os + (size_t)s * t.used * hd);
       y.x = __builtin_fmaf(x.x, f[s], y.x);
       y.y = __builtin_fmaf(x.y, f[s], y.y);
       y.z = __builtin_fmaf(x.z, f[s], y.z);
@@ -853,20 +873,21 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   t.pieces = (int)std::max(1L, 512 / ht);
   const long cuts = t.direct ? t.pieces : 1024 / (t.units * ht);
   t.splits = (int)std::max(1L, std::min({(long)most, cuts, (long)kAttnMaxSplits8}));
+  t.slots = t.direct ? t.pieces + requests : t.units * t.splits;
+  t.used = t.grp <= t.vecs ? t.rows_per * t.grp : t.vecs;
   return t;
 }
 
-static size_t attn_workgroups(const AttnTiles& t, int requests, int kv_heads) {
-  return (size_t)kv_heads * t.group_tiles * (t.direct ? (size_t)t.pieces + requests : (size_t)t.units * t.splits);
-}
+static size_t attn_workgroups(const AttnTiles& t, int kv_heads) { return (size_t)kv_heads * t.group_tiles * t.slots; }
 
 size_t attention_kv8_workgroups(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
-  return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd), requests, kv_heads);
+  return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd), kv_heads);
 }
 
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
   const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd);
-  return t.splits > 1 ? split_pairs(rows, heads, t.splits) + (size_t)rows * heads * t.splits * hd + t.units : 0;
+  const size_t n = piece_vectors(t, kv_heads);
+  return t.splits > 1 ? sums_at(n) + n * hd + 2 * (size_t)t.units : 0;
 }
 
 template <int NB>
@@ -880,7 +901,7 @@ static void launch_attention_hd(const PagedBatch& b, const Kv8Cache& c, const At
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s) {
   const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.heads, c.kv_heads, c.hd);
   const unsigned heads = (unsigned)(c.kv_heads * t.group_tiles);
-  const unsigned n = (unsigned)attn_workgroups(t, b.requests, c.kv_heads);
+  const unsigned n = (unsigned)attn_workgroups(t, c.kv_heads);
   switch (c.hd / 32) {
     case 1: launch_attention_hd<1>(b, c, a, t, n, s); break;
     case 2: launch_attention_hd<2>(b, c, a, t, n, s); break;
@@ -897,8 +918,7 @@ hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const At
     hipLaunchKernelGGL(attention_kv8_join_few_kernel, dim3((unsigned)t.units, heads), dim3(256), 0, s, b, c, a, t);
     return hipGetLastError();
   }
-  const int vecs = t.grp <= t.vecs ? t.rows_per * t.grp : t.vecs;
-  hipLaunchKernelGGL(attention_kv8_join_kernel, dim3((unsigned)t.units, heads, (unsigned)vecs), dim3(256), 0, s, b, c, a,
+  hipLaunchKernelGGL(attention_kv8_join_kernel, dim3((unsigned)t.units, heads, (unsigned)t.used), dim3(256), 0, s, b, c, a,
                      t);
   return hipGetLastError();
 }
