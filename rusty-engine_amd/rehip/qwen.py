@@ -505,7 +505,7 @@ class DeviceDecoder:
     V are kept in int8 pages of 64 tokens with a scale for each page and KV head (a quarter of the f32
     caches' memory, any max_seq): per layer bias, rotary positions, append and attention over the pages
     are launches of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32).
-    A prefill at position 0 (seq_len 0) begins a new sequence."""
+    A prefill goes on at seq_len, also where that was set back: 0 begins a new sequence."""
 
     def __init__(self, mb: ModelBytes, max_seq: int, mode: int = MODE_F32, prefill_rows: int = 1024,
                  use_graph: bool = True, kv_cache: str = "f32"):
@@ -674,8 +674,7 @@ class DeviceDecoder:
         self.toks.upload(prompt)
         embed_dev(self.embed, self.mb.n_vocab, d, self.toks, rows, self.x, s)
         if self.pages is not None:
-            if self.seq_len == 0:
-                self.pages.clear()
+            self.pages.go_to(self.seq_len)
             self.pages.new.upload(np.array([rows], np.int32))
             self.pages.plan(self.pages.new, rows, s)
         for blk in self.blocks:
@@ -821,13 +820,14 @@ class _Int8Pages:
         i32 = lambda n: B.from_array(np.zeros(n, np.int32))   # noqa: E731
         self.new, self.kv_len, self.n_free, self.row_start, self.row_count = (i32(1) for _ in range(5))
         self.one = B.from_array(np.ones(1, np.int32))
-        self.table, self.free, self.status = i32(self.count), i32(self.count), i32(2)
+        self.table, self.status = i32(self.count), i32(2)
+        self.free = B.from_array(np.arange(self.count, dtype=np.int32)[::-1])
         self.row_seq, self.row_pos, self.row_slot = (i32(self.cap) for _ in range(3))
         self.freqs = B.from_array(rope_freqs(g.rope_freq_base, g.head_dim)[0])
         self.work_bytes = max(attention_kv8_work_bytes(r, 1, r, max_seq, g.n_heads, g.n_kv_heads, g.head_dim)
                               for r in range(1, self.cap + 1))
         self.work = B(max(self.work_bytes, 16))
-        self.clear()
+        self.go_to(0)
 
     def new_cache(self):
         """One layer's K codes, V codes and their scales."""
@@ -835,10 +835,10 @@ class _Int8Pages:
         n = self.count * self.g.n_kv_heads
         return tuple(B(n * size) for size in (self.PAGE * self.g.head_dim,) * 2 + (4, 4))
 
-    def clear(self):
-        self.kv_len.upload(np.zeros(1, np.int32))
-        self.free.upload(np.arange(self.count, dtype=np.int32)[::-1])
-        self.n_free.upload(np.array([self.count], np.int32))
+    def go_to(self, length):
+        """The sequence holds its first `length` tokens; pages are taken in order, so the rest are the stack."""
+        self.kv_len.upload(np.array([length], np.int32))
+        self.n_free.upload(np.array([self.count - -(-length // self.PAGE)], np.int32))
 
     def plan(self, new, rows, stream):
         from . import kv_plan_dev

@@ -67,6 +67,26 @@ def test_int8_new_conversations_and_replays(tiny):
     assert qwen.logit_profile_check(whole, chunked)["ok"]
 
 
+def test_int8_a_sequence_set_back(tiny):
+    """Tokens behind a page boundary taken back: what follows is as if they had never been there."""
+    rng = np.random.default_rng(5)
+    prompt, other = rng.integers(0, 1000, 100), rng.integers(0, 1000, 150)
+    got = []
+    for detour in (False, True):
+        dd = qwen.DeviceDecoder(tiny, max_seq=400, prefill_rows=200, kv_cache="int8")
+        dd.prefill(prompt[:64])
+        if detour:
+            dd.prefill(other)
+            dd.step()
+            dd.seq_len = 64
+            dd.pos.upload(np.array([64], np.int32))
+        tokens = [dd.prefill(prompt[64:])] + [dd.step() for _ in range(8)]
+        got.append((tokens, dd.logits()))
+        dd.close()
+    assert got[0][0] == got[1][0]
+    np.testing.assert_array_equal(got[0][1], got[1][1])
+
+
 @pytest.mark.parametrize("kv_cache", ["f32", "int8"])
 def test_score(tiny, kv_cache):
     """Each row's numbers are those of the logits that prefilling up to it gives; the sequence goes on as after
