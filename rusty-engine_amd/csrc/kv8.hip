@@ -306,10 +306,14 @@ __device__ __forceinline__ int steps_per(int steps, int pieces) {
   return max(kAttnMinSteps, ((steps + pieces - 1) / pieces + 3) & ~3);
 }
 
-// .. of a piece of the whole batch's sum; a float sum is at most 2^-8 too small, and pieces that are too small in all
-// would be more than the launch has workgroups for
-__device__ __forceinline__ int piece_steps(float sum, int pieces) {
-  return max(kAttnMinSteps, ((int)fminf(ceilf(sum * 1.005f / (float)pieces), 1e9f) + 3) & ~3);
+// .. of a piece of the whole batch's sum over `live` requests. Their last pieces are half empty on average; while they are
+// few that half is taken off, so that there are about `pieces` workgroups in all (us without / with: 64 requests of up to
+// 16384, 4 heads of 128 38.8 / 35.4, 16 of up to 20000, 8 of 256 43.8 / 36.2; but 128 requests, 64 pieces a head 90 / 99,
+// 48 of up to 32000, 64 69 / 82: the longest piece then comes last). A float sum is at most 2^-8 too small, and pieces
+// that are too small in all would be more than the launch has workgroups for.
+__device__ __forceinline__ int piece_steps(float sum, float live, int pieces) {
+  const float n = 2.0f * live <= (float)pieces ? (float)pieces - 0.5f * live : (float)pieces;
+  return max(kAttnMinSteps, ((int)fminf(ceilf(sum * 1.005f / n), 1e9f) + 3) & ~3);
 }
 
 // inclusive sums over the lanes of a wave
@@ -352,7 +356,8 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
     const int i = threadIdx.x & 63, r = min(i, b.requests - 1);
     const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
     const bool has = place_tile(b, a, t, q, 0, o) && i < b.requests;
-    const int per = max(piece_steps(wave_sum(has ? (float)o.steps : 0.0f), t.pieces), steps_per(o.steps, t.splits));
+    const int piece = piece_steps(wave_sum(has ? (float)o.steps : 0.0f), (float)__popcll(__ballot(has)), t.pieces);
+    const int per = max(piece, steps_per(o.steps, t.splits));
     const int mine = has ? max(1, (o.steps + per - 1) / per) : 0, upto = wave_scan(mine);
     const unsigned long long at = __ballot(u < upto);
     if (at == 0) return false;
@@ -365,18 +370,21 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
   }
   __shared__ AttnTile found;
   __shared__ int found_sp;
-  __shared__ float sums[4];
+  __shared__ float sums[2][4];
   const int chunk = (b.requests + 255) / 256, r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
-  float sum = 0.0f;
+  float sum = 0.0f, live = 0.0f;
   bool has = false;
   for (int r = r0; r < r1; ++r) {
     has = place_request(b, a, t, r, o);
     sum += has ? (float)o.steps : 0.0f;
+    live += has ? 1.0f : 0.0f;
   }
   sum = wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+  live = wave_sum(live);
+  if ((threadIdx.x & 63) == 0) { sums[0][threadIdx.x >> 6] = sum; sums[1][threadIdx.x >> 6] = live; }
   __syncthreads();
-  const int piece = piece_steps((sums[0] + sums[1]) + (sums[2] + sums[3]), t.pieces);
+  const int piece = piece_steps((sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]),
+                                (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]), t.pieces);
   auto pieces_of = [&] {
     o.per = max(piece, steps_per(o.steps, t.splits));
     return has ? max(1, (o.steps + o.per - 1) / o.per) : 0;
@@ -868,9 +876,11 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   }
   const long ht = (long)kv_heads * t.group_tiles;
   const int most = (std::max(max_len, 1) + 32 * kAttnMinSteps - 1) / (32 * kAttnMinSteps);
-  // two workgroups of a piece for each CU (us of 512 / 1024 / 2048 / 8192 workgroups: one request of 131071 tokens, 8
-  // heads of 128, 55.7 / 59.6 / 63.4 / 74; 64 requests of 1 .. 16384, 4 heads, 44.9 / 47.6 / 47.5 / 53.9)
-  t.pieces = (int)std::max(1L, 512 / ht);
+  // two workgroups of a piece for each CU, four of heads up to 64, whose steps are half as many bytes on their way (us of
+  // 512 / 1024 / 1536: one request of 131071 tokens, 8 heads of 128 50.5 / 53.7 / 56, 64 of up to 16384, 4 of 128 35.4 /
+  // 41 / 42; but one of 131071, 2 of 64 17.5 / 16.8 / 16.8, 128 of up to 8000, 4 of 64 32.7 / 24.4 / 26.7, 300, 2 of 32
+  // 31.5 / 24.4 / 25.0)
+  t.pieces = (int)std::max(1L, (hd <= 64 ? 1024 : 512) / ht);
   const long cuts = t.direct ? t.pieces : 1024 / (t.units * ht);
   t.splits = (int)std::max(1L, std::min({(long)most, cuts, (long)kAttnMaxSplits8}));
   t.slots = t.direct ? t.pieces + requests : t.units * t.splits;
