@@ -331,9 +331,9 @@ int re_ffn_block_dev(re_ffn *f, re_qmat *down, const float *d_x, size_t rows, co
 
 /* The plan of a step from the requests' lengths. Request b holds d_kv_len[b] tokens and brings
  * d_new_len[b] more (0: none this time; up to 262144); a negative number ends it: its pages go back to
- * the pool, request after request, and its length becomes 0 (so not a request that shares pages). d_free is a stack of free pages, n_pages entries of
- * which the first *d_n_free are set; the step's new pages are taken from its top in request order and
- * written to d_table (other entries are left). A request whose pages, with those of the requests
+ * the pool, request after request, and its length becomes 0 (so not a request that shares pages). d_free
+ * is a stack of free pages, n_pages entries of which the first *d_n_free are set; the step's new pages are
+ * taken from its top in request order and written to d_table (other entries are left). A request whose pages, with those of the requests
  * before it, exceed the free ones, or whose tokens exceed table_ld * page, is refused: row_count 0,
  * length and pages unchanged. Outputs: d_kv_len_out and d_n_free_out (may be d_kv_len and d_n_free);
  * d_row_start (rows packed in request order, refused ones included, as the caller packed them from

@@ -16,6 +16,10 @@ namespace rehip {
 // it needs none or S_b <= the pages there are, so every thread decides for its own requests after one prefix sum.
 // The accepted and refused alike keep their rows (the caller laid them out from new_len); a refused one gets count 0
 // and keeps its length.
+//
+// Bound by latency (a few KB): loads, two scans, the stack, the table, then the rows, one after the other in one workgroup:
+// 64 requests 7.6 us a call, 5.4 in the kernel; 1024 requests and 19000 rows 12.5 us, 8.6 and 4.1 for the rows' launch (of
+// more rows than two per thread; in the plan's own workgroup they would take a trip to memory per 1024 of them).
 
 // exclusive prefix sums over the workgroup of three numbers per thread; totals in tot
 template <int THREADS>
@@ -177,7 +181,9 @@ hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s) {
 
 // ---- rotary positions ----------------------------------------------------------------------------
 // Pair i of each head of row r turns by pos[r] * freqs[i] radians and is scaled by mscale. The angle is taken in turns
-// and reduced to half a turn in 64 bits: at position 131071 an angle in 32 bits is off by up to 4e-3.
+// and reduced to half a turn in 64 bits: at position 131071 an angle in 32 bits is off by up to 4e-3. A row's angles are
+// taken once for all its heads. Bound by HBM: 8192 rows of 36 heads of 128, 302 MB, 57.8 us, 5.2 TB/s (as a large copy);
+// 8 rows by the launch, 7 us a call and 2.8 in the kernel.
 __device__ __forceinline__ void turn_cs(int pos, double freq, float mscale, float& c, float& s) {
   const double t = (double)pos * (freq * 0.15915494309189533577);
   const float f = (float)(2.0 * (t - rint(t)));
@@ -263,6 +269,9 @@ hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s) {
 // the others the keys above the border are appended. When the list is full its k best stay, ranked by counting. A first
 // border comes from the first batch: the k-th largest of the 64 lanes' maxima has at least k values at or above it.
 // Values in random order push about k ln(batches) keys behind the first batch; a rising row pushes all.
+//
+// Bound by HBM: 961 rows of 151936, 20 best, 584 MB in 100 us, 5.8 TB/s (without candidates 93, 6.3 TB/s); one row 10.5 us,
+// 7.0 and 4.4 in its two launches: latency.
 constexpr int kTopCap = 256;             // candidates of a wave
 constexpr int kLogBatch = 16;            // logits of a lane at a time
 constexpr int kLogWaves = 4;
