@@ -26,7 +26,8 @@ namespace rehip {
 // |q| <= 127 (1 + 2^-23), and q + 1.5 2^23 rounds it to an integer, whose low byte is the code.
 //
 // Bound by HBM for prompts: 9260 rows of 8 heads of 128, 94.8 MB, 18.0 us, 5.3 TB/s (a copy of 1 GiB runs at 5.1). A decode
-// step (64 rows, 0.33 MB) is three dependent trips to memory, the rows' places, the page number, the values: 8.0 us.
+// step (64 rows, 0.33 MB) is three dependent trips to memory, the rows' places, the page number, the values: 4.8 us in the
+// kernel.
 constexpr float kCodeMagic = 12582912.0f;
 
 __device__ __forceinline__ unsigned code_of(float x, float s, float y) {
@@ -45,6 +46,52 @@ __device__ __forceinline__ unsigned bytes4(unsigned a, unsigned b, unsigned c, u
   return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
+// Token of a lane's first code in a block (blocks of the page in order, nb for 32 tokens), and of its code e.
+template <bool IS_V>
+__device__ __forceinline__ int first_token(int blk, int nb) {
+  const int lane = threadIdx.x & 63;
+  return 32 * (blk / nb) + (IS_V ? 4 * (lane >> 4) : lane & 15);
+}
+template <bool IS_V>
+__device__ __forceinline__ int token_of(int first, int e) {
+  return first + (IS_V ? 16 * ((e >> 2) & 1) + (e & 3) : 16 * (e >> 3));
+}
+__device__ __forceinline__ int held_code(const uint4& u, int e) { return (int)(int8_t)((&u.x)[e >> 2] >> (8 * (e & 3))); }
+
+// The page's scale from the threads' largest magnitudes of the new tokens and of what it held (s_old).
+struct PageScale {
+  float s, ratio, inverse;   // of old codes to new ones; 1 / s
+  bool grown, plain;         // plain: every value is finite and the quotient may be taken by remainders
+};
+__device__ __forceinline__ PageScale page_scale(float top, float odd, float s_old, const float* __restrict__ x, int ld,
+                                                int o0, int o1, int hd, float (*red)[4]) {
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  top = wave_max(top);
+  odd = wave_sum(odd);
+  if (lane == 0) { red[0][w] = top; red[1][w] = odd; }
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  odd = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  if (odd != odd) {                        // the finite ones only
+    top = 0.0f;
+    for (int e = tid; e < (o1 - o0) * hd; e += 256) {
+      const float v = fabsf(x[e / hd * ld + e % hd]);
+      if (v < INFINITY) top = fmaxf(top, v);
+    }
+    top = wave_max(top);
+    __syncthreads();
+    if (lane == 0) red[0][w] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  }
+  if (o0 == 0) s_old = 0.0f;               // the page is begun: what it held before does not count
+  float s = top * (1.0f / 127.0f);
+  if (s < 1.17549435e-38f) s = 0.0f;
+  s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(s, s_old))));
+  const bool grown = o0 > 0 && s > s_old;
+  return {s, grown ? s_old / s : 1.0f, 1.0f / s, grown, s >= 7.8886091e-31f && odd == odd};
+}
+
 // One page's new tokens o0 .. o1 - 1 of one head: x is token o0's row, codes and scale the page's. A thread has U units of
 // 16 codes that lie together in memory (K: 2 tokens x 8 dimensions, V: 8 tokens x 2), 64 lanes' units a block of 32 x 32:
 // it loads their values, and the codes of a page that is not all new, before the largest magnitude is known, so that all
@@ -56,12 +103,10 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   const int nb = hd >> 5, blocks = (page >> 5) * nb;
   const bool all_new = o0 == 0 && o1 == page;
-  auto first_token = [&](int blk) { return 32 * (blk / nb) + (IS_V ? 4 * g : m); };
-  auto token_of = [&](int t, int e) { return t + (IS_V ? 16 * ((e >> 2) & 1) + (e & 3) : 16 * (e >> 3)); };
   auto load = [&](int blk, float (&y)[16]) {
-    const int t = first_token(blk), d = 32 * (blk % nb) + (IS_V ? m : 8 * g);
+    const int t = first_token<IS_V>(blk, nb), d = 32 * (blk % nb) + (IS_V ? m : 8 * g);
     // (of a token that is not new, some new one's values: a load under a condition of its lane waits for the one before)
-    auto row = [&](int e) { return x + ((min(max(token_of(t, e), o0), o1 - 1) - o0) * ld + d); };
+    auto row = [&](int e) { return x + ((min(max(token_of<IS_V>(t, e), o0), o1 - 1) - o0) * ld + d); };
     if constexpr (IS_V) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -81,7 +126,7 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
   uint4* const units = reinterpret_cast<uint4*>(codes) + lane;    // unit of block blk: units[64 * blk]
   float y[U > 0 ? U : 1][16];
   uint4 old[U > 0 ? U : 1];
-  float s_old = *scale;
+  const float s_old = *scale;
   float top = 0.0f, odd = 0.0f;            // odd: NaN once an infinity or a NaN was seen
   auto largest = [&](const float (&z)[16]) {
 #pragma unroll
@@ -105,48 +150,25 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
       largest(y[0]);
     }
   }
-  top = wave_max(top);
-  odd = wave_sum(odd);
-  if (lane == 0) { red[0][w] = top; red[1][w] = odd; }
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  odd = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  if (odd != odd) {                        // the finite ones only
-    top = 0.0f;
-    for (int e = tid; e < (o1 - o0) * hd; e += 256) {
-      const float v = fabsf(x[e / hd * ld + e % hd]);
-      if (v < INFINITY) top = fmaxf(top, v);
-    }
-    top = wave_max(top);
-    __syncthreads();
-    if (lane == 0) red[0][w] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  }
-  if (o0 == 0) s_old = 0.0f;               // the page is begun: what it held before does not count
-  float s = top * (1.0f / 127.0f);
-  if (s < 1.17549435e-38f) s = 0.0f;
-  s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(s, s_old))));
-  const bool grown = o0 > 0 && s > s_old, plain = s >= 7.8886091e-31f && odd == odd;
-  const float ratio = grown ? s_old / s : 1.0f, inverse = 1.0f / s;
+  const PageScale sc = page_scale(top, odd, s_old, x, ld, o0, o1, hd, red);
   auto store = [&](int blk, const float (&z)[16], const uint4& was) {
     unsigned c[16], out[4];
-    if (plain) {
+    if (sc.plain) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) c[e] = code_of(z[e], s, inverse);
+      for (int e = 0; e < 16; ++e) c[e] = code_of(z[e], sc.s, sc.inverse);
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) c[e] = code_of_any(z[e], s);
+      for (int e = 0; e < 16; ++e) c[e] = code_of_any(z[e], sc.s);
     }
     if (!all_new) {
-      const int t = first_token(blk);
+      const int t = first_token<IS_V>(blk, nb);
       bool changes = false;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int tok = token_of(t, e), held = (int)(int8_t)((&was.x)[e >> 2] >> (8 * (e & 3)));
-        if (tok < o0) c[e] = grown ? (unsigned)(int)rintf((float)held * ratio) : (unsigned)held;
+        const int tok = token_of<IS_V>(t, e), held = held_code(was, e);
+        if (tok < o0) c[e] = sc.grown ? (unsigned)(int)rintf((float)held * sc.ratio) : (unsigned)held;
         if (tok >= o1) c[e] = (unsigned)held;
-        changes |= tok < o1 && (tok >= o0 || grown);
+        changes |= tok < o1 && (tok >= o0 || sc.grown);
       }
       if (!changes) return;
     }
@@ -165,7 +187,68 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
       store(blk, y[0], old[0]);
     }
   }
-  if (tid == 0) *scale = s;
+  if (tid == 0) *scale = sc.s;
+}
+
+// The same where the new tokens have up to 1024 values, four for each thread: their codes go straight to their bytes, and
+// the page's other codes are read and written only if its scale grows (us of 64 tokens, 4 heads of 128 4.8 in the kernel
+// instead of 8.7 by whole units; 256 tokens, 8 heads of 256, pages of 256 15 / 162; 512 times 8 rows, 4 of 128 19 / 34. Old
+// codes loaded beforehand, on their way with the values, did not pay: 1000 tokens, 8 heads of 128 64 -> 72).
+constexpr int kAppendFew = 1024;
+
+template <bool IS_V>
+__device__ __forceinline__ void append_few(const float* __restrict__ x, int ld, int o0, int o1, int page, int hd,
+                                           int8_t* codes, float* scale, float (*red)[4]) {
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nb = hd >> 5, blocks = (page >> 5) * nb, n = (o1 - o0) * hd;
+  const int at = min(4 * tid, n - 4), row = at / hd, d = at - row * hd;
+  const float4 y = *reinterpret_cast<const float4*>(x + (row * ld + d));
+  const float z[4] = {y.x, y.y, y.z, y.w};
+  float top = 0.0f, odd = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    top = fmaxf(top, fabsf(z[e]));
+    odd = __builtin_fmaf(z[e], 0.0f, odd);
+  }
+  const PageScale sc = page_scale(top, odd, *scale, x, ld, o0, o1, hd, red);
+  if (sc.grown) {
+    uint4* const units = reinterpret_cast<uint4*>(codes) + lane;
+    for (int b0 = w; b0 < blocks; b0 += 16) {
+      uint4 old[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) old[i] = units[64 * min(b0 + 4 * i, blocks - 1)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int blk = b0 + 4 * i, t = first_token<IS_V>(blk, nb);
+        if (blk >= blocks) break;
+        unsigned c[16], out[4];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int held = held_code(old[i], e);
+          c[e] = token_of<IS_V>(t, e) < o0 ? (unsigned)(int)rintf((float)held * sc.ratio) : (unsigned)held;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = bytes4(c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]);
+        units[64 * blk] = make_uint4(out[0], out[1], out[2], out[3]);
+      }
+    }
+    __syncthreads();                       // the new codes come after
+  }
+  if (tid == 0) *scale = sc.s;
+  if (4 * tid >= n) return;
+  unsigned c[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] = sc.plain ? code_of(z[e], sc.s, sc.inverse) : code_of_any(z[e], sc.s);
+  const int tok = o0 + row, t = tok & 31, dd = d & 31;
+  int8_t* const block = codes + 1024 * ((tok >> 5) * nb + (d >> 5));
+  if constexpr (IS_V) {
+    int8_t* const o = block + 256 * (t >> 2 & 3) + 16 * (dd & 15) + 8 * (dd >> 4) + 4 * (t >> 4) + (t & 3);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[16 * e] = (int8_t)c[e];
+  } else {
+    *reinterpret_cast<unsigned*>(block + 256 * (dd >> 3) + 16 * (t & 15) + 8 * (t >> 4) + (dd & 7)) =
+        bytes4(c[0], c[1], c[2], c[3]);
+  }
 }
 
 // One workgroup per (run of one request's new rows inside one page, head, K or V).
@@ -184,10 +267,16 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache 
   if (pid < 0 || pid >= b.n_pages) return;
   const int o0 = lo - pi * b.page, o1 = hi - pi * b.page;
   const size_t row = q.row0 + lo - first, at = (size_t)pid * c.kv_heads + head, codes = at * b.page * c.hd;
-  if (blockIdx.z == 0)
-    append_page<false, U>(k + row * ldk + head * c.hd, ldk, o0, o1, b.page, c.hd, c.k + codes, c.ks + at, red);
-  else
-    append_page<true, U>(v + row * ldv + head * c.hd, ldv, o0, o1, b.page, c.hd, c.v + codes, c.vs + at, red);
+  const bool few = (o1 - o0) * c.hd <= kAppendFew;
+  if (blockIdx.z == 0) {
+    const float* x = k + row * ldk + head * c.hd;
+    if (few) append_few<false>(x, ldk, o0, o1, b.page, c.hd, c.k + codes, c.ks + at, red);
+    else append_page<false, U>(x, ldk, o0, o1, b.page, c.hd, c.k + codes, c.ks + at, red);
+  } else {
+    const float* x = v + row * ldv + head * c.hd;
+    if (few) append_few<true>(x, ldv, o0, o1, b.page, c.hd, c.v + codes, c.vs + at, red);
+    else append_page<true, U>(x, ldv, o0, o1, b.page, c.hd, c.v + codes, c.vs + at, red);
+  }
 }
 
 hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,

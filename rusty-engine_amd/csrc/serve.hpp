@@ -110,36 +110,23 @@ __device__ __forceinline__ RequestRows lane_rows(const RequestRows& q, int l) {
 }
 
 // Request of unit u, where request b owns the units from start[b] / div + mult * b on: the last one whose first unit is
-// at most u (req -1: none, or starts that do not ascend). Every thread of a workgroup of 256 calls it. A thread has read
-// what it hands on, so the search is one round trip to memory. Up to 64 requests every wave has them all, a lane each,
-// and nothing goes through LDS.
+// at most u (req -1: none; of starts that do not ascend, any one). Every wave looks at 64 requests at a time, a lane each,
+// spread over the range that is left: one trip to memory up to 64 requests, two up to 4096, and nothing goes through LDS.
 __device__ __forceinline__ RequestRows request_of_unit(int u, const PagedBatch& b, int div, int mult) {
-  if (b.requests <= 64) {
-    const int i = threadIdx.x & 63, r = min(i, b.requests - 1);
-    const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
-    const int n = __popcll(__ballot(i < b.requests && q.row0 / div + mult * i <= u));
-    return n == 0 ? RequestRows{-1, 0, 0, 0} : lane_rows(q, n - 1);
+  const int lane = threadIdx.x & 63;
+  int base = 0, n = b.requests;
+  while (n > 64) {
+    const int step = (n + 63) >> 6, i = base + lane * step;
+    const int row0 = min(max(b.start[min(i, b.requests - 1)], 0), b.rows);
+    const int k = __popcll(__ballot(lane * step < n && row0 / div + mult * i <= u));
+    if (k == 0) return {-1, 0, 0, 0};
+    base += (k - 1) * step;
+    n = min(step, n - (k - 1) * step);
   }
-  __shared__ int part[4];
-  __shared__ RequestRows found;
-  RequestRows mine{-1, 0, 0, 0};
-  int n = 0;
-  for (int i = threadIdx.x; i < b.requests; i += 256) {
-    const RequestRows q = request_rows(i, b.start[i], b.count[i], b.len[i], b.rows);
-    if (q.row0 / div + mult * i <= u) {
-      ++n;
-      mine = q;
-    }
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
-  if (threadIdx.x == 0) found = RequestRows{-1, 0, 0, 0};
-  __syncthreads();
-  n = part[0] + part[1] + part[2] + part[3];
-  if (mine.req >= 0 && mine.req == n - 1) found = mine;
-  __syncthreads();
-  return found;
+  const int r = base + min(lane, n - 1);
+  const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
+  const int k = __popcll(__ballot(lane < n && q.row0 / div + mult * r <= u));
+  return k == 0 ? RequestRows{-1, 0, 0, 0} : lane_rows(q, k - 1);
 }
 
 }  // namespace rehip
