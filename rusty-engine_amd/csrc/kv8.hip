@@ -26,7 +26,7 @@ namespace rehip {
 // |q| <= 127 (1 + 2^-23), and q + 1.5 2^23 rounds it to an integer, whose low byte is the code.
 //
 // Bound by HBM for prompts: 9260 rows of 8 heads of 128, 94.8 MB, 18.0 us, 5.3 TB/s (a copy of 1 GiB runs at 5.1). A decode
-// step (64 rows, 0.33 MB) is three dependent trips to memory, the rows' places, the page number, the values: 4.8 us in the
+// step (64 rows, 0.33 MB) is three dependent trips to memory, the rows' places, the page number, the values: 4.0 us in the
 // kernel.
 constexpr float kCodeMagic = 12582912.0f;
 
@@ -58,31 +58,40 @@ __device__ __forceinline__ int token_of(int first, int e) {
 }
 __device__ __forceinline__ int held_code(const uint4& u, int e) { return (int)(int8_t)((&u.x)[e >> 2] >> (8 * (e & 3))); }
 
-// The page's scale from the threads' largest magnitudes of the new tokens and of what it held (s_old).
+// The page's scale from the threads' largest magnitudes of the new tokens and of what it held (s_old). W waves work
+// together, the whole workgroup or one.
 struct PageScale {
   float s, ratio, inverse;   // of old codes to new ones; 1 / s
   bool grown, plain;         // plain: every value is finite and the quotient may be taken by remainders
 };
+template <int W>
+__device__ __forceinline__ float append_max(float v, float (*red)[4]) {
+  v = wave_max(v);
+  if constexpr (W == 1) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+}
+template <int W>
 __device__ __forceinline__ PageScale page_scale(float top, float odd, float s_old, const float* __restrict__ x, int ld,
                                                 int o0, int o1, int hd, float (*red)[4]) {
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   top = wave_max(top);
   odd = wave_sum(odd);
-  if (lane == 0) { red[0][w] = top; red[1][w] = odd; }
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  odd = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  if constexpr (W > 1) {
+    if ((tid & 63) == 0) { red[0][w] = top; red[1][w] = odd; }
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    odd = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  }
   if (odd != odd) {                        // the finite ones only
     top = 0.0f;
-    for (int e = tid; e < (o1 - o0) * hd; e += 256) {
+    for (int e = tid; e < (o1 - o0) * hd; e += 64 * W) {
       const float v = fabsf(x[e / hd * ld + e % hd]);
       if (v < INFINITY) top = fmaxf(top, v);
     }
-    top = wave_max(top);
-    __syncthreads();
-    if (lane == 0) red[0][w] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    top = append_max<W>(top, red);
   }
   if (o0 == 0) s_old = 0.0f;               // the page is begun: what it held before does not count
   float s = top * (1.0f / 127.0f);
@@ -150,7 +159,7 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
       largest(y[0]);
     }
   }
-  const PageScale sc = page_scale(top, odd, s_old, x, ld, o0, o1, hd, red);
+  const PageScale sc = page_scale<4>(top, odd, s_old, x, ld, o0, o1, hd, red);
   auto store = [&](int blk, const float (&z)[16], const uint4& was) {
     unsigned c[16], out[4];
     if (sc.plain) {
@@ -190,16 +199,14 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
   if (tid == 0) *scale = sc.s;
 }
 
-// The same where the new tokens have up to 1024 values, four for each thread: their codes go straight to their bytes, and
-// the page's other codes are read and written only if its scale grows (us of 64 tokens, 4 heads of 128 4.8 in the kernel
-// instead of 8.7 by whole units; 256 tokens, 8 heads of 256, pages of 256 15 / 162; 512 times 8 rows, 4 of 128 19 / 34. Old
-// codes loaded beforehand, on their way with the values, did not pay: 1000 tokens, 8 heads of 128 64 -> 72).
-constexpr int kAppendFew = 1024;
-
-template <bool IS_V>
+// The same where the new tokens have at most four values for each thread of W waves: their codes go straight to their bytes, and
+// the page's other codes are read and written only if its scale grows (us of the workgroup's four waves / by whole units: 64
+// tokens, 4 heads of 128 4.8 / 8.7 in the kernel, 256 tokens, 8 heads of 256, pages of 256 15 / 162, 512 times 8 rows, 4 of
+// 128 19 / 34. Old codes loaded beforehand, on their way with the values, did not pay: 1000 tokens, 8 heads of 128 64 -> 72).
+template <bool IS_V, int W>
 __device__ __forceinline__ void append_few(const float* __restrict__ x, int ld, int o0, int o1, int page, int hd,
                                            int8_t* codes, float* scale, float (*red)[4]) {
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, w = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = 64 * w + lane;
   const int nb = hd >> 5, blocks = (page >> 5) * nb, n = (o1 - o0) * hd;
   const int at = min(4 * tid, n - 4), row = at / hd, d = at - row * hd;
   const float4 y = *reinterpret_cast<const float4*>(x + (row * ld + d));
@@ -210,16 +217,16 @@ __device__ __forceinline__ void append_few(const float* __restrict__ x, int ld, 
     top = fmaxf(top, fabsf(z[e]));
     odd = __builtin_fmaf(z[e], 0.0f, odd);
   }
-  const PageScale sc = page_scale(top, odd, *scale, x, ld, o0, o1, hd, red);
+  const PageScale sc = page_scale<W>(top, odd, *scale, x, ld, o0, o1, hd, red);
   if (sc.grown) {
     uint4* const units = reinterpret_cast<uint4*>(codes) + lane;
-    for (int b0 = w; b0 < blocks; b0 += 16) {
+    for (int b0 = w; b0 < blocks; b0 += 4 * W) {
       uint4 old[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) old[i] = units[64 * min(b0 + 4 * i, blocks - 1)];
+      for (int i = 0; i < 4; ++i) old[i] = units[64 * min(b0 + W * i, blocks - 1)];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int blk = b0 + 4 * i, t = first_token<IS_V>(blk, nb);
+        const int blk = b0 + W * i, t = first_token<IS_V>(blk, nb);
         if (blk >= blocks) break;
         unsigned c[16], out[4];
 #pragma unroll
@@ -232,7 +239,8 @@ __device__ __forceinline__ void append_few(const float* __restrict__ x, int ld, 
         units[64 * blk] = make_uint4(out[0], out[1], out[2], out[3]);
       }
     }
-    __syncthreads();                       // the new codes come after
+    if constexpr (W == 1) wave_sync();     // the new codes come after
+    else __syncthreads();
   }
   if (tid == 0) *scale = sc.s;
   if (4 * tid >= n) return;
@@ -251,12 +259,18 @@ __device__ __forceinline__ void append_few(const float* __restrict__ x, int ld, 
   }
 }
 
-// One workgroup per (run of one request's new rows inside one page, head, K or V).
-template <int U>
-__global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache c, const float* __restrict__ k, int ldk,
-                                                         const float* __restrict__ v, int ldv) {
-  __shared__ float red[2][4];
-  const int u = blockIdx.x, head = blockIdx.y;
+// One workgroup per (run of one request's new rows inside one page, head or four heads, K or V).
+template <bool IS_V, int U>
+__device__ __forceinline__ void append_head(const float* __restrict__ x, int ld, int o0, int o1, int page, int hd,
+                                            int8_t* codes, float* scale, float (*red)[4]) {
+  if ((o1 - o0) * hd <= 1024) append_few<IS_V, 4>(x, ld, o0, o1, page, hd, codes, scale, red);
+  else append_page<IS_V, U>(x, ld, o0, o1, page, hd, codes, scale, red);
+}
+
+template <bool IS_V, int U, bool FOUR>
+__device__ __forceinline__ void append_run(const PagedBatch& b, const Kv8Cache& c, const float* __restrict__ x, int ld,
+                                           int8_t* codes, float* scale, float (*red)[4]) {
+  const int u = blockIdx.x;
   const RequestRows q = request_of_unit(u, b, b.page, 2);
   const int n = q.count, len = q.len, first = len - n;
   if (n == 0 || first < 0 || len > b.table_ld * b.page) return;
@@ -265,27 +279,51 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache 
   if (lo >= hi) return;
   const int pid = b.table[(size_t)q.req * b.table_ld + pi];
   if (pid < 0 || pid >= b.n_pages) return;
-  const int o0 = lo - pi * b.page, o1 = hi - pi * b.page;
-  const size_t row = q.row0 + lo - first, at = (size_t)pid * c.kv_heads + head, codes = at * b.page * c.hd;
-  const bool few = (o1 - o0) * c.hd <= kAppendFew;
-  if (blockIdx.z == 0) {
-    const float* x = k + row * ldk + head * c.hd;
-    if (few) append_few<false>(x, ldk, o0, o1, b.page, c.hd, c.k + codes, c.ks + at, red);
-    else append_page<false, U>(x, ldk, o0, o1, b.page, c.hd, c.k + codes, c.ks + at, red);
+  const int o0 = lo - pi * b.page, o1 = hi - pi * b.page, size = b.page * c.hd;
+  const size_t page0 = (size_t)pid * c.kv_heads;
+  x += (size_t)(q.row0 + lo - first) * ld;
+  if constexpr (!FOUR) {
+    const int h = blockIdx.y;
+    append_head<IS_V, U>(x + h * c.hd, ld, o0, o1, b.page, c.hd, codes + (page0 + h) * size, scale + page0 + h, red);
   } else {
-    const float* x = v + row * ldv + head * c.hd;
-    if (few) append_few<true>(x, ldv, o0, o1, b.page, c.hd, c.v + codes, c.vs + at, red);
-    else append_page<true, U>(x, ldv, o0, o1, b.page, c.hd, c.v + codes, c.vs + at, red);
+    const int h0 = 4 * blockIdx.y, h1 = min(h0 + 4, c.kv_heads);
+    if ((o1 - o0) * c.hd <= 256) {
+      const int h = h0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      if (h < h1)
+        append_few<IS_V, 1>(x + h * c.hd, ld, o0, o1, b.page, c.hd, codes + (page0 + h) * size, scale + page0 + h, red);
+      return;
+    }
+    for (int h = h0; h < h1; ++h) {
+      append_head<IS_V, U>(x + h * c.hd, ld, o0, o1, b.page, c.hd, codes + (page0 + h) * size, scale + page0 + h, red);
+      __syncthreads();
+    }
   }
+}
+
+template <int U, bool FOUR>
+__global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache c, const float* __restrict__ k, int ldk,
+                                                         const float* __restrict__ v, int ldv) {
+  __shared__ float red[2][4];
+  if (blockIdx.z == 0) append_run<false, U, FOUR>(b, c, k, ldk, c.k, c.ks, red);
+  else append_run<true, U, FOUR>(b, c, v, ldv, c.v, c.vs, red);
+}
+
+template <bool FOUR>
+static void launch_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,
+                          hipStream_t s) {
+  const dim3 grid((unsigned)(b.rows / b.page + 2 * b.requests), (unsigned)(FOUR ? (c.kv_heads + 3) / 4 : c.kv_heads), 2);
+  const int units = b.page * c.hd / 16;
+  auto* f = units <= 256 ? kv8_append_kernel<1, FOUR> : units <= 512 ? kv8_append_kernel<2, FOUR>
+          : units <= 1024 ? kv8_append_kernel<4, FOUR> : kv8_append_kernel<0, FOUR>;
+  hipLaunchKernelGGL(f, grid, dim3(256), 0, s, b, c, k, ldk, v, ldv);
 }
 
 hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,
                              hipStream_t s) {
-  const dim3 grid((unsigned)(b.rows / b.page + 2 * b.requests), (unsigned)c.kv_heads, 2);
-  const int units = b.page * c.hd / 16;
-  auto* f = units <= 256 ? kv8_append_kernel<1> : units <= 512 ? kv8_append_kernel<2> : units <= 1024 ? kv8_append_kernel<4>
-                                                                                           : kv8_append_kernel<0>;
-  hipLaunchKernelGGL(f, grid, dim3(256), 0, s, b, c, k, ldk, v, ldv);
+  // a token for each request at most on average: a wave per head, four to a workgroup (us of that / of a workgroup per head:
+  // 64 tokens, 4 heads of 128 4.0 / 4.8 in the kernel, 1000, 8 of 128 18 / 47, 4000, 2 of 64 25 / 42: starting workgroups)
+  if (b.rows <= b.requests) launch_append<true>(b, c, k, ldk, v, ldv, s);
+  else launch_append<false>(b, c, k, ldk, v, ldv, s);
   return hipGetLastError();
 }
 

@@ -90,6 +90,48 @@ def test_append_of_odd_values_in_large_pages():
     cache.check()
 
 
+@pytest.mark.parametrize("page,hd,kv_heads", [(32, 64, 5), (64, 128, 9), (256, 160, 3), (96, 256, 4), (64, 32, 1)])
+def test_append_of_a_decode_step_with_a_prompt_in_it(page, hd, kv_heads):
+    """No more rows than requests, but not one each: some idle, some with a few, one with more than a page; then tokens one by
+    one, with scales that grow and stay, infinities and NaN among them."""
+    rng = np.random.default_rng(page + hd)
+    n = 450
+    rows_of = np.zeros(n, int)
+    rows_of[[3, 7, 70, 200, 449]] = 1, 9, page + 40, 3, 1
+    rows_of[100:180] = 1
+    rows_of[300:306] = 2
+    len_of = rows_of + rng.integers(0, 2 * page, n)
+    bt = Batch(rng, rows_of, len_of, page, spare=2)
+    assert bt.rows <= n
+    cache = Cache(rng, bt.n_pages, kv_heads, page, hd)
+    for turn in range(4):
+        k, v = ((rng.standard_normal((bt.rows, kv_heads, hd)) * np.exp(2 * rng.standard_normal((bt.rows, kv_heads, 1))))
+                .astype(np.float32) for _ in range(2))
+        k[rng.integers(0, bt.rows, 5), 0, 3] = np.inf
+        v[rng.integers(0, bt.rows, 5), kv_heads - 1, hd - 1] = np.nan
+        append_both(cache, bt, k, v)
+        cache.check()
+        bt.len = np.minimum(bt.len + 1, bt.ld * page).astype(np.int32)
+        bt.count = np.minimum(bt.count, 1).astype(np.int32)
+
+
+@pytest.mark.parametrize("n", [64, 65, 200, 4096, 4097, 5000])
+def test_batches_of_many_requests(n):
+    """Requests on both sides of every step of the search for a request, most idle, unused rows among them."""
+    rng = np.random.default_rng(n)
+    rows_of = (rng.random(n) < 0.3) * rng.integers(1, 4, n)
+    rows_of[n - 1] = 2
+    bt = Batch(rng, rows_of, rows_of + rng.integers(0, 40, n), 32)
+    cache = Cache(rng, bt.n_pages, 1, 32, 32)
+    k, v = (rng.standard_normal((bt.rows, 1, 32)).astype(np.float32) for _ in range(2))
+    append_both(cache, bt, k, v)
+    cache.check()
+    q = rng.standard_normal((bt.rows, 20, 32)).astype(np.float32)   # (20 heads a row: tiles of one row or two)
+    cache.ks *= np.float32(0.02)
+    cache.upload()
+    check_attention(cache, bt, q, 0.2)
+
+
 # ---- offsets past 32 bits of rows ------------------------------------------------------------------
 def test_row_strides_past_32_bits():
     """Three rows 2^30 floats apart (the third begins at byte 2^33): log probabilities, rotary positions, attention."""
