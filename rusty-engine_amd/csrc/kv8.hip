@@ -402,11 +402,13 @@ __device__ __forceinline__ float column_sum(float v) {
 // grp heads (grp <= vecs), or vecs of the grp heads of one row (group_tiles of them).
 //   direct: no request has more than one tile. Its keys are cut into pieces of about the same size over all requests,
 //     `pieces` of them in all (and one more for each request), of at least kAttnMinSteps steps: a batch of lengths 1 ..
-//     16384 then takes the time of its sum, not of its longest request.
+//     16384 then takes the time of its sum, not of its longest request. Up to kAttnScanned requests every workgroup finds
+//     its piece from all the lengths; of more a launch before lists them (listed, at float `list` of the workspace).
 //   else: unit u is a tile, every tile is cut into `splits` pieces.
 // A head's pieces have `slots` places in the workspace, a tile's one behind the other, each of `used` vectors.
 struct AttnTiles {
-  int vecs, grp, rows_per, group_tiles, units, direct, splits, pieces, slots, used;
+  int vecs, grp, rows_per, group_tiles, units, direct, splits, pieces, slots, used, listed;
+  size_t list;
 };
 
 // A tile's place: request, rows, and the 32-key steps it has to walk, and their cut into splits.
@@ -419,6 +421,7 @@ struct AttnTile {
 
 constexpr int kAttnMaxSplits8 = 256;  // one thread of the join each
 constexpr int kAttnMinSteps = 16;     // steps of a split, at least (four waves take turns)
+constexpr int kAttnScanned = 256;     // one thread of a workgroup each
 
 // rows i0 .. of a request; false if it has none
 __device__ __forceinline__ bool place_tile(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t,
@@ -463,16 +466,35 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// The sum over a workgroup of 256 threads, and in `before` that of the threads below this one.
-__device__ __forceinline__ int scan256(int v, int& before) {
-  __shared__ int part[4];
+// The sum over a workgroup of WAVES waves, and in `before` that of the threads below this one.
+template <int WAVES>
+__device__ __forceinline__ int scan_block(int v, int& before) {
+  __shared__ int part[WAVES];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, inc = wave_scan(v);
   if (lane == 63) part[w] = inc;
   __syncthreads();
-  const int p0 = part[0], p1 = part[1], p2 = part[2], p3 = part[3];
+  int all = 0;
+  before = inc - v;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    before += i < w ? part[i] : 0;
+    all += part[i];
+  }
   __syncthreads();
-  before = inc - v + (w > 0 ? p0 : 0) + (w > 1 ? p1 : 0) + (w > 2 ? p2 : 0);
-  return p0 + p1 + p2 + p3;
+  return all;
+}
+// .. of floats, in one order
+template <int WAVES>
+__device__ __forceinline__ float sum_block(float v) {
+  __shared__ float part[WAVES];
+  v = wave_sum(v);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float all = 0.0f;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) all += part[i];
+  __syncthreads();
+  return all;
 }
 
 // The tile and split of workgroup `u` of a head; false if there is none.
@@ -488,7 +510,7 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
     return sp == 0 || sp * o.per < o.steps;
   }
   // steps of a piece over the whole batch, then the request that piece u falls into: up to 64 requests a lane of every
-  // wave each (nothing then goes through LDS), else some for each thread
+  // wave each (nothing then goes through LDS), else one for each thread
   if (b.requests <= 64) {
     const int i = threadIdx.x & 63, r = min(i, b.requests - 1);
     const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
@@ -505,48 +527,27 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
     o.slot = u - sp;
     return true;
   }
+  if (t.listed) {
+    const int4 e = reinterpret_cast<const int4*>(a.work + t.list)[u];
+    if (e.x < 0) return false;
+    place_request(b, a, t, e.x, o);
+    o.per = e.z;
+    sp = e.y;
+    o.slot = u - sp;
+    return true;
+  }
   __shared__ AttnTile found;
   __shared__ int found_sp;
-  __shared__ float sums[2][4];
-  const int chunk = (b.requests + 255) / 256, r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
-  float sum = 0.0f, live = 0.0f;
-  bool has = false;
-  for (int r = r0; r < r1; ++r) {
-    has = place_request(b, a, t, r, o);
-    sum += has ? (float)o.steps : 0.0f;
-    live += has ? 1.0f : 0.0f;
-  }
-  sum = wave_sum(sum);
-  live = wave_sum(live);
-  if ((threadIdx.x & 63) == 0) { sums[0][threadIdx.x >> 6] = sum; sums[1][threadIdx.x >> 6] = live; }
-  __syncthreads();
-  const int piece = piece_steps((sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]),
-                                (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]), t.pieces);
-  auto pieces_of = [&] {
-    o.per = max(piece, steps_per(o.steps, t.splits));
-    return has ? max(1, (o.steps + o.per - 1) / o.per) : 0;
-  };
-  int mine = 0;
-  if (chunk == 1) mine = pieces_of();
-  else
-    for (int r = r0; r < r1; ++r) {
-      has = place_request(b, a, t, r, o);
-      mine += pieces_of();
-    }
+  const int i = threadIdx.x;
+  const bool has = place_request(b, a, t, min(i, b.requests - 1), o) && i < b.requests;
+  const float sum = sum_block<4>(has ? (float)o.steps : 0.0f), live = sum_block<4>(has ? 1.0f : 0.0f);
+  o.per = max(piece_steps(sum, live, t.pieces), steps_per(o.steps, t.splits));
+  const int mine = has ? max(1, (o.steps + o.per - 1) / o.per) : 0;
   int before;
-  const int all = scan256(mine, before);
-  if (u >= all) return false;
+  if (u >= scan_block<4>(mine, before)) return false;
   if (u >= before && u < before + mine) {
-    int k = u - before;
-    if (chunk > 1)
-      for (int r = r0;; ++r) {
-        has = place_request(b, a, t, r, o);
-        const int n = pieces_of();
-        if (k < n) break;
-        k -= n;
-      }
     found = o;
-    found_sp = k;
+    found_sp = u - before;
   }
   __syncthreads();
   o = found;
@@ -555,8 +556,39 @@ __device__ __forceinline__ bool find_piece(const PagedBatch& b, const Attn8Args&
   return true;
 }
 
+// The list of pieces of a large batch: {request, split, steps per split} for each, request -1 behind the last. One
+// workgroup, every thread some requests that follow one another.
+__global__ __launch_bounds__(1024) void attention_kv8_pieces_kernel(PagedBatch b, Attn8Args a, AttnTiles t) {
+  int4* const list = reinterpret_cast<int4*>(a.work + t.list);
+  const int chunk = (b.requests + 1023) / 1024, r0 = threadIdx.x * chunk, r1 = min(r0 + chunk, b.requests);
+  AttnTile o;
+  float sum = 0.0f, live = 0.0f;
+  for (int r = r0; r < r1; ++r)
+    if (place_request(b, a, t, r, o)) {
+      sum += (float)o.steps;
+      live += 1.0f;
+    }
+  sum = sum_block<16>(sum);
+  live = sum_block<16>(live);
+  const int piece = piece_steps(sum, live, t.pieces);
+  auto pieces_of = [&](int r, int& per) {
+    if (!place_request(b, a, t, r, o)) return 0;
+    per = max(piece, steps_per(o.steps, t.splits));
+    return max(1, (o.steps + per - 1) / per);
+  };
+  int mine = 0, per = 0, at;
+  for (int r = r0; r < r1; ++r) mine += pieces_of(r, per);
+  const int all = scan_block<16>(mine, at);
+  for (int r = r0; r < r1; ++r) {
+    const int n = pieces_of(r, per);
+    for (int sp = 0; sp < n; ++sp, ++at)
+      if (at < t.slots) list[at] = make_int4(r, sp, per, 0);
+  }
+  for (int u = all + threadIdx.x; u < t.slots; u += 1024) list[u] = make_int4(-1, 0, 0, 0);
+}
+
 // The workspace holds (m, l) of every vector of every piece, then (16-byte aligned) their sums, then every unit's number
-// of splits and first place.
+// of splits and first place, then the list of pieces.
 __host__ __device__ inline size_t piece_vectors(const AttnTiles& t, int kv_heads) {
   return (size_t)kv_heads * t.group_tiles * t.slots * t.used;
 }
@@ -1022,6 +1054,9 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   t.splits = (int)std::max(1L, std::min({(long)most, cuts, (long)kAttnMaxSplits8}));
   t.slots = t.direct ? t.pieces + requests : t.units * t.splits;
   t.used = t.grp <= t.vecs ? t.rows_per * t.grp : t.vecs;
+  t.listed = t.direct && requests > kAttnScanned;
+  const size_t n = piece_vectors(t, kv_heads);
+  t.list = t.splits > 1 ? (sums_at(n) + n * hd + 2 * (size_t)t.units + 3) & ~(size_t)3 : 0;
   return t;
 }
 
@@ -1033,8 +1068,7 @@ size_t attention_kv8_workgroups(int rows, int requests, int max_rows, int max_le
 
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
   const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd);
-  const size_t n = piece_vectors(t, kv_heads);
-  return t.splits > 1 ? sums_at(n) + n * hd + 2 * (size_t)t.units : 0;
+  return t.list + (t.listed ? 4 * (size_t)t.slots : 0);
 }
 
 template <int NB>
@@ -1049,6 +1083,11 @@ hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const At
   const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.heads, c.kv_heads, c.hd);
   const unsigned heads = (unsigned)(c.kv_heads * t.group_tiles);
   const unsigned n = (unsigned)attn_workgroups(t, c.kv_heads);
+  if (t.listed) {
+    hipLaunchKernelGGL(attention_kv8_pieces_kernel, dim3(1), dim3(1024), 0, s, b, a, t);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   switch (c.hd / 32) {
     case 1: launch_attention_hd<1>(b, c, a, t, n, s); break;
     case 2: launch_attention_hd<2>(b, c, a, t, n, s); break;
