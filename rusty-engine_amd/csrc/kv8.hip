@@ -1024,7 +1024,9 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
 // the most groups of 16 vectors of a tile: their sums, 64 and 128 registers, leave a SIMD two waves
 constexpr int most_groups(int hd) { return hd <= 128 ? 4 : 2; }
 
-static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
+// (a window only ever makes the workspace smaller)
+static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int window, int heads, int kv_heads,
+                            int hd) {
   AttnTiles t;
   t.grp = heads / kv_heads;
   const long vecs = (long)max_rows * t.grp;
@@ -1044,30 +1046,38 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
     if (2 * vecs > t.vecs && (t.direct ? (long)requests * kv_heads * (max_len / 32) >= 16384 : tiles >= 1024)) break;
   }
   const long ht = (long)kv_heads * t.group_tiles;
-  const int most = (std::max(max_len, 1) + 32 * kAttnMinSteps - 1) / (32 * kAttnMinSteps);
+  long steps = (std::max(max_len, 1) + 31) / 32;                   // of the longest tile
+  if (window > 0) steps = std::min(steps, ((long)window + t.rows_per - 2) / 32 + 2);
   // two workgroups of a piece for each CU, four of heads up to 64, whose steps are half as many bytes on their way (us of
   // 512 / 1024 / 1536: one request of 131071 tokens, 8 heads of 128 50.5 / 53.7 / 56, 64 of up to 16384, 4 of 128 35.4 /
   // 41 / 42; but one of 131071, 2 of 64 17.5 / 16.8 / 16.8, 128 of up to 8000, 4 of 64 32.7 / 24.4 / 26.7, 300, 2 of 32
   // 31.5 / 24.4 / 25.0)
   t.pieces = (int)std::max(1L, (hd <= 64 ? 1024 : 512) / ht);
-  const long cuts = t.direct ? t.pieces : 1024 / (t.units * ht);
-  t.splits = (int)std::max(1L, std::min({(long)most, cuts, (long)kAttnMaxSplits8}));
+  // Prompts' tiles are cut into about three pieces for each CU; a cut in two that makes more than two for each CU does not pay
+  // (us of 1024 / 768 / 512: three prompts of 77 rows behind 1500 tokens, 8 heads of 128, 264 tiles 24.5 / 22.8 / 18.7, 50
+  // rows each behind 4000 of 4, 12 heads of 64, 192 tiles 18.2 / 18.7 / 19.3, 100 behind 20000, 104 tiles 45.8 / 45.0 / 48.8)
+  const long tiles = t.units * ht, cuts = t.direct ? t.pieces : tiles <= 256 ? 768 / tiles : 512 / tiles;
+  const long n = std::min({(steps + kAttnMinSteps - 1) / kAttnMinSteps, cuts, (long)kAttnMaxSplits8});
+  // The second launch takes 4 .. 6 us, a step of 32 keys about hd / 170 us of a wave: cut if it takes more than that off (us
+  // whole / cut: one row, 8 heads of 128, 544 tokens 11.1 / 13.6, 1024 13.5 / 14.1; 4 heads, 1500 17.6 / 14.4; 100 rows, 8
+  // heads of 128, 1000 tokens 15.4 / 20.4; one row, 8 heads of 256, 902 tokens 20.6 / 17.4)
+  t.splits = n > 1 && steps * hd * (n - 1) > 2816 * n ? (int)n : 1;
   t.slots = t.direct ? t.pieces + requests : t.units * t.splits;
   t.used = t.grp <= t.vecs ? t.rows_per * t.grp : t.vecs;
   t.listed = t.direct && requests > kAttnScanned;
-  const size_t n = piece_vectors(t, kv_heads);
-  t.list = t.splits > 1 ? (sums_at(n) + n * hd + 2 * (size_t)t.units + 3) & ~(size_t)3 : 0;
+  const size_t vectors = piece_vectors(t, kv_heads);
+  t.list = t.splits > 1 ? (sums_at(vectors) + vectors * hd + 2 * (size_t)t.units + 3) & ~(size_t)3 : 0;
   return t;
 }
 
 static size_t attn_workgroups(const AttnTiles& t, int kv_heads) { return (size_t)kv_heads * t.group_tiles * t.slots; }
 
 size_t attention_kv8_workgroups(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
-  return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd), kv_heads);
+  return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, 0, heads, kv_heads, hd), kv_heads);
 }
 
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
-  const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, heads, kv_heads, hd);
+  const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, 0, heads, kv_heads, hd);
   return t.list + (t.listed ? 4 * (size_t)t.slots : 0);
 }
 
@@ -1080,7 +1090,7 @@ static void launch_attention_hd(const PagedBatch& b, const Kv8Cache& c, const At
 }
 
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s) {
-  const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.heads, c.kv_heads, c.hd);
+  const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.window, a.heads, c.kv_heads, c.hd);
   const unsigned heads = (unsigned)(c.kv_heads * t.group_tiles);
   const unsigned n = (unsigned)attn_workgroups(t, c.kv_heads);
   if (t.listed) {
