@@ -602,18 +602,22 @@ __global__ __launch_bounds__(kLogJoin) void logprobs_join_kernel(LogprobArgs a, 
 
 // About three workgroups for each CU; a part is at least one batch of every wave (64 rows of 151936, top 20: 32.0 / 28.8
 // / 30.2 us at 256 / 768 / 1024 workgroups; 256 rows: 54.0 / 43.9 / 45.0).
-static int logprob_parts(int rows, int vocab) {
-  const int most = std::min((vocab + kLogPart - 1) / kLogPart, kLogMaxParts);
-  return std::max(1, std::min(most, 768 / std::max(rows, 1)));
+// The join's launch takes 3 us, a batch 0.2 and more with candidates: parts if they take more than that off (us whole / in
+// parts: one row of 32000, none 7.2 / 10.5, 20 best 22 / 12; 12289, 2 best 8.5 / 10.7; 12963, 17 best 15 / 11; 157 rows of
+// 29551, none 7.8 / 10.6, 4 best 19.4 / 15.1); two of them only of long rows (300 of 20000 20 / 23, 380 of 151936 50 / 47).
+static int logprob_parts(int rows, int vocab, int k) {
+  const int batches = (vocab + kLogPart - 1) / kLogPart;           // of a wave of a whole row
+  const int parts = std::min({batches, kLogMaxParts, 768 / std::max(rows, 1)});
+  return (parts > 2 || (parts == 2 && batches >= 16)) && (long)batches * (parts - 1) * (1 + k) > 20L * parts ? parts : 1;
 }
 
 size_t logprobs_work_floats(int rows, int vocab, int k) {
-  const int parts = logprob_parts(rows, vocab);
+  const int parts = logprob_parts(rows, vocab, k);
   return parts > 1 ? (size_t)rows * parts * (4 + 2 * k) : 0;
 }
 
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s) {
-  const int parts = logprob_parts(a.rows, a.vocab);
+  const int parts = logprob_parts(a.rows, a.vocab, a.k);
   // a wave per row where one batch is the row, or where rows alone fill the GPU's waves (us of a wave / a workgroup per
   // row, top 5 or 20: 4000 x 1000 11.8 / 25.8, 2000 x 32000 54 / 67, 8000 x 32000 176 / 238; but 1000 x 16000 31.5 / 26.9)
   if (a.vocab <= 64 * kLogBatch || a.rows >= 1536) {
