@@ -64,26 +64,29 @@ struct PageScale {
   float s, ratio, inverse;   // of old codes to new ones; 1 / s
   bool grown, plain;         // plain: every value is finite and the quotient may be taken by remainders
 };
+constexpr int kAppendWaves = 16;
+typedef float AppendRed[2][kAppendWaves];
+
 template <int W>
-__device__ __forceinline__ float append_max(float v, float (*red)[4]) {
-  v = wave_max(v);
-  if constexpr (W == 1) return v;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+__device__ __forceinline__ float largest_of(const float (&v)[kAppendWaves]) {
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) m = fmaxf(m, v[i]);
+  return m;
 }
 template <int W>
 __device__ __forceinline__ PageScale page_scale(float top, float odd, float s_old, const float* __restrict__ x, int ld,
-                                                int o0, int o1, int hd, float (*red)[4]) {
+                                                int o0, int o1, int hd, AppendRed& red) {
   const int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   top = wave_max(top);
   odd = wave_sum(odd);
   if constexpr (W > 1) {
     if ((tid & 63) == 0) { red[0][w] = top; red[1][w] = odd; }
     __syncthreads();
-    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    odd = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    top = largest_of<W>(red[0]);
+    odd = red[1][0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) odd += red[1][i];
   }
   if (odd != odd) {                        // the finite ones only
     top = 0.0f;
@@ -91,7 +94,13 @@ __device__ __forceinline__ PageScale page_scale(float top, float odd, float s_ol
       const float v = fabsf(x[e / hd * ld + e % hd]);
       if (v < INFINITY) top = fmaxf(top, v);
     }
-    top = append_max<W>(top, red);
+    top = wave_max(top);
+    if constexpr (W > 1) {
+      __syncthreads();
+      if ((tid & 63) == 0) red[0][w] = top;
+      __syncthreads();
+      top = largest_of<W>(red[0]);
+    }
   }
   if (o0 == 0) s_old = 0.0f;               // the page is begun: what it held before does not count
   float s = top * (1.0f / 127.0f);
@@ -105,10 +114,10 @@ __device__ __forceinline__ PageScale page_scale(float top, float odd, float s_ol
 // 16 codes that lie together in memory (K: 2 tokens x 8 dimensions, V: 8 tokens x 2), 64 lanes' units a block of 32 x 32:
 // it loads their values, and the codes of a page that is not all new, before the largest magnitude is known, so that all
 // of this is one round trip to memory. Units past the page's (U rounded up) repeat the last and are not stored.
-// U = 0: the units in turn, their values read twice.
-template <bool IS_V, int U>
+// U = 0 (a prompt of large pages in a decode step): the units in turn, their values read twice.
+template <bool IS_V, int U, int W>
 __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld, int o0, int o1, int page, int hd,
-                                            int8_t* codes, float* scale, float (*red)[4]) {
+                                            int8_t* codes, float* scale, AppendRed& red) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   const int nb = hd >> 5, blocks = (page >> 5) * nb;
   const bool all_new = o0 == 0 && o1 == page;
@@ -146,20 +155,20 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
   };
   if constexpr (U > 0) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) load(min(w + 4 * i, blocks - 1), y[i]);
+    for (int i = 0; i < U; ++i) load(min(w + W * i, blocks - 1), y[i]);
     if (!all_new) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) old[i] = units[64 * min(w + 4 * i, blocks - 1)];
+      for (int i = 0; i < U; ++i) old[i] = units[64 * min(w + W * i, blocks - 1)];
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) largest(y[i]);
   } else {
-    for (int blk = w; blk < blocks; blk += 4) {
+    for (int blk = w; blk < blocks; blk += W) {
       load(blk, y[0]);
       largest(y[0]);
     }
   }
-  const PageScale sc = page_scale<4>(top, odd, s_old, x, ld, o0, o1, hd, red);
+  const PageScale sc = page_scale<W>(top, odd, s_old, x, ld, o0, o1, hd, red);
   auto store = [&](int blk, const float (&z)[16], const uint4& was) {
     unsigned c[16], out[4];
     if (sc.plain) {
@@ -188,9 +197,9 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
   if constexpr (U > 0) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (w + 4 * i < blocks) store(w + 4 * i, y[i], old[i]);
+      if (w + W * i < blocks) store(w + W * i, y[i], old[i]);
   } else {
-    for (int blk = w; blk < blocks; blk += 4) {
+    for (int blk = w; blk < blocks; blk += W) {
       load(blk, y[0]);
       if (!all_new) old[0] = units[64 * blk];
       store(blk, y[0], old[0]);
@@ -205,7 +214,7 @@ __device__ __forceinline__ void append_page(const float* __restrict__ x, int ld,
 // 128 19 / 34. Old codes loaded beforehand, on their way with the values, did not pay: 1000 tokens, 8 heads of 128 64 -> 72).
 template <bool IS_V, int W>
 __device__ __forceinline__ void append_few(const float* __restrict__ x, int ld, int o0, int o1, int page, int hd,
-                                           int8_t* codes, float* scale, float (*red)[4]) {
+                                           int8_t* codes, float* scale, AppendRed& red) {
   const int lane = threadIdx.x & 63, w = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = 64 * w + lane;
   const int nb = hd >> 5, blocks = (page >> 5) * nb, n = (o1 - o0) * hd;
   const int at = min(4 * tid, n - 4), row = at / hd, d = at - row * hd;
@@ -260,16 +269,16 @@ __device__ __forceinline__ void append_few(const float* __restrict__ x, int ld, 
 }
 
 // One workgroup per (run of one request's new rows inside one page, head or four heads, K or V).
-template <bool IS_V, int U>
+template <bool IS_V, int U, int W>
 __device__ __forceinline__ void append_head(const float* __restrict__ x, int ld, int o0, int o1, int page, int hd,
-                                            int8_t* codes, float* scale, float (*red)[4]) {
-  if ((o1 - o0) * hd <= 1024) append_few<IS_V, 4>(x, ld, o0, o1, page, hd, codes, scale, red);
-  else append_page<IS_V, U>(x, ld, o0, o1, page, hd, codes, scale, red);
+                                            int8_t* codes, float* scale, AppendRed& red) {
+  if ((o1 - o0) * hd <= 256 * W) append_few<IS_V, W>(x, ld, o0, o1, page, hd, codes, scale, red);
+  else append_page<IS_V, U, W>(x, ld, o0, o1, page, hd, codes, scale, red);
 }
 
-template <bool IS_V, int U, bool FOUR>
+template <bool IS_V, int U, int W, bool FOUR>
 __device__ __forceinline__ void append_run(const PagedBatch& b, const Kv8Cache& c, const float* __restrict__ x, int ld,
-                                           int8_t* codes, float* scale, float (*red)[4]) {
+                                           int8_t* codes, float* scale, AppendRed& red) {
   const int u = blockIdx.x;
   const RequestRows q = request_of_unit(u, b, b.page, 2);
   const int n = q.count, len = q.len, first = len - n;
@@ -284,7 +293,7 @@ __device__ __forceinline__ void append_run(const PagedBatch& b, const Kv8Cache& 
   x += (size_t)(q.row0 + lo - first) * ld;
   if constexpr (!FOUR) {
     const int h = blockIdx.y;
-    append_head<IS_V, U>(x + h * c.hd, ld, o0, o1, b.page, c.hd, codes + (page0 + h) * size, scale + page0 + h, red);
+    append_head<IS_V, U, W>(x + h * c.hd, ld, o0, o1, b.page, c.hd, codes + (page0 + h) * size, scale + page0 + h, red);
   } else {
     const int h0 = 4 * blockIdx.y, h1 = min(h0 + 4, c.kv_heads);
     if ((o1 - o0) * c.hd <= 256) {
@@ -294,36 +303,46 @@ __device__ __forceinline__ void append_run(const PagedBatch& b, const Kv8Cache& 
       return;
     }
     for (int h = h0; h < h1; ++h) {
-      append_head<IS_V, U>(x + h * c.hd, ld, o0, o1, b.page, c.hd, codes + (page0 + h) * size, scale + page0 + h, red);
+      append_head<IS_V, U, W>(x + h * c.hd, ld, o0, o1, b.page, c.hd, codes + (page0 + h) * size, scale + page0 + h, red);
       __syncthreads();
     }
   }
 }
 
-template <int U, bool FOUR>
-__global__ __launch_bounds__(256) void kv8_append_kernel(PagedBatch b, Kv8Cache c, const float* __restrict__ k, int ldk,
-                                                         const float* __restrict__ v, int ldv) {
-  __shared__ float red[2][4];
-  if (blockIdx.z == 0) append_run<false, U, FOUR>(b, c, k, ldk, c.k, c.ks, red);
-  else append_run<true, U, FOUR>(b, c, v, ldv, c.v, c.vs, red);
+template <int U, int W, bool FOUR>
+__global__ __launch_bounds__(64 * W) void kv8_append_kernel(PagedBatch b, Kv8Cache c, const float* __restrict__ k, int ldk,
+                                                            const float* __restrict__ v, int ldv) {
+  __shared__ AppendRed red;
+  if (blockIdx.z == 0) append_run<false, U, W, FOUR>(b, c, k, ldk, c.k, c.ks, red);
+  else append_run<true, U, W, FOUR>(b, c, v, ldv, c.v, c.vs, red);
 }
 
-template <bool FOUR>
+template <int U, int W, bool FOUR>
 static void launch_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,
                           hipStream_t s) {
   const dim3 grid((unsigned)(b.rows / b.page + 2 * b.requests), (unsigned)(FOUR ? (c.kv_heads + 3) / 4 : c.kv_heads), 2);
-  const int units = b.page * c.hd / 16;
-  auto* f = units <= 256 ? kv8_append_kernel<1, FOUR> : units <= 512 ? kv8_append_kernel<2, FOUR>
-          : units <= 1024 ? kv8_append_kernel<4, FOUR> : kv8_append_kernel<0, FOUR>;
-  hipLaunchKernelGGL(f, grid, dim3(256), 0, s, b, c, k, ldk, v, ldv);
+  hipLaunchKernelGGL((kv8_append_kernel<U, W, FOUR>), grid, dim3(64 * W), 0, s, b, c, k, ldk, v, ldv);
 }
 
 hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float* k, int ldk, const float* v, int ldv,
                              hipStream_t s) {
+  const int units = b.page * c.hd / 16;
   // a token for each request at most on average: a wave per head, four to a workgroup (us of that / of a workgroup per head:
   // 64 tokens, 4 heads of 128 4.0 / 4.8 in the kernel, 1000, 8 of 128 18 / 47, 4000, 2 of 64 25 / 42: starting workgroups)
-  if (b.rows <= b.requests) launch_append<true>(b, c, k, ldk, v, ldv, s);
-  else launch_append<false>(b, c, k, ldk, v, ldv, s);
+  if (b.rows <= b.requests) {
+    if (units <= 256) launch_append<1, 4, true>(b, c, k, ldk, v, ldv, s);
+    else if (units <= 512) launch_append<2, 4, true>(b, c, k, ldk, v, ldv, s);
+    else if (units <= 1024) launch_append<4, 4, true>(b, c, k, ldk, v, ldv, s);
+    else launch_append<0, 4, true>(b, c, k, ldk, v, ldv, s);
+  } else {
+    // more waves for large pages, not units in turn (us: chunks of 737 rows of 11 requests, 4 heads of 256, pages of 128 17 /
+    // 26, of 300 of 4, 8 heads of 256, pages of 256 16 / 26); twice the waves with half the units each does as well
+    if (units <= 256) launch_append<1, 4, false>(b, c, k, ldk, v, ldv, s);
+    else if (units <= 512) launch_append<2, 4, false>(b, c, k, ldk, v, ldv, s);
+    else if (units <= 1024) launch_append<4, 4, false>(b, c, k, ldk, v, ldv, s);
+    else if (units <= 2048) launch_append<4, 8, false>(b, c, k, ldk, v, ldv, s);
+    else launch_append<4, 16, false>(b, c, k, ldk, v, ldv, s);
+  }
   return hipGetLastError();
 }
 
