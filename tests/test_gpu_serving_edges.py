@@ -132,6 +132,24 @@ def test_batches_of_many_requests(n):
     check_attention(cache, bt, q, 0.2)
 
 
+@pytest.mark.parametrize("n", [200, 300, 1100])
+@pytest.mark.parametrize("max_len", [4000, 60000])
+def test_many_requests_and_a_few_long_ones(n, max_len):
+    """Pieces of a few long requests among many short, idle and empty ones; few splits and many (planned for)."""
+    rng = np.random.default_rng(n)
+    len_of = rng.integers(1, 40, n)
+    len_of[[5, n // 2, n - 1]] = 4000, 2111, 1500
+    rows_of = (rng.random(n) < 0.6).astype(int)
+    rows_of[[5, n // 2, n - 1]] = 1
+    rows_of[7], len_of[7] = 1, 0                            # (a row before the first token)
+    bt, cache, q = make(rng, rows_of, len_of, 64, 6, 2, 64)
+    check_attention(cache, bt, q, 0.125, max_len=max_len)
+    check_attention(cache, bt, q, 0.125, 1000, max_len=max_len)
+    bt.count[:] = 0
+    bt.count[n // 2] = 1
+    check_attention(cache, bt, q, 0.125, max_len=max_len)
+
+
 # ---- offsets past 32 bits of rows ------------------------------------------------------------------
 def test_row_strides_past_32_bits():
     """Three rows 2^30 floats apart (the third begins at byte 2^33): log probabilities, rotary positions, attention."""
