@@ -503,8 +503,8 @@ class DeviceDecoder:
 
     Same computation as `DenseDecoder` (runner.rs:205-282, forward.rs:347-586). With kv_cache="int8" K and
     V are kept in int8 pages of 64 tokens with a scale for each page and KV head (a quarter of the f32
-    caches' memory, any max_seq): per layer bias, rotary positions, append and attention over the pages
-    are launches of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32).
+    caches' memory, any max_seq): per layer rotary positions, append and attention over the pages are launches
+    of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32).
     A prefill goes on at seq_len, also where that was set back: 0 begins a new sequence."""
 
     def __init__(self, mb: ModelBytes, max_seq: int, mode: int = MODE_F32, prefill_rows: int = 1024,
@@ -622,11 +622,10 @@ class DeviceDecoder:
                       work_bytes=self.work_bytes if rows < 8 else 0, stream=self.stream)
 
     def _paged_attention(self, blk, rows):
-        """int8 pages: bias, rotary positions, append and attention of the rows that the step's plan gave."""
-        from . import ROPE_HALF, add_dev, attention_kv8_dev, kv8_append_dev, rope_rows_dev
+        """int8 pages: rotary positions, append and attention of the rows that the step's plan gave."""
+        from . import ROPE_HALF, attention_kv8_dev, kv8_append_dev, rope_rows_dev
         g, d, kv, p, s = self.g, self.g.d_model, self.kv, self.pages, self.stream
         ld = d + 2 * kv
-        add_dev(self.qkv, blk["bias"], rows * ld, ld, self.qkv, s)
         rope_rows_dev(self.qkv, ld, rows, g.n_heads + g.n_kv_heads, g.head_dim, g.head_dim, ROPE_HALF, p.freqs, 1.0,
                       p.row_pos, self.qkv, ld, s)
         batch = (rows, 1, p.row_start, p.row_count, p.kv_len, p.table, p.count, p.PAGE, p.count, *blk["cache"])
@@ -649,7 +648,7 @@ class DeviceDecoder:
         if self.pages is not None:
             self.pages.plan(self.pages.one, 1, s)
         for blk in self.blocks:
-            blk["qkv"].matvec_ex_dev(self.x, self.qkv, norm_w=blk["attn_norm"], eps=eps, stream=s)
+            blk["qkv"].matvec_ex_dev(self.x, self.qkv, norm_w=blk["attn_norm"], eps=eps, add=blk.get("bias"), stream=s)
             if self.pages is None:
                 self._decode_attention(blk)
             else:
@@ -684,6 +683,7 @@ class DeviceDecoder:
                 self._qkv_post(blk, rows)
                 self._attention(blk, rows)
             else:
+                add_dev(self.qkv, blk["bias"], rows * (d + 2 * self.kv), d + 2 * self.kv, self.qkv, s)
                 self._paged_attention(blk, rows)
             blk["o"].matmul_dev(self.ctx, rows, self.ob, m, stream=s)
             add_dev(self.x, self.ob, rows * d, rows * d, self.x, s)
