@@ -422,11 +422,12 @@ __device__ __forceinline__ float column_sum(float v) {
 //   direct: no request has more than one tile. Its keys are cut into pieces of about the same size over all requests,
 //     `pieces` of them in all (and one more for each request), of at least kAttnMinSteps steps: a batch of lengths 1 ..
 //     16384 then takes the time of its sum, not of its longest request. Up to kAttnScanned requests every workgroup finds
-//     its piece from all the lengths; of more a launch before lists them (listed, at float `list` of the workspace).
+//     its piece from all the lengths; of more a launch before lists them (listed, at float `list` of the workspace), and with
+//     16 vectors a tile of short contexts a wave takes a piece alone, four to a workgroup (solo).
 //   else: unit u is a tile, every tile is cut into `splits` pieces.
 // A head's pieces have `slots` places in the workspace, a tile's one behind the other, each of `used` vectors.
 struct AttnTiles {
-  int vecs, grp, rows_per, group_tiles, units, direct, splits, pieces, slots, used, listed;
+  int vecs, grp, rows_per, group_tiles, units, direct, splits, pieces, slots, used, listed, solo;
   size_t list;
 };
 
@@ -638,11 +639,13 @@ constexpr int kAttnPages = 256;       // pages whose numbers and scales are stag
 // loads while the softmax and V's products run, the next V block while K's do. With one group its q stays in
 // registers; with more (prompts) the groups' q lies in LDS, in fragment order too, and every code is converted to f16
 // once for all of them.
-template <int NB, int VT>
+// SOLO (listed pieces, one group): every wave its own piece, no joins between waves.
+template <int NB, int VT, bool SOLO>
 __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
-  constexpr int HD = 32 * NB, LD = HD + 4;
-  __shared__ int ids[kAttnPages];
-  __shared__ float kss[kAttnPages], vss[kAttnPages];
+  constexpr int HD = 32 * NB, LD = HD + 4, kW = SOLO ? 1 : 4, kPages = SOLO ? kAttnPages / 4 : kAttnPages;
+  static_assert(!SOLO || VT == 1, "a wave alone has one group");
+  __shared__ int all_ids[kAttnPages];
+  __shared__ float all_kss[kAttnPages], all_vss[kAttnPages];
   __shared__ float Ms[4][16], Ls[4][16];
   constexpr size_t kQ = VT > 1 ? (size_t)VT * NB * 2 * 1024 : 0, kO = sizeof(float) * 4 * 16 * LD;
   __shared__ __attribute__((aligned(16))) char big[kQ > kO ? kQ : kO];    // q, and after the steps the waves' sums
@@ -651,12 +654,21 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   __shared__ float qss[VT][16];
   AttnTile tile;
   const int ht = c.kv_heads * t.group_tiles, yy = blockIdx.x % ht;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = SOLO ? 0 : wave, tid = SOLO ? lane : threadIdx.x;            // within the piece
+  const int u = blockIdx.x / ht * (4 / kW) + (SOLO ? wave : 0);
   int sp;
-  if (!find_piece(b, a, t, blockIdx.x / ht, tile, sp)) return;
+  if (u >= t.slots || !find_piece(b, a, t, u, tile, sp)) return;
+  int* const ids = all_ids + (SOLO ? kPages * wave : 0);
+  float* const kss = all_kss + (SOLO ? kPages * wave : 0);
+  float* const vss = all_vss + (SOLO ? kPages * wave : 0);
+  auto sync = [] {
+    if constexpr (SOLO) wave_sync();
+    else __syncthreads();
+  };
   tile = uniform(tile);
   sp = __builtin_amdgcn_readfirstlane(sp);
   const int head = yy / t.group_tiles, g0 = (yy % t.group_tiles) * t.vecs;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int s0 = tile.first + sp * tile.per, s1 = min(s0 + tile.per, tile.first + tile.steps);
   // every vector of the tile sees the keys see_from .. see_all (a place without one may see anything: it is not stored)
@@ -746,20 +758,20 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     for (int k = 0; k < NB; ++k) o[v][k][0] = o[v][k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   bool huge = false;                     // some vector's m is beyond 2^20
-  for (int pg0 = page0; pg0 * page_steps < s1; pg0 += kAttnPages) {
+  for (int pg0 = page0; pg0 * page_steps < s1; pg0 += kPages) {
     // the pages of these steps: their numbers and scales
     if (pg0 != page0) {
       my_page = entry(min(pg0 + tid, page_last));
       my_ks = c.ks[(size_t)max(my_page, 0) * c.kv_heads + head];
       my_vs = c.vs[(size_t)max(my_page, 0) * c.kv_heads + head];
-      __syncthreads();                   // the pages before have been read
+      sync();                            // the pages before have been read
     }
     ids[tid] = my_page;
     kss[tid] = my_page >= 0 ? my_ks : 0.0f;
     vss[tid] = my_page >= 0 ? my_vs : 0.0f;
-    __syncthreads();
+    sync();
     // steps from here on count from page pg0's first (below kAttnPages * 8): the quotient by page_steps is exact
-    const int c0 = pg0 * page_steps, e0 = max(s0 - c0, 0), e1 = min(s1 - c0, kAttnPages * page_steps);
+    const int c0 = pg0 * page_steps, e0 = max(s0 - c0, 0), e1 = min(s1 - c0, kPages * page_steps);
     auto page_of = [&](int s) { return (int)((unsigned)s * page_inv >> 16); };
     auto next_block = [&](const int8_t* base, int s) {
       const int pi = page_of(s);
@@ -770,8 +782,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       load(next_block(c.k, s), kf);
       load(next_block(c.v, s), vf);
     }
-    for (; s < e1; s += 4) {
-      const int next = min(s + 4, e1 - 1);
+    for (; s < e1; s += kW) {
+      const int next = min(s + kW, e1 - 1);
       const int pi = page_of(s), key0 = 32 * (s + c0);
       const bool have = ids[pi] >= 0;
       const float ks = kss[pi], vs = vss[pi];
@@ -874,13 +886,14 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       load(next_block(c.v, next), vf);
     }
   }
-  // the four waves' (m, l, O) joined in wave order, group after group
+  // the waves' (m, l, O) joined in wave order, group after group
   const bool whole = tile.steps <= tile.per;                      // one split: nothing left to join
   if (t.splits > 1 && sp == 0 && yy == 0 && tid == 0)
     splits_at(a, t, c.kv_heads, HD)[t.direct ? tile.req : tile.row0 / t.rows_per + tile.req + tile.i0 / t.rows_per] =
         make_int2((tile.steps + tile.per - 1) / tile.per, tile.slot);
   const size_t place = place_of(t, tile, yy) + (size_t)sp * t.used;
   float* const sums = a.work + sums_at(piece_vectors(t, c.kv_heads));
+  const int first_wave = SOLO ? wave : 0;
 #pragma unroll
   for (int v = 0; v < VT; ++v) {
     const float lv = column_sum(l[v]);
@@ -889,39 +902,44 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     for (int k = 0; k < NB; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float4*>(&Os[w][col][32 * k + 16 * h + 4 * g]) =
+        *reinterpret_cast<float4*>(&Os[wave][col][32 * k + 16 * h + 4 * g]) =
             make_float4(o[v][k][h][0], o[v][k][h][1], o[v][k][h][2], o[v][k][h][3]);
-    if (g == 0) { Ms[w][col] = m[v]; Ls[w][col] = lv; }
-    __syncthreads();
-    const int vec = tid >> 4, oi = row_of(16 * v + vec), oh = head_of(16 * v + vec);
-    if (oi >= tile.i1 || oh >= t.grp) continue;
-    const float M = fmaxf(fmaxf(Ms[0][vec], Ms[1][vec]), fmaxf(Ms[2][vec], Ms[3][vec]));
-    float f[4], L = 0.0f;
+    if (g == 0) { Ms[wave][col] = m[v]; Ls[wave][col] = lv; }
+    sync();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      // (a wave that saw nothing: m = -inf, l = 0 and O = 0, unless the vector holds NaN)
-      f[k] = Ms[k][vec] == M ? 1.0f : pow2(Ms[k][vec] - M);
-      L = __builtin_fmaf(Ls[k][vec], f[k], L);
-    }
-    const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh;
-    const float inv = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
-    const size_t mine = place + 16 * v + vec;
-    float* out = whole ? a.ctx + at * HD : sums + mine * HD;
-    for (int d = 4 * (tid & 15); d < HD; d += 64) {
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int vec = tid >> 4; vec < 16; vec += 4 * kW) {
+      const int oi = row_of(16 * v + vec), oh = head_of(16 * v + vec);
+      if (oi >= tile.i1 || oh >= t.grp) continue;
+      float M = Ms[first_wave][vec];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 x = *reinterpret_cast<const float4*>(&Os[k][vec][d]);
-        y.x = __builtin_fmaf(x.x, f[k], y.x);
-        y.y = __builtin_fmaf(x.y, f[k], y.y);
-        y.z = __builtin_fmaf(x.z, f[k], y.z);
-        y.w = __builtin_fmaf(x.w, f[k], y.w);
+      for (int k = 1; k < kW; ++k) M = fmaxf(M, Ms[k][vec]);
+      float f[kW], L = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kW; ++k) {
+        // (a wave that saw nothing: m = -inf, l = 0 and O = 0, unless the vector holds NaN)
+        const float mk = Ms[first_wave + k][vec];
+        f[k] = mk == M ? 1.0f : pow2(mk - M);
+        L = __builtin_fmaf(Ls[first_wave + k][vec], f[k], L);
       }
-      *reinterpret_cast<float4*>(out + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-    }
-    if (!whole && (tid & 15) == 0) {
-      a.work[2 * mine] = M;
-      a.work[2 * mine + 1] = L;
+      const size_t at = (size_t)(tile.row0 + oi) * a.heads + (size_t)head * t.grp + oh, mine = place + 16 * v + vec;
+      const float inv = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
+      float* out = whole ? a.ctx + at * HD : sums + mine * HD;
+      for (int d = 4 * (tid & 15); d < HD; d += 64) {
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kW; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(&Os[first_wave + k][vec][d]);
+          y.x = __builtin_fmaf(x.x, f[k], y.x);
+          y.y = __builtin_fmaf(x.y, f[k], y.y);
+          y.z = __builtin_fmaf(x.z, f[k], y.z);
+          y.w = __builtin_fmaf(x.w, f[k], y.w);
+        }
+        *reinterpret_cast<float4*>(out + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+      }
+      if (!whole && (tid & 15) == 0) {
+        a.work[2 * mine] = M;
+        a.work[2 * mine + 1] = L;
+      }
     }
   }
 }
@@ -1065,13 +1083,18 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
     if (2 * vecs > t.vecs && (t.direct ? (long)requests * kv_heads * (max_len / 32) >= 16384 : tiles >= 1024)) break;
   }
   const long ht = (long)kv_heads * t.group_tiles;
+  t.listed = t.direct && requests > kAttnScanned;
+  // a wave for each short request: there are enough of them, and most of a workgroup's four waves would have no step (us of a
+  // wave / four: 1000 requests of up to 64 tokens, 8 heads of 128 39 / 79, of up to 500 74 / 96, 500 of up to 2000, 4 of 256
+  // 97 / 99, 8 of 64 52 / 55; but 1000 of up to 4096, 8 of 128 268 / 247, 300 of up to 16384 303 / 277)
+  t.solo = t.listed && t.vecs == 16 && max_len <= 2048;
   long steps = (std::max(max_len, 1) + 31) / 32;                   // of the longest tile
   if (window > 0) steps = std::min(steps, ((long)window + t.rows_per - 2) / 32 + 2);
   // two workgroups of a piece for each CU, four of heads up to 64, whose steps are half as many bytes on their way (us of
   // 512 / 1024 / 1536: one request of 131071 tokens, 8 heads of 128 50.5 / 53.7 / 56, 64 of up to 16384, 4 of 128 35.4 /
   // 41 / 42; but one of 131071, 2 of 64 17.5 / 16.8 / 16.8, 128 of up to 8000, 4 of 64 32.7 / 24.4 / 26.7, 300, 2 of 32
   // 31.5 / 24.4 / 25.0)
-  t.pieces = (int)std::max(1L, (hd <= 64 ? 1024 : 512) / ht);
+  t.pieces = (int)std::max(1L, (hd <= 64 ? 1024 : 512) * (t.solo ? 4 : 1) / ht);
   // Prompts' tiles are cut into about three pieces for each CU; a cut in two that makes more than two for each CU does not pay
   // (us of 1024 / 768 / 512: three prompts of 77 rows behind 1500 tokens, 8 heads of 128, 264 tiles 24.5 / 22.8 / 18.7, 50
   // rows each behind 4000 of 4, 12 heads of 64, 192 tiles 18.2 / 18.7 / 19.3, 100 behind 20000, 104 tiles 45.8 / 45.0 / 48.8)
@@ -1083,13 +1106,14 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   t.splits = n > 1 && steps * hd * (n - 1) > 2816 * n ? (int)n : 1;
   t.slots = t.direct ? t.pieces + requests : t.units * t.splits;
   t.used = t.grp <= t.vecs ? t.rows_per * t.grp : t.vecs;
-  t.listed = t.direct && requests > kAttnScanned;
   const size_t vectors = piece_vectors(t, kv_heads);
   t.list = t.splits > 1 ? (sums_at(vectors) + vectors * hd + 2 * (size_t)t.units + 3) & ~(size_t)3 : 0;
   return t;
 }
 
-static size_t attn_workgroups(const AttnTiles& t, int kv_heads) { return (size_t)kv_heads * t.group_tiles * t.slots; }
+static size_t attn_workgroups(const AttnTiles& t, int kv_heads) {
+  return (size_t)kv_heads * t.group_tiles * (t.solo ? (t.slots + 3) / 4 : t.slots);
+}
 
 size_t attention_kv8_workgroups(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
   return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, 0, heads, kv_heads, hd), kv_heads);
@@ -1103,8 +1127,8 @@ size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_l
 template <int NB>
 static void launch_attention_hd(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, const AttnTiles& t,
                                 unsigned workgroups, hipStream_t s) {
-  auto* k = t.vecs == 16 ? attention_kv8_kernel<NB, 1> : t.vecs == 32 ? attention_kv8_kernel<NB, 2>
-                                                                      : attention_kv8_kernel<NB, most_groups(32 * NB)>;
+  auto* k = t.solo ? attention_kv8_kernel<NB, 1, true> : t.vecs == 16 ? attention_kv8_kernel<NB, 1, false>
+          : t.vecs == 32 ? attention_kv8_kernel<NB, 2, false> : attention_kv8_kernel<NB, most_groups(32 * NB), false>;
   hipLaunchKernelGGL(k, dim3(workgroups), dim3(256), 0, s, b, c, a, t);
 }
 

@@ -133,16 +133,16 @@ def test_batches_of_many_requests(n):
 
 
 @pytest.mark.parametrize("n", [200, 300, 1100])
-@pytest.mark.parametrize("max_len", [4000, 60000])
-def test_many_requests_and_a_few_long_ones(n, max_len):
-    """Pieces of a few long requests among many short, idle and empty ones; few splits and many (planned for)."""
+@pytest.mark.parametrize("page,max_len", [(64, 4000), (64, 60000), (64, 2000), (32, 500)])
+def test_many_requests_and_a_few_long_ones(n, page, max_len):
+    """Pieces of a few long requests among many short, idle and empty ones; few splits, many and none (planned for)."""
     rng = np.random.default_rng(n)
     len_of = rng.integers(1, 40, n)
     len_of[[5, n // 2, n - 1]] = 4000, 2111, 1500
     rows_of = (rng.random(n) < 0.6).astype(int)
     rows_of[[5, n // 2, n - 1]] = 1
     rows_of[7], len_of[7] = 1, 0                            # (a row before the first token)
-    bt, cache, q = make(rng, rows_of, len_of, 64, 6, 2, 64)
+    bt, cache, q = make(rng, rows_of, len_of, page, 6, 2, 64)
     check_attention(cache, bt, q, 0.125, max_len=max_len)
     check_attention(cache, bt, q, 0.125, 1000, max_len=max_len)
     bt.count[:] = 0
@@ -293,6 +293,21 @@ def test_rope_at_the_last_positions():
 
 
 # ---- wide tiles ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,kv_heads,hd", [(14, 2, 64), (5, 1, 32), (40, 2, 96), (16, 2, 256), (3, 3, 160)])
+def test_waves_alone(heads, kv_heads, hd):
+    """Many short requests, a wave each: odd queries, holes, windows, groups of more heads than a tile has vectors."""
+    rng = np.random.default_rng(hd)
+    n = 270
+    len_of = rng.integers(0, 70, n)
+    len_of[::50] = rng.integers(300, 600, 6)
+    bt, cache, q = make(rng, np.ones(n, int), len_of, 32, heads, kv_heads, hd, gap=1)
+    live = np.flatnonzero(len_of > 0)
+    q[bt.start[live[0]], 0, 3], q[bt.start[live[1]], heads - 1, 0], q[bt.start[live[2]]] = np.nan, np.inf, 0
+    bt.table[live[3], 0], bt.table[live[4]] = -1, bt.n_pages
+    check_attention(cache, bt, q, hd ** -0.5, max_len=600)
+    check_attention(cache, bt, q, -hd ** -0.5, 40, max_len=1500)
+
+
 def test_odd_queries_in_wide_tiles():
     """Tiles of 64 vectors with queries of NaN, infinities, zeros and huge scores: each spoils its own row and head only,
     and scores past 2^20 keep their neighbours' precision."""
