@@ -1084,10 +1084,11 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   }
   const long ht = (long)kv_heads * t.group_tiles;
   t.listed = t.direct && requests > kAttnScanned;
-  // a wave for each short request: there are enough of them, and most of a workgroup's four waves would have no step (us of a
-  // wave / four: 1000 requests of up to 64 tokens, 8 heads of 128 39 / 79, of up to 500 74 / 96, 500 of up to 2000, 4 of 256
-  // 97 / 99, 8 of 64 52 / 55; but 1000 of up to 4096, 8 of 128 268 / 247, 300 of up to 16384 303 / 277)
-  t.solo = t.listed && t.vecs == 16 && max_len <= 2048;
+  // A wave for each short request where there are enough of them: most of a workgroup's four waves would have no step, but a
+  // wave alone takes four times as long (us of a wave / four: 1000 requests of up to 64 tokens, 8 heads of 128 39 / 79, of up
+  // to 500 74 / 96, 300 of up to 64, 4 heads 15.2 / 20.5; but of up to 500 27 / 24, 500 of up to 500, 2 of 64 21 / 16, 1000 of
+  // up to 4096, 8 of 128 268 / 247)
+  t.solo = t.listed && t.vecs == 16 && max_len <= 2048 && requests * ht >= 4L * max_len;
   long steps = (std::max(max_len, 1) + 31) / 32;                   // of the longest tile
   if (window > 0) steps = std::min(steps, ((long)window + t.rows_per - 2) / 32 + 2);
   // two workgroups of a piece for each CU, four of heads up to 64, whose steps are half as many bytes on their way (us of
