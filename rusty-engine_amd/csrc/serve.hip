@@ -507,7 +507,9 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
   }
   s = wave_join(s);
   if constexpr (TOP) {
-    if (c.n > 64) c.keep_best();           // (k at most 64: a workgroup's lists then have a thread per key)
+    // (k at most 64: a workgroup's lists then have a thread per key. Longer lists of a small k would be ranked against each
+    // other below: 300 rows of 20000, 5 best 17.7 us instead of 16.6)
+    if (c.n > min(a.k + 8, 64)) c.keep_best();
   }
   if constexpr (SHORT) {
     if (TOP && lane < kPad) c.list[c.n + lane] = 0;
