@@ -505,7 +505,7 @@ class DeviceDecoder:
     V are kept in int8 pages of 64 tokens with a scale for each page and KV head (a quarter of the f32
     caches' memory, any max_seq): per layer rotary positions, append and attention over the pages are launches
     of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32).
-    A prefill goes on at seq_len, also where that was set back: 0 begins a new sequence."""
+    Prefills and steps go on at seq_len, also where that was set back: 0 begins a new sequence."""
 
     def __init__(self, mb: ModelBytes, max_seq: int, mode: int = MODE_F32, prefill_rows: int = 1024,
                  use_graph: bool = True, kv_cache: str = "f32"):
@@ -568,7 +568,25 @@ class DeviceDecoder:
             self.rope = B(max_seq * hd * 4)
             rope_table_dev(g.rope_freq_base, hd, max_seq, self.rope, self.stream)
         self.graph = None
-        self.seq_len = 0
+        self._seq_len = 0
+
+    @property
+    def seq_len(self) -> int:
+        """Tokens that the sequence holds. Setting it takes the sequence back to its first ones (0: a new sequence),
+        position and pages with it: the next prefill or step goes on there (a step decodes the token in `tok`, as
+        before). A part-filled int8 page keeps the scale that the tokens behind had raised."""
+        return self._seq_len
+
+    @seq_len.setter
+    def seq_len(self, length: int) -> None:
+        most = self.max_seq if self.pages is None else self._seq_len     # (int8 pages behind have no codes yet)
+        if not 0 <= length <= most:
+            raise ValueError(f"DeviceDecoder: seq_len {length} of a sequence of {self._seq_len} (0 .. {most})")
+        self.stream.synchronize()
+        self.pos.upload(np.array([length], np.int32))
+        if self.pages is not None:
+            self.pages.go_to(length)
+        self._seq_len = int(length)
 
     @staticmethod
     def _check_supported(mb: ModelBytes) -> None:
@@ -696,7 +714,7 @@ class DeviceDecoder:
         """Batched prefill of the prompt (runner.rs:236-260); returns the first greedy token."""
         rows = self._forward_rows(prompt)
         self._head_and_advance(_Offset(self.x, (rows - 1) * self.g.d_model * 4), rows)
-        self.seq_len += rows
+        self._seq_len += rows
         self.stream.synchronize()
         return int(self.tok.download(np.int32, 1)[0])
 
@@ -729,7 +747,7 @@ class DeviceDecoder:
                          at(out["ids"], r * top_k) if top_k else None, at(out["top"], r * top_k) if top_k else None,
                          work, nbytes, s)
         self._head_and_advance(_Offset(self.x, (rows - 1) * d * 4), rows)
-        self.seq_len += rows
+        self._seq_len += rows
         s.synchronize()
         got = {k: b.download(np.int32 if k == "ids" else np.float32, rows * (top_k if k in ("ids", "top") else 1))
                for k, b in out.items()}
@@ -752,7 +770,7 @@ class DeviceDecoder:
             self._step_body()
         else:
             self._graph().launch()
-        self.seq_len += 1
+        self._seq_len += 1
         self.stream.synchronize()
         return int(self.tok.download(np.int32, 1)[0])
 
@@ -767,7 +785,7 @@ class DeviceDecoder:
                 self._graph().launch()
             else:
                 self._step_body()
-        self.seq_len += steps
+        self._seq_len += steps
         self.stream.synchronize()
 
     def history(self, start: int, count: int) -> list:
