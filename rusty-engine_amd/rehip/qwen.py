@@ -569,6 +569,7 @@ class DeviceDecoder:
             rope_table_dev(g.rope_freq_base, hd, max_seq, self.rope, self.stream)
         self.graph = None
         self._seq_len = 0
+        self._whole = True                 # no call ended on its way since the last one that came through
 
     @property
     def seq_len(self) -> int:
@@ -587,6 +588,18 @@ class DeviceDecoder:
         if self.pages is not None:
             self.pages.go_to(length)
         self._seq_len = int(length)
+        self._whole = True
+
+    def _begin(self) -> None:
+        """Before a call's launches: after one that raised on its way, the device goes back to what the host counted
+        (the plan of int8 pages moves before the layers run)."""
+        if not self._whole:
+            self.seq_len = self._seq_len
+        self._whole = False
+
+    def _done(self, rows: int) -> None:
+        self._seq_len += rows
+        self._whole = True
 
     @staticmethod
     def _check_supported(mb: ModelBytes) -> None:
@@ -688,10 +701,10 @@ class DeviceDecoder:
             raise ValueError(f"prefill of {rows} rows at position {self.seq_len} (cap {self.cap}, max_seq {self.max_seq})")
         if prompt.min() < 0 or prompt.max() >= self.mb.n_vocab:
             raise ValueError("prompt token outside the vocabulary")
+        self._begin()
         self.toks.upload(prompt)
         embed_dev(self.embed, self.mb.n_vocab, d, self.toks, rows, self.x, s)
         if self.pages is not None:
-            self.pages.go_to(self.seq_len)
             self.pages.new.upload(np.array([rows], np.int32))
             self.pages.plan(self.pages.new, rows, s)
         for blk in self.blocks:
@@ -714,7 +727,7 @@ class DeviceDecoder:
         """Batched prefill of the prompt (runner.rs:236-260); returns the first greedy token."""
         rows = self._forward_rows(prompt)
         self._head_and_advance(_Offset(self.x, (rows - 1) * self.g.d_model * 4), rows)
-        self._seq_len += rows
+        self._done(rows)
         self.stream.synchronize()
         return int(self.tok.download(np.int32, 1)[0])
 
@@ -747,7 +760,7 @@ class DeviceDecoder:
                          at(out["ids"], r * top_k) if top_k else None, at(out["top"], r * top_k) if top_k else None,
                          work, nbytes, s)
         self._head_and_advance(_Offset(self.x, (rows - 1) * d * 4), rows)
-        self._seq_len += rows
+        self._done(rows)
         s.synchronize()
         got = {k: b.download(np.int32 if k == "ids" else np.float32, rows * (top_k if k in ("ids", "top") else 1))
                for k, b in out.items()}
@@ -762,15 +775,19 @@ class DeviceDecoder:
             self.graph = hip.Graph(self.stream, self._step_body)
         return self.graph
 
+    def _decode_one(self) -> None:
+        self._begin()
+        if self.use_graph:
+            self._graph().launch()
+        else:
+            self._step_body()
+        self._done(1)
+
     def step(self) -> int:
         """Decode the token in *tok at the next position; returns the following greedy token."""
         if self.seq_len >= self.max_seq:
             raise ValueError(f"decode past max_seq {self.max_seq}")
-        if not self.use_graph:
-            self._step_body()
-        else:
-            self._graph().launch()
-        self._seq_len += 1
+        self._decode_one()
         self.stream.synchronize()
         return int(self.tok.download(np.int32, 1)[0])
 
@@ -781,11 +798,7 @@ class DeviceDecoder:
         if self.seq_len + steps > self.max_seq:
             raise ValueError(f"decode past max_seq {self.max_seq}")
         for _ in range(steps):
-            if self.use_graph:
-                self._graph().launch()
-            else:
-                self._step_body()
-        self._seq_len += steps
+            self._decode_one()
         self.stream.synchronize()
 
     def history(self, start: int, count: int) -> list:

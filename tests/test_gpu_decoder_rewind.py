@@ -87,3 +87,27 @@ def test_positions_that_the_sequence_does_not_have(tiny):
         assert dd.seq_len == 20
         dd.seq_len = 20
         dd.close()
+
+
+@pytest.mark.parametrize("kv_cache", ["f32", "int8"])
+def test_calls_that_fail_leave_the_sequence(tiny, kv_cache, monkeypatch):
+    """A prefill and a scoring that raise on their way (no memory, say): the next step goes on where the sequence was."""
+    import rehip
+    prompt = np.random.default_rng(52).integers(0, 1000, 64)
+    dd = decoder(tiny, kv_cache)
+    t0 = dd.prefill(prompt)
+    want = [dd.step() for _ in range(5)]
+    logits = dd.logits()
+    for call, name in ((dd.prefill, "add_dev"), (dd.score, "logprobs_dev")):
+        dd.seq_len = 64
+        with monkeypatch.context() as m:
+            def fail(*a, **k):
+                raise RuntimeError("no memory")
+            m.setattr(rehip, name, fail)
+            with pytest.raises(RuntimeError):
+                call(prompt[:30])
+        assert dd.seq_len == 64
+        token(dd, t0)
+        assert [dd.step() for _ in range(5)] == want
+        np.testing.assert_array_equal(dd.logits(), logits)
+    dd.close()
