@@ -504,7 +504,8 @@ class DeviceDecoder:
     Same computation as `DenseDecoder` (runner.rs:205-282, forward.rs:347-586). With kv_cache="int8" K and
     V are kept in int8 pages of 64 tokens with a scale for each page and KV head (a quarter of the f32
     caches' memory, any max_seq): per layer rotary positions, append and attention over the pages are launches
-    of their own, planned on the device, in prefill and decode alike (head_dim a multiple of 32).
+    of their own, planned on the device, in prefill and decode alike (head_dim a
+    multiple of 32, prefills of up to 262144 rows).
     Prefills and steps go on at seq_len, also where that was set back: 0 begins a new sequence."""
 
     def __init__(self, mb: ModelBytes, max_seq: int, mode: int = MODE_F32, prefill_rows: int = 1024,
@@ -697,8 +698,9 @@ class DeviceDecoder:
         d = g.d_model
         prompt = np.asarray(prompt, np.int32)
         rows = prompt.size
-        if not (0 < rows <= self.cap and self.seq_len + rows <= self.max_seq):
-            raise ValueError(f"prefill of {rows} rows at position {self.seq_len} (cap {self.cap}, max_seq {self.max_seq})")
+        cap = self.cap if self.pages is None else min(self.cap, self.pages.MOST_ROWS)
+        if not (0 < rows <= cap and self.seq_len + rows <= self.max_seq):
+            raise ValueError(f"prefill of {rows} rows at position {self.seq_len} (cap {cap}, max_seq {self.max_seq})")
         if prompt.min() < 0 or prompt.max() >= self.mb.n_vocab:
             raise ValueError("prompt token outside the vocabulary")
         self._begin()
@@ -839,6 +841,7 @@ class _Int8Pages:
     """One sequence's pages of the int8 K/V cache and the plan of its steps, on the device; the layers' codes
     and scales share the page table."""
     PAGE = 64
+    MOST_ROWS = 1 << 18                    # of a prefill: the plan refuses more new tokens of a request
 
     def __init__(self, mb: ModelBytes, max_seq: int, cap: int):
         from . import attention_kv8_work_bytes, rope_freqs

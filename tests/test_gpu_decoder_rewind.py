@@ -111,3 +111,26 @@ def test_calls_that_fail_leave_the_sequence(tiny, kv_cache, monkeypatch):
         assert [dd.step() for _ in range(5)] == want
         np.testing.assert_array_equal(dd.logits(), logits)
     dd.close()
+
+
+def test_prefills_past_what_a_plan_takes():
+    """The plan of int8 pages takes up to 262144 new tokens of a request: a longer prefill is refused, not run on
+    rows without a place, and the decoder goes on as if it had not been asked."""
+    g = qwen.Geometry(d_model=32, n_heads=1, n_kv_heads=1, d_ff=32, rope_freq_base=1e4, rms_eps=1e-5)
+    dd = qwen.DeviceDecoder(qwen.synth_model(9, g, n_layers=1, n_vocab=64), max_seq=(1 << 18) + 100,
+                            prefill_rows=(1 << 18) + 1, kv_cache="int8")
+    first = dd.prefill([3, 4, 5])
+    for call in (dd.prefill, dd.score):
+        with pytest.raises(ValueError):
+            call(np.zeros((1 << 18) + 1, np.int32))
+    dd.seq_len = 0
+    assert dd.prefill([3, 4, 5]) == first
+    logits = []
+    prompt = np.random.default_rng(53).integers(0, 64, 1 << 18)
+    for n in (1 << 16, 1 << 18):                            # the longest prefill is what its parts are
+        dd.seq_len = 0
+        for i in range(0, 1 << 18, n):
+            dd.prefill(prompt[i:i + n])
+        logits.append(dd.logits())
+    assert qwen.logit_profile_check(*logits)["ok"]
+    dd.close()
