@@ -317,8 +317,8 @@ int re_ffn_block_dev(re_ffn *f, re_qmat *down, const float *d_x, size_t rows, co
  * row_count[b]; rows between and behind them are left as they were. kv_len[b] counts the request's
  * tokens, its new rows included: row i stands at position kv_len[b] - row_count[b] + i. Token t of
  * it lies in page d_table[b * table_ld + t / page] at place t % page; an entry outside 0 .. n_pages - 1
- * holds no page. A request's pages are distinct, and a page that is being appended to belongs to one
- * request; full pages may be shared.
+ * holds no page, nor does what is behind the table's columns. A request's pages are distinct, and a page
+ * that is being appended to belongs to one request; full pages may be shared.
  *
  * The cache: d_kcodes and d_vcodes hold n_pages x n_kv_heads x page x head_dim int8 codes (page and
  * head_dim multiples of 32 up to 256; 16-byte aligned), d_kscale and d_vscale n_pages x n_kv_heads f32

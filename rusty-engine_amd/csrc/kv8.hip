@@ -348,7 +348,7 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 
 // ---- attention -----------------------------------------------------------------------------------
 // Row i of request r stands at position p = len - count + i and sees the keys max(0, p - window + 1) .. p that lie
-// in a page: softmax over scale * q . k, then the weighted values. A row that sees no key gets zeros.
+// in a page (none does behind the table): softmax over scale * q . k, then the weighted values. A row that sees no key gets zeros.
 //
 // All products run on v_mfma_f32_16x16x32_f16: an int8 code is exact in f16, and the f32 operands (q, the
 // probabilities) are split into two f16 parts, hi + lo, good to 2^-22 of the largest: two instructions per product,
@@ -449,13 +449,13 @@ __device__ __forceinline__ bool place_tile(const PagedBatch& b, const Attn8Args&
   o.req = q.req;
   o.row0 = q.row0;
   o.n = min(q.count, a.max_rows);
-  o.p0 = min(max(q.len, 0), b.table_ld * b.page) - q.count;
+  o.p0 = max(q.len, 0) - q.count;
   o.i0 = i0;
   o.i1 = min(i0 + t.rows_per, o.n);
-  const int last = o.p0 + o.i1 - 1;
+  const int last = min(o.p0 + o.i1, b.table_ld * b.page) - 1;      // (no key behind the table)
   const int lo = a.window > 0 ? max(0, o.p0 + i0 - a.window + 1) : 0;
-  o.first = lo >> 5;
-  o.steps = last < 0 ? 0 : (last >> 5) - o.first + 1;
+  o.first = last < lo ? 0 : lo >> 5;
+  o.steps = last < lo ? 0 : (last >> 5) - o.first + 1;
   return i0 >= 0 && i0 < o.n;
 }
 __device__ __forceinline__ bool place_request(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int r,
