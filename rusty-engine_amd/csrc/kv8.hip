@@ -25,8 +25,8 @@ namespace rehip {
 // right: Markstein). Below 2^-100 remainders could underflow: there the division itself is used. Of finite values
 // |q| <= 127 (1 + 2^-23), and q + 1.5 2^23 rounds it to an integer, whose low byte is the code.
 //
-// Bound by HBM for prompts: 9260 rows of 8 heads of 128, 94.8 MB, 18.2 us, 5.2 TB/s (a copy of 1 GiB runs at 5.1). A decode
-// step (64 rows, 0.33 MB) is three dependent trips to memory, the rows' places, the page number, the values: 4.0 us in the
+// Bound by HBM for prompts: 9260 rows of 8 heads of 128, 94.8 MB, 18.4 us, 5.1 TB/s (as a copy of 1 GiB). A decode
+// step (64 rows, 0.33 MB) is three dependent trips to memory, the rows' places, the page number, the values: 3.9 us in the
 // kernel.
 constexpr float kCodeMagic = 12582912.0f;
 
@@ -359,10 +359,10 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 // zero and scaled by the page's scale in f32 (scales taken into the f16 weights cost a row that sees only pages of small
 // scale its precision).
 //
-// Measured, with the join: one row of 24 heads behind 131071 tokens (8 heads of 128, 268 MB) 48.8 us, 5.5 TB/s: HBM; 64
-// requests of 1 .. 16384 tokens (4 heads of 128, 135 MB) 34.5 us, 30 of them here: HBM behind the first three trips to
-// memory; one row of 14 heads, 211 tokens 9.4 us, 6.6 in the kernel: those trips. Prompts of 1000 rows behind up to 5000
-// tokens (four, 32 heads of 128) 193 us, 466 TFLOP/s of products and as many again of low parts: 0.88 of the rate of a large
+// Measured, with the join: one row of 24 heads behind 131071 tokens (8 heads of 128, 268 MB) 49.0 us, 5.5 TB/s: HBM; 64
+// requests of 1 .. 16384 tokens (4 heads of 128, 135 MB) 34.4 us, 30 of them here: HBM behind the first three trips to
+// memory; one row of 14 heads, 211 tokens 9.6 us, 6.7 in the kernel: those trips. Prompts of 1000 rows behind up to 5000
+// tokens (four, 32 heads of 128) 189 us, 475 TFLOP/s of products and as many again of low parts: 0.90 of the rate of a large
 // f16 matrix product (1.06 PFLOP/s) on the matrix cores.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -691,7 +691,9 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     return base + ((size_t)__builtin_amdgcn_readfirstlane(max(pid, 0)) * c.kv_heads + head) * head_bytes +
            (size_t)in_page * (NB * 1024);
   };
-  // (a decode step reads every code once; prompts' tiles read them again, from L2)
+  // (a decode step reads every code once, tiles of 32 and 64 vectors read them again, from L2: us of nontemporal / plain
+  // loads for one row behind 131071 tokens 50 / 56, 64 requests of up to 16384 36 / 35. Prompts in tiles of 16 take either: 961
+  // rows of 14 heads in 2 of 64 16.4 / 16.5, behind 4000 tokens 69 / 70.6, 100 of 32 in 8 of 128 behind 1000 21.7 / 21.7)
   auto load = [&](const int8_t* p, u32x4 (&x)[NB]) {
 #pragma unroll
     for (int k = 0; k < NB; ++k) {

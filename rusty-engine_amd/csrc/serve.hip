@@ -18,7 +18,7 @@ namespace rehip {
 // and keeps its length.
 //
 // Bound by latency (a few KB): loads, two scans, the stack, the table, then the rows, one after the other in one workgroup:
-// 64 requests 7.6 us a call, 5.4 in the kernel; 1024 requests and 19000 rows 12.5 us, 8.6 and 4.1 for the rows' launch (of
+// 64 requests 7.8 us a call, 5.5 in the kernel; 1024 requests and 19000 rows 12.6 us, 8.7 and 4.1 for the rows' launch (of
 // more rows than two per thread; in the plan's own workgroup they would take a trip to memory per 1024 of them).
 
 // exclusive prefix sums over the workgroup of three numbers per thread; totals in tot
@@ -182,8 +182,8 @@ hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s) {
 // ---- rotary positions ----------------------------------------------------------------------------
 // Pair i of each head of row r turns by pos[r] * freqs[i] radians and is scaled by mscale. The angle is taken in turns
 // and reduced to half a turn in 64 bits: at position 131071 an angle in 32 bits is off by up to 4e-3. A row's angles are
-// taken once for all its heads. Bound by HBM: 8192 rows of 36 heads of 128, 302 MB, 57.8 us, 5.2 TB/s (as a large copy);
-// 8 rows by the launch, 7 us a call and 2.8 in the kernel.
+// taken once for all its heads. Bound by HBM: 8192 rows of 36 heads of 128, 302 MB, 57.6 us, 5.2 TB/s (as a large copy);
+// 8 rows by the launch, 7 us a call and 2.9 in the kernel.
 __device__ __forceinline__ void turn_cs(int pos, double freq, float mscale, float& c, float& s) {
   const double t = (double)pos * (freq * 0.15915494309189533577);
   const float f = (float)(2.0 * (t - rint(t)));
@@ -270,8 +270,8 @@ hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s) {
 // border comes from the first batch: the k-th largest of the 64 lanes' maxima has at least k values at or above it.
 // Values in random order push about k ln(batches) keys behind the first batch; a rising row pushes all.
 //
-// Bound by HBM: 961 rows of 151936, 20 best, 584 MB in 100 us, 5.8 TB/s (without candidates 93, 6.3 TB/s); one row 10.5 us,
-// 7.0 and 4.4 in its two launches: latency.
+// Bound by HBM: 961 rows of 151936, 20 best, 584 MB in 98 us, 5.9 TB/s (without candidates 93, 6.3 TB/s); one row 11 us,
+// 7.3 and 4.4 in its two launches: latency.
 constexpr int kTopCap = 256;             // candidates of a wave
 constexpr int kLogBatch = 16;            // logits of a lane at a time
 constexpr int kLogWaves = 4;
@@ -621,7 +621,8 @@ size_t logprobs_work_floats(int rows, int vocab, int k) {
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s) {
   const int parts = logprob_parts(a.rows, a.vocab, a.k);
   // a wave per row where one batch is the row, or where rows alone fill the GPU's waves (us of a wave / a workgroup per
-  // row, top 5 or 20: 4000 x 1000 11.8 / 25.8, 2000 x 32000 54 / 67, 8000 x 32000 176 / 238; but 1000 x 16000 31.5 / 26.9)
+  // row, top 5 or 20: 4000 x 1000 11.8 / 25.8, 2000 x 32000 54 / 67, 8000 x 32000 176 / 238; but 1000 x 16000 31.5 / 26.9;
+  // long rows just above the border, top 20: 1536 x 50000 67.4 / 69.4, x 151936 161 / 163, 2048 x 151936 199 / 202)
   if (a.vocab <= 64 * kLogBatch || a.rows >= 1536) {
     auto* k = a.k > 0 ? logprobs_kernel<true, true> : logprobs_kernel<false, true>;
     hipLaunchKernelGGL(k, dim3((unsigned)((a.rows + kLogWaves - 1) / kLogWaves)), dim3(64 * kLogWaves), 0, s, a, 1);
