@@ -739,7 +739,8 @@ class DeviceDecoder:
         """Prefill of the prompt with, for each of its rows, what the model says of the token that follows:
         "logprob" of the prompt's own next token (0 for the last row), "entropy" in nats, and the top_k
         alternatives' "ids" and "top" log probabilities (ties to the lower id). The sequence goes on as after
-        `prefill` (whose greedy token is returned as "next")."""
+        `prefill` (whose greedy token is returned as "next"). Of a prompt given in several calls, what the last row of
+        one says of the first token of the next is in `logits()` between them."""
         from . import logprobs_dev, logprobs_work_bytes, rmsnorm_dev
         from .hip import DeviceBuffer as B
         g, s, d, v = self.g, self.stream, self.g.d_model, self.mb.n_vocab
