@@ -261,7 +261,9 @@ hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s) {
 // With m a row's largest logit, d = x - m, Z = sum e^d and T = sum d e^d: log p = d_target - ln Z, entropy = ln Z - T / Z.
 // One pass over the logits: each lane keeps (m, Z, T) of what it has seen and moves them when its maximum rises,
 //   Z' = c Z, T' = c (T + (m - m') Z), c = e^(m - m');
-// a logit of -inf has e^d = 0 and adds nothing, and so do terms whose c is 0 (d may be -inf there).
+// a logit of -inf has e^d = 0 and adds nothing, and so do terms whose c is 0 (d may be -inf there). A lane sums a batch
+// and adds that to its sums with their rounding errors kept (2370 equal terms of a row of 151936, added one after the other,
+// could round the same way every time: ln Z was off by 3.7e-5).
 //
 // The k largest (ties to the lower index) in the same pass. A candidate is one 64-bit key, larger for the better one:
 // the value's bits made order-preserving, then the index inverted. A wave keeps its candidates in LDS, and a border that
@@ -449,6 +451,12 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
   const int b0 = (int)((long long)batches * part / parts), b1 = (int)((long long)batches * (part + 1) / parts);
   Candidates c{lists + (TOP ? w * (kTopCap + kPad) : 0), 0, a.k, 0, -INFINITY};
   Stats s{-INFINITY, 0.0f, 0.0f};
+  float lost_z = 0.0f, lost_t = 0.0f;      // what the sums' roundings left out, s.z + lost_z the better sum
+  auto add = [](float& sum, float& lost, float v) {
+    const float was = sum;
+    sum += v;
+    lost += v - (sum - was);
+  };
   bool first = true;
   auto take = [&](const float (&v)[kLogBatch], int base) {
     float mx = -INFINITY;
@@ -458,15 +466,20 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
     if (mn > s.m) {
       const float d = s.m - mn, f = exp_of(d);
       s.t = f == 0.0f ? 0.0f : f * (s.t + d * s.z);
+      lost_t = f == 0.0f ? 0.0f : f * (lost_t + d * lost_z);
       s.z *= f;
+      lost_z *= f;
       s.m = mn;
     }
+    float z = 0.0f, t = 0.0f;
 #pragma unroll
     for (int q = 0; q < kLogBatch; ++q) {
       const float d = v[q] - ref, e = exp_of(d);
-      s.z += e;
-      s.t = __builtin_fmaf(e, fmaxf(d, -3e38f), s.t);
+      z += e;
+      t = __builtin_fmaf(e, fmaxf(d, -3e38f), t);
     }
+    add(s.z, lost_z, z);
+    add(s.t, lost_t, t);
     if constexpr (TOP) {
       c.batch(v, mx, [&](int q) {
         const int at = base + 256 * (q >> 2) + (q & 3);
@@ -505,6 +518,8 @@ __global__ __launch_bounds__(64 * kLogWaves) void logprobs_kernel(LogprobArgs a,
     }
     take(v, base);
   }
+  s.z += lost_z;
+  s.t += lost_t;
   s = wave_join(s);
   if constexpr (TOP) {
     // (k at most 64: a workgroup's lists then have a thread per key. Longer lists of a small k would be ranked against each
