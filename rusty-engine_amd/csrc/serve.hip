@@ -617,11 +617,11 @@ __global__ __launch_bounds__(kLogJoin) void logprobs_join_kernel(LogprobArgs a, 
   finish_row(a, r, target, all, list, n, tid, kLogJoin);
 }
 
-// About three workgroups for each CU; a part is at least one batch of every wave (64 rows of 151936, top 20: 32.0 / 28.8
-// / 30.2 us at 256 / 768 / 1024 workgroups; 256 rows: 54.0 / 43.9 / 45.0).
+// About three workgroups for each CU; a part is at least one batch of every wave (64 rows of 151936, top 20: 29.7 / 25.3
+// / 26.6 us at 256 / 768 / 1024 workgroups; 256 rows: 53.1 / 42.3 / 42.6).
 // The join's launch takes 3 us, a batch 0.2 and more with candidates: parts if they take more than that off (us whole / in
-// parts: one row of 32000, none 7.2 / 10.5, 20 best 22 / 12; 12289, 2 best 8.5 / 10.7; 12963, 17 best 15 / 11; 157 rows of
-// 29551, none 7.8 / 10.6, 4 best 19.4 / 15.1); two of them only of long rows (300 of 20000 20 / 23, 380 of 151936 50 / 47).
+// parts: one row of 32000, none 8.0 / 11.3, 20 best 21 / 12; 12289, 2 best 8.5 / 11.3; 12963, 17 best 14 / 11.6; 157 rows of
+// 29551, none 8.4 / 11.0, 4 best 18.2 / 15.9); two of them only of long rows (300 of 20000 16.5 / 18.1, 380 of 151936 50 / 46).
 static int logprob_parts(int rows, int vocab, int k) {
   const int batches = (vocab + kLogPart - 1) / kLogPart;           // of a wave of a whole row
   const int parts = std::min({batches, kLogMaxParts, 768 / std::max(rows, 1)});
@@ -636,8 +636,8 @@ size_t logprobs_work_floats(int rows, int vocab, int k) {
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s) {
   const int parts = logprob_parts(a.rows, a.vocab, a.k);
   // a wave per row where one batch is the row, or where rows alone fill the GPU's waves (us of a wave / a workgroup per
-  // row, top 5 or 20: 4000 x 1000 11.8 / 25.8, 2000 x 32000 54 / 67, 8000 x 32000 176 / 238; but 1000 x 16000 31.5 / 26.9;
-  // long rows just above the border, top 20: 1536 x 50000 67.4 / 69.4, x 151936 161 / 163, 2048 x 151936 199 / 202)
+  // row, top 5 or 20: 4000 x 1000 11.5 / 25, 2000 x 32000 54 / 63, 8000 x 32000 161 / 182; but 1000 x 16000 25.4 / 20.2;
+  // long rows just above the border, top 20: 1536 x 50000 67.4 / 67.6, x 151936 156 / 158, 2048 x 151936 192 / 197)
   if (a.vocab <= 64 * kLogBatch || a.rows >= 1536) {
     auto* k = a.k > 0 ? logprobs_kernel<true, true> : logprobs_kernel<false, true>;
     hipLaunchKernelGGL(k, dim3((unsigned)((a.rows + kLogWaves - 1) / kLogWaves)), dim3(64 * kLogWaves), 0, s, a, 1);
