@@ -746,10 +746,11 @@ class DeviceDecoder:
         g, s, d, v = self.g, self.stream, self.g.d_model, self.mb.n_vocab
         if not 0 <= top_k <= min(64, v):
             raise ValueError(f"score: top {top_k} of {v} tokens (up to 64)")
+        prompt = np.asarray(prompt, np.int32).reshape(-1)      # (a target for each row, whatever its shape was)
         rows = self._forward_rows(prompt)
         rmsnorm_dev(self.x, self.output_norm, rows, d, g.rms_eps, self.n, s)
         step = min(rows, self.SCORE_ROWS)
-        targets = B.from_array(np.append(np.asarray(prompt, np.int32)[1:], np.int32(-1)))
+        targets = B.from_array(np.append(prompt[1:], np.int32(-1)))
         logits, out = B(step * v * 4), {"logprob": B(rows * 4), "entropy": B(rows * 4)}
         if top_k:
             out.update(ids=B(rows * top_k * 4), top=B(rows * top_k * 4))

@@ -134,3 +134,17 @@ def test_prefills_past_what_a_plan_takes():
         logits.append(dd.logits())
     assert qwen.logit_profile_check(*logits)["ok"]
     dd.close()
+
+
+def test_score_of_a_prompt_with_a_batch_axis(tiny):
+    """prefill() takes prompts of any shape; scoring one gives a target to every row."""
+    prompt = np.random.default_rng(54).integers(0, 1000, 30)
+    dd = decoder(tiny, "f32")
+    want = dd.score(prompt, 3)
+    for shaped in (prompt[None], prompt.reshape(5, 6), prompt.tolist()):
+        dd.seq_len = 0
+        got = dd.score(shaped, 3)
+        assert got["next"] == want["next"]
+        for k in ("logprob", "entropy", "ids", "top"):
+            np.testing.assert_array_equal(got[k], want[k])
+    dd.close()
