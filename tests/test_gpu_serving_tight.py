@@ -66,3 +66,22 @@ def test_score_of_the_last_row(mode):
         if n > 1:                                           # the row before says of the last token: by entropy alone
             assert got["entropy"][-2] <= np.log(1000) + 2e-3 and got["logprob"][-2] < 0
     dd.close()
+
+
+def test_int8_pages_of_a_decoder_with_unquantized_weights():
+    """The bias of a step goes into the q|k|v product: of dense weights that is another kernel. Prompt and steps against
+    the f32 caches, by the gate that the bf16 paths pass."""
+    from test_gpu_layer import TINY, dense_model
+    mb = dense_model(11, TINY, n_layers=3, n_vocab=1000)
+    prompt = np.random.default_rng(71).integers(0, 1000, 100)
+    a, b = (qwen.DeviceDecoder(mb, max_seq=200, prefill_rows=100, kv_cache=c) for c in ("f32", "int8"))
+    t = a.prefill(prompt)
+    b.prefill(prompt)
+    for i in range(40):
+        gate = qwen.logit_profile_check(a.logits(), b.logits())
+        assert gate["ok"], (i, gate)
+        b.tok.upload(np.array([t], np.int32))
+        t = a.step()
+        b.step()
+    a.close()
+    b.close()
