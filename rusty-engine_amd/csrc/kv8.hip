@@ -362,7 +362,7 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 // Measured, with the join: one row of 24 heads behind 131071 tokens (8 heads of 128, 268 MB) 49.0 us, 5.5 TB/s: HBM; 64
 // requests of 1 .. 16384 tokens (4 heads of 128, 135 MB) 34.4 us, 30 of them here: HBM behind the first three trips to
 // memory; one row of 14 heads, 211 tokens 9.6 us, 6.7 in the kernel: those trips. Prompts of 1000 rows behind up to 5000
-// tokens (four, 32 heads of 128) 189 us, 475 TFLOP/s of products and as many again of low parts: 0.90 of the rate of a large
+// tokens (four, 32 heads of 128) 189 .. 194 us, 465 .. 475 TFLOP/s of products and as many again of low parts: 0.9 of the rate of a large
 // f16 matrix product (1.06 PFLOP/s) on the matrix cores.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));

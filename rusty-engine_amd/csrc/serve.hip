@@ -18,7 +18,7 @@ namespace rehip {
 // and keeps its length.
 //
 // Bound by latency (a few KB): loads, two scans, the stack, the table, then the rows, one after the other in one workgroup:
-// 64 requests 7.8 us a call, 5.5 in the kernel; 1024 requests and 19000 rows 12.6 us, 8.7 and 4.1 for the rows' launch (of
+// 64 requests 7.8 us a call, 5.5 in the kernel; 1024 requests and 19000 rows 12.6 us, 8.5 and 4.2 for the rows' launch (of
 // more rows than two per thread; in the plan's own workgroup they would take a trip to memory per 1024 of them).
 
 // exclusive prefix sums over the workgroup of three numbers per thread; totals in tot
@@ -272,8 +272,8 @@ hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s) {
 // border comes from the first batch: the k-th largest of the 64 lanes' maxima has at least k values at or above it.
 // Values in random order push about k ln(batches) keys behind the first batch; a rising row pushes all.
 //
-// Bound by HBM: 961 rows of 151936, 20 best, 584 MB in 98 us, 5.9 TB/s (without candidates 93, 6.3 TB/s); one row 11 us,
-// 7.3 and 4.4 in its two launches: latency.
+// Bound by HBM: 961 rows of 151936, 20 best, 584 MB in 99 us, 5.9 TB/s (without candidates 93, 6.3 TB/s); one row 11 us,
+// 7.2 and 4.4 in its two launches: latency.
 constexpr int kTopCap = 256;             // candidates of a wave
 constexpr int kLogBatch = 16;            // logits of a lane at a time
 constexpr int kLogWaves = 4;
