@@ -403,6 +403,82 @@ int re_attention_kv8_dev(const float *d_q, size_t ldq, size_t rows, size_t reque
                          size_t head_dim, float scale, size_t window, float *d_ctx, void *d_work, size_t work_bytes,
                          void *stream);
 
+/* The same with a few first tokens that stay visible behind the window: row at position p sees the tokens t <= p with
+ * t > p - window or t < sinks (up to 1024; of no effect with window 0). A row costs window + sinks tokens however long its
+ * request is; pages that no row sees any more are not read. d_lse: NULL, or rows x n_heads, the natural logarithm of each
+ * row and head's sum of exp(scale * q . k) (-inf where it sees nothing). The workspace is re_attention_kv8_work_bytes' too. */
+int re_attention_kv8_sinks_dev(const float *d_q, size_t ldq, size_t rows, size_t requests, const int *d_row_start,
+                               const int *d_row_count, const int *d_kv_len, const int *d_table, size_t table_ld,
+                               size_t page, size_t n_pages, const int8_t *d_kcodes, const int8_t *d_vcodes,
+                               const float *d_kscale, const float *d_vscale, size_t max_rows, size_t max_len,
+                               size_t n_heads, size_t n_kv_heads, size_t head_dim, float scale, size_t window,
+                               size_t sinks, float *d_ctx, float *d_lse, void *d_work, size_t work_bytes, void *stream);
+
+/* The weight that a step's attention gives each cached token, added to what it has: d_mass holds n_pages x n_kv_heads x
+ * page f32, d_mass[page][head][place] += the sum over the request's rows that see the token and over the query heads of that
+ * KV head of exp(scale * q . k - lse), with the q, window and sinks of the attention call and the d_lse that it gave. A
+ * token that the step brought starts from 0, so pages need no preparation. A row whose q or lse is not finite adds
+ * nothing. Accurate to about 2^-23 |lse| of a weight. Here a page belongs to one request. No workspace; d_q and d_mass
+ * 16-byte aligned. */
+int re_kv8_mass_dev(const float *d_q, size_t ldq, const float *d_lse, size_t rows, size_t requests,
+                    const int *d_row_start, const int *d_row_count, const int *d_kv_len, const int *d_table,
+                    size_t table_ld, size_t page, size_t n_pages, const int8_t *d_kcodes, const float *d_kscale,
+                    size_t max_rows, size_t max_len, size_t n_heads, size_t n_kv_heads, size_t head_dim, float scale,
+                    size_t window, size_t sinks, float *d_mass, void *stream);
+
+/* Eviction: requests that hold more than `limit` tokens are cut to `keep` (1 .. limit) of them, in fresh pages, so that one
+ * plan serves the caches of all layers. re_kv_evict_plan_dev, once a step: each cut request, in request order, takes
+ * ceil(keep / page) pages from the top of the stack and then gives its old ones back (behind the free ones, entries that
+ * hold no page left out); one whose new pages are not there is left as it is. Outputs: lengths, table, stack and its height
+ * (d_kv_len_out, d_table_out, d_free_out, d_n_free_out may be the inputs; entries of d_table_out behind a cut request's
+ * pages are -1); d_from_len: a cut request's old length, 0 for the others; d_from_table (requests x table_ld): a cut
+ * request's old entries (may be d_table if d_table_out is another buffer; never d_table_out); d_dropped: NULL, or per
+ * request += the tokens it lost, 0 where it holds none (positions of its next tokens are its length and these);
+ * d_status[0] requests over the limit that were left, d_status[1] cut ones. Up to 4096 requests.
+ *
+ * re_kv8_evict_dev, for each layer: of a cut request's tokens the first `first`, the last `recent` and the heaviest of
+ * those between them stay, `keep` in all, KV head by KV head (ties to the earlier token; a NaN counts as -inf, a token
+ * without a page below that), and move to the new pages in their order, K, V and mass. A new page's scale is the largest of
+ * the pages that its tokens come from, a code round(c * (old / new)), ties to even; places behind the last token get code
+ * and mass 0. d_kept: requests x n_kv_heads x keep, the old places of what stayed (of cut requests). d_mass may be NULL if
+ * first + recent = keep. Old pages are only read: they must not be given out before the last layer's call. max_len: the
+ * largest d_from_len to plan for (longer ones are computed too, only slower). */
+int re_kv_evict_plan_dev(size_t requests, size_t page, size_t limit, size_t keep, const int *d_kv_len,
+                         const int *d_table, size_t table_ld, const int *d_free, size_t n_pages, const int *d_n_free,
+                         int *d_kv_len_out, int *d_table_out, int *d_free_out, int *d_n_free_out, int *d_from_len,
+                         int *d_from_table, int *d_dropped, int *d_status, void *stream);
+int re_kv8_evict_dev(size_t requests, const int *d_from_len, const int *d_from_table, const int *d_table,
+                     size_t table_ld, size_t page, size_t n_pages, int8_t *d_kcodes, int8_t *d_vcodes, float *d_kscale,
+                     float *d_vscale, float *d_mass, size_t n_kv_heads, size_t head_dim, size_t keep, size_t first,
+                     size_t recent, size_t max_len, int *d_kept, void *stream);
+
+/* Drafted tokens against the target's probabilities. Request b has d_row_count[b] rows of logits from d_row_start[b] on
+ * (ranges ascending and disjoint, as above; 0: none): row i is the target's after token d_tokens[row i], d_tokens[row i + 1] the
+ * token drafted there, and the last row has no draft behind it, so that a request of one row just draws a token. p =
+ * softmax(logits / T), T = d_temperature[b] (NULL: 1). d_probs (stride ldp), or NULL: the distributions q that the drafts were
+ * drawn from, row by row; finite, not negative. A draft d is accepted if d_accept_u[row] * q(d) < p(d) (without d_probs:
+ * q(d) = 1). In the place of the first that is not, a token is drawn from max(0, p - q) over its sum (without d_probs: from
+ * p without d; where nothing is left, from p), behind the last from p. Drawn: the lowest token t with sum over j <= t
+ * of the weights > d_sample_u[b] * their sum; both random numbers from [0, 1). T <= 0 or NaN: greedy, a draft is accepted
+ * if it is the largest logit (ties to the lower id), and the token behind is the largest. Sums are taken in 64 bits. A
+ * draft outside 0 .. vocab - 1 is not accepted. A row with NaN or +inf among its logits, or nothing above -inf, has no
+ * distribution: its draft is not accepted, and the token in its place is -1. Outputs: d_accepted[b] drafts, d_back[b] = the
+ * others (for re_kv_rewind_dev), d_out_tokens[row i]: the accepted drafts, the token behind them, -1 after that; rows
+ * outside the requests' are left. d_work: re_draft_verify_work_bytes bytes, 16-byte aligned; as above. */
+size_t re_draft_verify_work_bytes(size_t rows, size_t requests, size_t vocab);
+int re_draft_verify_dev(const float *d_logits, size_t ld, size_t rows, size_t vocab, size_t requests,
+                        const int *d_row_start, const int *d_row_count, const int *d_tokens, const float *d_probs,
+                        size_t ldp, const float *d_temperature, const float *d_accept_u, const float *d_sample_u,
+                        int *d_accepted, int *d_back, int *d_out_tokens, void *d_work, size_t work_bytes, void *stream);
+
+/* Takes d_back[b] tokens (negative: none; more than there are: all) off the ends of the requests' lengths; pages that hold
+ * none of the rest go back to the stack, behind the free ones in request order. d_kv_len_out and d_n_free_out may be
+ * d_kv_len and d_n_free; the table is left. Lengths outside 0 .. table_ld * page stay. Such pages belong to one request. A
+ * part-filled page keeps the scale that the tokens behind had raised. Up to 4096 requests. */
+int re_kv_rewind_dev(size_t requests, size_t page, const int *d_back, const int *d_kv_len, const int *d_table,
+                     size_t table_ld, int *d_free, size_t n_pages, const int *d_n_free, int *d_kv_len_out,
+                     int *d_n_free_out, void *stream);
+
 /* Of rows x vocab logits (row stride ld): d_logprob[r] = log softmax of logit d_targets[r] (a target outside
  * 0 .. vocab - 1: 0, so that a sum over rows skips it), d_entropy[r] in nats, and the top_k (up to 64)
  * largest logits' ids and log probabilities in descending order, ties to the lower id; rows x top_k. d_logprob

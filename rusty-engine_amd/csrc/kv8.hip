@@ -9,6 +9,7 @@
 
 #include <algorithm>
 
+#include "kv8.hpp"
 #include "serve.hpp"
 #include "wave.hpp"
 
@@ -349,6 +350,8 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 // ---- attention -----------------------------------------------------------------------------------
 // Row i of request r stands at position p = len - count + i and sees the keys max(0, p - window + 1) .. p that lie
 // in a page (none does behind the table): softmax over scale * q . k, then the weighted values. A row that sees no key gets zeros.
+// With sinks (first tokens that stay visible behind the window) it sees the keys below `sinks` too: a tile then walks their
+// steps first and skips from there to the window's, so that a row costs window + sinks keys however long its request is.
 //
 // All products run on v_mfma_f32_16x16x32_f16: an int8 code is exact in f16, and the f32 operands (q, the
 // probabilities) are split into two f16 parts, hi + lo, good to 2^-22 of the largest: two instructions per product,
@@ -364,58 +367,7 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 // memory; one row of 14 heads, 211 tokens 9.6 us, 6.7 in the kernel: those trips. Prompts of 1000 rows behind up to 5000
 // tokens (four, 32 heads of 128) 189 .. 194 us, 465 .. 475 TFLOP/s of products and as many again of low parts: 0.9 of the rate of a large
 // f16 matrix product (1.06 PFLOP/s) on the matrix cores.
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr float kTermBits = 10.0f, kSlack = 5.0f;     // 2^(10 + 5) stays below f16's 65504
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
-// eight codes as f16: 0x6400 + u is the f16 value 1024 + u for a byte u = c + 128, less 1152 is c
-__device__ __forceinline__ h8 codes8(unsigned a, unsigned b) {
-  union { unsigned u[4]; h2 h[4]; h8 v; } r;
-  a ^= 0x80808080u;
-  b ^= 0x80808080u;
-  r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
-  r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
-  r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
-  r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
-  const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r.h[i] += off;
-  return r.v;
-}
-
-// x = hi + lo, each rounded to the nearest f16. minus_one: -1, but unknown to the compiler, which then subtracts hi in
-// one mixed-precision fma instead of converting it back first
-__device__ __forceinline__ void split8(const float (&x)[8], float minus_one, h8& hi, h8& lo) {
-  union { h2 h[4]; h8 v; } a, b;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a.h[i] = __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), h2);
-    const f32x2 r = {__builtin_fmaf((float)a.h[i][0], minus_one, x[2 * i]),
-                     __builtin_fmaf((float)a.h[i][1], minus_one, x[2 * i + 1])};
-    b.h[i] = __builtin_convertvector(r, h2);
-  }
-  hi = a.v;
-  lo = b.v;
-}
-
-// 2^x for x <= 16: what is below the smallest normal float may come out as 0
-__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// the largest over the four lanes that share a column of the 16 x 16 layouts (one of the swapped values is the lane's
-// own, so both may be taken), and the sum
-__device__ __forceinline__ float column_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float column_sum(float v) {
-  v += lane_xor<16>(v);
-  return v + lane_xor<32>(v);
-}
 
 // How a launch cuts the batch: a tile holds up to vecs query vectors of one request and KV head, rows_per rows of its
 // grp heads (grp <= vecs), or vecs of the grp heads of one row (group_tiles of them).
@@ -431,11 +383,13 @@ struct AttnTiles {
   size_t list;
 };
 
-// A tile's place: request, rows, and the 32-key steps it has to walk, and their cut into splits.
+// A tile's place: request, rows, and the 32-key steps it has to walk, and their cut into splits. The steps are those of the
+// sinks, 0 .. sinks - 1, then the window's from `first` on; sinks is 0 where the two meet, and then all start at `first`.
 struct AttnTile {
   int req, row0, n, i0, i1;  // request, its first row, its rows, the tile's rows i0 .. i1 - 1 of them
   int p0;                    // position of the request's row 0 (may be below 0)
   int first, steps, per;     // first step, number of steps, steps per split
+  int sinks;                 // the sinks' steps before the first, counted in `steps`
   int slot;                  // its first place in the workspace
 };
 
@@ -456,6 +410,19 @@ __device__ __forceinline__ bool place_tile(const PagedBatch& b, const Attn8Args&
   const int lo = a.window > 0 ? max(0, o.p0 + i0 - a.window + 1) : 0;
   o.first = last < lo ? 0 : lo >> 5;
   o.steps = last < lo ? 0 : (last >> 5) - o.first + 1;
+  o.sinks = 0;
+  if (a.sinks > 0 && a.window > 0 && last >= 0) {
+    const int sinks = (min(a.sinks, last + 1) + 31) >> 5;
+    if (last < lo) {
+      o.sinks = o.first = o.steps = sinks;             // (the window is behind the table)
+    } else if (o.first > sinks) {
+      o.sinks = sinks;
+      o.steps += sinks;
+    } else {
+      o.first = 0;
+      o.steps = (last >> 5) + 1;
+    }
+  }
   return i0 >= 0 && i0 < o.n;
 }
 __device__ __forceinline__ bool place_request(const PagedBatch& b, const Attn8Args& a, const AttnTiles& t, int r,
@@ -476,34 +443,7 @@ __device__ __forceinline__ int piece_steps(float sum, float live, int pieces) {
   return max(kAttnMinSteps, ((int)fminf(ceilf(sum * 1.005f / n), 1e9f) + 3) & ~3);
 }
 
-// inclusive sums over the lanes of a wave
-__device__ __forceinline__ int wave_scan(int v) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(v, off, 64);
-    if ((int)(threadIdx.x & 63) >= off) v += y;
-  }
-  return v;
-}
-
-// The sum over a workgroup of WAVES waves, and in `before` that of the threads below this one.
-template <int WAVES>
-__device__ __forceinline__ int scan_block(int v, int& before) {
-  __shared__ int part[WAVES];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, inc = wave_scan(v);
-  if (lane == 63) part[w] = inc;
-  __syncthreads();
-  int all = 0;
-  before = inc - v;
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) {
-    before += i < w ? part[i] : 0;
-    all += part[i];
-  }
-  __syncthreads();
-  return all;
-}
-// .. of floats, in one order
+// The sum of floats over a workgroup of WAVES waves, in one order.
 template <int WAVES>
 __device__ __forceinline__ float sum_block(float v) {
   __shared__ float part[WAVES];
@@ -621,12 +561,17 @@ __device__ __forceinline__ size_t place_of(const AttnTiles& t, const AttnTile& t
 // the same in every lane, so that what follows from it is scalar
 __device__ __forceinline__ AttnTile uniform(const AttnTile& o) {
   auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  return {u(o.req), u(o.row0), u(o.n), u(o.i0), u(o.i1), u(o.p0), u(o.first), u(o.steps), u(o.per), u(o.slot)};
+  return {u(o.req), u(o.row0), u(o.n), u(o.i0), u(o.i1), u(o.p0), u(o.first), u(o.steps), u(o.per), u(o.sinks), u(o.slot)};
 }
 
 __device__ __forceinline__ int2* splits_at(const Attn8Args& a, const AttnTiles& t, int kv_heads, int hd) {
   const size_t n = piece_vectors(t, kv_heads);
   return reinterpret_cast<int2*>(a.work + sums_at(n) + n * hd);
+}
+
+// ln of a vector's sum of exponentials from its m and l; -inf where it saw nothing
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return (m + (__builtin_amdgcn_logf(l) - kTermBits)) * 0.6931471805599453f;
 }
 
 constexpr int kAttnPages = 256;       // pages whose numbers and scales are staged at a time: one per thread
@@ -640,7 +585,9 @@ constexpr int kAttnPages = 256;       // pages whose numbers and scales are stag
 // registers; with more (prompts) the groups' q lies in LDS, in fragment order too, and every code is converted to f16
 // once for all of them.
 // SOLO (listed pieces, one group): every wave its own piece, no joins between waves.
-template <int NB, int VT, bool SOLO>
+// SINKS: a piece's steps are numbers within the tile's list of steps, its pages within the list of the sinks' pages and the
+// window's; without, both count from the request's first.
+template <int NB, int VT, bool SOLO, bool SINKS>
 __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cache c, Attn8Args a, AttnTiles t) {
   constexpr int HD = 32 * NB, LD = HD + 4, kW = SOLO ? 1 : 4, kPages = SOLO ? kAttnPages / 4 : kAttnPages;
   static_assert(!SOLO || VT == 1, "a wave alone has one group");
@@ -670,7 +617,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   sp = __builtin_amdgcn_readfirstlane(sp);
   const int head = yy / t.group_tiles, g0 = (yy % t.group_tiles) * t.vecs;
   const int col = lane & 15, g = lane >> 4;
-  const int s0 = tile.first + sp * tile.per, s1 = min(s0 + tile.per, tile.first + tile.steps);
+  const int base = SINKS ? 0 : tile.first;
+  const int s0 = base + sp * tile.per, s1 = min(s0 + tile.per, base + tile.steps);
   // every vector of the tile sees the keys see_from .. see_all (a place without one may see anything: it is not stored)
   const int see_all = tile.p0 + tile.i0, see_from = a.window > 0 ? tile.p0 + tile.i1 - a.window : 0;
   // vector col of group v: row and head, the last key it sees (-1: no such vector)
@@ -681,9 +629,21 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   for (int v = 0; v < VT; ++v)
     pos[v] = row_of(16 * v + col) < tile.i1 && head_of(16 * v + col) < t.grp ? tile.p0 + row_of(16 * v + col) : -1;
   const size_t head_bytes = (size_t)b.page * HD;
-  const int page_steps = b.page >> 5, page0 = s0 / page_steps, page_last = max(s1 - 1, 0) / page_steps;
+  const int page_steps = b.page >> 5;
+  // (SINKS) pages of the sinks, the window's first page and its first step's place in that
+  const int sink_pages = SINKS ? (tile.sinks + page_steps - 1) / page_steps : 0;
+  const int win_page = SINKS ? tile.first / page_steps : 0, win_off = SINKS ? tile.first - win_page * page_steps : 0;
+  auto listed_page = [&](int s) {                                  // of a step
+    if (!SINKS) return s / page_steps;
+    return s < tile.sinks ? s / page_steps : sink_pages + (s - tile.sinks + win_off) / page_steps;
+  };
+  auto first_step = [&](int pg) {                                  // of a listed page
+    return pg < sink_pages ? pg * page_steps : tile.sinks + max((pg - sink_pages) * page_steps - win_off, 0);
+  };
+  const int page0 = listed_page(s0), page_last = listed_page(max(s1 - 1, 0));
   const unsigned page_inv = 65536u / page_steps + 1;
   auto entry = [&](int pg) {
+    if (SINKS && pg >= sink_pages) pg += win_page - sink_pages;
     const int pid = b.table[(size_t)tile.req * b.table_ld + pg];
     return pid >= 0 && pid < b.n_pages ? pid : -1;
   };
@@ -706,7 +666,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
   const int first = max(min(s0 + w, s1 - 1), 0);
   int my_page = entry(min(page0 + tid, page_last));
   {
-    const int pid = entry(first / page_steps), in_page = first - first / page_steps * page_steps;
+    const int at = SINKS && first >= tile.sinks ? first - tile.sinks + win_off : first;
+    const int pid = entry(listed_page(first)), in_page = at - at / page_steps * page_steps;
     load(block(c.k, pid, in_page), kf);
     load(block(c.v, pid, in_page), vf);
   }
@@ -760,7 +721,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     for (int k = 0; k < NB; ++k) o[v][k][0] = o[v][k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   bool huge = false;                     // some vector's m is beyond 2^20
-  for (int pg0 = page0; pg0 * page_steps < s1; pg0 += kPages) {
+  for (int pg0 = page0; SINKS ? pg0 <= page_last && s0 < s1 : pg0 * page_steps < s1; pg0 += kPages) {
     // the pages of these steps: their numbers and scales
     if (pg0 != page0) {
       my_page = entry(min(pg0 + tid, page_last));
@@ -772,12 +733,23 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     kss[tid] = my_page >= 0 ? my_ks : 0.0f;
     vss[tid] = my_page >= 0 ? my_vs : 0.0f;
     sync();
-    // steps from here on count from page pg0's first (below kAttnPages * 8): the quotient by page_steps is exact
-    const int c0 = pg0 * page_steps, e0 = max(s0 - c0, 0), e1 = min(s1 - c0, kPages * page_steps);
-    auto page_of = [&](int s) { return (int)((unsigned)s * page_inv >> 16); };
+    // steps from here on count from page pg0's first (below kAttnPages * 8): the quotient by page_steps is exact. SINKS: they
+    // go on counting within the list, and the window's are taken from page pg0's first, or the window's first, for the quotient
+    const int c0 = SINKS ? 0 : pg0 * page_steps, e0 = SINKS ? max(s0, first_step(pg0)) : max(s0 - c0, 0);
+    const int e1 = SINKS ? min(s1, first_step(pg0 + kPages)) : min(s1 - c0, kPages * page_steps);
+    const int win_from = tile.sinks - win_off + max(pg0 - sink_pages, 0) * page_steps;
+    const int win_at = max(sink_pages - pg0, 0);
+    auto page_of = [&](int s, int& in_page) {
+      const bool sink = SINKS && s < tile.sinks;
+      if (SINKS && !sink) s -= win_from;
+      const int pi = (int)((unsigned)s * page_inv >> 16);
+      in_page = s - pi * page_steps;
+      return SINKS ? (sink ? pi - pg0 : pi + win_at) : pi;
+    };
     auto next_block = [&](const int8_t* base, int s) {
-      const int pi = page_of(s);
-      return block(base, ids[pi], s - pi * page_steps);
+      int in_page;
+      const int pi = page_of(s, in_page);
+      return block(base, ids[pi], in_page);
     };
     int s = e0 + w;
     if (pg0 != page0 && s < e1) {
@@ -786,7 +758,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
     }
     for (; s < e1; s += kW) {
       const int next = min(s + kW, e1 - 1);
-      const int pi = page_of(s), key0 = 32 * (s + c0);
+      int in_page;
+      const int pi = page_of(s, in_page), key0 = 32 * (SINKS && s >= tile.sinks ? s - tile.sinks + tile.first : s + c0);
       const bool have = ids[pi] >= 0;
       const float ks = kss[pi], vs = vss[pi];
       f32x4 st[VT][2] = {};
@@ -808,7 +781,8 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
       load(next_block(c.k, next), kf);
       // f > 0, so the largest product is the largest score (0 would make NaN of the hidden ones' -inf)
       float f[VT], mx[VT];
-      const bool hides = !have || key0 + 31 > see_all || key0 < see_from;      // some vector does not see some key
+      // some vector does not see some key
+      const bool hides = !have || key0 + 31 > see_all || (key0 < see_from && (!SINKS || key0 + 31 >= a.sinks));
       if (hides) {
 #pragma unroll
         for (int v = 0; v < VT; ++v) {
@@ -816,7 +790,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int j = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
-            if (!have || j > pos[v] || j < low) st[v][e >> 2][e & 3] = -INFINITY;
+            if (!have || j > pos[v] || (j < low && (!SINKS || j >= a.sinks))) st[v][e >> 2][e & 3] = -INFINITY;
           }
         }
       }
@@ -942,6 +916,7 @@ __global__ __launch_bounds__(256) void attention_kv8_kernel(PagedBatch b, Kv8Cac
         a.work[2 * mine] = M;
         a.work[2 * mine + 1] = L;
       }
+      if (SINKS && whole && a.lse && (tid & 15) == 0) a.lse[at] = lse_of(M, L);
     }
   }
 }
@@ -999,6 +974,7 @@ __global__ __launch_bounds__(256) void attention_kv8_join_few_kernel(PagedBatch 
       y.z = __builtin_fmaf(x.z, f, y.z);
       y.w = __builtin_fmaf(x.w, f, y.w);
     }
+    if (a.lse && col == 0) a.lse[at] = lse_of(M, L);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     *reinterpret_cast<float4*>(a.ctx + at * hd + 4 * col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
   }
@@ -1056,6 +1032,7 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
     y.z += x.z;
     y.w += x.w;
   }
+  if (a.lse && tid == 0) a.lse[at] = lse_of(M, L);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   *reinterpret_cast<float4*>(a.ctx + at * hd + 4 * tid) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
@@ -1064,8 +1041,8 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(PagedBatch b, K
 constexpr int most_groups(int hd) { return hd <= 128 ? 4 : 2; }
 
 // (a window only ever makes the workspace smaller)
-static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int window, int heads, int kv_heads,
-                            int hd) {
+static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, int window, int sinks, int heads,
+                            int kv_heads, int hd) {
   AttnTiles t;
   t.grp = heads / kv_heads;
   const long vecs = (long)max_rows * t.grp;
@@ -1092,7 +1069,7 @@ static AttnTiles attn_tiles(int rows, int requests, int max_rows, int max_len, i
   // up to 4096, 8 of 128 268 / 247)
   t.solo = t.listed && t.vecs == 16 && max_len <= 2048 && requests * ht >= 4L * max_len;
   long steps = (std::max(max_len, 1) + 31) / 32;                   // of the longest tile
-  if (window > 0) steps = std::min(steps, ((long)window + t.rows_per - 2) / 32 + 2);
+  if (window > 0) steps = std::min(steps, ((long)window + t.rows_per - 2) / 32 + 2 + ((long)sinks + 31) / 32);
   // two workgroups of a piece for each CU, four of heads up to 64, whose steps are half as many bytes on their way (us of
   // 512 / 1024 / 1536: one request of 131071 tokens, 8 heads of 128 50.5 / 53.7 / 56, 64 of up to 16384, 4 of 128 35.4 /
   // 41 / 42; but one of 131071, 2 of 64 17.5 / 16.8 / 16.8, 128 of up to 8000, 4 of 64 32.7 / 24.4 / 26.7, 300, 2 of 32
@@ -1119,24 +1096,32 @@ static size_t attn_workgroups(const AttnTiles& t, int kv_heads) {
 }
 
 size_t attention_kv8_workgroups(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
-  return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, 0, heads, kv_heads, hd), kv_heads);
+  return attn_workgroups(attn_tiles(rows, requests, max_rows, max_len, 0, 0, heads, kv_heads, hd), kv_heads);
 }
 
 size_t attention_kv8_work_floats(int rows, int requests, int max_rows, int max_len, int heads, int kv_heads, int hd) {
-  const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, 0, heads, kv_heads, hd);
+  const AttnTiles t = attn_tiles(rows, requests, max_rows, max_len, 0, 0, heads, kv_heads, hd);
   return t.list + (t.listed ? 4 * (size_t)t.slots : 0);
 }
 
+template <int NB, bool SINKS>
+static void launch_attention_as(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, const AttnTiles& t,
+                                unsigned workgroups, hipStream_t s) {
+  auto* k = t.solo ? attention_kv8_kernel<NB, 1, true, SINKS> : t.vecs == 16 ? attention_kv8_kernel<NB, 1, false, SINKS>
+          : t.vecs == 32 ? attention_kv8_kernel<NB, 2, false, SINKS>
+                         : attention_kv8_kernel<NB, most_groups(32 * NB), false, SINKS>;
+  hipLaunchKernelGGL(k, dim3(workgroups), dim3(256), 0, s, b, c, a, t);
+}
+// (sinks behind a window, and the sums of exponentials, are another kernel, so that the plain one keeps its registers)
 template <int NB>
 static void launch_attention_hd(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, const AttnTiles& t,
                                 unsigned workgroups, hipStream_t s) {
-  auto* k = t.solo ? attention_kv8_kernel<NB, 1, true> : t.vecs == 16 ? attention_kv8_kernel<NB, 1, false>
-          : t.vecs == 32 ? attention_kv8_kernel<NB, 2, false> : attention_kv8_kernel<NB, most_groups(32 * NB), false>;
-  hipLaunchKernelGGL(k, dim3(workgroups), dim3(256), 0, s, b, c, a, t);
+  if (a.sinks > 0 || a.lse) launch_attention_as<NB, true>(b, c, a, t, workgroups, s);
+  else launch_attention_as<NB, false>(b, c, a, t, workgroups, s);
 }
 
 hipError_t launch_attention_kv8(const PagedBatch& b, const Kv8Cache& c, const Attn8Args& a, hipStream_t s) {
-  const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.window, a.heads, c.kv_heads, c.hd);
+  const AttnTiles t = attn_tiles(b.rows, b.requests, a.max_rows, a.max_len, a.window, a.sinks, a.heads, c.kv_heads, c.hd);
   const unsigned heads = (unsigned)(c.kv_heads * t.group_tiles);
   const unsigned n = (unsigned)attn_workgroups(t, c.kv_heads);
   if (t.listed) {

@@ -53,17 +53,6 @@ __device__ __forceinline__ void scan3(int (&v)[3], int (&tot)[3]) {
   __syncthreads();
 }
 
-// the last of list[0 .. n) (ascending, list[0] <= x) that is at most x
-__device__ __forceinline__ int last_at_most(const int* list, int n, int x) {
-  int lo = 0, hi = n;                      // list[lo] <= x < list[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (list[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // seq, pos and slot of row t from the finished plan; rows that no request of the step owns get -1
 __device__ __forceinline__ void plan_row(const PlanArgs& a, const int* start, const int* count, const int* len, int t) {
   const int b = last_at_most(start, a.requests, t), n = count[b], i = t - start[b];

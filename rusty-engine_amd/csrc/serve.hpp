@@ -72,6 +72,8 @@ struct LogprobArgs {
 };
 
 constexpr int kLogprobsMaxTop = 64;
+constexpr size_t kAttnMaxSinks = 1024;     // their pages, and a few more, are staged at once
+constexpr size_t kMassMaxWorkgroups = (size_t)1 << 23;
 
 struct Attn8Args {
   const float* q;
@@ -80,9 +82,80 @@ struct Attn8Args {
   size_t ldq;
   float scale;
   int window, heads, max_rows, max_len;
+  int sinks;                 // first tokens that every row sees (0: none), of no effect without a window
+  float* lse;                // ln of each row and head's sum of exponentials, or null
+};
+
+// What attention leaves in the cache's masses: of every page, KV head and place the weight that it has got.
+struct MassArgs {
+  const float* q;
+  const float* lse;
+  float* mass;
+  size_t ldq;
+  float scale;
+  int window, sinks, heads, max_rows, max_len;
+};
+
+struct EvictPlanArgs {
+  const int* len;
+  const int* table;
+  const int* free_pages;
+  const int* n_free;
+  int* len_out;
+  int* table_out;
+  int* free_out;
+  int* n_free_out;
+  int* from_len;
+  int* from_table;
+  int* dropped;
+  int* status;
+  int requests, page, table_ld, n_pages, limit, keep;
+};
+
+struct EvictArgs {
+  const int* from_len;
+  const int* from_table;
+  const int* table;
+  float* mass;
+  int* kept;
+  int requests, table_ld, page, n_pages, keep, first, recent, max_len;
+};
+
+struct RewindArgs {
+  const int* back;
+  const int* len;
+  const int* table;
+  int* free_pages;
+  const int* n_free;
+  int* len_out;
+  int* n_free_out;
+  int requests, page, table_ld, n_pages;
+};
+
+struct VerifyArgs {
+  const float* x;
+  const int* start;
+  const int* count;
+  const int* tokens;
+  const float* probs;
+  const float* temperature;
+  const float* accept_u;
+  const float* sample_u;
+  int* accepted;
+  int* back;
+  int* out;
+  void* work;
+  size_t ld, ldp;
+  int rows, vocab, requests;
 };
 
 hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
+hipError_t launch_kv_evict_plan(const EvictPlanArgs& a, hipStream_t s);
+hipError_t launch_kv_rewind(const RewindArgs& a, hipStream_t s);
+hipError_t launch_kv8_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s);
+hipError_t launch_kv8_evict(const EvictArgs& a, const Kv8Cache& c, hipStream_t s);
+size_t verify_work_bytes(int rows, int requests, int vocab);
+hipError_t launch_verify(const VerifyArgs& a, hipStream_t s);
 hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s);
 size_t logprobs_work_floats(int rows, int vocab, int k);
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s);
@@ -101,6 +174,17 @@ struct RequestRows {
 __device__ __forceinline__ RequestRows request_rows(int r, int start, int count, int len, int rows) {
   const int row0 = min(max(start, 0), rows);
   return {r, row0, min(max(count, 0), rows - row0), len};
+}
+
+// the last of list[0 .. n) (ascending, list[0] <= x) that is at most x
+__device__ __forceinline__ int last_at_most(const int* list, int n, int x) {
+  int lo = 0, hi = n;                      // list[lo] <= x < list[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (list[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
 // lane l's of a wave, in every lane (l the same in all of them)

@@ -64,6 +64,34 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v + lane_xor<1>(v);
 }
 
+// inclusive sums over the lanes of a wave
+__device__ __forceinline__ int wave_scan(int v) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(v, off, 64);
+    if ((int)(threadIdx.x & 63) >= off) v += y;
+  }
+  return v;
+}
+
+// The sum over a workgroup of WAVES waves, and in `before` that of the threads below this one.
+template <int WAVES>
+__device__ __forceinline__ int scan_block(int v, int& before) {
+  __shared__ int part[WAVES];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, inc = wave_scan(v);
+  if (lane == 63) part[w] = inc;
+  __syncthreads();
+  int all = 0;
+  before = inc - v;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    before += i < w ? part[i] : 0;
+    all += part[i];
+  }
+  __syncthreads();
+  return all;
+}
+
 // What the wave's lanes wrote to LDS before this, all its lanes read after it. LDS serves a wave in order, so this is
 // no instruction: it keeps the compiler from moving or reusing reads across it.
 __device__ __forceinline__ void wave_sync() {
