@@ -15,15 +15,16 @@ namespace rehip {
 // leaves nothing, from p); behind the last draft it comes from p. Drawn: the lowest t with sum over j <= t of w_j > r W.
 //
 // Which token r falls on depends on sums over the whole vocabulary to about 1 / vocab of a share each: with sums off by
-// 2^-24 one row in a hundred of 151936 would draw a neighbour. So exponentials and sums are in 64 bits: 2^y by its
-// Taylor series at the nearest integer, |f| <= 1/2, 13 terms, off by (ln 2 / 2)^13 / 13! = 2e-16.
+// 2^-24 one row in a hundred of 151936 would draw a neighbour. So exponentials and sums are in 64 bits. 2^(k / 256 + f / 256),
+// |f| <= 1/2: from a table of 256 in LDS and the series of 2^(f / 256) - 1 to its third power, off by (ln 2 / 512)^4 / 24 = 1.4e-13.
 //
 // Three launches: maxima and sums of parts of all rows; every request's last row found from them, and the sums of its
-// weights by parts of the vocabulary; the part where r falls, and the token in it.
+// weights by blocks of the vocabulary; the block where r falls, and the token in it.
 constexpr int kVerWaves = 4;
-constexpr int kVerBatch = 8;             // logits of a lane at a time
+constexpr int kVerBatch = 16;            // logits of a lane at a time
 constexpr int kVerStep = 64 * kVerBatch * kVerWaves;
 constexpr int kVerParts = 64;            // a lane each
+constexpr int kVerTable = 256;
 
 struct RowPart {
   double z;                              // sum of 2^((x - m) c)
@@ -39,6 +40,9 @@ struct Decision {
 };
 constexpr int kNone = 0, kGreedy = 1, kTarget = 2, kRest = 3;  // no distribution; the largest; p; p without the draft
 
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// 2^y, y <= 0: the series at the nearest integer, 13 terms, off by (ln 2 / 2)^13 / 13! = 2e-16
 __device__ __forceinline__ double pow2_64(double y) {
   y = fmax(y, -1100.0);
   const double n = rint(y), f = (y - n) * 0.69314718055994530942;
@@ -58,123 +62,164 @@ __device__ __forceinline__ double pow2_64(double y) {
   return ldexp(p, (int)n);
 }
 
-__device__ __forceinline__ double lane_xor64(double v, int off) {
-  const int lo = __shfl_xor(__double2loint(v), off, 64), hi = __shfl_xor(__double2hiint(v), off, 64);
-  return __hiloint2double(hi, lo);
+// The table: 2^(i / 256). All threads of the workgroup call it.
+template <int THREADS>
+__device__ __forceinline__ void fill_table(double* table) {
+  for (int i = threadIdx.x; i < kVerTable; i += THREADS) table[i] = 2.0 * pow2_64((double)(i - kVerTable) / kVerTable);
+  __syncthreads();
+}
+
+// 2^((x - m) c), c256 = 256 c; what is below 2^-1000 comes out as that
+__device__ __forceinline__ double share_of(float x, double m, double c256, const double* table) {
+  constexpr double kRound = 6755399441055744.0;                // 1.5 2^52: a sum's low word is then the nearest integer
+  constexpr double k1 = 0.69314718055994530942 / kVerTable, k2 = k1 * k1 / 2.0, k3 = k1 * k1 * k1 / 6.0;
+  const double y = fmax(((double)x - m) * c256, -1000.0 * kVerTable), t = y + kRound;
+  const double f = y - (t - kRound);
+  const int n = __double2loint(t);
+  const double b = table[n & (kVerTable - 1)];
+  const double q = f * fma(f, fma(f, k3, k2), k1), w = fma(b, q, b);
+  return __hiloint2double(__double2hiint(w) + (n >> 8) * (1 << 20), __double2loint(w));
+}
+// .. and exactly 0 there and for a logit of -inf
+__device__ __forceinline__ double weight_of(float x, double m, double c256, const double* table) {
+  const double w = share_of(x, m, c256, table);
+  return x == -INFINITY || ((double)x - m) * c256 < -1000.0 * kVerTable ? 0.0 : w;
+}
+
+template <int OFF>
+__device__ __forceinline__ double lane_xor64(double v) {
+  return __hiloint2double((int)lane_xor_u32<OFF>((unsigned)__double2hiint(v)), (int)lane_xor_u32<OFF>((unsigned)__double2loint(v)));
 }
 __device__ __forceinline__ double wave_sum64(double v) {
+  wave_butterfly([&](auto off) { v += lane_xor64<decltype(off)::value>(v); });
+  return v;
+}
+// inclusive sums over the lanes of a wave
+__device__ __forceinline__ double wave_scan64(double v) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += lane_xor64(v, off);
+  for (int off = 1; off < 64; off <<= 1) {
+    const double y = __hiloint2double(__shfl_up(__double2hiint(v), off, 64), __shfl_up(__double2loint(v), off, 64));
+    if ((int)(threadIdx.x & 63) >= off) v += y;
+  }
   return v;
 }
 
-// powers of 2 for each unit of logit; greedy below 0
+// 256 powers of 2 for each unit of logit; greedy below 0
 __device__ __forceinline__ double units_of(const VerifyArgs& a, int req) {
   const float t = a.temperature ? a.temperature[req] : 1.0f;
-  return t > 0.0f ? 1.4426950408889634074 / (double)t : -1.0;
-}
-// 2^((x - m) c), 0 for a logit of -inf
-__device__ __forceinline__ double weight(float x, float m, double c) {
-  return x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)m) * c);
+  return t > 0.0f ? kVerTable * 1.4426950408889634074 / (double)t : -1.0;
 }
 
 __device__ __forceinline__ PagedBatch rows_of(const VerifyArgs& a) {
   return {a.start, a.count, a.count, nullptr, a.requests, a.rows, 1, 1, 1};
 }
 
+// A wave's lanes joined, the same in every lane: sums of shares to the largest maximum.
+__device__ __forceinline__ RowPart joined_wave(const RowPart& p, double c256) {
+  const float m = wave_max(p.m);
+  double z = 0.0;
+  if (c256 >= 0.0) z = wave_sum64(p.m > -INFINITY ? p.z * pow2_64(((double)p.m - (double)m) * (c256 / kVerTable)) : 0.0);
+  int best = p.m == m ? p.best : 0x7fffffff, bad = p.bad;
+  wave_butterfly([&](auto off) {
+    constexpr int X = decltype(off)::value;
+    best = min(best, (int)lane_xor_u32<X>((unsigned)best));
+    bad |= (int)lane_xor_u32<X>((unsigned)bad);
+  });
+  return {z, m, best, bad, 0};
+}
+
 // One workgroup per (row, part).
 __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs a, int parts) {
+  __shared__ double table[kVerTable];
   __shared__ RowPart ws[kVerWaves];
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
   const RequestRows q = request_of_unit(r, rows_of(a), 1, 0);
   if (q.req < 0 || r >= q.row0 + q.count) return;
-  const double c = units_of(a, q.req);
+  const double c256 = units_of(a, q.req);
   const float* x = a.x + (size_t)r * a.ld;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int steps = (a.vocab + kVerStep - 1) / kVerStep;
   const int s0 = (int)((long long)steps * part / parts), s1 = (int)((long long)steps * (part + 1) / parts);
-  RowPart mine{0.0, -INFINITY, 0x7fffffff, 0, 0};
-  for (int s = s0; s < s1; ++s) {
-    const int base = s * kVerStep + w * 64 * kVerBatch + lane;
-    float v[kVerBatch], mx = -INFINITY;
+  // element k of a lane in step s: whole steps by fours
+  auto place = [&](int s, int k) { return s * kVerStep + w * 64 * kVerBatch + 256 * (k >> 2) + 4 * lane + (k & 3); };
+  auto load = [&](int s, float (&v)[kVerBatch]) {
+    if ((s + 1) * kVerStep <= a.vocab) {
 #pragma unroll
-    for (int k = 0; k < kVerBatch; ++k) {
-      const int at = base + 64 * k;
-      const float y = x[min(at, a.vocab - 1)];
-      v[k] = at < a.vocab ? y : -INFINITY;
+      for (int k = 0; k < kVerBatch; k += 4)
+        *reinterpret_cast<f32x4u*>(&v[k]) = *reinterpret_cast<const f32x4u*>(x + place(s, k));
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVerBatch; ++k) {
+        const int at = place(s, k);
+        const float y = x[min(at, a.vocab - 1)];
+        v[k] = at < a.vocab ? y : -INFINITY;
+      }
     }
+  };
+  RowPart mine{0.0, -INFINITY, 0x7fffffff, 0, 0};
+  float v[kVerBatch], nx[kVerBatch];
+  if (s0 < s1) load(s0, v);
+  fill_table<64 * kVerWaves>(table);
+  for (int s = s0; s < s1; ++s) {
+    load(min(s + 1, s1 - 1), nx);
+    float mx = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kVerBatch; ++k) {
       mine.bad |= !(v[k] < INFINITY);
       mx = fmaxf(mx, v[k]);
     }
     if (mx > mine.m) {
-      mine.z *= mine.m == -INFINITY ? 0.0 : weight(mine.m, mx, fabs(c));
+      if (c256 >= 0.0 && mine.m > -INFINITY) mine.z *= share_of(mine.m, (double)mx, c256, table);
       mine.m = mx;
 #pragma unroll
       for (int k = kVerBatch - 1; k >= 0; --k)
-        if (v[k] == mx) mine.best = base + 64 * k;
+        if (v[k] == mx) mine.best = place(s, k);
     }
-    if (c >= 0.0 && mine.m > -INFINITY) {
+    if (c256 >= 0.0 && mine.m > -INFINITY) {
+      double z[4] = {};
+      const double m = (double)mine.m;
 #pragma unroll
-      for (int k = 0; k < kVerBatch; ++k) mine.z += weight(v[k], mine.m, c);
+      for (int k = 0; k < kVerBatch; ++k) z[k & 3] += share_of(v[k], m, c256, table);
+      mine.z += (z[0] + z[1]) + (z[2] + z[3]);
     }
+#pragma unroll
+    for (int k = 0; k < kVerBatch; ++k) v[k] = nx[k];
   }
-  auto join = [&](const RowPart& x, const RowPart& y) {
-    RowPart o{0.0, fmaxf(x.m, y.m), x.m > y.m ? x.best : y.m > x.m ? y.best : min(x.best, y.best), x.bad | y.bad, 0};
-    if (x.m > -INFINITY) o.z += x.z * weight(x.m, o.m, fabs(c));
-    if (y.m > -INFINITY) o.z += y.z * weight(y.m, o.m, fabs(c));
-    return o;
-  };
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1)
-    mine = join(mine, RowPart{lane_xor64(mine.z, off), __shfl_xor(mine.m, off, 64), __shfl_xor(mine.best, off, 64),
-                              __shfl_xor(mine.bad, off, 64), 0});
-  if (lane == 0) ws[w] = mine;
+  const RowPart all = joined_wave(mine, c256);
+  if (lane == 0) ws[w] = all;
   __syncthreads();
-  if (threadIdx.x == 0)
-    reinterpret_cast<RowPart*>(a.work)[blockIdx.x] = join(join(ws[0], ws[1]), join(ws[2], ws[3]));
-}
-
-// A row's parts joined, the same in every lane.
-__device__ __forceinline__ RowPart joined_row(const VerifyArgs& a, int row, int parts, double c) {
-  const int lane = threadIdx.x & 63;
-  RowPart p = reinterpret_cast<const RowPart*>(a.work)[(size_t)row * parts + min(lane, parts - 1)];
-  if (lane >= parts) p = {0.0, -INFINITY, 0x7fffffff, 0, 0};
-  float m = wave_max(p.m);
-  const double z = wave_sum64(p.m > -INFINITY ? p.z * weight(p.m, m, fabs(c)) : 0.0);
-  int best = p.m == m ? p.best : 0x7fffffff, bad = p.bad;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    best = min(best, __shfl_xor(best, off, 64));
-    bad |= __shfl_xor(bad, off, 64);
+  if (w == 0) {
+    const RowPart p = lane < kVerWaves ? ws[lane] : RowPart{0.0, -INFINITY, 0x7fffffff, 0, 0};
+    const RowPart o = joined_wave(p, c256);
+    if (lane == 0) reinterpret_cast<RowPart*>(a.work)[blockIdx.x] = o;
   }
-  return {z, m, best, bad | (m == -INFINITY), 0};
 }
 
 // How many drafts of a request are accepted, and where its next token comes from. Every wave of the workgroup looks at a row of
 // its own at a time.
 template <int WAVES>
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& q, int parts) {
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& q, double c256, int parts) {
   __shared__ Decision found[WAVES];
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const double c = units_of(a, q.req);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Decision d{};
   for (int i0 = 0; i0 < q.count; i0 += WAVES) {
     const int i = i0 + w, row = q.row0 + min(i, q.count - 1);
-    const RowPart p = joined_row(a, row, parts, c);
+    const bool drafted = i < q.count - 1;
+    // (the draft's logit and probability are on their way with the row's parts)
+    const int t = drafted ? a.tokens[row + 1] : 0, at = min(max(t, 0), a.vocab - 1);
+    const float x = a.x[(size_t)row * a.ld + at], share = a.probs ? a.probs[(size_t)row * a.ldp + at] : 1.0f;
+    const float u = a.accept_u[row];
+    RowPart p = reinterpret_cast<const RowPart*>(a.work)[(size_t)row * parts + min(lane, parts - 1)];
+    if (lane >= parts) p = {0.0, -INFINITY, 0x7fffffff, 0, 0};
+    p = joined_wave(p, c256);
+    const bool none = p.bad || p.m == -INFINITY;
     bool accepted = false;
-    if (i < q.count - 1 && !p.bad) {
-      const int t = a.tokens[row + 1];
-      if (c < 0.0) {
-        accepted = t == p.best;
-      } else if (t >= 0 && t < a.vocab) {
-        const double share = a.probs ? (double)a.probs[(size_t)row * a.ldp + t] : 1.0;
-        accepted = (double)a.accept_u[row] * share * p.z < weight(a.x[(size_t)row * a.ld + t], p.m, c);
-      }
-    }
-    if ((threadIdx.x & 63) == 0)
-      found[w] = {p.z, p.m, accepted ? -1 : i, row, p.bad ? kNone : c < 0.0 ? kGreedy : i < q.count - 1 ? kRest : kTarget, p.best, 0};
+    if (drafted && !none && t == at)
+      accepted = c256 < 0.0 ? t == p.best
+                            : (double)u * (double)share * p.z <
+                                  (x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)p.m) * (c256 / kVerTable)));
+    if (lane == 0)
+      found[w] = {p.z, p.m, accepted ? -1 : i, row, none ? kNone : c256 < 0.0 ? kGreedy : drafted ? kRest : kTarget, p.best, 0};
     __syncthreads();
     bool done = false;
 #pragma unroll
@@ -189,108 +234,162 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
   return d;
 }
 
-// The weight of token t: p, less the draft's share of it
+// The weight of token t, of logit x and the draft's probability there: p, less the draft's share of it
 struct Weights {
   const float* x;
   const float* probs;                    // the draft's row, or null
-  double c, z;
-  float m;
+  double c256, m, inverse;               // 1 / z
   int drop;                              // a draft without a distribution: this token has no weight (-1: none)
-  __device__ __forceinline__ double operator()(int t) const {
-    const double e = weight(x[t], m, c);
-    if (probs) return fmax(e / z - (double)probs[t], 0.0);
+  const double* table;
+  __device__ __forceinline__ double operator()(int t, float xt, float qt) const {
+    const double e = weight_of(xt, m, c256, table);
+    if (probs) return fmax(fma(e, inverse, -(double)qt), 0.0);
     return t == drop ? 0.0 : e;
   }
 };
-__device__ __forceinline__ Weights weights_of(const VerifyArgs& a, const Decision& d, double c, bool rest) {
+__device__ __forceinline__ Weights weights_of(const VerifyArgs& a, const Decision& d, double c256, bool rest, const double* table) {
   const int t = rest && !a.probs ? a.tokens[d.row + 1] : -1;
-  return {a.x + (size_t)d.row * a.ld, rest && a.probs ? a.probs + (size_t)d.row * a.ldp : nullptr, c, d.z, d.m, t};
+  return {a.x + (size_t)d.row * a.ld, rest && a.probs ? a.probs + (size_t)d.row * a.ldp : nullptr, c256, (double)d.m,
+          1.0 / d.z, t, table};
 }
 
 __device__ __forceinline__ Decision* decisions_at(const VerifyArgs& a, int parts) {
   return reinterpret_cast<Decision*>(reinterpret_cast<RowPart*>(a.work) + (size_t)a.rows * parts);
 }
-
-// One workgroup per (request, part of the vocabulary): the sum of its weights.
-constexpr int kRestWaves = 4;
-__global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs a, int parts, int cuts) {
-  __shared__ double sums[kRestWaves];
-  const int req = blockIdx.x / cuts, cut = blockIdx.x % cuts, tid = threadIdx.x;
-  const RequestRows q = request_rows(req, a.start[req], a.count[req], 0, a.rows);
-  if (q.count <= 0) return;
-  const Decision d = decide<kRestWaves>(a, q, parts);
-  Decision* const at = decisions_at(a, parts);
-  if (cut == 0 && tid == 0) at[req] = d;
-  if (d.state != kTarget && d.state != kRest) return;
-  const Weights of = weights_of(a, d, units_of(a, req), d.state == kRest);
-  const int t0 = (int)((long long)a.vocab * cut / cuts), t1 = (int)((long long)a.vocab * (cut + 1) / cuts);
-  double s = 0.0;
-  for (int t = t0 + tid; t < t1; t += 64 * kRestWaves) s += of(t);
-  s = wave_sum64(s);
-  if ((tid & 63) == 0) sums[tid >> 6] = s;
-  __syncthreads();
-  if (tid == 0) reinterpret_cast<double*>(at + a.requests)[(size_t)req * cuts + cut] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+__device__ __forceinline__ double* sums_at(const VerifyArgs& a, int parts) {
+  return reinterpret_cast<double*>(decisions_at(a, parts) + a.requests);
 }
 
-// The lowest token of t0 .. t1 - 1 whose running sum, from `from` on, is above `target`; the last with any weight if rounding
-// leaves none (-1: no weight at all). All threads call it.
-constexpr int kDrawThreads = 512;
-__device__ __forceinline__ int draw_from(const Weights& of, int t0, int t1, double from, double target) {
-  __shared__ double part[kDrawThreads / 64];
-  __shared__ int lowest[kDrawThreads / 64], highest[kDrawThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int per = (t1 - t0 + kDrawThreads - 1) / kDrawThreads, a0 = min(t0 + tid * per, t1), a1 = min(a0 + per, t1);
-  double s = 0.0;
+// One workgroup per (request, run of blocks of the vocabulary), a block to a wave at a time: the sums of their weights.
+constexpr int kRestWaves = 8;
+constexpr int kBlock = 1024;             // tokens of a block
+__global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs a, int parts, int cuts, int blocks) {
+  __shared__ double table[kVerTable];
+  const int req = blockIdx.x / cuts, cut = blockIdx.x % cuts, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const RequestRows q = request_rows(req, a.start[req], a.count[req], 0, a.rows);
+  if (q.count <= 0) return;
+  const double c256 = units_of(a, req);
+  const Decision d = decide<kRestWaves>(a, q, c256, parts);
+  if (cut == 0 && threadIdx.x == 0) decisions_at(a, parts)[req] = d;
+  if (d.state != kTarget && d.state != kRest) return;
+  const Weights of = weights_of(a, d, c256, d.state == kRest, table);
+  fill_table<64 * kRestWaves>(table);
+  const int b0 = (int)((long long)blocks * cut / cuts), b1 = (int)((long long)blocks * (cut + 1) / cuts);
+  for (int b = b0 + w; b < b1; b += kRestWaves) {
+    float x[16], p[16];
+    auto place = [&](int k) { return b * kBlock + 256 * (k >> 2) + 4 * lane + (k & 3); };
+    if ((b + 1) * kBlock <= a.vocab) {
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        *reinterpret_cast<f32x4u*>(&x[k]) = *reinterpret_cast<const f32x4u*>(of.x + place(k));
+        if (of.probs) *reinterpret_cast<f32x4u*>(&p[k]) = *reinterpret_cast<const f32x4u*>(of.probs + place(k));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int t = min(place(k), a.vocab - 1);
+        x[k] = place(k) < a.vocab ? of.x[t] : -INFINITY;
+        p[k] = of.probs ? of.probs[t] : 0.0f;
+      }
+    }
+    double s[4] = {};
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s[k & 3] += of(place(k), x[k], p[k]);
+    const double all = wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
+    if (lane == 0) sums_at(a, parts)[(size_t)req * blocks + b] = all;
+  }
+}
+
+// Exclusive sums over a workgroup of WAVES waves; the total in `all`.
+template <int WAVES>
+__device__ __forceinline__ double scan_block64(double v, double& all) {
+  __shared__ double part[WAVES];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const double inc = wave_scan64(v);
+  if (lane == 63) part[w] = inc;
+  __syncthreads();
+  double before = 0.0;
+  all = 0.0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    before += i < w ? part[i] : 0.0;
+    all += part[i];
+  }
+  __syncthreads();
+  return before + (inc - v);
+}
+// the least over the workgroup, and the largest
+template <int WAVES>
+__device__ __forceinline__ int2 ends_block(int low, int high) {
+  __shared__ int part[2][WAVES];
+  wave_butterfly([&](auto off) {
+    constexpr int X = decltype(off)::value;
+    low = min(low, (int)lane_xor_u32<X>((unsigned)low));
+    high = max(high, (int)lane_xor_u32<X>((unsigned)high));
+  });
+  const int w = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    part[0][w] = low;
+    part[1][w] = high;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    low = min(low, part[0][i]);
+    high = max(high, part[1][i]);
+  }
+  __syncthreads();
+  return make_int2(low, high);
+}
+
+// Of places t0 .. t1 - 1 with value(t) each the lowest whose running sum, from `from` on, is above `target`, or the last with
+// a value above 0 if rounding leaves none (-1: there is none at all); `upto`: the sum of the places before it. A thread has
+// `per` places that follow one another. All threads call it.
+constexpr int kDrawWaves = 4;
+template <class F>
+__device__ __forceinline__ int first_above(F value, int t0, int t1, int per, double from, double target, double& upto) {
+  __shared__ double found;
+  const int a0 = min(t0 + (int)threadIdx.x * per, t1), a1 = min(a0 + per, t1);
+  double s = 0.0, all;
   int some = -1;
   for (int t = a0; t < a1; ++t) {
-    const double v = of(t);
+    const double v = value(t);
     s += v;
     if (v > 0.0) some = t;
   }
-  double inc = s;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double y = __hiloint2double(__shfl_up(__double2hiint(inc), off, 64), __shfl_up(__double2loint(inc), off, 64));
-    if (lane >= off) inc += y;
-  }
-  if (lane == 63) part[w] = inc;
-  __syncthreads();
-  double before = from;
-  for (int i = 0; i < w; ++i) before += part[i];
-  const double start = before + (inc - s);
+  double run = from + scan_block64<kDrawWaves>(s, all), before = run;
+  const int last = some;
   int low = 0x7fffffff;
-  if (before + inc > target || start > target) {
-    double run = start;
+  if (some >= 0 && !(run + s <= target)) {
     for (int t = a0; t < a1; ++t) {
-      const double v = of(t);
-      run += v;
-      if (v > 0.0 && run > target) {
+      const double v = value(t);
+      if (v > 0.0 && run + v > target) {
         low = t;
         break;
       }
+      run += v;
     }
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    low = min(low, __shfl_xor(low, off, 64));
-    some = max(some, __shfl_xor(some, off, 64));
-  }
-  if (lane == 0) {
-    lowest[w] = low;
-    highest[w] = some;
-  }
-  __syncthreads();
-  for (int i = 0; i < kDrawThreads / 64; ++i) {
-    low = min(low, lowest[i]);
-    some = max(some, highest[i]);
+  const int2 e = ends_block<kDrawWaves>(low, some);
+  const int at = e.x < 0x7fffffff ? e.x : e.y;
+  if (at >= 0 && (e.x < 0x7fffffff ? low == at : last == at)) {
+    if (e.x == 0x7fffffff) {             // (up to the last one)
+      run = before;
+      for (int t = a0; t < at; ++t) run += value(t);
+    }
+    found = run;
   }
   __syncthreads();
-  return low < 0x7fffffff ? low : some;
+  upto = found;
+  __syncthreads();
+  return at;
 }
 
 // One workgroup per request: the token, and the request's outputs.
-__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a, int parts, int cuts) {
-  const int req = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+__global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs a, int parts, int blocks) {
+  constexpr int kThreads = 64 * kDrawWaves;
+  __shared__ double table[kVerTable];
+  const int req = blockIdx.x, tid = threadIdx.x;
   const RequestRows q = request_rows(req, a.start[req], a.count[req], 0, a.rows);
   if (q.count <= 0) {
     if (tid == 0) a.accepted[req] = a.back[req] = 0;
@@ -299,29 +398,24 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a,
   const Decision d = decisions_at(a, parts)[req];
   int token = d.state == kGreedy ? d.best : -1;
   if (d.state == kTarget || d.state == kRest) {
-    const double c = units_of(a, req), r = (double)a.sample_u[req];
-    const Weights of = weights_of(a, d, c, d.state == kRest);
-    const double* sums = reinterpret_cast<const double*>(decisions_at(a, parts) + a.requests) + (size_t)req * cuts;
-    const double mine = lane < cuts ? sums[lane] : 0.0;
-    double inc = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double y = __hiloint2double(__shfl_up(__double2hiint(inc), off, 64), __shfl_up(__double2loint(inc), off, 64));
-      if (lane >= off) inc += y;
-    }
-    const double all = __hiloint2double(__shfl(__double2hiint(inc), 63, 64), __shfl(__double2loint(inc), 63, 64));
+    const double c256 = units_of(a, req), r = (double)a.sample_u[req];
+    const double* sums = sums_at(a, parts) + (size_t)req * blocks;
+    fill_table<kThreads>(table);
+    Weights of = weights_of(a, d, c256, d.state == kRest, table);
+    auto value = [&](int t) { return of(t, of.x[t], of.probs ? of.probs[t] : 0.0f); };
+    const int per = (blocks + kThreads - 1) / kThreads;
+    double all, upto, none, mine = 0.0;
+    for (int b = tid * per; b < min(tid * per + per, blocks); ++b) mine += sums[b];
+    scan_block64<kDrawWaves>(mine, all);
     if (all > 0.0) {
-      const double target = r * all;
-      const unsigned long long above = __ballot(mine > 0.0 && inc > target), any = __ballot(mine > 0.0);
-      const int k = above ? __ffsll(above) - 1 : 63 - __clzll(any);
-      const double upto = inc - mine;
-      const double from = __hiloint2double(__shfl(__double2hiint(upto), k, 64), __shfl(__double2loint(upto), k, 64));
-      token = draw_from(of, (int)((long long)a.vocab * k / cuts), (int)((long long)a.vocab * (k + 1) / cuts), from, target);
+      const int b = first_above([&](int k) { return sums[k]; }, 0, blocks, per, 0.0, r * all, upto);
+      token = first_above(value, b * kBlock, min((b + 1) * kBlock, a.vocab), kBlock / kThreads, upto, r * all, none);
     } else {                             // nothing is left of p: from p itself
-      token = draw_from(weights_of(a, d, c, false), 0, a.vocab, 0.0, r * d.z);
+      of = weights_of(a, d, c256, false, table);
+      token = first_above(value, 0, a.vocab, (a.vocab + kThreads - 1) / kThreads, 0.0, r * d.z, none);
     }
   }
-  for (int i = tid; i < q.count; i += kDrawThreads)
+  for (int i = tid; i < q.count; i += kThreads)
     a.out[q.row0 + i] = i < d.accepted ? a.tokens[q.row0 + i + 1] : i == d.accepted ? token : -1;
   if (tid == 0) {
     a.accepted[req] = d.accepted;
@@ -332,24 +426,24 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a,
 static int verify_parts(int rows, int vocab) {
   return std::max(1, std::min({(vocab + kVerStep - 1) / kVerStep, kVerParts, 1536 / std::max(rows, 1)}));
 }
-static int verify_cuts(int requests, int vocab) {
-  return std::max(1, std::min({(vocab + 2047) / 2048, kVerParts, 1024 / std::max(requests, 1)}));
-}
+static int verify_blocks(int vocab) { return (vocab + kBlock - 1) / kBlock; }
 
 size_t verify_work_bytes(int rows, int requests, int vocab) {
   return (size_t)rows * verify_parts(rows, vocab) * sizeof(RowPart) + (size_t)requests * sizeof(Decision) +
-         (size_t)requests * verify_cuts(requests, vocab) * sizeof(double);
+         (size_t)requests * verify_blocks(vocab) * sizeof(double);
 }
 
 hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
-  const int parts = verify_parts(a.rows, a.vocab), cuts = verify_cuts(a.requests, a.vocab);
+  const int parts = verify_parts(a.rows, a.vocab), blocks = verify_blocks(a.vocab);
+  const int cuts = std::max(1, std::min((blocks + kRestWaves - 1) / kRestWaves, 1024 / a.requests));
   hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(a.rows * parts)), dim3(64 * kVerWaves), 0, s, a, parts);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.requests * cuts)), dim3(64 * kRestWaves), 0, s, a, parts, cuts);
+  hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.requests * cuts)), dim3(64 * kRestWaves), 0, s, a, parts, cuts,
+                     blocks);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)a.requests), dim3(kDrawThreads), 0, s, a, parts, cuts);
+  hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)a.requests), dim3(64 * kDrawWaves), 0, s, a, parts, blocks);
   return hipGetLastError();
 }
 
