@@ -15,16 +15,22 @@ namespace rehip {
 // leaves nothing, from p); behind the last draft it comes from p. Drawn: the lowest t with sum over j <= t of w_j > r W.
 //
 // Which token r falls on depends on sums over the whole vocabulary to about 1 / vocab of a share each: with sums off by
-// 2^-24 one row in a hundred of 151936 would draw a neighbour. So exponentials and sums are in 64 bits. 2^(k / 256 + f / 256),
-// |f| <= 1/2: from a table of 256 in LDS and the series of 2^(f / 256) - 1 to its third power, off by (ln 2 / 512)^4 / 24 = 1.4e-13.
+// 2^-24 one row in a hundred of 151936 would draw a neighbour. So exponentials and sums are in 64 bits. 2^(k / 64 + f / 64),
+// |f| <= 1/2: from a table of 64 in LDS and the series of 2^(f / 64) - 1 to its third power, off by (ln 2 / 128)^4 / 24 = 3.6e-11
+// at most: a token at the border of 151936 equal ones is then taken for its neighbour once in 200000 times.
 //
 // Three launches: maxima and sums of parts of all rows; every request's last row found from them, and the sums of its
 // weights by blocks of the vocabulary; the block where r falls, and the token in it.
+//
+// 64 requests of up to 4 drafts, 189 rows of 151936 and the drafts' probabilities, 153 MB: 54 us, 33 + 18 + 7.6 in the three
+// kernels. The rows: 115 MB, 3.5 TB/s; without the exponentials they take 23, with them the vector units' 64-bit rate bounds (5 clocks
+// for each of 15 operations; a table of 32 and one term more: 34.5). One
+// request of 4 drafts 14 us: three launches of latency, 5.6 + 6.6 + 5.6.
 constexpr int kVerWaves = 4;
 constexpr int kVerBatch = 16;            // logits of a lane at a time
 constexpr int kVerStep = 64 * kVerBatch * kVerWaves;
 constexpr int kVerParts = 64;            // a lane each
-constexpr int kVerTable = 256;
+constexpr int kVerTable = 64;
 
 struct RowPart {
   double z;                              // sum of 2^((x - m) c)
@@ -62,28 +68,27 @@ __device__ __forceinline__ double pow2_64(double y) {
   return ldexp(p, (int)n);
 }
 
-// The table: 2^(i / 256). All threads of the workgroup call it.
-template <int THREADS>
+// The table: 2^(i / 64). All threads of the workgroup call it.
 __device__ __forceinline__ void fill_table(double* table) {
-  for (int i = threadIdx.x; i < kVerTable; i += THREADS) table[i] = 2.0 * pow2_64((double)(i - kVerTable) / kVerTable);
+  if (threadIdx.x < kVerTable) table[threadIdx.x] = 2.0 * pow2_64(((int)threadIdx.x - kVerTable) / (double)kVerTable);
   __syncthreads();
 }
 
-// 2^((x - m) c), c256 = 256 c; what is below 2^-1000 comes out as that
-__device__ __forceinline__ double share_of(float x, double m, double c256, const double* table) {
+// 2^((x - m) c), c64 = 64 c; what is below 2^-1000 comes out as that
+__device__ __forceinline__ double share_of(float x, double m, double c64, const double* table) {
   constexpr double kRound = 6755399441055744.0;                // 1.5 2^52: a sum's low word is then the nearest integer
   constexpr double k1 = 0.69314718055994530942 / kVerTable, k2 = k1 * k1 / 2.0, k3 = k1 * k1 * k1 / 6.0;
-  const double y = fmax(((double)x - m) * c256, -1000.0 * kVerTable), t = y + kRound;
+  const double y = fmax(((double)x - m) * c64, -1000.0 * kVerTable), t = y + kRound;
   const double f = y - (t - kRound);
   const int n = __double2loint(t);
   const double b = table[n & (kVerTable - 1)];
   const double q = f * fma(f, fma(f, k3, k2), k1), w = fma(b, q, b);
-  return __hiloint2double(__double2hiint(w) + (n >> 8) * (1 << 20), __double2loint(w));
+  return __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
 }
 // .. and exactly 0 there and for a logit of -inf
-__device__ __forceinline__ double weight_of(float x, double m, double c256, const double* table) {
-  const double w = share_of(x, m, c256, table);
-  return x == -INFINITY || ((double)x - m) * c256 < -1000.0 * kVerTable ? 0.0 : w;
+__device__ __forceinline__ double weight_of(float x, double m, double c64, const double* table) {
+  const double w = share_of(x, m, c64, table);
+  return x == -INFINITY || ((double)x - m) * c64 < -1000.0 * kVerTable ? 0.0 : w;
 }
 
 template <int OFF>
@@ -104,7 +109,7 @@ __device__ __forceinline__ double wave_scan64(double v) {
   return v;
 }
 
-// 256 powers of 2 for each unit of logit; greedy below 0
+// 64 powers of 2 for each unit of logit; greedy below 0
 __device__ __forceinline__ double units_of(const VerifyArgs& a, int req) {
   const float t = a.temperature ? a.temperature[req] : 1.0f;
   return t > 0.0f ? kVerTable * 1.4426950408889634074 / (double)t : -1.0;
@@ -115,10 +120,10 @@ __device__ __forceinline__ PagedBatch rows_of(const VerifyArgs& a) {
 }
 
 // A wave's lanes joined, the same in every lane: sums of shares to the largest maximum.
-__device__ __forceinline__ RowPart joined_wave(const RowPart& p, double c256) {
+__device__ __forceinline__ RowPart joined_wave(const RowPart& p, double c64) {
   const float m = wave_max(p.m);
   double z = 0.0;
-  if (c256 >= 0.0) z = wave_sum64(p.m > -INFINITY ? p.z * pow2_64(((double)p.m - (double)m) * (c256 / kVerTable)) : 0.0);
+  if (c64 >= 0.0) z = wave_sum64(p.m > -INFINITY ? p.z * pow2_64(((double)p.m - (double)m) * (c64 / kVerTable)) : 0.0);
   int best = p.m == m ? p.best : 0x7fffffff, bad = p.bad;
   wave_butterfly([&](auto off) {
     constexpr int X = decltype(off)::value;
@@ -133,35 +138,27 @@ __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs 
   __shared__ double table[kVerTable];
   __shared__ RowPart ws[kVerWaves];
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
-  const RequestRows q = request_of_unit(r, rows_of(a), 1, 0);
-  if (q.req < 0 || r >= q.row0 + q.count) return;
-  const double c256 = units_of(a, q.req);
   const float* x = a.x + (size_t)r * a.ld;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int steps = (a.vocab + kVerStep - 1) / kVerStep;
   const int s0 = (int)((long long)steps * part / parts), s1 = (int)((long long)steps * (part + 1) / parts);
-  // element k of a lane in step s: whole steps by fours
+  // element k of a lane in step s
   auto place = [&](int s, int k) { return s * kVerStep + w * 64 * kVerBatch + 256 * (k >> 2) + 4 * lane + (k & 3); };
   auto load = [&](int s, float (&v)[kVerBatch]) {
-    if ((s + 1) * kVerStep <= a.vocab) {
 #pragma unroll
-      for (int k = 0; k < kVerBatch; k += 4)
-        *reinterpret_cast<f32x4u*>(&v[k]) = *reinterpret_cast<const f32x4u*>(x + place(s, k));
-    } else {
-#pragma unroll
-      for (int k = 0; k < kVerBatch; ++k) {
-        const int at = place(s, k);
-        const float y = x[min(at, a.vocab - 1)];
-        v[k] = at < a.vocab ? y : -INFINITY;
-      }
-    }
+    for (int k = 0; k < kVerBatch; k += 4)
+      *reinterpret_cast<f32x4u*>(&v[k]) = *reinterpret_cast<const f32x4u*>(x + place(s, k));
   };
-  RowPart mine{0.0, -INFINITY, 0x7fffffff, 0, 0};
+  // whole steps, the next one loading meanwhile (a load under a condition would be waited for), then the row's last part of one
+  const int whole = min(s1, a.vocab / kVerStep);
   float v[kVerBatch], nx[kVerBatch];
-  if (s0 < s1) load(s0, v);
-  fill_table<64 * kVerWaves>(table);
-  for (int s = s0; s < s1; ++s) {
-    load(min(s + 1, s1 - 1), nx);
+  if (s0 < whole) load(s0, v);           // (on its way while the row's request is found)
+  const RequestRows q = request_of_unit(r, rows_of(a), 1, 0);
+  if (q.req < 0 || r >= q.row0 + q.count) return;
+  const double c64 = units_of(a, q.req);
+  fill_table(table);
+  RowPart mine{0.0, -INFINITY, 0x7fffffff, 0, 0};
+  auto take = [&](const float (&v)[kVerBatch], int s) {
     float mx = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kVerBatch; ++k) {
@@ -169,28 +166,42 @@ __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs 
       mx = fmaxf(mx, v[k]);
     }
     if (mx > mine.m) {
-      if (c256 >= 0.0 && mine.m > -INFINITY) mine.z *= share_of(mine.m, (double)mx, c256, table);
+      if (c64 >= 0.0 && mine.m > -INFINITY) mine.z *= share_of(mine.m, (double)mx, c64, table);
       mine.m = mx;
 #pragma unroll
       for (int k = kVerBatch - 1; k >= 0; --k)
         if (v[k] == mx) mine.best = place(s, k);
     }
-    if (c256 >= 0.0 && mine.m > -INFINITY) {
+    if (c64 >= 0.0 && mine.m > -INFINITY) {
       double z[4] = {};
       const double m = (double)mine.m;
 #pragma unroll
-      for (int k = 0; k < kVerBatch; ++k) z[k & 3] += share_of(v[k], m, c256, table);
+      for (int k = 0; k < kVerBatch; ++k) z[k & 3] += share_of(v[k], m, c64, table);
       mine.z += (z[0] + z[1]) + (z[2] + z[3]);
     }
+  };
+  int s = s0;
+  for (; s < whole; ++s) {
+    load(min(s + 1, whole - 1), nx);
+    take(v, s);
 #pragma unroll
     for (int k = 0; k < kVerBatch; ++k) v[k] = nx[k];
   }
-  const RowPart all = joined_wave(mine, c256);
+  if (s < s1) {
+#pragma unroll
+    for (int k = 0; k < kVerBatch; ++k) {
+      const int at = place(s, k);
+      const float y = x[min(at, a.vocab - 1)];
+      v[k] = at < a.vocab ? y : -INFINITY;
+    }
+    take(v, s);
+  }
+  const RowPart all = joined_wave(mine, c64);
   if (lane == 0) ws[w] = all;
   __syncthreads();
   if (w == 0) {
     const RowPart p = lane < kVerWaves ? ws[lane] : RowPart{0.0, -INFINITY, 0x7fffffff, 0, 0};
-    const RowPart o = joined_wave(p, c256);
+    const RowPart o = joined_wave(p, c64);
     if (lane == 0) reinterpret_cast<RowPart*>(a.work)[blockIdx.x] = o;
   }
 }
@@ -198,7 +209,7 @@ __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs 
 // How many drafts of a request are accepted, and where its next token comes from. Every wave of the workgroup looks at a row of
 // its own at a time.
 template <int WAVES>
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& q, double c256, int parts) {
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& q, double c64, int parts) {
   __shared__ Decision found[WAVES];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Decision d{};
@@ -211,15 +222,15 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
     const float u = a.accept_u[row];
     RowPart p = reinterpret_cast<const RowPart*>(a.work)[(size_t)row * parts + min(lane, parts - 1)];
     if (lane >= parts) p = {0.0, -INFINITY, 0x7fffffff, 0, 0};
-    p = joined_wave(p, c256);
+    p = joined_wave(p, c64);
     const bool none = p.bad || p.m == -INFINITY;
     bool accepted = false;
     if (drafted && !none && t == at)
-      accepted = c256 < 0.0 ? t == p.best
+      accepted = c64 < 0.0 ? t == p.best
                             : (double)u * (double)share * p.z <
-                                  (x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)p.m) * (c256 / kVerTable)));
+                                  (x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)p.m) * (c64 / kVerTable)));
     if (lane == 0)
-      found[w] = {p.z, p.m, accepted ? -1 : i, row, none ? kNone : c256 < 0.0 ? kGreedy : drafted ? kRest : kTarget, p.best, 0};
+      found[w] = {p.z, p.m, accepted ? -1 : i, row, none ? kNone : c64 < 0.0 ? kGreedy : drafted ? kRest : kTarget, p.best, 0};
     __syncthreads();
     bool done = false;
 #pragma unroll
@@ -238,18 +249,18 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
 struct Weights {
   const float* x;
   const float* probs;                    // the draft's row, or null
-  double c256, m, inverse;               // 1 / z
+  double c64, m, inverse;               // 1 / z
   int drop;                              // a draft without a distribution: this token has no weight (-1: none)
   const double* table;
   __device__ __forceinline__ double operator()(int t, float xt, float qt) const {
-    const double e = weight_of(xt, m, c256, table);
+    const double e = weight_of(xt, m, c64, table);
     if (probs) return fmax(fma(e, inverse, -(double)qt), 0.0);
     return t == drop ? 0.0 : e;
   }
 };
-__device__ __forceinline__ Weights weights_of(const VerifyArgs& a, const Decision& d, double c256, bool rest, const double* table) {
+__device__ __forceinline__ Weights weights_of(const VerifyArgs& a, const Decision& d, double c64, bool rest, const double* table) {
   const int t = rest && !a.probs ? a.tokens[d.row + 1] : -1;
-  return {a.x + (size_t)d.row * a.ld, rest && a.probs ? a.probs + (size_t)d.row * a.ldp : nullptr, c256, (double)d.m,
+  return {a.x + (size_t)d.row * a.ld, rest && a.probs ? a.probs + (size_t)d.row * a.ldp : nullptr, c64, (double)d.m,
           1.0 / d.z, t, table};
 }
 
@@ -263,40 +274,58 @@ __device__ __forceinline__ double* sums_at(const VerifyArgs& a, int parts) {
 // One workgroup per (request, run of blocks of the vocabulary), a block to a wave at a time: the sums of their weights.
 constexpr int kRestWaves = 8;
 constexpr int kBlock = 1024;             // tokens of a block
+constexpr int kRestMost = 512;           // workgroups, about
+template <bool PROBS>
 __global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs a, int parts, int cuts, int blocks) {
   __shared__ double table[kVerTable];
   const int req = blockIdx.x / cuts, cut = blockIdx.x % cuts, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const RequestRows q = request_rows(req, a.start[req], a.count[req], 0, a.rows);
   if (q.count <= 0) return;
-  const double c256 = units_of(a, req);
-  const Decision d = decide<kRestWaves>(a, q, c256, parts);
+  const double c64 = units_of(a, req);
+  fill_table(table);
+  const Decision d = decide<kRestWaves>(a, q, c64, parts);
   if (cut == 0 && threadIdx.x == 0) decisions_at(a, parts)[req] = d;
   if (d.state != kTarget && d.state != kRest) return;
-  const Weights of = weights_of(a, d, c256, d.state == kRest, table);
-  fill_table<64 * kRestWaves>(table);
+  const Weights of = weights_of(a, d, c64, d.state == kRest, table);
   const int b0 = (int)((long long)blocks * cut / cuts), b1 = (int)((long long)blocks * (cut + 1) / cuts);
-  for (int b = b0 + w; b < b1; b += kRestWaves) {
-    float x[16], p[16];
-    auto place = [&](int k) { return b * kBlock + 256 * (k >> 2) + 4 * lane + (k & 3); };
-    if ((b + 1) * kBlock <= a.vocab) {
+  auto place = [&](int b, int k) { return b * kBlock + 256 * (k >> 2) + 4 * lane + (k & 3); };
+  const float* probs = of.probs ? of.probs : of.x;                 // (loaded whatever)
+  auto load = [&](int b, float (&x)[16], float (&p)[16]) {
 #pragma unroll
-      for (int k = 0; k < 16; k += 4) {
-        *reinterpret_cast<f32x4u*>(&x[k]) = *reinterpret_cast<const f32x4u*>(of.x + place(k));
-        if (of.probs) *reinterpret_cast<f32x4u*>(&p[k]) = *reinterpret_cast<const f32x4u*>(of.probs + place(k));
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const int t = min(place(k), a.vocab - 1);
-        x[k] = place(k) < a.vocab ? of.x[t] : -INFINITY;
-        p[k] = of.probs ? of.probs[t] : 0.0f;
-      }
+    for (int k = 0; k < 16; k += 4) {
+      *reinterpret_cast<f32x4u*>(&x[k]) = *reinterpret_cast<const f32x4u*>(of.x + place(b, k));
+      if (PROBS) *reinterpret_cast<f32x4u*>(&p[k]) = *reinterpret_cast<const f32x4u*>(probs + place(b, k));
     }
+  };
+  auto take = [&](const float (&x)[16], const float (&p)[16], int b) {
     double s[4] = {};
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s[k & 3] += of(place(k), x[k], p[k]);
+    for (int k = 0; k < 16; ++k) s[k & 3] += of(place(b, k), x[k], PROBS ? p[k] : 0.0f);
     const double all = wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
     if (lane == 0) sums_at(a, parts)[(size_t)req * blocks + b] = all;
+  };
+  float x[16], p[16], nx[16], np[16];
+  const int whole = min(b1, a.vocab / kBlock);
+  int b = b0 + w;
+  if (b < whole) load(b, x, p);
+  for (; b < whole; b += kRestWaves) {
+    load(b + kRestWaves < whole ? b + kRestWaves : b, nx, np);
+    take(x, p, b);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      x[k] = nx[k];
+      if (PROBS) p[k] = np[k];
+    }
+  }
+  if (b < b1) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int t = min(place(b, k), a.vocab - 1);
+      const float y = of.x[t];
+      x[k] = place(b, k) < a.vocab ? y : -INFINITY;
+      if (PROBS) p[k] = probs[t];
+    }
+    take(x, p, b);
   }
 }
 
@@ -398,10 +427,10 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs
   const Decision d = decisions_at(a, parts)[req];
   int token = d.state == kGreedy ? d.best : -1;
   if (d.state == kTarget || d.state == kRest) {
-    const double c256 = units_of(a, req), r = (double)a.sample_u[req];
+    const double c64 = units_of(a, req), r = (double)a.sample_u[req];
     const double* sums = sums_at(a, parts) + (size_t)req * blocks;
-    fill_table<kThreads>(table);
-    Weights of = weights_of(a, d, c256, d.state == kRest, table);
+    fill_table(table);
+    Weights of = weights_of(a, d, c64, d.state == kRest, table);
     auto value = [&](int t) { return of(t, of.x[t], of.probs ? of.probs[t] : 0.0f); };
     const int per = (blocks + kThreads - 1) / kThreads;
     double all, upto, none, mine = 0.0;
@@ -411,7 +440,7 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs
       const int b = first_above([&](int k) { return sums[k]; }, 0, blocks, per, 0.0, r * all, upto);
       token = first_above(value, b * kBlock, min((b + 1) * kBlock, a.vocab), kBlock / kThreads, upto, r * all, none);
     } else {                             // nothing is left of p: from p itself
-      of = weights_of(a, d, c256, false, table);
+      of = weights_of(a, d, c64, false, table);
       token = first_above(value, 0, a.vocab, (a.vocab + kThreads - 1) / kThreads, 0.0, r * d.z, none);
     }
   }
@@ -435,11 +464,11 @@ size_t verify_work_bytes(int rows, int requests, int vocab) {
 
 hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
   const int parts = verify_parts(a.rows, a.vocab), blocks = verify_blocks(a.vocab);
-  const int cuts = std::max(1, std::min((blocks + kRestWaves - 1) / kRestWaves, 1024 / a.requests));
+  const int cuts = std::max(1, std::min((blocks + kRestWaves - 1) / kRestWaves, kRestMost / a.requests));
   hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(a.rows * parts)), dim3(64 * kVerWaves), 0, s, a, parts);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.requests * cuts)), dim3(64 * kRestWaves), 0, s, a, parts, cuts,
+  hipLaunchKernelGGL(a.probs ? verify_rest_kernel<true> : verify_rest_kernel<false>, dim3((unsigned)(a.requests * cuts)), dim3(64 * kRestWaves), 0, s, a, parts, cuts,
                      blocks);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
