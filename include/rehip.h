@@ -440,8 +440,8 @@ int re_kv8_mass_dev(const float *d_q, size_t ldq, const float *d_lse, size_t row
  * those between them stay, `keep` in all, KV head by KV head (ties to the earlier token; a NaN counts as -inf, a token
  * without a page below that), and move to the new pages in their order, K, V and mass. A new page's scale is the largest of
  * the pages that its tokens come from, a code round(c * (old / new)), ties to even; places behind the last token get code
- * and mass 0. d_kept: requests x n_kv_heads x keep, the old places of what stayed (of cut requests). d_mass may be NULL if
- * first + recent = keep. Old pages are only read: they must not be given out before the last layer's call. max_len: the
+ * and mass 0. d_kept: requests x n_kv_heads x keep, the old places of what stayed (of cut requests). d_mass (16-byte
+ * aligned) may be NULL if first + recent = keep. Old pages are only read: they must not be given out before the last layer's call. max_len: the
  * largest d_from_len to plan for (longer ones are computed too, only slower). */
 int re_kv_evict_plan_dev(size_t requests, size_t page, size_t limit, size_t keep, const int *d_kv_len,
                          const int *d_table, size_t table_ld, const int *d_free, size_t n_pages, const int *d_n_free,

@@ -208,179 +208,229 @@ __device__ __forceinline__ unsigned mass_key(float x) {
   return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 
+// One workgroup per (request, head). A thread has up to kPickMost tokens that follow one another, by fours: a page's places
+// come in fours that lie together.
 __global__ __launch_bounds__(kPickThreads) void kv8_evict_pick_kernel(EvictArgs a, int kv_heads) {
   __shared__ int bins[kPickBins];
-  __shared__ int found_bin, found_above;
+  __shared__ int found_bin, found_above, found_in;
   const int req = blockIdx.x / kv_heads, head = blockIdx.x % kv_heads, tid = threadIdx.x;
   const int T = a.from_len[req];
   if (T <= a.keep || T > a.table_ld * a.page) return;
   int* const kept = a.kept + (size_t)blockIdx.x * a.keep;
   const int* const table = a.from_table + (size_t)req * a.table_ld;
-  const int N = T - a.recent - a.first, M = a.keep - a.first - a.recent;
+  const int M = a.keep - a.first - a.recent, end = T - a.recent;   // M of the tokens first .. end - 1
   for (int i = tid; i < a.first; i += kPickThreads) kept[i] = i;
-  for (int i = tid; i < a.recent; i += kPickThreads) kept[a.keep - a.recent + i] = T - a.recent + i;
+  for (int i = tid; i < a.recent; i += kPickThreads) kept[a.keep - a.recent + i] = end + i;
   if (M == 0) return;
-  constexpr int kBlock = kPickThreads * kPickMost;
-  // tokens at .. at + kPickMost - 1 of the middle's
+  const int per = min(kPickMost, ((end + kPickThreads - 1) / kPickThreads + 3) & ~3), block = kPickThreads * per;
+  // tokens at .. at + per - 1 (those behind the middle: some of its own)
   auto load = [&](int at, unsigned (&key)[kPickMost]) {
+    float4 x[kPickMost / 4];
+    int pid[kPickMost / 4];
 #pragma unroll
-    for (int e = 0; e < kPickMost; ++e) {
-      const int i = at + e, t = a.first + min(i, N - 1), pg = t / a.page, pid = table[pg];
-      const bool there = pid >= 0 && pid < a.n_pages;
-      const float x = a.mass[((size_t)(there ? pid : 0) * kv_heads + head) * a.page + t - pg * a.page];
-      key[e] = there ? mass_key(x) : 0;
+    for (int e = 0; e < kPickMost / 4; ++e) pid[e] = table[min(at + min(4 * e, per - 4), end - 1) / a.page];
+#pragma unroll
+    for (int e = 0; e < kPickMost / 4; ++e) {
+      const int t = min(at + min(4 * e, per - 4), (end - 1) & ~3);
+      const bool there = pid[e] >= 0 && pid[e] < a.n_pages;
+      x[e] = *reinterpret_cast<const float4*>(a.mass + ((size_t)(there ? pid[e] : 0) * kv_heads + head) * a.page + t % a.page);
+      if (!there) pid[e] = -1;
     }
+#pragma unroll
+    for (int e = 0; e < kPickMost; ++e) key[e] = pid[e / 4] >= 0 ? mass_key((&x[e / 4].x)[e & 3]) : 0;
   };
   unsigned key[kPickMost];
-  const bool once = N <= kBlock;
-  if (once) load(tid * kPickMost, key);
+  const bool once = end <= block;
+  auto middle = [&](int at, int e) { return e < per && at + e >= a.first && at + e < end; };
+  if (once) load(tid * per, key);
   unsigned high = 0;                     // the digits found, and what of M is left below the larger ones
-  int want = M;
-  constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
+  int want = M, shift = 32;
+  constexpr int kBits[3] = {11, 11, 10};
 #pragma unroll
   for (int d = 0; d < 3; ++d) {
-    const int size = 1 << kBits[d];
+    const int size = 1 << kBits[d], below = shift - kBits[d];
     for (int i = tid; i < size; i += kPickThreads) bins[i] = 0;
     __syncthreads();
-    for (int base = 0; base < N; base += kBlock) {
-      const int at = base + tid * kPickMost;
+    for (int base = 0; base < end; base += block) {
+      const int at = base + tid * per;
       if (!once) load(at, key);
 #pragma unroll
       for (int e = 0; e < kPickMost; ++e) {
-        const bool same = d == 0 || (key[e] >> (kShift[d] + kBits[d])) == (high >> (kShift[d] + kBits[d]));
-        if (at + e < N && same) atomicAdd(&bins[(key[e] >> kShift[d]) & (size - 1)], 1);
+        const bool same = d == 0 || (key[e] >> shift) == (high >> shift);
+        if (middle(at, e) && same) atomicAdd(&bins[(key[e] >> below) & (size - 1)], 1);
       }
     }
     __syncthreads();
     // thread i has the bins size - 1 - 2 i and the next one down (one, of the last digit's)
-    const int per = size / kPickThreads, top = size - 1 - per * tid;
-    int mine[2] = {bins[top], per > 1 ? bins[top - 1] : 0}, before;
+    const int own = size / kPickThreads, top = size - 1 - own * tid;
+    const int mine[2] = {bins[top], own > 1 ? bins[top - 1] : 0};
+    int before;
     scan_block<kPickThreads / 64>(mine[0] + mine[1], before);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (before < want && before + mine[i] >= want) {
         found_bin = top - i;
         found_above = before;
+        found_in = mine[i];
       }
       before += mine[i];
     }
     __syncthreads();
-    high |= (unsigned)found_bin << kShift[d];
+    high |= (unsigned)found_bin << below;
     want -= found_above;
+    shift = below;
+    if (found_in == want) break;         // all of them stay: what their lower digits are does not matter
     __syncthreads();
   }
-  // `want` of those equal to `high` stay
+  // keys above `high` (in their digits down to `shift`) stay, and the first `want` of those equal to it
+  high >>= shift;
   int at_kept = a.first, equals = 0;
-  for (int base = 0; base < N; base += kBlock) {
-    const int at = base + tid * kPickMost;
+  for (int base = 0; base < end; base += block) {
+    const int at = base + tid * per;
     if (!once) load(at, key);
-    int more = 0, same = 0, more_before, same_before;
+    int more = 0, same = 0, before;
 #pragma unroll
     for (int e = 0; e < kPickMost; ++e) {
-      more += at + e < N && key[e] > high;
-      same += at + e < N && key[e] == high;
+      more += middle(at, e) && (key[e] >> shift) > high;
+      same += middle(at, e) && (key[e] >> shift) == high;
     }
-    const int all_more = scan_block<kPickThreads / 64>(more, more_before);
-    const int all_same = scan_block<kPickThreads / 64>(same, same_before);
-    int s = equals + same_before, o = at_kept + more_before + min(s, want) - min(equals, want);
+    // (both counts in one sum: of at most 2^14 tokens)
+    const int all = scan_block<kPickThreads / 64>(more | same << 16, before);
+    int s = equals + (before >> 16), o = at_kept + (before & 0xffff) + min(s, want) - min(equals, want);
 #pragma unroll
     for (int e = 0; e < kPickMost; ++e) {
-      const bool in = at + e < N, stays = in && (key[e] > high || (key[e] == high && s < want));
-      s += in && key[e] == high;
-      if (stays) kept[o++] = a.first + at + e;
+      const bool in = middle(at, e), equal = in && (key[e] >> shift) == high;
+      if ((in && (key[e] >> shift) > high) || (equal && s < want)) kept[o++] = at + e;
+      s += equal;
     }
-    at_kept += all_more + min(equals + all_same, want) - min(equals, want);
-    equals += all_same;
+    at_kept += (all & 0xffff) + min(equals + (all >> 16), want) - min(equals, want);
+    equals += all >> 16;
   }
 }
 
 // ---- the move --------------------------------------------------------------------------------------
 // Place o of new page p holds token kept[p * page + o]; the page's scale is the largest among the pages that its tokens come
 // from, so that no code grows, a code round(c * (s_old / s_new)), ties to even. Places behind the last token get code 0 and
-// mass 0. One workgroup for each page and head, K and V.
-__global__ __launch_bounds__(256) void kv8_evict_move_kernel(EvictArgs a, Kv8Cache c, int units) {
-  __shared__ int src_page[256], src_at[256];
-  __shared__ float ratio[2][256];
-  __shared__ float red[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fresh = (a.keep + a.page - 1) / a.page;
+// mass 0.
+//
+// One workgroup for each new page and head, K or V. A lane makes 16 bytes of a block of 32 tokens x 32 dimensions: K's are
+// two tokens' 8 dimensions, two loads of 8 bytes; V's are 8 tokens' 2 dimensions, and of each of them the 16 old bytes
+// that hold them with 7 neighbours are loaded. Where a lane's tokens lie is found once for all blocks of dimensions.
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// the code in byte i of x, rounded to another scale: q + 1.5 2^23 rounds q to an integer, whose low byte is the code
+__device__ __forceinline__ unsigned moved(unsigned x, int i, float r) {
+  const float q = (float)((int)(x << (24 - 8 * i)) >> 24) * r;
+  return __float_as_uint(q + 12582912.0f);
+}
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+
+template <bool IS_V>
+__device__ __forceinline__ void move_page(const EvictArgs& a, const Kv8Cache& c, int req, int p, int pid, int head) {
+  __shared__ const int8_t* src[256];     // the old page's first block of the token's 32
+  __shared__ int place[256];             // .. and the token's place in it
+  __shared__ float ratio[256], red[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nb = c.hd >> 5, m = lane & 15, g = lane >> 4;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int head = u % c.kv_heads, p = u / c.kv_heads % fresh, req = u / c.kv_heads / fresh;
+  int8_t* const codes = IS_V ? c.v : c.k;
+  float* const scales = IS_V ? c.vs : c.ks;
+  const int T = a.from_len[req], count = min(a.page, a.keep - p * a.page);
+  const size_t head_bytes = (size_t)a.page * c.hd, mine = (size_t)pid * c.kv_heads + head;
+  int from = -1, at = 0;
+  float s = 0.0f;
+  if (tid < count) {
+    const int t = a.kept[((size_t)req * c.kv_heads + head) * a.keep + p * a.page + tid];
+    if (t >= 0 && t < T) {
+      const int pg = t / a.page, id = a.from_table[(size_t)req * a.table_ld + pg];
+      at = t - pg * a.page;
+      if (id >= 0 && id < a.n_pages) {
+        from = id;
+        s = scales[(size_t)id * c.kv_heads + head];
+      }
+    }
+  }
+  const float mass = !IS_V && a.mass && from >= 0 ? a.mass[((size_t)from * c.kv_heads + head) * a.page + at] : 0.0f;
+  float top = wave_max(s);
+  if (lane == 0) red[w] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (tid < a.page) {                    // (a place without a token: its own page, times 0)
+    ratio[tid] = from >= 0 && top > 0.0f ? s / top : 0.0f;
+    src[tid] = codes + (from >= 0 ? (size_t)from * c.kv_heads + head : mine) * head_bytes + (size_t)(at >> 5) * (nb * 1024);
+    place[tid] = at & 31;
+    if (!IS_V && a.mass) a.mass[mine * a.page + tid] = mass;
+  }
+  if (tid == 0) scales[mine] = top;
+  __syncthreads();
+  // waves: blocks of tokens, and where there are fewer than four, every so-manieth block of dimensions
+  const int tokens = a.page >> 5, step = tokens >= 4 ? 1 : 4 / tokens;
+  for (int tb = w / step; tb < tokens; tb += 4) {
+    int8_t* const out = codes + mine * head_bytes + (size_t)tb * (nb * 1024) + 16 * lane;
+    if constexpr (IS_V) {
+      const u32x4* at8[8];
+      int shift[8];
+      float r[8];
+      bool later[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int o = 32 * tb + 16 * (e >> 2) + 4 * g + (e & 3), x = place[o];
+        at8[e] = reinterpret_cast<const u32x4*>(src[o] + 256 * (x >> 2 & 3) + 16 * m);
+        shift[e] = x & 3;
+        later[e] = x & 16;
+        r[e] = ratio[o];
+      }
+      for (int d = w % step; d < nb; d += step) {
+        u32x4 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = at8[e][64 * d];
+        unsigned y[2][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) y[b][e] = moved(later[e] ? x[e][2 * b + 1] : x[e][2 * b], shift[e], r[e]);
+        *reinterpret_cast<u32x4*>(out + 1024 * d) =
+            u32x4{low_bytes(y[0][0], y[0][1], y[0][2], y[0][3]), low_bytes(y[0][4], y[0][5], y[0][6], y[0][7]),
+                  low_bytes(y[1][0], y[1][1], y[1][2], y[1][3]), low_bytes(y[1][4], y[1][5], y[1][6], y[1][7])};
+      }
+    } else {
+      const u32x2* at8[2];
+      float r[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int o = 32 * tb + 16 * t + m, x = place[o];
+        at8[t] = reinterpret_cast<const u32x2*>(src[o] + 256 * g + 16 * (x & 15) + 8 * (x >> 4));
+        r[t] = ratio[o];
+      }
+#pragma unroll 4
+      for (int d = w % step; d < nb; d += step) {
+        u32x4 z;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const u32x2 x = at8[t][128 * d];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            z[2 * t + h] = low_bytes(moved(x[h], 0, r[t]), moved(x[h], 1, r[t]), moved(x[h], 2, r[t]), moved(x[h], 3, r[t]));
+        }
+        *reinterpret_cast<u32x4*>(out + 1024 * d) = z;
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void kv8_evict_move_kernel(EvictArgs a, Kv8Cache c, long units) {
+  const int fresh = (a.keep + a.page - 1) / a.page;
+  for (long u = blockIdx.x; u < units; u += gridDim.x) {
+    const long page = u >> 1;
+    const int head = (int)(page % c.kv_heads), p = (int)(page / c.kv_heads % fresh), req = (int)(page / c.kv_heads / fresh);
     const int T = a.from_len[req];
     if (T <= a.keep || T > a.table_ld * a.page) continue;
     const int pid = a.table[(size_t)req * a.table_ld + p];
     if (pid < 0 || pid >= a.n_pages) continue;
-    const int count = min(a.page, a.keep - p * a.page);
-    int from = -1, at = 0;
-    float s[2] = {0.0f, 0.0f};
-    if (tid < count) {
-      const int t = a.kept[((size_t)req * c.kv_heads + head) * a.keep + p * a.page + tid];
-      const int pg = t / a.page;
-      const int id = t >= 0 && t < T ? a.from_table[(size_t)req * a.table_ld + pg] : -1;
-      from = id >= 0 && id < a.n_pages ? id : -1;
-      at = t - pg * a.page;
-      if (from >= 0) {
-        s[0] = c.ks[(size_t)from * c.kv_heads + head];
-        s[1] = c.vs[(size_t)from * c.kv_heads + head];
-      }
-    }
-    float top[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = wave_max(s[i]);
-      if (lane == 0) red[i][w] = top[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = fmaxf(fmaxf(red[i][0], red[i][1]), fmaxf(red[i][2], red[i][3]));
-      ratio[i][tid] = from >= 0 && top[i] > 0.0f ? s[i] / top[i] : 0.0f;
-    }
-    src_page[tid] = max(from, 0);
-    src_at[tid] = from >= 0 ? at : 0;
-    const size_t mine = (size_t)pid * c.kv_heads + head;
-    if (a.mass && tid < a.page)
-      a.mass[mine * a.page + tid] = from >= 0 ? a.mass[((size_t)from * c.kv_heads + head) * a.page + at] : 0.0f;
-    if (tid == 0) {
-      c.ks[mine] = top[0];
-      c.vs[mine] = top[1];
-    }
-    __syncthreads();
-    const int blocks = (a.page >> 5) * nb;
-    const size_t head_bytes = (size_t)a.page * c.hd;
-    // byte of token place o, dimension block d, of its page and head
-    auto base = [&](const int8_t* codes, int o, int d) {
-      return codes + ((size_t)src_page[o] * c.kv_heads + head) * head_bytes + ((src_at[o] >> 5) * nb + d) * 1024;
-    };
-    for (int blk = w; blk < 2 * blocks; blk += 4) {
-      const bool is_v = blk >= blocks;
-      const int q = is_v ? blk - blocks : blk, d = q % nb, o0 = 32 * (q / nb);
-      int8_t out[16];
-      if (!is_v) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int o = o0 + 16 * t + m, x = src_at[o] & 31;
-          const float r = ratio[0][o];
-          const uint2 v = *reinterpret_cast<const uint2*>(base(c.k, o, d) + 256 * g + 16 * (x & 15) + 8 * (x >> 4));
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            out[8 * t + j] = (int8_t)(int)rintf((float)(int8_t)((j < 4 ? v.x : v.y) >> (8 * (j & 3))) * r);
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int o = o0 + 16 * t + 4 * g + i, x = src_at[o] & 31;
-            const float r = ratio[1][o];
-            const int8_t* at8 = base(c.v, o, d) + 256 * (x >> 2 & 3) + 16 * m + 4 * (x >> 4) + (x & 3);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) out[8 * b + 4 * t + i] = (int8_t)(int)rintf((float)at8[8 * b] * r);
-          }
-      }
-      int8_t* const to = (is_v ? c.v : c.k) + mine * head_bytes + (size_t)q * 1024 + 16 * lane;
-      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(out);
-    }
+    if (u & 1) move_page<true>(a, c, req, p, pid, head);
+    else move_page<false>(a, c, req, p, pid, head);
     __syncthreads();
   }
 }
@@ -389,9 +439,8 @@ hipError_t launch_kv8_evict(const EvictArgs& a, const Kv8Cache& c, hipStream_t s
   hipLaunchKernelGGL(kv8_evict_pick_kernel, dim3((unsigned)(a.requests * c.kv_heads)), dim3(kPickThreads), 0, s, a, c.kv_heads);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int fresh = (a.keep + a.page - 1) / a.page;
-  const long units = (long)a.requests * c.kv_heads * fresh;        // (below 2^31: checked by the caller)
-  hipLaunchKernelGGL(kv8_evict_move_kernel, dim3((unsigned)std::min(units, 1L << 22)), dim3(256), 0, s, a, c, (int)units);
+  const long units = 2L * a.requests * c.kv_heads * ((a.keep + a.page - 1) / a.page);
+  hipLaunchKernelGGL(kv8_evict_move_kernel, dim3((unsigned)std::min(units, 1L << 22)), dim3(256), 0, s, a, c, units);
   return hipGetLastError();
 }
 

@@ -309,6 +309,7 @@ int re_kv8_evict_dev(size_t requests, const int* d_from_len, const int* d_from_t
   if (d_table == d_from_table) return report_error(RE_ERR_ARG, "the old table and the new one must be two buffers");
   if (keep == 0 || keep > (1u << 30) || first > keep || recent > keep - first)
     return report_error(RE_ERR_SIZE, "%zu first and %zu last tokens of %zu to keep (up to 2^30)", first, recent, keep);
+  if (!a16(d_mass)) return report_error(RE_ERR_ARG, "masses must be 16-byte aligned");
   if (!d_mass && first + recent < keep)
     return report_error(RE_ERR_ARG, "without masses the first and last tokens must be all of the %zu to keep", keep);
   const size_t pages = (keep + page - 1) / page;

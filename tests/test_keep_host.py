@@ -78,7 +78,7 @@ EVICT = dict(requests=4, from_len=A, from_table=A, table=B, table_ld=8, page=64,
 
 @pytest.mark.parametrize("code,change", POOL + nulls("from_len", "from_table", "table", "kcodes", "vcodes", "kscale", "vscale",
                                                      "kept") + [
-    (ARG, {"table": A}), (ARG, {"mass": None}), (ARG, {"kcodes": A + 8}), (ARG, {"vcodes": A + 4}),
+    (ARG, {"table": A}), (ARG, {"mass": None}), (ARG, {"mass": A + 8}), (ARG, {"kcodes": A + 8}), (ARG, {"vcodes": A + 4}),
     *[(SIZE, c) for c in ({"keep": 0}, {"keep": (1 << 30) + 1}, {"first": 101}, {"recent": 97}, {"first": 100, "recent": 1},
                           {"page": 48}, {"page": 288}, {"head_dim": 80}, {"head_dim": 0}, {"n_kv_heads": 0},
                           {"requests": 4096, "n_kv_heads": 1024}, {"first": (1 << 64) - 1, "recent": 2},
