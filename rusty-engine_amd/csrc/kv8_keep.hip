@@ -200,7 +200,7 @@ hipError_t launch_kv8_mass(const PagedBatch& b, const Kv8Cache& c, const MassArg
 // below that). The M-th largest key is found by its digits, 11, 11 and 10 bits from the top: a histogram of those whose
 // higher digits are the ones found so far, and a scan of it from the top. Then a token stays if its key is larger, or equal
 // and among the first of those.
-constexpr int kPickThreads = 1024, kPickMost = 16;                 // tokens of a thread at a time
+constexpr int kPickMost = 16;            // tokens of a thread at a time
 constexpr int kPickBins = 2048;
 
 __device__ __forceinline__ unsigned mass_key(float x) {
@@ -210,7 +210,8 @@ __device__ __forceinline__ unsigned mass_key(float x) {
 
 // One workgroup per (request, head). A thread has up to kPickMost tokens that follow one another, by fours: a page's places
 // come in fours that lie together.
-__global__ __launch_bounds__(kPickThreads) void kv8_evict_pick_kernel(EvictArgs a, int kv_heads) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void kv8_evict_pick_kernel(EvictArgs a, int kv_heads) {
   __shared__ int bins[kPickBins];
   __shared__ int found_bin, found_above, found_in;
   const int req = blockIdx.x / kv_heads, head = blockIdx.x % kv_heads, tid = threadIdx.x;
@@ -219,10 +220,10 @@ __global__ __launch_bounds__(kPickThreads) void kv8_evict_pick_kernel(EvictArgs 
   int* const kept = a.kept + (size_t)blockIdx.x * a.keep;
   const int* const table = a.from_table + (size_t)req * a.table_ld;
   const int M = a.keep - a.first - a.recent, end = T - a.recent;   // M of the tokens first .. end - 1
-  for (int i = tid; i < a.first; i += kPickThreads) kept[i] = i;
-  for (int i = tid; i < a.recent; i += kPickThreads) kept[a.keep - a.recent + i] = end + i;
+  for (int i = tid; i < a.first; i += THREADS) kept[i] = i;
+  for (int i = tid; i < a.recent; i += THREADS) kept[a.keep - a.recent + i] = end + i;
   if (M == 0) return;
-  const int per = min(kPickMost, ((end + kPickThreads - 1) / kPickThreads + 3) & ~3), block = kPickThreads * per;
+  const int per = min(kPickMost, ((end + THREADS - 1) / THREADS + 3) & ~3), block = THREADS * per;
   // tokens at .. at + per - 1 (those behind the middle: some of its own)
   auto load = [&](int at, unsigned (&key)[kPickMost]) {
     float4 x[kPickMost / 4];
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(kPickThreads) void kv8_evict_pick_kernel(EvictArgs 
 #pragma unroll
   for (int d = 0; d < 3; ++d) {
     const int size = 1 << kBits[d], below = shift - kBits[d];
-    for (int i = tid; i < size; i += kPickThreads) bins[i] = 0;
+    for (int i = tid; i < size; i += THREADS) bins[i] = 0;
     __syncthreads();
     for (int base = 0; base < end; base += block) {
       const int at = base + tid * per;
@@ -261,13 +262,18 @@ __global__ __launch_bounds__(kPickThreads) void kv8_evict_pick_kernel(EvictArgs 
       }
     }
     __syncthreads();
-    // thread i has the bins size - 1 - 2 i and the next one down (one, of the last digit's)
-    const int own = size / kPickThreads, top = size - 1 - own * tid;
-    const int mine[2] = {bins[top], own > 1 ? bins[top - 1] : 0};
-    int before;
-    scan_block<kPickThreads / 64>(mine[0] + mine[1], before);
+    // a thread has bins that follow one another, from the top down
+    constexpr int kOwn = kPickBins / THREADS;
+    const int own = size / THREADS, top = size - 1 - own * tid;
+    int mine[kOwn], sum = 0, before;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kOwn; ++i) {
+      mine[i] = i < own ? bins[top - i] : 0;
+      sum += mine[i];
+    }
+    scan_block<THREADS / 64>(sum, before);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
       if (before < want && before + mine[i] >= want) {
         found_bin = top - i;
         found_above = before;
@@ -295,7 +301,7 @@ __global__ __launch_bounds__(kPickThreads) void kv8_evict_pick_kernel(EvictArgs 
       same += middle(at, e) && (key[e] >> shift) == high;
     }
     // (both counts in one sum: of at most 2^14 tokens)
-    const int all = scan_block<kPickThreads / 64>(more | same << 16, before);
+    const int all = scan_block<THREADS / 64>(more | same << 16, before);
     int s = equals + (before >> 16), o = at_kept + (before & 0xffff) + min(s, want) - min(equals, want);
 #pragma unroll
     for (int e = 0; e < kPickMost; ++e) {
@@ -436,7 +442,11 @@ __global__ __launch_bounds__(256) void kv8_evict_move_kernel(EvictArgs a, Kv8Cac
 }
 
 hipError_t launch_kv8_evict(const EvictArgs& a, const Kv8Cache& c, hipStream_t s) {
-  hipLaunchKernelGGL(kv8_evict_pick_kernel, dim3((unsigned)(a.requests * c.kv_heads)), dim3(kPickThreads), 0, s, a, c.kv_heads);
+  const dim3 picks((unsigned)(a.requests * c.kv_heads));
+  // the fewest waves that hold a request's tokens at once: their barriers are shorter
+  if (a.max_len <= 256 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<256>, picks, dim3(256), 0, s, a, c.kv_heads);
+  else if (a.max_len <= 512 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<512>, picks, dim3(512), 0, s, a, c.kv_heads);
+  else hipLaunchKernelGGL(kv8_evict_pick_kernel<1024>, picks, dim3(1024), 0, s, a, c.kv_heads);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const long units = 2L * a.requests * c.kv_heads * ((a.keep + a.page - 1) / a.page);

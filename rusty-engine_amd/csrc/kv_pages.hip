@@ -8,22 +8,33 @@
 namespace rehip {
 
 // The table entries of requests b, columns from first[b] (null: 0) on, at[b + 1] - at[b] of them, `total` in all, that hold a page
-// go to out[base ..] in that order, `room` at most. Returns how many. All threads of the workgroup call it.
+// go to out[base ..] in that order, `room` at most. Returns how many. All threads of the workgroup call it; a thread has four
+// entries that follow one another, so that 4 THREADS of them cost one trip to memory and one scan.
 template <int THREADS>
 __device__ __forceinline__ int push_pages(const int* at, const int* first, int requests, int total, const int* table,
                                           int table_ld, int n_pages, int* out, int base, int room) {
   int done = 0;
-  for (int k0 = 0; k0 < total; k0 += THREADS) {
-    const int k = k0 + (int)threadIdx.x;
-    int pid = -1;
-    if (k < total) {
-      const int b = last_at_most(at, requests, k);
-      pid = table[(size_t)b * table_ld + (first ? first[b] : 0) + (k - at[b])];
+  for (int k0 = 0; k0 < total; k0 += 4 * THREADS) {
+    int pid[4], mine = 0, before;
+    const int k = k0 + 4 * (int)threadIdx.x;
+    int b = k < total ? last_at_most(at, requests, k) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i > 0 && k + i < total && b + 1 < requests && at[b + 1] <= k + i) b = last_at_most(at, requests, k + i);
+      pid[i] = k + i < total ? table[(size_t)b * table_ld + (first ? first[b] : 0) + (k + i - at[b])] : -1;
     }
-    const bool holds = pid >= 0 && pid < n_pages;
-    int before;
-    const int all = scan_block<THREADS / 64>(holds ? 1 : 0, before);
-    if (holds && done + before < room) out[base + done + before] = pid;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (pid[i] < 0 || pid[i] >= n_pages) pid[i] = -1;
+      mine += pid[i] >= 0;
+    }
+    const int all = scan_block<THREADS / 64>(mine, before);
+    before += done;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (pid[i] >= 0 && before < room) out[base + before] = pid[i];
+      before += pid[i] >= 0;
+    }
     done += all;
   }
   return min(done, room);
@@ -37,8 +48,7 @@ __device__ __forceinline__ int push_pages(const int* at, const int* first, int r
 template <int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(EvictPlanArgs a, int copy_table, int copy_free) {
   constexpr int kMost = THREADS * PER;
-  __shared__ int at[kMost], row_of[kMost];                  // row_of[i]: the i-th request that is cut
-  __shared__ bool cut[kMost];
+  __shared__ int at[kMost], row_of[kMost], rank_of[kMost];         // row_of[i]: the i-th request that is cut; its i, or -1
   const int tid = threadIdx.x, b0 = tid * PER;
   const int free0 = min(max(*a.n_free, 0), a.n_pages);
   const int room = a.table_ld * a.page, fresh = (a.keep + a.page - 1) / a.page;
@@ -49,14 +59,15 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(EvictPlanArgs a,
     over += len[i] > a.limit && len[i] <= room;
   }
   const int wanted = scan_block<THREADS / 64>(over, before);
-  const int cuts = min(wanted, free0 / fresh);
-  int held = 0;
+  const int cuts = min(wanted, free0 / fresh), left = free0 - cuts * fresh;
+  int held[PER], sum = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = b0 + i;
     const bool is = len[i] > a.limit && len[i] <= room, ok = is && before < cuts;
+    held[i] = ok ? (len[i] + a.page - 1) / a.page : 0;
     if (b < a.requests) {
-      cut[b] = ok;
+      rank_of[b] = ok ? before : -1;
       if (ok) row_of[before] = b;
       a.len_out[b] = ok ? a.keep : len[i];
       a.from_len[b] = ok ? len[i] : 0;
@@ -66,42 +77,50 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(EvictPlanArgs a,
       }
     }
     before += is;
-    held += ok ? (len[i] + a.page - 1) / a.page : 0;
+    sum += held[i];
   }
-  int sum;
-  const int total = scan_block<THREADS / 64>(held, sum);
+  int upto;
+  const int total = scan_block<THREADS / 64>(sum, upto);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (b0 + i >= a.requests) break;
-    at[b0 + i] = sum;
-    sum += cut[b0 + i] ? (len[i] + a.page - 1) / a.page : 0;
+    at[b0 + i] = upto;
+    upto += held[i];
   }
   __syncthreads();
-  // the old rows, where the table is written over
-  if (a.from_table != a.table) {
-    for (int k = tid; k < total; k += THREADS) {
-      const int b = last_at_most(at, a.requests, k);
-      const size_t e = (size_t)b * a.table_ld + (k - at[b]);
-      a.from_table[e] = a.table[e];
+  // Rows: the cut ones' old entries kept and new ones written, the others copied. An entry is read and written by one thread,
+  // so that the table may be written in place.
+  const int rows = copy_table ? a.requests : cuts, entries = rows * a.table_ld;
+  for (int k0 = tid; k0 < entries; k0 += 4 * THREADS) {
+    int e[4], rank[4], j[4], old[4], got[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = min(k0 + i * THREADS, entries - 1), r = k / a.table_ld, b = copy_table ? r : row_of[r];
+      j[i] = k - r * a.table_ld;
+      e[i] = b * a.table_ld + j[i];
+      rank[i] = rank_of[b];
+      old[i] = a.table[e[i]];
+      got[i] = rank[i] >= 0 && j[i] < fresh ? a.free_pages[free0 - 1 - (rank[i] * fresh + j[i])] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (k0 + i * THREADS >= entries) break;
+      if (rank[i] >= 0 && a.from_table != a.table) a.from_table[e[i]] = old[i];
+      a.table_out[e[i]] = rank[i] >= 0 ? got[i] : old[i];
     }
   }
-  if (copy_table) {
-    for (int k = tid; k < a.requests * a.table_ld; k += THREADS)
-      if (!cut[k / a.table_ld]) a.table_out[k] = a.table[k];
-  }
   if (copy_free) {
-    for (int k = tid; k < free0 - cuts * fresh; k += THREADS) a.free_out[k] = a.free_pages[k];
+    for (int k0 = tid; k0 < left; k0 += 4 * THREADS) {
+      int x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = a.free_pages[min(k0 + i * THREADS, left - 1)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k0 + i * THREADS < left) a.free_out[k0 + i * THREADS] = x[i];
+    }
   }
   __threadfence_block();
-  __syncthreads();
-  // (a request's columns side by side: the stack is read and the rows written in order)
-  for (int k = tid; k < cuts * a.table_ld; k += THREADS) {
-    const int i = k / a.table_ld, j = k - i * a.table_ld;
-    a.table_out[(size_t)row_of[i] * a.table_ld + j] = j < fresh ? a.free_pages[free0 - 1 - (i * fresh + j)] : -1;
-  }
-  __threadfence_block();
-  __syncthreads();
-  const int left = free0 - cuts * fresh;
+  __syncthreads();                       // (the stack's top has been read, the old rows are there)
   const int pushed = push_pages<THREADS>(at, nullptr, a.requests, total, a.from_table, a.table_ld, a.n_pages, a.free_out, left,
                                          a.n_pages - left);
   if (tid == 0) {
@@ -125,7 +144,7 @@ static void launch_evict_plan(const EvictPlanArgs& a, bool copy_table, bool copy
 
 hipError_t launch_kv_evict_plan(const EvictPlanArgs& a, hipStream_t s) {
   // Tables and stacks of more than a few numbers for each of the plan's threads are copied by many workgroups before
-  constexpr int kCopiedHere = 16384;
+  constexpr int kCopiedHere = 32768;
   const int entries = a.requests * a.table_ld;
   bool copy_table = a.table_out != a.table, copy_free = a.free_out != a.free_pages;
   if (copy_table && entries > kCopiedHere) {
@@ -136,7 +155,8 @@ hipError_t launch_kv_evict_plan(const EvictPlanArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(copy_ints_kernel, dim3(512), dim3(256), 0, s, a.free_pages, a.free_out, a.n_free, 0, a.n_pages);
     copy_free = false;
   }
-  if (a.requests <= 256) launch_evict_plan<256, 1>(a, copy_table, copy_free, s);
+  // (four waves for a small table: their barriers are shorter)
+  if (a.requests <= 256 && entries <= 1024) launch_evict_plan<256, 1>(a, copy_table, copy_free, s);
   else if (a.requests <= 1024) launch_evict_plan<1024, 1>(a, copy_table, copy_free, s);
   else launch_evict_plan<1024, kPlanMaxRequests / 1024>(a, copy_table, copy_free, s);
   return hipGetLastError();
@@ -144,39 +164,71 @@ hipError_t launch_kv_evict_plan(const EvictPlanArgs& a, hipStream_t s) {
 
 // ---- rewind --------------------------------------------------------------------------------------
 // A request of len tokens gives back min(back, len) of them; the pages ceil(left / page) .. ceil(len / page) - 1 hold none of
-// the rest and go to the stack, request after request. One workgroup, as the plan.
+// the rest and go to the stack, request after request. One workgroup, as the plan: the lengths, then the table's entries, then
+// a scan. Where no request gives back more than kFew pages (drafts are shorter than that) a thread reads those of its own
+// requests itself; else entries are handed out one by one, whatever request they are of.
 template <int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void kv_rewind_kernel(RewindArgs a) {
-  constexpr int kMost = THREADS * PER;
+  constexpr int kMost = THREADS * PER, kFew = 2;
   __shared__ int at[kMost], stay[kMost];
   const int tid = threadIdx.x, b0 = tid * PER;
   const int free0 = min(max(*a.n_free, 0), a.n_pages), room = a.table_ld * a.page;
-  int gone[PER], sum = 0;
+  int gone[PER], from[PER], sum = 0, most = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int b = b0 + i;
-    const bool in = b < a.requests;
-    const int len = in ? a.len[b] : 0, back = in ? a.back[b] : 0;
-    const bool sound = len >= 0 && len <= room;
-    const int left = sound ? len - min(max(back, 0), len) : len;
-    gone[i] = sound ? (len + a.page - 1) / a.page - (left + a.page - 1) / a.page : 0;
-    if (in) {
-      a.len_out[b] = left;
-      stay[b] = sound ? (left + a.page - 1) / a.page : 0;
-    }
+    const int b = min(b0 + i, a.requests - 1);
+    gone[i] = a.len[b];
+    from[i] = a.back[b];
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int b = b0 + i, len = gone[i];
+    const bool sound = len >= 0 && len <= room && b < a.requests;
+    const int left = sound ? len - min(max(from[i], 0), len) : len;
+    from[i] = sound ? (left + a.page - 1) / a.page : 0;
+    gone[i] = sound ? (len + a.page - 1) / a.page - from[i] : 0;
+    if (b < a.requests) a.len_out[b] = left;
     sum += gone[i];
+    most = max(most, gone[i]);
   }
-  int before;
-  const int total = scan_block<THREADS / 64>(sum, before);
+  int before, pushed;
+  if (!__syncthreads_or(most > kFew)) {
+    int pid[PER][kFew], mine = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (b0 + i >= a.requests) break;
-    at[b0 + i] = before;
-    before += gone[i];
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < kFew; ++j) {
+        pid[i][j] = -1;
+        if (j < gone[i]) pid[i][j] = a.table[(size_t)(b0 + i) * a.table_ld + from[i] + j];
+      }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < kFew; ++j) {
+        if (pid[i][j] >= a.n_pages) pid[i][j] = -1;
+        mine += pid[i][j] >= 0;
+      }
+    pushed = min(scan_block<THREADS / 64>(mine, before), a.n_pages - free0);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < kFew; ++j) {
+        if (pid[i][j] >= 0 && before < a.n_pages - free0) a.free_pages[free0 + before] = pid[i][j];
+        before += pid[i][j] >= 0;
+      }
+  } else {
+    const int total = scan_block<THREADS / 64>(sum, before);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (b0 + i >= a.requests) break;
+      at[b0 + i] = before;
+      stay[b0 + i] = from[i];
+      before += gone[i];
+    }
+    __syncthreads();
+    pushed = push_pages<THREADS>(at, stay, a.requests, total, a.table, a.table_ld, a.n_pages, a.free_pages, free0,
+                                 a.n_pages - free0);
   }
-  __syncthreads();
-  const int pushed = push_pages<THREADS>(at, stay, a.requests, total, a.table, a.table_ld, a.n_pages, a.free_pages, free0,
-                                         a.n_pages - free0);
   if (tid == 0) *a.n_free_out = free0 + pushed;
 }
 
