@@ -13,171 +13,276 @@ namespace rehip {
 // ---- weights of a step -----------------------------------------------------------------------------
 // Key j of a request and KV head gets sum over its rows and the heads of the group of exp(scale q . k_j - lse), lse the log of
 // the row's sum of exponentials as attention left it, over the rows that see the key. Products as in attention: codes exact in
-// f16, q in two f16 parts, f32 sums. A key belongs to one wave, so its sum is taken in one order.
+// f16, q in two f16 parts, f32 sums. A key belongs to one wave or workgroup, so its sum is taken in one order.
 //
-// A workgroup of four waves holds 128 KS keys of one head as f16 operands in registers, KS steps of 32 for each wave, and
-// walks the query vectors that see some of them, 64 at a time (a tile of 16 for each wave to split, all four tiles for every
-// wave to multiply). Sums over the 16 vectors of a tile stay in the lanes until the end.
+// A piece is 32 KS keys of one request and head, held as f16 operands in registers; tiles of 16 query vectors that see some of
+// them go past, each split by the wave that multiplies it (the matrix operand's lanes are those that load it), the next
+// one on its way meanwhile. Sums over a tile's vectors stay in the lanes until the end. Steps of few vectors: a wave takes a
+// piece alone (W = 1). Prompts: the four waves of a workgroup share a piece and take every fourth tile (W = 4). The launch has as
+// many waves as run at once, and each takes every so-manieth piece of the whole batch, found from the lengths: a piece for each
+// wave of the longest request's would leave most of a ragged batch's waves without any.
+#ifndef MWG
+#define MWG 1024
+#endif
+constexpr int kMassWorkgroups = MWG;
 struct MassCut {
-  int chunks;                            // workgroups of a request and head
+  int chunks;                            // pieces of a request and head, of the longest planned
+  int mode;                              // how a piece is found: below
 };
+constexpr int kMassLanes = 0, kMassListed = 1, kMassEven = 2;      // requests a lane each; listed in LDS; chunks of each
+constexpr int kMassList = 1024;
 
-template <int NB, int KS>
-__global__ __launch_bounds__(256) void kv8_mass_kernel(PagedBatch b, Kv8Cache c, MassArgs a, MassCut t) {
-  constexpr int HD = 32 * NB, kKeys = 128 * KS;
-  __shared__ __attribute__((aligned(16))) char big[4 * NB * 2 * 1024];
-  h8* const qf = reinterpret_cast<h8*>(big);                       // [tile][NB][hi, lo][lane]
-  __shared__ float qss[4][16], cut[4][16];                         // a vector's factor, its lse in powers of 2
-  const int head = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
-  const int req = rest / t.chunks;
-  const RequestRows q = request_rows(req, b.start[req], b.count[req], b.len[req], b.rows);
-  const int n = min(q.count, a.max_rows);
-  if (n <= 0) return;
-  const int grp = a.heads / c.kv_heads, p0 = max(q.len, 0) - q.count;
-  const int last = min(p0 + n, b.table_ld * b.page) - 1;           // (no key behind the table)
-  if (last < 0) return;
-  const int lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
-  const int sink_chunks = a.window > 0 ? (min(a.sinks, last + 1) + kKeys - 1) / kKeys : 0;
-  const int first = max(lo / kKeys, sink_chunks), all = sink_chunks + max(last / kKeys - first + 1, 0);
+// A request's pieces: those of the sinks, then those from `first` on that some row sees; n rows from position p0 to `last`.
+struct MassPlace {
+  int n, p0, last, sinks, first, all;
+};
+__device__ __forceinline__ MassPlace mass_place(const PagedBatch& b, const MassArgs& a, const RequestRows& q, int keys) {
+  MassPlace o;
+  o.n = min(q.count, a.max_rows);
+  o.p0 = max(q.len, 0) - q.count;
+  o.last = min(o.p0 + o.n, b.table_ld * b.page) - 1;               // (no key behind the table)
+  const int lo = a.window > 0 ? max(0, o.p0 - a.window + 1) : 0;
+  o.sinks = a.window > 0 ? (min(a.sinks, o.last + 1) + keys - 1) / keys : 0;
+  o.first = max(lo / keys, o.sinks);
+  o.all = o.n <= 0 || o.last < 0 ? 0 : o.sinks + max(o.last / keys - o.first + 1, 0);
+  return o;
+}
+
+template <int NB, int W>
+__global__ __launch_bounds__(256, 2) void kv8_mass_kernel(PagedBatch b, Kv8Cache c, MassArgs a, MassCut t) {
+  constexpr int HD = 32 * NB, KS = NB <= 2 ? 4 : NB <= 4 ? 2 : 1, kKeys = 32 * KS;
+  __shared__ float4 red[W > 1 ? W - 1 : 1][2 * KS][4];
+  __shared__ int at[kMassList];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, g = lane >> 4, page_steps = b.page >> 5;
+  const int col = lane & 15, g = lane >> 4, page_steps = b.page >> 5, grp = a.heads / c.kv_heads;
   float minus_one = -1.0f;
   asm volatile("" : "+v"(minus_one));
-  for (int ch = rest % t.chunks; ch < all; ch += t.chunks) {
-    const int k0 = (ch < sink_chunks ? ch : ch - sink_chunks + first) * kKeys;
-    // this wave's keys
+
+  auto piece = [&](int req, int row0, const MassPlace& o, int ch, int head) {
+    const int k0 = (ch < o.sinks ? ch : ch - o.sinks + o.first) * kKeys;
     int pid[KS], in_page[KS];
     u32x4 kc[KS][NB];
     float ks[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int step = (k0 >> 5) + w * KS + s, pg = step / page_steps;
+      const int step = (k0 >> 5) + s, pg = step / page_steps;
       in_page[s] = step - pg * page_steps;
-      int p = -1;
-      if (32 * step <= last) p = b.table[(size_t)req * b.table_ld + pg];
-      pid[s] = __builtin_amdgcn_readfirstlane(p >= 0 && p < b.n_pages ? p : -1);
-      const int8_t* at = c.k + ((size_t)max(pid[s], 0) * c.kv_heads + head) * ((size_t)b.page * HD) + in_page[s] * (NB * 1024);
-#pragma unroll
-      for (int k = 0; k < NB; ++k) kc[s][k] = *reinterpret_cast<const u32x4*>(at + 1024 * k + 16 * lane);
-      ks[s] = c.ks[(size_t)max(pid[s], 0) * c.kv_heads + head];
+      pid[s] = b.table[(size_t)req * b.table_ld + min(pg, b.table_ld - 1)];
+      if (32 * step > o.last || pid[s] >= b.n_pages) pid[s] = -1;
     }
-    f32x4 sum[KS][2] = {};
-    // rows that see some key of the workgroup's
-    const int i0 = max(0, k0 - p0);
-    const int i1 = a.window > 0 && k0 >= a.sinks ? (int)min((long long)n, (long long)k0 + kKeys - 1 + a.window - p0) : n;
-    const int tile1 = (i1 * grp + 15) >> 4;
-    for (int t0 = (i0 * grp) >> 4; t0 < tile1; t0 += 4) {
-      __syncthreads();                   // the tiles before have been read
-      if (t0 + w < tile1) {
-        const int vec = 16 * (t0 + w) + col, row = vec / grp, hq = head * grp + vec - row * grp;
-        const bool live = row < n;
-        const float* at = a.q + (size_t)(q.row0 + (live ? row : 0)) * a.ldq + (size_t)(live ? hq : 0) * HD + 8 * g;
-        const float lse = live ? a.lse[(size_t)(q.row0 + row) * a.heads + hq] : INFINITY;
-        float x[NB][8];
-        unsigned top = 0;
-#pragma unroll
-        for (int k = 0; k < NB; ++k) {
-          *reinterpret_cast<float4*>(&x[k][0]) = *reinterpret_cast<const float4*>(at + 32 * k);
-          *reinterpret_cast<float4*>(&x[k][4]) = *reinterpret_cast<const float4*>(at + 32 * k + 4);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
-        }
-        top = max(top, lane_xor_u32<16>(top));
-        top = max(top, lane_xor_u32<32>(top));
-        const int e = (int)(top >> 23), f = min(267 - e, 253);     // 2^13 <= largest * 2^(f - 127) < 2^14
-        // (a row that is not there, sees nothing or is not finite gives no weight: q = 0, lse = inf)
-        const bool ok = e != 255 && fabsf(lse) < INFINITY;
-        const float up = ok ? copysignf(__uint_as_float((unsigned)f << 23), a.scale) : 0.0f;
-#pragma unroll
-        for (int k = 0; k < NB; ++k) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[k][j] = ok ? x[k][j] * up : 0.0f;
-          h8 hi, lo8;
-          split8(x[k], minus_one, hi, lo8);
-          qf[((w * NB + k) * 2 + 0) * 64 + lane] = hi;
-          qf[((w * NB + k) * 2 + 1) * 64 + lane] = lo8;
-        }
-        if (g == 0) {
-          qss[w][col] = ok ? __uint_as_float((unsigned)(254 - f) << 23) * (fabsf(a.scale) * 1.4426950408889634f) : 0.0f;
-          cut[w][col] = ok ? lse * 1.4426950408889634f : INFINITY;
-        }
-      }
-      __syncthreads();
-      for (int u = 0; u < 4 && t0 + u < tile1; ++u) {
-        const float qs = qss[u][col], m = cut[u][col];
-        const int low_row = 16 * (t0 + u) / grp, pos = p0 + (16 * (t0 + u) + col) / grp;
-        const int pos_low = p0 + low_row, pos_high = p0 + (16 * (t0 + u) + 15) / grp;
-        f32x4 st[KS][2] = {};
-#pragma unroll
-        for (int k = 0; k < NB; ++k) {
-          const h8 hi = qf[((u * NB + k) * 2 + 0) * 64 + lane], lo8 = qf[((u * NB + k) * 2 + 1) * 64 + lane];
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            const h8 a0 = codes8(kc[s][k][0], kc[s][k][1]), a1 = codes8(kc[s][k][2], kc[s][k][3]);
-            st[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, hi, st[s][0], 0, 0, 0);
-            st[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, hi, st[s][1], 0, 0, 0);
-            st[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, lo8, st[s][0], 0, 0, 0);
-            st[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, lo8, st[s][1], 0, 0, 0);
-          }
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int key0 = k0 + 32 * (w * KS + s);
-          const float f = ks[s] * qs;
-          const bool hides = key0 + 31 > pos_low || (a.window > 0 && key0 <= pos_high - a.window && key0 + 31 >= a.sinks);
-          const int low = a.window > 0 ? pos - a.window + 1 : 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float p = pow2(__builtin_fmaf(st[s][e >> 2][e & 3], f, -m));
-            if (hides) {
-              const int j = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
-              if (j > pos || (j < low && j >= a.sinks)) p = 0.0f;
-            }
-            sum[s][e >> 2][e & 3] += p;
-          }
-        }
-      }
-    }
-    // over the 16 vectors of the tiles' columns; a step's own tokens start from nothing
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int key0 = k0 + 32 * (w * KS + s);
+      pid[s] = __builtin_amdgcn_readfirstlane(pid[s]);
+      const int8_t* p = c.k + ((size_t)max(pid[s], 0) * c.kv_heads + head) * ((size_t)b.page * HD) + in_page[s] * (NB * 1024);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) kc[s][k] = *reinterpret_cast<const u32x4*>(p + 1024 * k + 16 * lane);
+      ks[s] = c.ks[(size_t)max(pid[s], 0) * c.kv_heads + head];
+    }
+    // this lane's four places of each half step, and what is there already
+    float4* place[KS][2];
+    float4 was[KS][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float y[4];
+        place[s][h] = reinterpret_cast<float4*>(a.mass + ((size_t)max(pid[s], 0) * c.kv_heads + head) * b.page +
+                                                32 * in_page[s] + 16 * h + 4 * g);
+        if (W == 1) was[s][h] = *place[s][h];
+      }
+    // tiles of the vectors that see some key of the piece
+    const int i0 = max(0, k0 - o.p0);
+    const int i1 = a.window > 0 && k0 >= a.sinks ? (int)min((long long)o.n, (long long)k0 + kKeys - 1 + a.window - o.p0) : o.n;
+    const int tile1 = (i1 * grp + 15) >> 4;
+    int tile = ((i0 * grp) >> 4) + (W > 1 ? w : 0);
+    float x[NB][8], lse;
+    int row;
+    auto load_q = [&](int tile, float (&x)[NB][8], float& lse, int& row) {
+      const int vec = 16 * tile + col;
+      row = vec / grp;
+      const int r = row0 + min(row, o.n - 1), hq = head * grp + vec - row * grp;
+      const float* p = a.q + (size_t)r * a.ldq + (size_t)hq * HD + 8 * g;
+      lse = a.lse[(size_t)r * a.heads + hq];
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        *reinterpret_cast<float4*>(&x[k][0]) = *reinterpret_cast<const float4*>(p + 32 * k);
+        *reinterpret_cast<float4*>(&x[k][4]) = *reinterpret_cast<const float4*>(p + 32 * k + 4);
+      }
+    };
+    f32x4 sum[KS][2] = {};
+    if (tile < tile1) load_q(tile, x, lse, row);
+    h8 kf[KS][NB][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        kf[s][k][0] = codes8(kc[s][k][0], kc[s][k][1]);
+        kf[s][k][1] = codes8(kc[s][k][2], kc[s][k][3]);
+      }
+    for (; tile < tile1; tile += W) {
+      unsigned top = 0;
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
+      top = max(top, lane_xor_u32<16>(top));
+      top = max(top, lane_xor_u32<32>(top));
+      const int e = (int)(top >> 23), f = min(267 - e, 253);       // 2^13 <= largest * 2^(f - 127) < 2^14
+      // (a row that is not there, sees nothing or is not finite gives no weight: q = 0, lse = inf)
+      const bool ok = e != 255 && row < o.n && fabsf(lse) < INFINITY;
+      const float up = copysignf(__uint_as_float((unsigned)f << 23), a.scale);
+      const float qs = ok ? __uint_as_float((unsigned)(254 - f) << 23) * (fabsf(a.scale) * 1.4426950408889634f) : 0.0f;
+      const float m = ok ? lse * 1.4426950408889634f : INFINITY;
+      h8 qh[NB], ql[NB];
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[k][j] = ok ? x[k][j] * up : 0.0f;
+        split8(x[k], minus_one, qh[k], ql[k]);
+      }
+      const int pos = o.p0 + row;
+      const int pos_low = __builtin_amdgcn_readlane(pos, 0), pos_high = __builtin_amdgcn_readlane(pos, 15);
+      load_q(tile + W < tile1 ? tile + W : tile, x, lse, row);     // (on its way while this one is multiplied)
+      f32x4 st[KS][2] = {};
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          st[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][0], qh[k], st[s][0], 0, 0, 0);
+          st[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][1], qh[k], st[s][1], 0, 0, 0);
+          st[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][0], ql[k], st[s][0], 0, 0, 0);
+          st[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][1], ql[k], st[s][1], 0, 0, 0);
+        }
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int key0 = k0 + 32 * s;
+        const float factor = ks[s] * qs;
+        const bool hides = key0 + 31 > pos_low || (a.window > 0 && key0 <= pos_high - a.window && key0 + 31 >= a.sinks);
+        const int low = a.window > 0 ? pos - a.window + 1 : 0;
+#pragma unroll
+        for (int e8 = 0; e8 < 8; ++e8) {
+          float p = pow2(__builtin_fmaf(st[s][e8 >> 2][e8 & 3], factor, -m));
+          if (hides) {
+            const int j = key0 + 16 * (e8 >> 2) + 4 * g + (e8 & 3);
+            if (j > pos || (j < low && j >= a.sinks)) p = 0.0f;
+          }
+          sum[s][e8 >> 2][e8 & 3] += p;
+        }
+      }
+    }
+    // over the 16 vectors of the tiles' columns, and the waves; a step's own tokens start from nothing
+    float4 y[KS][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = sum[s][h][i];
           v += lane_xor<8>(v);
           v += lane_xor<4>(v);
           v += lane_xor<2>(v);
-          y[i] = v + lane_xor<1>(v);
+          (&y[s][h].x)[i] = v + lane_xor<1>(v);
         }
-        const int j = key0 + 16 * h + 4 * g;
-        if (pid[s] < 0 || j > last || col != 0) continue;
-        float4* const at = reinterpret_cast<float4*>(
-            a.mass + ((size_t)pid[s] * c.kv_heads + head) * b.page + 32 * in_page[s] + 16 * h + 4 * g);
-        const float4 was = *at;
-        float z[4] = {was.x, was.y, was.z, was.w};
+    if constexpr (W > 1) {
+      __syncthreads();                   // the piece before has been read
+      if (w > 0 && col == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j + i <= last) z[i] = j + i >= p0 ? y[i] : z[i] + y[i];
-        *at = make_float4(z[0], z[1], z[2], z[3]);
+        for (int s = 0; s < 2 * KS; ++s) red[w - 1][s][g] = y[s >> 1][s & 1];
       }
+      __syncthreads();
+      if (w > 0) return;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          was[s][h] = *place[s][h];
+#pragma unroll
+          for (int i = 0; i < W - 1; ++i) {
+            const float4 z = red[i][2 * s + h][g];
+            y[s][h] = make_float4(y[s][h].x + z.x, y[s][h].y + z.y, y[s][h].z + z.z, y[s][h].w + z.w);
+          }
+        }
     }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = k0 + 32 * s + 16 * h + 4 * g;
+        if (pid[s] < 0 || j > o.last || col != 0) continue;
+        float z[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float old = (&was[s][h].x)[i], add = (&y[s][h].x)[i];
+          z[i] = j + i > o.last ? old : j + i >= o.p0 ? add : old + add;
+        }
+        *place[s][h] = make_float4(z[0], z[1], z[2], z[3]);
+      }
+  };
+
+  const int first = W > 1 ? blockIdx.x : 4 * blockIdx.x + w, stride = W > 1 ? gridDim.x : 4 * gridDim.x;
+  if (t.mode == kMassLanes) {
+    const int i = min(lane, b.requests - 1);
+    const RequestRows q = request_rows(i, b.start[i], b.count[i], b.len[i], b.rows);
+    const MassPlace o = mass_place(b, a, q, kKeys);
+    const int mine = lane < b.requests ? o.all : 0, upto = wave_scan(mine);
+    const int total = __builtin_amdgcn_readlane(upto, 63) * c.kv_heads;
+    for (int u = first; u < total; u += stride) {
+      const int ch = u / c.kv_heads, l = __ffsll(__ballot(ch < upto)) - 1;
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+      piece(l, of(q.row0), MassPlace{of(o.n), of(o.p0), of(o.last), of(o.sinks), of(o.first), of(o.all)}, ch - of(upto - mine),
+            u - ch * c.kv_heads);
+    }
+    return;
+  }
+  if (t.mode == kMassListed) {
+    constexpr int kOwn = kMassList / 256;
+    int mine[kOwn], sum = 0, before;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int r = kOwn * threadIdx.x + i, in = min(r, b.requests - 1);
+      const MassPlace o = mass_place(b, a, request_rows(in, b.start[in], b.count[in], b.len[in], b.rows), kKeys);
+      mine[i] = r < b.requests ? o.all : 0;
+      sum += mine[i];
+    }
+    const int total = scan_block<4>(sum, before) * c.kv_heads;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      at[kOwn * threadIdx.x + i] = before;
+      before += mine[i];
+    }
+    __syncthreads();
+    for (int u = first; u < total; u += stride) {
+      const int ch = u / c.kv_heads, r = last_at_most(at, b.requests, ch);
+      const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
+      piece(r, q.row0, mass_place(b, a, q, kKeys), ch - at[r], u - ch * c.kv_heads);
+    }
+    return;
+  }
+  const long long all = (long long)b.requests * t.chunks * c.kv_heads;
+  for (long long u = first; u < all; u += stride) {
+    const int head = (int)(u % c.kv_heads), r = (int)(u / c.kv_heads / t.chunks);
+    const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
+    const MassPlace o = mass_place(b, a, q, kKeys);
+    for (int ch = (int)(u / c.kv_heads % t.chunks); ch < o.all; ch += t.chunks) piece(r, q.row0, o, ch, head);
   }
 }
 
-template <int NB>
-static void launch_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
-  constexpr int KS = 2, kKeys = 128 * KS;
+template <int NB, int W>
+static void launch_mass_as(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
+  constexpr int kKeys = 32 * (NB <= 2 ? 4 : NB <= 4 ? 2 : 1);
   long chunks = (std::max(a.max_len, 1) + kKeys - 1) / kKeys;
   if (a.window > 0)
     chunks = std::min(chunks, (long)(a.sinks + kKeys - 1) / kKeys + ((long)a.window + a.max_rows - 2) / kKeys + 2);
-  const size_t heads = (size_t)b.requests * c.kv_heads;
-  chunks = std::max(1L, std::min(chunks, (long)(kMassMaxWorkgroups / heads)));
-  hipLaunchKernelGGL((kv8_mass_kernel<NB, KS>), dim3((unsigned)(heads * chunks)), dim3(256), 0, s, b, c, a,
-                     MassCut{(int)chunks});
+  const int mode = b.requests <= 64 ? kMassLanes : b.requests <= kMassList ? kMassListed : kMassEven;
+  if (mode == kMassEven) chunks = std::min(chunks, 16L);           // (a longer request's waves take several)
+  const long waves = (long)b.requests * c.kv_heads * chunks;
+  const long groups = std::min(W > 1 ? waves : (waves + 3) / 4, (long)kMassWorkgroups);
+  hipLaunchKernelGGL((kv8_mass_kernel<NB, W>), dim3((unsigned)groups), dim3(256), 0, s, b, c, a, MassCut{(int)chunks, mode});
+}
+template <int NB>
+static void launch_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
+  if ((long)a.max_rows * (a.heads / c.kv_heads) > 64) launch_mass_as<NB, 4>(b, c, a, s);
+  else launch_mass_as<NB, 1>(b, c, a, s);
 }
 
 hipError_t launch_kv8_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
