@@ -16,15 +16,18 @@ namespace rehip {
 // f16, q in two f16 parts, f32 sums. A key belongs to one wave or workgroup, so its sum is taken in one order.
 //
 // A piece is 32 KS keys of one request and head, held as f16 operands in registers; tiles of 16 query vectors that see some of
-// them go past, each split by the wave that multiplies it (the matrix operand's lanes are those that load it), the next
-// one on its way meanwhile. Sums over a tile's vectors stay in the lanes until the end. Steps of few vectors: a wave takes a
-// piece alone (W = 1). Prompts: the four waves of a workgroup share a piece and take every fourth tile (W = 4). The launch has as
-// many waves as run at once, and each takes every so-manieth piece of the whole batch, found from the lengths: a piece for each
-// wave of the longest request's would leave most of a ragged batch's waves without any.
-#ifndef MWG
-#define MWG 1024
-#endif
-constexpr int kMassWorkgroups = MWG;
+// them go past, each split by the wave that multiplies it (the matrix operand's lanes are those that load it), the next one
+// on its way meanwhile. Sums over a tile's vectors stay in the lanes until the end, and are then taken by halves, so that
+// every lane ends with a key or two of its own. Steps of few vectors: a wave takes a piece alone (W = 1). Prompts: a
+// workgroup's W waves share a piece and take every W-th tile. The launch has about as many workgroups as run at once, and each
+// takes every so-manieth piece of the whole batch, found from the lengths: with a piece for each of the longest request's, most
+// workgroups of a ragged batch would find nothing (64 requests of up to 8192 tokens 32 us instead of 17).
+//
+// 64 requests of up to 8192 tokens, 32 heads in 4 of 128, 36 MB: 16.8 us, 2.1 TB/s: two pieces a wave, one after the other, four
+// trips to memory each. Two prompts of up to 1000 rows behind up to 5000 tokens, 16 heads in 8 of 64, 9.7 GFLOP and as many of low
+// parts: 47 us: exponentials, the split of q (each vector for every 128 keys) and few pieces of unequal length (the first keys
+// are seen by every row), two waves on a SIMD half of the time waiting. Passing split tiles on in LDS between waves of
+// different keys did not pay (57; 32 heads in 4 of 128 268 us instead of 117: then a quarter of the pieces).
 struct MassCut {
   int chunks;                            // pieces of a request and head, of the longest planned
   int mode;                              // how a piece is found: below
@@ -48,240 +51,317 @@ __device__ __forceinline__ MassPlace mass_place(const PagedBatch& b, const MassA
   return o;
 }
 
-template <int NB, int W>
-__global__ __launch_bounds__(256, 2) void kv8_mass_kernel(PagedBatch b, Kv8Cache c, MassArgs a, MassCut t) {
-  constexpr int HD = 32 * NB, KS = NB <= 2 ? 4 : NB <= 4 ? 2 : 1, kKeys = 32 * KS;
-  __shared__ float4 red[W > 1 ? W - 1 : 1][2 * KS][4];
-  __shared__ int at[kMassList];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, g = lane >> 4, page_steps = b.page >> 5, grp = a.heads / c.kv_heads;
-  float minus_one = -1.0f;
-  asm volatile("" : "+v"(minus_one));
+// f(request, its first row, its place, piece, head) for every `stride`-th piece of the batch from `u` on. `at`: kMassList places in
+// LDS. All threads of the workgroup call it.
+template <int WAVES, class F>
+__device__ __forceinline__ void mass_pieces(const PagedBatch& b, const MassArgs& a, const MassCut& t, int kv_heads, int keys,
+                                            int u, int stride, int* at, F f) {
+  const int lane = threadIdx.x & 63, i = min(lane, b.requests - 1);
+  RequestRows q{};
+  MassPlace mine{};
+  int upto = 0;
+  long long total = (long long)b.requests * t.chunks * kv_heads;
+  if (t.mode == kMassLanes) {
+    q = request_rows(i, b.start[i], b.count[i], b.len[i], b.rows);
+    mine = mass_place(b, a, q, keys);
+    if (lane >= b.requests) mine.all = 0;
+    upto = wave_scan(mine.all);
+    total = (long long)__builtin_amdgcn_readlane(upto, 63) * kv_heads;
+  } else if (t.mode == kMassListed) {
+    constexpr int kOwn = kMassList / (64 * WAVES);
+    int n[kOwn], sum = 0, before;
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) {
+      const int r = kOwn * threadIdx.x + e, in = min(r, b.requests - 1);
+      const MassPlace o = mass_place(b, a, request_rows(in, b.start[in], b.count[in], b.len[in], b.rows), keys);
+      n[e] = r < b.requests ? o.all : 0;
+      sum += n[e];
+    }
+    total = (long long)scan_block<WAVES>(sum, before) * kv_heads;
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) {
+      at[kOwn * threadIdx.x + e] = before;
+      before += n[e];
+    }
+    __syncthreads();
+  }
+  for (long long v = u; v < total; v += stride) {
+    const int c = (int)(v / kv_heads), head = (int)(v - (long long)c * kv_heads);
+    int r, row0, ch, step = 0x40000000;
+    MassPlace o;
+    if (t.mode == kMassLanes) {
+      r = __ffsll(__ballot(c < upto)) - 1;
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, r); };
+      row0 = of(q.row0);
+      o = {of(mine.n), of(mine.p0), of(mine.last), of(mine.sinks), of(mine.first), of(mine.all)};
+      ch = c - of(upto - mine.all);
+    } else {
+      if (t.mode == kMassListed) {
+        r = __builtin_amdgcn_readfirstlane(last_at_most(at, b.requests, c));
+        ch = c - at[r];
+      } else {
+        r = c / t.chunks;
+        ch = c - r * t.chunks;
+        step = t.chunks;
+      }
+      const RequestRows y = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
+      o = mass_place(b, a, y, keys);
+      row0 = y.row0;
+    }
+    for (; ch < o.all; ch += step) f(r, row0, o, ch, head);
+  }
+}
 
-  auto piece = [&](int req, int row0, const MassPlace& o, int ch, int head) {
-    const int k0 = (ch < o.sinks ? ch : ch - o.sinks + o.first) * kKeys;
+// A vector as its lanes load it: vector `lane % 16` of a tile, dimensions 32 k + 8 (lane / 16) ..
+template <int NB>
+struct MassVector {
+  float x[NB][8], lse;
+  int row;
+  __device__ __forceinline__ void load(const MassArgs& a, const MassPlace& o, int row0, int grp, int head, int tile) {
+    const int vec = 16 * tile + (threadIdx.x & 15);
+    row = vec / grp;
+    const int r = row0 + min(row, o.n - 1), hq = head * grp + vec - row * grp;
+    const float* p = a.q + (size_t)r * a.ldq + (size_t)hq * (32 * NB) + 8 * ((threadIdx.x & 63) >> 4);
+    lse = a.lse[(size_t)r * a.heads + hq];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      *reinterpret_cast<float4*>(&x[k][0]) = *reinterpret_cast<const float4*>(p + 32 * k);
+      *reinterpret_cast<float4*>(&x[k][4]) = *reinterpret_cast<const float4*>(p + 32 * k + 4);
+    }
+  }
+  // its two f16 parts, scaled by the power of two that takes the largest element to 2^13 .. 2^14; the factor of its products and
+  // its lse, in powers of 2. A row that is not there, sees nothing or is not finite gives no weight: q = 0, lse = inf
+  __device__ __forceinline__ float2 split(const MassArgs& a, const MassPlace& o, float minus_one, h8 (&hi)[NB], h8 (&lo)[NB]) {
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
+    top = max(top, lane_xor_u32<16>(top));
+    top = max(top, lane_xor_u32<32>(top));
+    const int e = (int)(top >> 23), f = min(267 - e, 253);
+    const bool ok = e != 255 && row < o.n && fabsf(lse) < INFINITY;
+    const float up = copysignf(__uint_as_float((unsigned)f << 23), a.scale);
+    if (__ballot(!ok) != 0) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[k][j] = ok ? x[k][j] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[k][j] *= up;
+      split8(x[k], minus_one, hi[k], lo[k]);
+    }
+    return ok ? make_float2(__uint_as_float((unsigned)(254 - f) << 23) * (fabsf(a.scale) * 1.4426950408889634f),
+                            lse * 1.4426950408889634f)
+              : make_float2(0.0f, INFINITY);
+  }
+};
+
+// A wave's keys, from k0 on, and their sums.
+template <int NB, int KS>
+struct MassKeys {
+  u32x4 raw[KS][NB];
+  float scale[KS];
+  int k0;
+  f32x4 sum[KS][2];
+  // a lane's own keys (KS = 1: of every other lane), -1 where there is none, their places and what is there
+  static constexpr int kLeft = KS > 1 ? KS / 2 : 1;
+  int mine[kLeft];
+  float* place[kLeft];
+  float was[kLeft];
+  __device__ __forceinline__ void load(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, const MassPlace& o, int req, int head,
+                                       int from) {
+    const int page_steps = b.page >> 5, lane = threadIdx.x & 63, col = lane & 15;
+    k0 = from;
     int pid[KS], in_page[KS];
-    u32x4 kc[KS][NB];
-    float ks[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int step = (k0 >> 5) + s, pg = step / page_steps;
       in_page[s] = step - pg * page_steps;
-      pid[s] = b.table[(size_t)req * b.table_ld + min(pg, b.table_ld - 1)];
-      if (32 * step > o.last || pid[s] >= b.n_pages) pid[s] = -1;
+      const int id = b.table[(size_t)req * b.table_ld + min(pg, b.table_ld - 1)];
+      pid[s] = 32 * step > o.last || id >= b.n_pages ? -1 : id;
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       pid[s] = __builtin_amdgcn_readfirstlane(pid[s]);
-      const int8_t* p = c.k + ((size_t)max(pid[s], 0) * c.kv_heads + head) * ((size_t)b.page * HD) + in_page[s] * (NB * 1024);
+      const size_t page = (size_t)max(pid[s], 0) * c.kv_heads + head;
+      const int8_t* p = c.k + page * ((size_t)b.page * (32 * NB)) + in_page[s] * (NB * 1024) + 16 * lane;
 #pragma unroll
-      for (int k = 0; k < NB; ++k) kc[s][k] = *reinterpret_cast<const u32x4*>(p + 1024 * k + 16 * lane);
-      ks[s] = c.ks[(size_t)max(pid[s], 0) * c.kv_heads + head];
+      for (int k = 0; k < NB; ++k) raw[s][k] = *reinterpret_cast<const u32x4*>(p + 1024 * k);
+      scale[s] = c.ks[page];
+      sum[s][0] = sum[s][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // this lane's four places of each half step, and what is there already
-    float4* place[KS][2];
-    float4 was[KS][2];
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int e = 0; e < kLeft; ++e) {
+      const int i = KS > 1 ? kLeft * col + e : col >> 1, s = i >> 3;                // its number: 8 step + 4 half + place
+      int page = 0, step = 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        place[s][h] = reinterpret_cast<float4*>(a.mass + ((size_t)max(pid[s], 0) * c.kv_heads + head) * b.page +
-                                                32 * in_page[s] + 16 * h + 4 * g);
-        if (W == 1) was[s][h] = *place[s][h];
+      for (int k = 0; k < KS; ++k) {
+        page = k == s ? pid[k] : page;
+        step = k == s ? in_page[k] : step;
       }
-    // tiles of the vectors that see some key of the piece
-    const int i0 = max(0, k0 - o.p0);
-    const int i1 = a.window > 0 && k0 >= a.sinks ? (int)min((long long)o.n, (long long)k0 + kKeys - 1 + a.window - o.p0) : o.n;
-    const int tile1 = (i1 * grp + 15) >> 4;
-    int tile = ((i0 * grp) >> 4) + (W > 1 ? w : 0);
-    float x[NB][8], lse;
-    int row;
-    auto load_q = [&](int tile, float (&x)[NB][8], float& lse, int& row) {
-      const int vec = 16 * tile + col;
-      row = vec / grp;
-      const int r = row0 + min(row, o.n - 1), hq = head * grp + vec - row * grp;
-      const float* p = a.q + (size_t)r * a.ldq + (size_t)hq * HD + 8 * g;
-      lse = a.lse[(size_t)r * a.heads + hq];
+      const int in = 16 * (i >> 2 & 1) + 4 * (lane >> 4) + (i & 3), key = k0 + 32 * s + in;
+      mine[e] = page >= 0 && key <= o.last && (KS > 1 || (col & 1) == 0) ? key : -1;
+      place[e] = a.mass + ((size_t)max(page, 0) * c.kv_heads + head) * b.page + 32 * step + in;
+      was[e] = *place[e];
+    }
+  }
+  // adds the weights of a tile of 16 vectors; st: their products, v: factor and lse, pos: positions (low, high: of the tile's
+  // first and last)
+  __device__ __forceinline__ void add(const MassArgs& a, const f32x4 (&st)[KS][2], float2 v, int pos, int low, int high) {
+    const int g = (threadIdx.x & 63) >> 4, from = a.window > 0 ? pos - a.window + 1 : 0;
 #pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        *reinterpret_cast<float4*>(&x[k][0]) = *reinterpret_cast<const float4*>(p + 32 * k);
-        *reinterpret_cast<float4*>(&x[k][4]) = *reinterpret_cast<const float4*>(p + 32 * k + 4);
-      }
-    };
-    f32x4 sum[KS][2] = {};
-    if (tile < tile1) load_q(tile, x, lse, row);
-    h8 kf[KS][NB][2];
+    for (int s = 0; s < KS; ++s) {
+      const int key0 = k0 + 32 * s;
+      const float f = scale[s] * v.x;
+      const bool hides = key0 + 31 > low || (a.window > 0 && key0 <= high - a.window && key0 + 31 >= a.sinks);
+      float p[8];
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+      for (int e = 0; e < 8; ++e) p[e] = pow2(__builtin_fmaf(st[s][e >> 2][e & 3], f, -v.y));
+      if (hides) {
 #pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        kf[s][k][0] = codes8(kc[s][k][0], kc[s][k][1]);
-        kf[s][k][1] = codes8(kc[s][k][2], kc[s][k][3]);
-      }
-    for (; tile < tile1; tile += W) {
-      unsigned top = 0;
-#pragma unroll
-      for (int k = 0; k < NB; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
-      top = max(top, lane_xor_u32<16>(top));
-      top = max(top, lane_xor_u32<32>(top));
-      const int e = (int)(top >> 23), f = min(267 - e, 253);       // 2^13 <= largest * 2^(f - 127) < 2^14
-      // (a row that is not there, sees nothing or is not finite gives no weight: q = 0, lse = inf)
-      const bool ok = e != 255 && row < o.n && fabsf(lse) < INFINITY;
-      const float up = copysignf(__uint_as_float((unsigned)f << 23), a.scale);
-      const float qs = ok ? __uint_as_float((unsigned)(254 - f) << 23) * (fabsf(a.scale) * 1.4426950408889634f) : 0.0f;
-      const float m = ok ? lse * 1.4426950408889634f : INFINITY;
-      h8 qh[NB], ql[NB];
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[k][j] = ok ? x[k][j] * up : 0.0f;
-        split8(x[k], minus_one, qh[k], ql[k]);
-      }
-      const int pos = o.p0 + row;
-      const int pos_low = __builtin_amdgcn_readlane(pos, 0), pos_high = __builtin_amdgcn_readlane(pos, 15);
-      load_q(tile + W < tile1 ? tile + W : tile, x, lse, row);     // (on its way while this one is multiplied)
-      f32x4 st[KS][2] = {};
-#pragma unroll
-      for (int k = 0; k < NB; ++k)
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          st[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][0], qh[k], st[s][0], 0, 0, 0);
-          st[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][1], qh[k], st[s][1], 0, 0, 0);
-          st[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][0], ql[k], st[s][0], 0, 0, 0);
-          st[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][1], ql[k], st[s][1], 0, 0, 0);
-        }
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int key0 = k0 + 32 * s;
-        const float factor = ks[s] * qs;
-        const bool hides = key0 + 31 > pos_low || (a.window > 0 && key0 <= pos_high - a.window && key0 + 31 >= a.sinks);
-        const int low = a.window > 0 ? pos - a.window + 1 : 0;
-#pragma unroll
-        for (int e8 = 0; e8 < 8; ++e8) {
-          float p = pow2(__builtin_fmaf(st[s][e8 >> 2][e8 & 3], factor, -m));
-          if (hides) {
-            const int j = key0 + 16 * (e8 >> 2) + 4 * g + (e8 & 3);
-            if (j > pos || (j < low && j >= a.sinks)) p = 0.0f;
-          }
-          sum[s][e8 >> 2][e8 & 3] += p;
+        for (int e = 0; e < 8; ++e) {
+          const int j = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
+          if (j > pos || (j < from && j >= a.sinks)) p[e] = 0.0f;
         }
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[s][e >> 2][e & 3] += p[e];
     }
-    // over the 16 vectors of the tiles' columns, and the waves; a step's own tokens start from nothing
-    float4 y[KS][2];
+  }
+  // The sums over the 16 lanes that share keys, by halves: a lane ends with those of its own kLeft keys. v[0 .. N - 1]: what is
+  // left, over the lanes xor X, X / 2, .., 1.
+  template <int N, int X>
+  static __device__ __forceinline__ void halve(float (&v)[8 * KS]) {
+    if constexpr (N == 1) {
+      v[0] += lane_xor<X>(v[0]);
+    } else {
+      const bool upper = threadIdx.x & X;
+#pragma unroll
+      for (int k = 0; k < N / 2; ++k) {
+        const float keep = upper ? v[k + N / 2] : v[k], give = upper ? v[k] : v[k + N / 2];
+        v[k] = keep + lane_xor<X>(give);
+      }
+    }
+    if constexpr (X > 1) halve<(N > 1 ? N / 2 : 1), X / 2>(v);
+  }
+  __device__ __forceinline__ void reduce(float (&out)[kLeft]) const {
+    float v[8 * KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = sum[s][h][i];
-          v += lane_xor<8>(v);
-          v += lane_xor<4>(v);
-          v += lane_xor<2>(v);
-          (&y[s][h].x)[i] = v + lane_xor<1>(v);
-        }
-    if constexpr (W > 1) {
-      __syncthreads();                   // the piece before has been read
-      if (w > 0 && col == 0) {
+        for (int i = 0; i < 4; ++i) v[8 * s + 4 * h + i] = sum[s][h][i];
+    halve<8 * KS, 8>(v);
 #pragma unroll
-        for (int s = 0; s < 2 * KS; ++s) red[w - 1][s][g] = y[s >> 1][s & 1];
-      }
-      __syncthreads();
-      if (w > 0) return;
+    for (int e = 0; e < kLeft; ++e) out[e] = v[e];
+  }
+  // .. added to what the keys have; a step's own tokens start from nothing
+  __device__ __forceinline__ void write(const MassPlace& o, const float (&v)[kLeft]) const {
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          was[s][h] = *place[s][h];
-#pragma unroll
-          for (int i = 0; i < W - 1; ++i) {
-            const float4 z = red[i][2 * s + h][g];
-            y[s][h] = make_float4(y[s][h].x + z.x, y[s][h].y + z.y, y[s][h].z + z.z, y[s][h].w + z.w);
-          }
-        }
-    }
+    for (int e = 0; e < kLeft; ++e)
+      if (mine[e] >= 0) *place[e] = mine[e] >= o.p0 ? v[e] : was[e] + v[e];
+  }
+};
+
+// tiles of the vectors that see some of `keys` keys from k0 on
+__device__ __forceinline__ int2 mass_tiles(const MassArgs& a, const MassPlace& o, int grp, int k0, int keys) {
+  const int i0 = max(0, k0 - o.p0);
+  const int i1 = a.window > 0 && k0 >= a.sinks ? (int)min((long long)o.n, (long long)k0 + keys - 1 + a.window - o.p0) : o.n;
+  return make_int2((i0 * grp) >> 4, (i1 * grp + 15) >> 4);
+}
+__device__ __forceinline__ int piece_key(const MassPlace& o, int ch, int keys) {
+  return (ch < o.sinks ? ch : ch - o.sinks + o.first) * keys;
+}
+
+// W = 1: a wave for each piece. Else a workgroup for each, whose W waves take every W-th tile.
+// Steps of a piece: as many as leave a SIMD two waves (us of 1 / 2 for a wave alone: 64 requests of up to 8192 tokens, 4 heads of
+// 128 20.9 / 16.8; of 2 / 4 for prompts of 8 heads of 64 62 / 52).
+constexpr int mass_steps(int nb, int w) { return w > 1 && nb <= 2 ? 4 : nb <= 4 ? 2 : 1; }
+template <int NB, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 2) void kv8_mass_kernel(PagedBatch b, Kv8Cache c, MassArgs a, MassCut t) {
+  constexpr int KS = mass_steps(NB, W), kKeys = 32 * KS, kLeft = MassKeys<NB, KS>::kLeft;
+  __shared__ float red[W > 1 ? W - 1 : 1][kLeft][64];
+  __shared__ int at[kMassList];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = a.heads / c.kv_heads;
+  float minus_one = -1.0f;
+  asm volatile("" : "+v"(minus_one));
+  mass_pieces<W == 1 ? 4 : W>(b, a, t, c.kv_heads, kKeys, W == 1 ? 4 * blockIdx.x + w : blockIdx.x, W == 1 ? 4 * gridDim.x : gridDim.x,
+                              at, [&](int req, int row0, const MassPlace& o, int ch, int head) {
+    const int k0 = piece_key(o, ch, kKeys);
+    MassKeys<NB, KS> keys;
+    keys.load(b, c, a, o, req, head, k0);
+    const int2 tiles = mass_tiles(a, o, grp, k0, kKeys);
+    int tile = tiles.x + (W == 1 ? 0 : w);
+    MassVector<NB> q;
+    if (tile < tiles.y) q.load(a, o, row0, grp, head, tile);
+    h8 kf[KS][NB][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int j = k0 + 32 * s + 16 * h + 4 * g;
-        if (pid[s] < 0 || j > o.last || col != 0) continue;
-        float z[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float old = (&was[s][h].x)[i], add = (&y[s][h].x)[i];
-          z[i] = j + i > o.last ? old : j + i >= o.p0 ? add : old + add;
-        }
-        *place[s][h] = make_float4(z[0], z[1], z[2], z[3]);
+      for (int k = 0; k < NB; ++k) {
+        kf[s][k][0] = codes8(keys.raw[s][k][0], keys.raw[s][k][1]);
+        kf[s][k][1] = codes8(keys.raw[s][k][2], keys.raw[s][k][3]);
       }
-  };
+    for (; tile < tiles.y; tile += W) {
+      h8 hi[NB], lo[NB];
+      const float2 v = q.split(a, o, minus_one, hi, lo);
+      const int pos = o.p0 + q.row;
+      q.load(a, o, row0, grp, head, tile + W < tiles.y ? tile + W : tile);          // (on its way meanwhile)
+      f32x4 st[KS][2] = {};
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              st[s][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][k][h], part ? lo[k] : hi[k], st[s][h], 0, 0, 0);
+      keys.add(a, st, v, pos, __builtin_amdgcn_readlane(pos, 0), __builtin_amdgcn_readlane(pos, 15));
+    }
+    float sums[kLeft];
+    keys.reduce(sums);
+    if constexpr (W > 1) {               // the waves' sums, in their order
+      __syncthreads();                   // (those of the piece before have been read)
+#pragma unroll
+      for (int e = 0; e < kLeft; ++e)
+        if (w > 0) red[w - 1][e][lane] = sums[e];
+      __syncthreads();
+      if (w > 0) return;
+#pragma unroll
+      for (int i = 0; i < W - 1; ++i)
+#pragma unroll
+        for (int e = 0; e < kLeft; ++e) sums[e] += red[i][e][lane];
+    }
+    keys.write(o, sums);
+  });
+}
 
-  const int first = W > 1 ? blockIdx.x : 4 * blockIdx.x + w, stride = W > 1 ? gridDim.x : 4 * gridDim.x;
-  if (t.mode == kMassLanes) {
-    const int i = min(lane, b.requests - 1);
-    const RequestRows q = request_rows(i, b.start[i], b.count[i], b.len[i], b.rows);
-    const MassPlace o = mass_place(b, a, q, kKeys);
-    const int mine = lane < b.requests ? o.all : 0, upto = wave_scan(mine);
-    const int total = __builtin_amdgcn_readlane(upto, 63) * c.kv_heads;
-    for (int u = first; u < total; u += stride) {
-      const int ch = u / c.kv_heads, l = __ffsll(__ballot(ch < upto)) - 1;
-      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-      piece(l, of(q.row0), MassPlace{of(o.n), of(o.p0), of(o.last), of(o.sinks), of(o.first), of(o.all)}, ch - of(upto - mine),
-            u - ch * c.kv_heads);
-    }
-    return;
-  }
-  if (t.mode == kMassListed) {
-    constexpr int kOwn = kMassList / 256;
-    int mine[kOwn], sum = 0, before;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      const int r = kOwn * threadIdx.x + i, in = min(r, b.requests - 1);
-      const MassPlace o = mass_place(b, a, request_rows(in, b.start[in], b.count[in], b.len[in], b.rows), kKeys);
-      mine[i] = r < b.requests ? o.all : 0;
-      sum += mine[i];
-    }
-    const int total = scan_block<4>(sum, before) * c.kv_heads;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      at[kOwn * threadIdx.x + i] = before;
-      before += mine[i];
-    }
-    __syncthreads();
-    for (int u = first; u < total; u += stride) {
-      const int ch = u / c.kv_heads, r = last_at_most(at, b.requests, ch);
-      const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
-      piece(r, q.row0, mass_place(b, a, q, kKeys), ch - at[r], u - ch * c.kv_heads);
-    }
-    return;
-  }
-  const long long all = (long long)b.requests * t.chunks * c.kv_heads;
-  for (long long u = first; u < all; u += stride) {
-    const int head = (int)(u % c.kv_heads), r = (int)(u / c.kv_heads / t.chunks);
-    const RequestRows q = request_rows(r, b.start[r], b.count[r], b.len[r], b.rows);
-    const MassPlace o = mass_place(b, a, q, kKeys);
-    for (int ch = (int)(u / c.kv_heads % t.chunks); ch < o.all; ch += t.chunks) piece(r, q.row0, o, ch, head);
-  }
+static MassCut mass_cut(const PagedBatch& b, const MassArgs& a, int keys) {
+  long chunks = (std::max(a.max_len, 1) + keys - 1) / keys;
+  if (a.window > 0) chunks = std::min(chunks, (long)(a.sinks + keys - 1) / keys + ((long)a.window + a.max_rows - 2) / keys + 2);
+  const int mode = b.requests <= 64 ? kMassLanes : b.requests <= kMassList ? kMassListed : kMassEven;
+  return {(int)(mode == kMassEven ? std::min(chunks, 16L) : chunks), mode};        // (a longer request's waves take several)
 }
 
 template <int NB, int W>
 static void launch_mass_as(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
-  constexpr int kKeys = 32 * (NB <= 2 ? 4 : NB <= 4 ? 2 : 1);
-  long chunks = (std::max(a.max_len, 1) + kKeys - 1) / kKeys;
-  if (a.window > 0)
-    chunks = std::min(chunks, (long)(a.sinks + kKeys - 1) / kKeys + ((long)a.window + a.max_rows - 2) / kKeys + 2);
-  const int mode = b.requests <= 64 ? kMassLanes : b.requests <= kMassList ? kMassListed : kMassEven;
-  if (mode == kMassEven) chunks = std::min(chunks, 16L);           // (a longer request's waves take several)
-  const long waves = (long)b.requests * c.kv_heads * chunks;
-  const long groups = std::min(W > 1 ? waves : (waves + 3) / 4, (long)kMassWorkgroups);
-  hipLaunchKernelGGL((kv8_mass_kernel<NB, W>), dim3((unsigned)groups), dim3(256), 0, s, b, c, a, MassCut{(int)chunks, mode});
+  const MassCut t = mass_cut(b, a, 32 * mass_steps(NB, W));
+  const long pieces = (long)b.requests * c.kv_heads * t.chunks;
+  const long groups = std::min(W == 1 ? (pieces + 3) / 4 : pieces, W == 4 ? 1024L : 512L);
+  hipLaunchKernelGGL((kv8_mass_kernel<NB, W>), dim3((unsigned)groups), dim3(W == 1 ? 256 : 64 * W), 0, s, b, c, a, t);
 }
 template <int NB>
 static void launch_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
-  if ((long)a.max_rows * (a.heads / c.kv_heads) > 64) launch_mass_as<NB, 4>(b, c, a, s);
+  // eight waves for the heads whose pieces are shorter (us of 4 / 8: prompts of 8 heads of 64 47 / 52, of 128 with a window of 1000
+  // 82 / 64)
+  constexpr int W = NB <= 2 ? 4 : 8;
+  if ((long)a.max_rows * (a.heads / c.kv_heads) > 64) launch_mass_as<NB, W>(b, c, a, s);
   else launch_mass_as<NB, 1>(b, c, a, s);
 }
 
