@@ -433,7 +433,7 @@ int re_kv8_mass_dev(const float *d_q, size_t ldq, const float *d_lse, size_t row
  * (d_kv_len_out, d_table_out, d_free_out, d_n_free_out may be the inputs; entries of d_table_out behind a cut request's
  * pages are -1); d_from_len: a cut request's old length, 0 for the others; d_from_table (requests x table_ld): a cut
  * request's old entries (may be d_table if d_table_out is another buffer; never d_table_out); d_dropped: NULL, or per
- * request += the tokens it lost, 0 where it holds none (positions of its next tokens are its length and these);
+ * request += the tokens it lost, 0 where it holds none (re_kv_positions_dev adds them to its rows' positions);
  * d_status[0] requests over the limit that were left, d_status[1] cut ones. Up to 4096 requests.
  *
  * re_kv8_evict_dev, for each layer: of a cut request's tokens the first `first`, the last `recent` and the heaviest of
@@ -451,6 +451,11 @@ int re_kv8_evict_dev(size_t requests, const int *d_from_len, const int *d_from_t
                      size_t table_ld, size_t page, size_t n_pages, int8_t *d_kcodes, int8_t *d_vcodes, float *d_kscale,
                      float *d_vscale, float *d_mass, size_t n_kv_heads, size_t head_dim, size_t keep, size_t first,
                      size_t recent, size_t max_len, int *d_kept, void *stream);
+
+/* Rotary positions of a step's rows after evictions: d_out[r] = d_row_pos[r] + d_dropped[d_row_seq[r]], -1 for rows without a
+ * request (of the plan's d_row_seq and d_row_pos, which count what the cache holds). d_out may be d_row_pos. */
+int re_kv_positions_dev(size_t rows, const int *d_row_seq, const int *d_row_pos, size_t requests, const int *d_dropped,
+                        int *d_out, void *stream);
 
 /* Drafted tokens against the target's probabilities. Request b has d_row_count[b] rows of logits from d_row_start[b] on
  * (ranges ascending and disjoint, as above; 0: none): row i is the target's after token d_tokens[row i], d_tokens[row i + 1] the

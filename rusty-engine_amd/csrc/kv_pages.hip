@@ -244,4 +244,21 @@ hipError_t launch_kv_rewind(const RewindArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// ---- positions -----------------------------------------------------------------------------------
+// A request that has been cut stands further on than its cache is long.
+__global__ __launch_bounds__(256) void kv_positions_kernel(const int* seq, const int* pos, int rows, const int* dropped,
+                                                           int requests, int* out) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= rows) return;
+  const int b = seq[r], p = pos[r];
+  out[r] = p >= 0 && b >= 0 && b < requests ? p + dropped[b] : -1;
+}
+
+hipError_t launch_kv_positions(const int* seq, const int* pos, int rows, const int* dropped, int requests, int* out,
+                               hipStream_t s) {
+  hipLaunchKernelGGL(kv_positions_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, seq, pos, rows, dropped,
+                     requests, out);
+  return hipGetLastError();
+}
+
 }  // namespace rehip

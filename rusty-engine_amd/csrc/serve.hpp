@@ -152,6 +152,8 @@ struct VerifyArgs {
 hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
 hipError_t launch_kv_evict_plan(const EvictPlanArgs& a, hipStream_t s);
 hipError_t launch_kv_rewind(const RewindArgs& a, hipStream_t s);
+hipError_t launch_kv_positions(const int* seq, const int* pos, int rows, const int* dropped, int requests, int* out,
+                               hipStream_t s);
 hipError_t launch_kv8_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s);
 hipError_t launch_kv8_evict(const EvictArgs& a, const Kv8Cache& c, hipStream_t s);
 size_t verify_work_bytes(int rows, int requests, int vocab);

@@ -336,6 +336,16 @@ int re_kv_rewind_dev(size_t requests, size_t page, const int* d_back, const int*
   return RE_OK;
 }
 
+int re_kv_positions_dev(size_t rows, const int* d_row_seq, const int* d_row_pos, size_t requests, const int* d_dropped,
+                        int* d_out, void* stream) {
+  if (!d_row_seq || !d_row_pos || !d_dropped || !d_out) return report_error(RE_ERR_ARG, "null pointer");
+  if (rows > (1u << 22) || requests == 0 || requests > (1u << 16))
+    return report_error(RE_ERR_SIZE, "positions of %zu rows, %zu requests (up to 4194304, 1 .. 65536)", rows, requests);
+  if (rows == 0) return RE_OK;
+  HIP_TRY(launch_kv_positions(d_row_seq, d_row_pos, (int)rows, d_dropped, (int)requests, d_out, (hipStream_t)stream));
+  return RE_OK;
+}
+
 size_t re_draft_verify_work_bytes(size_t rows, size_t requests, size_t vocab) {
   if (rows == 0 || requests == 0 || vocab == 0 || rows > (1u << 22) || requests > (1u << 16) || vocab > (1u << 24)) return 0;
   return verify_work_bytes((int)rows, (int)requests, (int)vocab);

@@ -57,7 +57,7 @@ EXPORTS = ("re_init", "re_last_error", "re_version", "re_row_bytes", "re_tiled_b
            "re_kv_plan_dev", "re_rope_freqs", "re_rope_rows_dev", "re_kv8_append_dev", "re_attention_kv8_work_bytes",
            "re_attention_kv8_dev", "re_logprobs_work_bytes", "re_logprobs_dev",
            "re_attention_kv8_sinks_dev", "re_kv8_mass_dev", "re_kv_evict_plan_dev", "re_kv8_evict_dev",
-           "re_draft_verify_work_bytes", "re_draft_verify_dev", "re_kv_rewind_dev")
+           "re_kv_positions_dev", "re_draft_verify_work_bytes", "re_draft_verify_dev", "re_kv_rewind_dev")
 GEMV_KERNELS = {0: "split", 1: "rows", 2: "tile", 3: "dense"}
 
 
@@ -182,6 +182,7 @@ def lib() -> C.CDLL:
                                       + [C.c_float, _sz, _sz, _vp, _vp])
         L.re_kv_evict_plan_dev.argtypes = [_sz] * 4 + [_vp, _vp, _sz, _vp, _sz] + [_vp] * 10
         L.re_kv8_evict_dev.argtypes = [_sz] + [_vp] * 3 + [_sz] * 3 + [_vp] * 5 + [_sz] * 6 + [_vp] * 2
+        L.re_kv_positions_dev.argtypes = [_sz, _vp, _vp, _sz, _vp, _vp, _vp]
         L.re_draft_verify_work_bytes.argtypes = [_sz] * 3
         L.re_draft_verify_work_bytes.restype = _sz
         L.re_draft_verify_dev.argtypes = [_vp] + [_sz] * 4 + [_vp] * 4 + [_sz] + [_vp] * 7 + [_sz, _vp]
@@ -698,6 +699,12 @@ def kv8_evict_dev(requests, from_len, from_table, table, table_ld, page, n_pages
     _check(lib().re_kv8_evict_dev(requests, _p(from_len), _p(from_table), _p(table), table_ld, page, n_pages, _p(kcodes),
                                   _p(vcodes), _p(kscale), _p(vscale), _p(mass), n_kv_heads, head_dim, keep, first, recent,
                                   max_len, _p(kept), _stream_ptr(stream)))
+
+
+def kv_positions_dev(rows, row_seq, row_pos, requests, dropped, out, stream=None):
+    """Rotary positions of a step's rows after evictions: what the plan counts and what the requests have lost
+    (re_kv_positions_dev); `out` may be `row_pos`."""
+    _check(lib().re_kv_positions_dev(rows, _p(row_seq), _p(row_pos), requests, _p(dropped), _p(out), _stream_ptr(stream)))
 
 
 def draft_verify_work_bytes(rows, requests, vocab) -> int:

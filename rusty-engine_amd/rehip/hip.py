@@ -169,3 +169,9 @@ class Graph:
 
 def synchronize() -> None:
     check(hip().hipDeviceSynchronize())
+
+
+def copy_device(dst: int, src: int, nbytes: int) -> None:
+    """Copies between two device addresses; waits for it."""
+    check(hip().hipMemcpy(C.c_void_p(dst), C.c_void_p(src), nbytes, D2D))
+    synchronize()

@@ -505,15 +505,19 @@ class DeviceDecoder:
     V are kept in int8 pages of 64 tokens with a scale for each page and KV head (a quarter of the f32
     caches' memory, any max_seq): per layer rotary positions, append and attention over the pages are launches
     of their own, planned on the device, in prefill and decode alike (head_dim a
-    multiple of 32, prefills of up to 262144 rows).
+    multiple of 32, prefills of up to 262144 rows). There a `window` makes every row see that many last tokens only, and the
+    sequence's first `sinks`: a step then costs the same however long the sequence is.
     Prefills and steps go on at seq_len, also where that was set back: 0 begins a new sequence."""
 
     def __init__(self, mb: ModelBytes, max_seq: int, mode: int = MODE_F32, prefill_rows: int = 1024,
-                 use_graph: bool = True, kv_cache: str = "f32"):
+                 use_graph: bool = True, kv_cache: str = "f32", window: int = 0, sinks: int = 0):
         from . import Ffn, attention_work_bytes, hip, rope_table_dev
         self._check_supported(mb)
         if kv_cache not in ("f32", "int8"):
             raise ValueError(f"DeviceDecoder: kv_cache {kv_cache!r} (f32 or int8)")
+        if window < 0 or not 0 <= sinks <= 1024 or ((window or sinks) and kv_cache != "int8"):
+            raise ValueError(f"DeviceDecoder: window {window}, sinks {sinks} (up to 1024) need the int8 pages")
+        self.window, self.sinks = window, sinks
         self.pages = _Int8Pages(mb, max_seq, prefill_rows) if kv_cache == "int8" else None
         self.mb, self.mode, self.max_seq = mb, mode, max_seq
         self.use_graph = use_graph
@@ -655,7 +659,7 @@ class DeviceDecoder:
 
     def _paged_attention(self, blk, rows):
         """int8 pages: rotary positions, append and attention of the rows that the step's plan gave."""
-        from . import ROPE_HALF, attention_kv8_dev, kv8_append_dev, rope_rows_dev
+        from . import ROPE_HALF, attention_kv8_dev, attention_kv8_sinks_dev, kv8_append_dev, rope_rows_dev
         g, d, kv, p, s = self.g, self.g.d_model, self.kv, self.pages, self.stream
         ld = d + 2 * kv
         rope_rows_dev(self.qkv, ld, rows, g.n_heads + g.n_kv_heads, g.head_dim, g.head_dim, ROPE_HALF, p.freqs, 1.0,
@@ -663,8 +667,12 @@ class DeviceDecoder:
         batch = (rows, 1, p.row_start, p.row_count, p.kv_len, p.table, p.count, p.PAGE, p.count, *blk["cache"])
         kv8_append_dev(_Offset(self.qkv, 4 * d), ld, _Offset(self.qkv, 4 * (d + kv)), ld, *batch, g.n_kv_heads,
                        g.head_dim, s)
-        attention_kv8_dev(self.qkv, ld, *batch, rows, self.max_seq, g.n_heads, g.n_kv_heads, g.head_dim,
-                          g.head_dim ** -0.5, 0, self.ctx, p.work, p.work_bytes, s)
+        shape = (rows, self.max_seq, g.n_heads, g.n_kv_heads, g.head_dim, g.head_dim ** -0.5)
+        if self.window:
+            attention_kv8_sinks_dev(self.qkv, ld, *batch, *shape, self.window, self.sinks, self.ctx, None, p.work,
+                                    p.work_bytes, s)
+        else:
+            attention_kv8_dev(self.qkv, ld, *batch, *shape, 0, self.ctx, p.work, p.work_bytes, s)
 
     def _head_and_advance(self, last_row, delta):
         from . import decode_advance_dev
@@ -795,6 +803,67 @@ class DeviceDecoder:
         self.stream.synchronize()
         return int(self.tok.download(np.int32, 1)[0])
 
+    def step_drafted(self, drafts, temperature: float = 0.0, probs=None, accept_u=None, sample_u=None) -> list:
+        """Decodes the token in `tok` and the drafted ones behind it in one pass; returns the drafts that the model
+        accepts and the token that it puts behind them, 1 to len(drafts) + 1 tokens (`draft_verify_dev`). Greedy at
+        temperature 0: the tokens that as many `step` calls would give. Else drafts (drawn from the rows of `probs`, or
+        certain without them) are accepted with the random numbers `accept_u`, one each, and the token behind is drawn
+        with `sample_u`, all from [0, 1): the tokens are then distributed as the model's own. Rejected drafts are
+        taken back as by setting seq_len."""
+        from . import draft_verify_dev, draft_verify_work_bytes, hip, rmsnorm_dev
+        B = hip.DeviceBuffer
+        g, s, v, n0 = self.g, self.stream, self.mb.n_vocab, self.seq_len
+        drafts = np.asarray(drafts, np.int32).reshape(-1)
+        n, rows = drafts.size, drafts.size + 1
+        if temperature > 0 and (sample_u is None or (n and accept_u is None)):
+            raise ValueError("step_drafted: a temperature needs random numbers")
+        u, r = np.zeros(rows, np.float32), np.float32(sample_u or 0)
+        if accept_u is not None:
+            u[:n] = np.asarray(accept_u, np.float32).reshape(n)
+        q = None
+        if probs is not None:
+            q = B.from_array(np.concatenate([np.asarray(probs, np.float32).reshape(n, v), np.zeros((1, v), np.float32)]))
+        s.synchronize()
+        tokens = np.concatenate([self.tok.download(np.int32, 1), drafts])
+        self._forward_rows(tokens)                             # (checks the tokens and the room)
+        rmsnorm_dev(self.x, self.output_norm, rows, g.d_model, g.rms_eps, self.n, s)
+        logits = B(rows * v * 4)
+        self.output.matmul_dev(self.n, rows, logits, self.mode, stream=s)
+        i32 = lambda a: B.from_array(np.asarray(a, np.int32))   # noqa: E731
+        accepted, back, out = i32([0]), i32([0]), i32(np.full(rows, -1))
+        nbytes = draft_verify_work_bytes(rows, 1, v)
+        args = [i32([0]), i32([rows]), i32(tokens), B.from_array(np.array([temperature], np.float32)), B.from_array(u),
+                B.from_array(np.array([r], np.float32)), B(nbytes)]
+        draft_verify_dev(logits, v, rows, v, 1, *args[:3], q, v, *args[3:6], accepted, back, out, args[6], nbytes, s)
+        s.synchronize()
+        k = int(accepted.download(np.int32, 1)[0])
+        got = out.download(np.int32, rows)[:k + 1]
+        self._done(rows)
+        if got[k] < 0:
+            self.seq_len = n0
+            raise ValueError("step_drafted: the model's logits are not finite")
+        self.seq_len = n0 + 1 + k
+        hip.copy_device(self.logits_buf.ptr, logits.ptr + 4 * k * v, 4 * v)
+        self.tok.upload(got[k:])
+        hist = self.hist.download(np.int32, self.max_seq)
+        places = np.arange(n0 + 1, min(n0 + 2 + k, self.max_seq))
+        hist[places] = got[:places.size]
+        self.hist.upload(hist)
+        return [int(t) for t in got]
+
+    def generate_drafted(self, prompt, max_new: int, most: int = 4, ngram: int = 2):
+        """`generate` with up to `most` tokens a step drafted by looking up the last `ngram` tokens earlier in the
+        sequence (`lookup_drafts`): the same greedy tokens in fewer steps where the text repeats itself."""
+        p0 = self.seq_len
+        prompt = [int(t) for t in np.asarray(prompt).reshape(-1)]
+        if p0 + len(prompt) + max_new > self.max_seq:
+            raise ValueError(f"{len(prompt)} + {max_new} tokens from position {p0} exceed max_seq {self.max_seq}")
+        out = [self.prefill(prompt)][:max_new]
+        while len(out) < max_new:
+            room = min(most, max_new - len(out) - 1, self.cap - 1)
+            out += self.step_drafted(lookup_drafts(prompt + out, room, ngram))
+        return out
+
     def replay(self, steps: int) -> None:
         """`steps` decode steps back to back with no host synchronisation in between (the token
         and position stay on the GPU; each token is recorded in the history); waits for the
@@ -881,6 +950,17 @@ class _Int8Pages:
         kv_plan_dev(1, self.PAGE, new, self.kv_len, self.table, self.count, self.free, self.count, self.n_free,
                     self.kv_len, self.n_free, self.row_start, self.row_count, rows, self.row_seq, self.row_pos,
                     self.row_slot, self.status, stream)
+
+
+def lookup_drafts(tokens, most: int, ngram: int = 2) -> list:
+    """Up to `most` tokens that followed the latest earlier occurrence of the last `ngram` tokens."""
+    if most <= 0 or ngram <= 0 or len(tokens) <= ngram:
+        return []
+    last = tokens[-ngram:]
+    for at in range(len(tokens) - ngram - 1, -1, -1):
+        if tokens[at:at + ngram] == last:
+            return list(tokens[at + ngram:at + ngram + most])
+    return []
 
 
 class _Offset:

@@ -111,7 +111,17 @@ def test_verify_refusals(code, change):
     refused(code, rehip.draft_verify_dev, **{**VERIFY, **change})
 
 
+POSITIONS = dict(rows=9, row_seq=A, row_pos=A, requests=3, dropped=A, out=A)
+
+
+@pytest.mark.parametrize("code,change", nulls("row_seq", "row_pos", "dropped", "out") + [
+    (SIZE, {"rows": (1 << 22) + 1}), (SIZE, {"requests": 0}), (SIZE, {"requests": 65537})])
+def test_positions_refusals(code, change):
+    refused(code, rehip.kv_positions_dev, **{**POSITIONS, **change})
+
+
 def test_no_rows_is_no_work():
+    rehip.kv_positions_dev(**{**POSITIONS, "rows": 0})
     rehip.attention_kv8_sinks_dev(**{**ATTN, "rows": 0, "work": None, "work_bytes": 0})
     rehip.kv8_mass_dev(**{**MASS, "rows": 0})
     rehip.draft_verify_dev(**{**VERIFY, "requests": 0, "rows": 0})
