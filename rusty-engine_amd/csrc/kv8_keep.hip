@@ -509,8 +509,10 @@ __global__ __launch_bounds__(THREADS) void kv8_evict_pick_kernel(EvictArgs a, in
 // that hold them with 7 neighbours are loaded. Where a lane's tokens lie is found once for all blocks of dimensions.
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-// the code in byte i of x, rounded to another scale: q + 1.5 2^23 rounds q to an integer, whose low byte is the code
+// the code in byte i of x, rounded to another scale: q + 1.5 2^23 rounds q to an integer, whose low byte is the code (q is a
+// rounded product: fused with the sum, codes next to a half would go the other way)
 __device__ __forceinline__ unsigned moved(unsigned x, int i, float r) {
+#pragma clang fp contract(off)
   const float q = (float)((int)(x << (24 - 8 * i)) >> 24) * r;
   return __float_as_uint(q + 12582912.0f);
 }

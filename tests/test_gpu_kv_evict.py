@@ -276,3 +276,32 @@ def test_rewind_and_plan_go_on():
         t = get(table, n * ld).reshape(n, ld)
         used = [t[b, :-(-length[b] // page)] for b in range(n)] + [get(free, pages)[:get(nf, 1)[0]]]
         assert sorted(np.concatenate(used)) == list(range(pages))
+
+
+def test_evict_rounds_the_rounded_product():
+    """Codes whose product with the ratio of scales is next to half a code: the product is rounded to f32 before it is rounded
+    to a code, so those that f32 takes to the half go to the even one."""
+    page, hd, n = 32, 64, 120
+    c = np.arange(1, 128)
+    ratios, hits = [], 0
+    for k in range(n):                   # (k + 1/2) / c of some c above k, rounded: c times it is next to k + 1/2
+        code = int(c[c > k][k * 7 % (127 - k)])
+        r = np.float32((k + 0.5) / code)
+        ratios.append(r)
+        exact = float(r) * code
+        hits += np.rint(np.float32(code) * r) != np.rint(exact)
+    assert hits > 10
+    p = Pool(np.random.default_rng(15), [64] * n, page, n + 1)
+    cache = Cache(np.random.default_rng(16), p.n_pages, 1, page, hd)
+    for b in range(n):                   # one page of this scale, one of scale 1, tokens of both in the new one
+        cache.ks[p.table[b, :2], 0] = cache.vs[p.table[b, :2], 0] = ratios[b], 1.0
+        for codes in (cache.k, cache.v):
+            codes[p.table[b, 0], 0] = np.arange(-64, 64)[None].repeat(16, 0).reshape(page, hd) if b % 2 else np.arange(
+                64, 128)[None].repeat(page, 0)
+    cache.upload()
+    got, want = check_plan(p, 40, 32, False)
+    d, kept = got["bufs"], np.zeros((n, 1, 32), np.int32)
+    rehip.kv8_evict_dev(n, d["from_len"], d["from_table"], d["table"], p.ld, page, p.n_pages, *cache.args(), None, 1, hd, 32, 31, 1, 64,
+                        i32(kept))
+    ref.evict(want[3], want[4], want[1], page, (cache.k, cache.v, cache.ks, cache.vs), None, 32, 31, 1, kept)
+    cache.check()
