@@ -19,7 +19,7 @@ namespace rehip {
 // |f| <= 1/2: from a table of 64 in LDS and the series of 2^(f / 64) - 1 to its third power, off by (ln 2 / 128)^4 / 24 = 3.6e-11
 // at most: a token at the border of 151936 equal ones is then taken for its neighbour once in 200000 times.
 //
-// Three launches: maxima and sums of parts of all rows; every request's last row found from them, and the sums of its
+// Small vocabularies: one launch. Else three: maxima and sums of parts of all rows; every request's last row found from them, and the sums of its
 // weights by blocks of the vocabulary; the block where r falls, and the token in it.
 //
 // 64 requests of up to 4 drafts, 189 rows of 151936 and the drafts' probabilities, 153 MB: 54 us, 33 + 18 + 7.6 in the three
@@ -133,31 +133,24 @@ __device__ __forceinline__ RowPart joined_wave(const RowPart& p, double c64) {
   return {z, m, best, bad, 0};
 }
 
-// One workgroup per (row, part).
-__global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs a, int parts) {
-  __shared__ double table[kVerTable];
-  __shared__ RowPart ws[kVerWaves];
-  const int r = blockIdx.x / parts, part = blockIdx.x % parts;
-  const float* x = a.x + (size_t)r * a.ld;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int steps = (a.vocab + kVerStep - 1) / kVerStep;
-  const int s0 = (int)((long long)steps * part / parts), s1 = (int)((long long)steps * (part + 1) / parts);
-  // element k of a lane in step s
-  auto place = [&](int s, int k) { return s * kVerStep + w * 64 * kVerBatch + 256 * (k >> 2) + 4 * lane + (k & 3); };
+// A lane's part of a row: elements 256 i + 4 lane .. + 3, i < 4, from `base` on, and so on every `step`, of steps s0 .. s1 - 1; whole
+// steps first, the next one loading meanwhile (a load under a condition would be waited for), then the row's last part of one.
+// begin() is called while the first is on its way; it gives the units, and whether the row counts.
+template <class Begin>
+__device__ __forceinline__ RowPart row_part(const float* x, int vocab, int s0, int s1, int step, int base, const double* table,
+                                            double& c64, Begin begin) {
+  const int lane = threadIdx.x & 63;
+  auto place = [&](int s, int k) { return s * step + base + 256 * (k >> 2) + 4 * lane + (k & 3); };
   auto load = [&](int s, float (&v)[kVerBatch]) {
 #pragma unroll
     for (int k = 0; k < kVerBatch; k += 4)
       *reinterpret_cast<f32x4u*>(&v[k]) = *reinterpret_cast<const f32x4u*>(x + place(s, k));
   };
-  // whole steps, the next one loading meanwhile (a load under a condition would be waited for), then the row's last part of one
-  const int whole = min(s1, a.vocab / kVerStep);
+  const int whole = min(s1, vocab / step);
   float v[kVerBatch], nx[kVerBatch];
-  if (s0 < whole) load(s0, v);           // (on its way while the row's request is found)
-  const RequestRows q = request_of_unit(r, rows_of(a), 1, 0);
-  if (q.req < 0 || r >= q.row0 + q.count) return;
-  const double c64 = units_of(a, q.req);
-  fill_table(table);
+  if (s0 < whole) load(s0, v);
   RowPart mine{0.0, -INFINITY, 0x7fffffff, 0, 0};
+  if (!begin()) return mine;
   auto take = [&](const float (&v)[kVerBatch], int s) {
     float mx = -INFINITY;
 #pragma unroll
@@ -191,11 +184,33 @@ __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs 
 #pragma unroll
     for (int k = 0; k < kVerBatch; ++k) {
       const int at = place(s, k);
-      const float y = x[min(at, a.vocab - 1)];
-      v[k] = at < a.vocab ? y : -INFINITY;
+      const float y = x[min(at, vocab - 1)];
+      v[k] = at < vocab ? y : -INFINITY;
     }
     take(v, s);
   }
+  return mine;
+}
+
+// One workgroup per (row, part).
+__global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs a, int parts) {
+  __shared__ double table[kVerTable];
+  __shared__ RowPart ws[kVerWaves];
+  const int r = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int steps = (a.vocab + kVerStep - 1) / kVerStep;
+  const int s0 = (int)((long long)steps * part / parts), s1 = (int)((long long)steps * (part + 1) / parts);
+  double c64 = 0.0;
+  bool counts = false;
+  const RowPart mine = row_part(a.x + (size_t)r * a.ld, a.vocab, s0, s1, kVerStep, w * 64 * kVerBatch, table, c64, [&] {
+    const RequestRows q = request_of_unit(r, rows_of(a), 1, 0);
+    counts = q.req >= 0 && r < q.row0 + q.count;
+    if (!counts) return false;
+    c64 = units_of(a, q.req);
+    fill_table(table);
+    return true;
+  });
+  if (!counts) return;
   const RowPart all = joined_wave(mine, c64);
   if (lane == 0) ws[w] = all;
   __syncthreads();
@@ -207,9 +222,9 @@ __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs 
 }
 
 // How many drafts of a request are accepted, and where its next token comes from. Every wave of the workgroup looks at a row of
-// its own at a time.
-template <int WAVES>
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& q, double c64, int parts) {
+// its own at a time; part(row) gives what its lanes hold of it.
+template <int WAVES, class Part>
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRows& q, double c64, Part part) {
   __shared__ Decision found[WAVES];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Decision d{};
@@ -220,15 +235,13 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
     const int t = drafted ? a.tokens[row + 1] : 0, at = min(max(t, 0), a.vocab - 1);
     const float x = a.x[(size_t)row * a.ld + at], share = a.probs ? a.probs[(size_t)row * a.ldp + at] : 1.0f;
     const float u = a.accept_u[row];
-    RowPart p = reinterpret_cast<const RowPart*>(a.work)[(size_t)row * parts + min(lane, parts - 1)];
-    if (lane >= parts) p = {0.0, -INFINITY, 0x7fffffff, 0, 0};
-    p = joined_wave(p, c64);
+    const RowPart p = joined_wave(part(row), c64);
     const bool none = p.bad || p.m == -INFINITY;
     bool accepted = false;
     if (drafted && !none && t == at)
       accepted = c64 < 0.0 ? t == p.best
-                            : (double)u * (double)share * p.z <
-                                  (x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)p.m) * (c64 / kVerTable)));
+                           : (double)u * (double)share * p.z <
+                                 (x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)p.m) * (c64 / kVerTable)));
     if (lane == 0)
       found[w] = {p.z, p.m, accepted ? -1 : i, row, none ? kNone : c64 < 0.0 ? kGreedy : drafted ? kRest : kTarget, p.best, 0};
     __syncthreads();
@@ -283,7 +296,10 @@ __global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs
   if (q.count <= 0) return;
   const double c64 = units_of(a, req);
   fill_table(table);
-  const Decision d = decide<kRestWaves>(a, q, c64, parts);
+  const Decision d = decide<kRestWaves>(a, q, c64, [&](int row) {
+    const RowPart p = reinterpret_cast<const RowPart*>(a.work)[(size_t)row * parts + min(lane, parts - 1)];
+    return lane < parts ? p : RowPart{0.0, -INFINITY, 0x7fffffff, 0, 0};
+  });
   if (cut == 0 && threadIdx.x == 0) decisions_at(a, parts)[req] = d;
   if (d.state != kTarget && d.state != kRest) return;
   const Weights of = weights_of(a, d, c64, d.state == kRest, table);
@@ -371,12 +387,11 @@ __device__ __forceinline__ int2 ends_block(int low, int high) {
   return make_int2(low, high);
 }
 
-// Of places t0 .. t1 - 1 with value(t) each the lowest whose running sum, from `from` on, is above `target`, or the last with
-// a value above 0 if rounding leaves none (-1: there is none at all); `upto`: the sum of the places before it. A thread has
-// `per` places that follow one another. All threads call it.
-constexpr int kDrawWaves = 4;
-template <class F>
-__device__ __forceinline__ int first_above(F value, int t0, int t1, int per, double from, double target, double& upto) {
+// Of places t0 .. t1 - 1 with value(t) each the lowest whose running sum, from `from` on, is above target(their sum), or the last
+// with a value above 0 if rounding leaves none (-1: there is none at all); `upto`: the sum of the places before it. A thread
+// has `per` places that follow one another. All threads call it.
+template <int WAVES, class F, class Target>
+__device__ __forceinline__ int first_above(F value, int t0, int t1, int per, double from, Target target_of, double& upto) {
   __shared__ double found;
   const int a0 = min(t0 + (int)threadIdx.x * per, t1), a1 = min(a0 + per, t1);
   double s = 0.0, all;
@@ -386,7 +401,8 @@ __device__ __forceinline__ int first_above(F value, int t0, int t1, int per, dou
     s += v;
     if (v > 0.0) some = t;
   }
-  double run = from + scan_block64<kDrawWaves>(s, all), before = run;
+  double run = from + scan_block64<WAVES>(s, all), before = run;
+  const double target = target_of(all);
   const int last = some;
   int low = 0x7fffffff;
   if (some >= 0 && !(run + s <= target)) {
@@ -399,7 +415,7 @@ __device__ __forceinline__ int first_above(F value, int t0, int t1, int per, dou
       run += v;
     }
   }
-  const int2 e = ends_block<kDrawWaves>(low, some);
+  const int2 e = ends_block<WAVES>(low, some);
   const int at = e.x < 0x7fffffff ? e.x : e.y;
   if (at >= 0 && (e.x < 0x7fffffff ? low == at : last == at)) {
     if (e.x == 0x7fffffff) {             // (up to the last one)
@@ -414,7 +430,18 @@ __device__ __forceinline__ int first_above(F value, int t0, int t1, int per, dou
   return at;
 }
 
+template <int WAVES>
+__device__ __forceinline__ void write_request(const VerifyArgs& a, const RequestRows& q, const Decision& d, int token) {
+  for (int i = threadIdx.x; i < q.count; i += 64 * WAVES)
+    a.out[q.row0 + i] = i < d.accepted ? a.tokens[q.row0 + i + 1] : i == d.accepted ? token : -1;
+  if (threadIdx.x == 0) {
+    a.accepted[q.req] = d.accepted;
+    a.back[q.req] = q.count - 1 - d.accepted;
+  }
+}
+
 // One workgroup per request: the token, and the request's outputs.
+constexpr int kDrawWaves = 4;
 __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs a, int parts, int blocks) {
   constexpr int kThreads = 64 * kDrawWaves;
   __shared__ double table[kVerTable];
@@ -433,23 +460,53 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs
     Weights of = weights_of(a, d, c64, d.state == kRest, table);
     auto value = [&](int t) { return of(t, of.x[t], of.probs ? of.probs[t] : 0.0f); };
     const int per = (blocks + kThreads - 1) / kThreads;
-    double all, upto, none, mine = 0.0;
-    for (int b = tid * per; b < min(tid * per + per, blocks); ++b) mine += sums[b];
-    scan_block64<kDrawWaves>(mine, all);
-    if (all > 0.0) {
-      const int b = first_above([&](int k) { return sums[k]; }, 0, blocks, per, 0.0, r * all, upto);
-      token = first_above(value, b * kBlock, min((b + 1) * kBlock, a.vocab), kBlock / kThreads, upto, r * all, none);
+    double target = 0.0, upto, none;
+    const int b = first_above<kDrawWaves>([&](int k) { return sums[k]; }, 0, blocks, per, 0.0,
+                                          [&](double all) { return target = r * all; }, upto);
+    if (b >= 0) {
+      token = first_above<kDrawWaves>(value, b * kBlock, min((b + 1) * kBlock, a.vocab), kBlock / kThreads, upto,
+                                      [&](double) { return target; }, none);
     } else {                             // nothing is left of p: from p itself
       of = weights_of(a, d, c64, false, table);
-      token = first_above(value, 0, a.vocab, (a.vocab + kThreads - 1) / kThreads, 0.0, r * d.z, none);
+      token = first_above<kDrawWaves>(value, 0, a.vocab, (a.vocab + kThreads - 1) / kThreads, 0.0,
+                                      [&](double) { return r * d.z; }, none);
     }
   }
-  for (int i = tid; i < q.count; i += kThreads)
-    a.out[q.row0 + i] = i < d.accepted ? a.tokens[q.row0 + i + 1] : i == d.accepted ? token : -1;
-  if (tid == 0) {
-    a.accepted[req] = d.accepted;
-    a.back[req] = q.count - 1 - d.accepted;
+  write_request<kDrawWaves>(a, q, d, token);
+}
+
+// Small vocabularies: all of a request in one workgroup, a wave for each row, then the weights from the row again. One launch
+// instead of three.
+constexpr int kSmallWaves = 8, kSmallVocab = 4096;
+__global__ __launch_bounds__(64 * kSmallWaves) void verify_small_kernel(VerifyArgs a) {
+  constexpr int kThreads = 64 * kSmallWaves, kStep = 64 * kVerBatch;
+  __shared__ double table[kVerTable];
+  const int req = blockIdx.x;
+  const RequestRows q = request_rows(req, a.start[req], a.count[req], 0, a.rows);
+  if (q.count <= 0) {
+    if (threadIdx.x == 0) a.accepted[req] = a.back[req] = 0;
+    return;
   }
+  double c64 = units_of(a, req);
+  fill_table(table);
+  const Decision d = decide<kSmallWaves>(a, q, c64, [&](int row) {
+    return row_part(a.x + (size_t)row * a.ld, a.vocab, 0, (a.vocab + kStep - 1) / kStep, kStep, 0, table, c64, [] { return true; });
+  });
+  int token = d.state == kGreedy ? d.best : -1;
+  if (d.state == kTarget || d.state == kRest) {
+    const double r = (double)a.sample_u[req];
+    Weights of = weights_of(a, d, c64, d.state == kRest, table);
+    auto value = [&](int t) { return of(t, of.x[t], of.probs ? of.probs[t] : 0.0f); };
+    const int per = (a.vocab + kThreads - 1) / kThreads;
+    auto target = [&](double all) { return r * all; };
+    double none;
+    token = first_above<kSmallWaves>(value, 0, a.vocab, per, 0.0, target, none);
+    if (token < 0) {                     // nothing is left of p: from p itself
+      of = weights_of(a, d, c64, false, table);
+      token = first_above<kSmallWaves>(value, 0, a.vocab, per, 0.0, target, none);
+    }
+  }
+  write_request<kSmallWaves>(a, q, d, token);
 }
 
 static int verify_parts(int rows, int vocab) {
@@ -463,6 +520,12 @@ size_t verify_work_bytes(int rows, int requests, int vocab) {
 }
 
 hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
+  // (us of one / three launches: one request of 500 tokens 9.2 / 13.2, of 4000 12.2 / 14.0, of 8000 16.0 / 13.6; 64 of 4000 18.2 /
+  // 19.0, of 8000 29.8 / 20.8)
+  if (a.vocab <= kSmallVocab) {
+    hipLaunchKernelGGL(verify_small_kernel, dim3((unsigned)a.requests), dim3(64 * kSmallWaves), 0, s, a);
+    return hipGetLastError();
+  }
   const int parts = verify_parts(a.rows, a.vocab), blocks = verify_blocks(a.vocab);
   const int cuts = std::max(1, std::min((blocks + kRestWaves - 1) / kRestWaves, kRestMost / a.requests));
   hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(a.rows * parts)), dim3(64 * kVerWaves), 0, s, a, parts);
