@@ -19,13 +19,14 @@ namespace rehip {
 // |f| <= 1/2: from a table of 64 in LDS and the series of 2^(f / 64) - 1 to its third power, off by (ln 2 / 128)^4 / 24 = 3.6e-11
 // at most: a token at the border of 151936 equal ones is then taken for its neighbour once in 200000 times.
 //
-// Small vocabularies: one launch. Else three: maxima and sums of parts of all rows; every request's last row found from them, and the sums of its
-// weights by blocks of the vocabulary; the block where r falls, and the token in it.
+// Small vocabularies: one launch. Else two: maxima and sums of parts of all rows; then every request's last row found from them, and
+// the sums of its weights by blocks of the vocabulary, of which the last workgroup finds the one where r falls, and the token in
+// it.
 //
-// 64 requests of up to 4 drafts, 189 rows of 151936 and the drafts' probabilities, 153 MB: 54 us, 33 + 18 + 7.6 in the three
-// kernels. The rows: 115 MB, 3.5 TB/s; without the exponentials they take 23, with them the vector units' 64-bit rate bounds (5 clocks
-// for each of 15 operations; a table of 32 and one term more: 34.5). One
-// request of 4 drafts 14 us: three launches of latency, 5.6 + 6.6 + 5.6.
+// 64 requests of up to 4 drafts, 189 rows of 151936 and the drafts' probabilities, 153 MB: 52 us, 32 + 22 in the two
+// kernels. The rows: 115 MB, 3.6 TB/s; without the exponentials they take 23, with them the vector units' 64-bit rate bounds (5 clocks
+// for each of 15 operations; a table of 32 and one term more: 34.5). One request of 4 drafts 13 us: two launches of latency,
+// 5.2 + 11. (With the token drawn by a launch of its own 54 and 14.5.)
 constexpr int kVerWaves = 4;
 constexpr int kVerBatch = 16;            // logits of a lane at a time
 constexpr int kVerStep = 64 * kVerBatch * kVerWaves;
@@ -42,7 +43,7 @@ struct Decision {
   double z;
   float m;
   int accepted, row, state;              // the row that the next token comes from; state: below
-  int best, pad;
+  int best;
 };
 constexpr int kNone = 0, kGreedy = 1, kTarget = 2, kRest = 3;  // no distribution; the largest; p; p without the draft
 
@@ -192,6 +193,14 @@ __device__ __forceinline__ RowPart row_part(const float* x, int vocab, int s0, i
   return mine;
 }
 
+// behind the rows' parts: of each request the workgroups that are done with it, then the sums of its blocks
+__device__ __forceinline__ int* done_at(const VerifyArgs& a, int parts) {
+  return reinterpret_cast<int*>(reinterpret_cast<RowPart*>(a.work) + (size_t)a.rows * parts);
+}
+__device__ __forceinline__ double* sums_at(const VerifyArgs& a, int parts) {
+  return reinterpret_cast<double*>(done_at(a, parts) + ((a.requests + 1) & ~1));
+}
+
 // One workgroup per (row, part).
 __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs a, int parts) {
   __shared__ double table[kVerTable];
@@ -207,6 +216,7 @@ __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs 
     counts = q.req >= 0 && r < q.row0 + q.count;
     if (!counts) return false;
     c64 = units_of(a, q.req);
+    if (r == q.row0 && part == 0 && threadIdx.x == 0) done_at(a, parts)[q.req] = 0;
     fill_table(table);
     return true;
   });
@@ -243,7 +253,7 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
                            : (double)u * (double)share * p.z <
                                  (x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)p.m) * (c64 / kVerTable)));
     if (lane == 0)
-      found[w] = {p.z, p.m, accepted ? -1 : i, row, none ? kNone : c64 < 0.0 ? kGreedy : drafted ? kRest : kTarget, p.best, 0};
+      found[w] = {p.z, p.m, accepted ? -1 : i, row, none ? kNone : c64 < 0.0 ? kGreedy : drafted ? kRest : kTarget, p.best};
     __syncthreads();
     bool done = false;
 #pragma unroll
@@ -275,74 +285,6 @@ __device__ __forceinline__ Weights weights_of(const VerifyArgs& a, const Decisio
   const int t = rest && !a.probs ? a.tokens[d.row + 1] : -1;
   return {a.x + (size_t)d.row * a.ld, rest && a.probs ? a.probs + (size_t)d.row * a.ldp : nullptr, c64, (double)d.m,
           1.0 / d.z, t, table};
-}
-
-__device__ __forceinline__ Decision* decisions_at(const VerifyArgs& a, int parts) {
-  return reinterpret_cast<Decision*>(reinterpret_cast<RowPart*>(a.work) + (size_t)a.rows * parts);
-}
-__device__ __forceinline__ double* sums_at(const VerifyArgs& a, int parts) {
-  return reinterpret_cast<double*>(decisions_at(a, parts) + a.requests);
-}
-
-// One workgroup per (request, run of blocks of the vocabulary), a block to a wave at a time: the sums of their weights.
-constexpr int kRestWaves = 8;
-constexpr int kBlock = 1024;             // tokens of a block
-constexpr int kRestMost = 512;           // workgroups, about
-template <bool PROBS>
-__global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs a, int parts, int cuts, int blocks) {
-  __shared__ double table[kVerTable];
-  const int req = blockIdx.x / cuts, cut = blockIdx.x % cuts, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const RequestRows q = request_rows(req, a.start[req], a.count[req], 0, a.rows);
-  if (q.count <= 0) return;
-  const double c64 = units_of(a, req);
-  fill_table(table);
-  const Decision d = decide<kRestWaves>(a, q, c64, [&](int row) {
-    const RowPart p = reinterpret_cast<const RowPart*>(a.work)[(size_t)row * parts + min(lane, parts - 1)];
-    return lane < parts ? p : RowPart{0.0, -INFINITY, 0x7fffffff, 0, 0};
-  });
-  if (cut == 0 && threadIdx.x == 0) decisions_at(a, parts)[req] = d;
-  if (d.state != kTarget && d.state != kRest) return;
-  const Weights of = weights_of(a, d, c64, d.state == kRest, table);
-  const int b0 = (int)((long long)blocks * cut / cuts), b1 = (int)((long long)blocks * (cut + 1) / cuts);
-  auto place = [&](int b, int k) { return b * kBlock + 256 * (k >> 2) + 4 * lane + (k & 3); };
-  const float* probs = of.probs ? of.probs : of.x;                 // (loaded whatever)
-  auto load = [&](int b, float (&x)[16], float (&p)[16]) {
-#pragma unroll
-    for (int k = 0; k < 16; k += 4) {
-      *reinterpret_cast<f32x4u*>(&x[k]) = *reinterpret_cast<const f32x4u*>(of.x + place(b, k));
-      if (PROBS) *reinterpret_cast<f32x4u*>(&p[k]) = *reinterpret_cast<const f32x4u*>(probs + place(b, k));
-    }
-  };
-  auto take = [&](const float (&x)[16], const float (&p)[16], int b) {
-    double s[4] = {};
-#pragma unroll
-    for (int k = 0; k < 16; ++k) s[k & 3] += of(place(b, k), x[k], PROBS ? p[k] : 0.0f);
-    const double all = wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
-    if (lane == 0) sums_at(a, parts)[(size_t)req * blocks + b] = all;
-  };
-  float x[16], p[16], nx[16], np[16];
-  const int whole = min(b1, a.vocab / kBlock);
-  int b = b0 + w;
-  if (b < whole) load(b, x, p);
-  for (; b < whole; b += kRestWaves) {
-    load(b + kRestWaves < whole ? b + kRestWaves : b, nx, np);
-    take(x, p, b);
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      x[k] = nx[k];
-      if (PROBS) p[k] = np[k];
-    }
-  }
-  if (b < b1) {
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int t = min(place(b, k), a.vocab - 1);
-      const float y = of.x[t];
-      x[k] = place(b, k) < a.vocab ? y : -INFINITY;
-      if (PROBS) p[k] = probs[t];
-    }
-    take(x, p, b);
-  }
 }
 
 // Exclusive sums over a workgroup of WAVES waves; the total in `all`.
@@ -440,44 +382,106 @@ __device__ __forceinline__ void write_request(const VerifyArgs& a, const Request
   }
 }
 
-// One workgroup per request: the token, and the request's outputs.
-constexpr int kDrawWaves = 4;
-__global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs a, int parts, int blocks) {
-  constexpr int kThreads = 64 * kDrawWaves;
+// One workgroup per (request, run of blocks of the vocabulary), a block to a wave at a time: the sums of their weights. The last one
+// of a request that is done with them draws the token (whichever it is, the sums are added in the blocks' order).
+constexpr int kRestWaves = 8;
+constexpr int kBlock = 1024;             // tokens of a block
+constexpr int kRestMost = 512;           // workgroups, about
+template <bool PROBS>
+__global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs a, int parts, int cuts, int blocks) {
+  constexpr int kThreads = 64 * kRestWaves;
   __shared__ double table[kVerTable];
-  const int req = blockIdx.x, tid = threadIdx.x;
+  __shared__ int last;
+  const int req = blockIdx.x / cuts, cut = blockIdx.x % cuts, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const RequestRows q = request_rows(req, a.start[req], a.count[req], 0, a.rows);
   if (q.count <= 0) {
-    if (tid == 0) a.accepted[req] = a.back[req] = 0;
+    if (cut == 0 && threadIdx.x == 0) a.accepted[req] = a.back[req] = 0;
     return;
   }
-  const Decision d = decisions_at(a, parts)[req];
-  int token = d.state == kGreedy ? d.best : -1;
-  if (d.state == kTarget || d.state == kRest) {
-    const double c64 = units_of(a, req), r = (double)a.sample_u[req];
-    const double* sums = sums_at(a, parts) + (size_t)req * blocks;
-    fill_table(table);
-    Weights of = weights_of(a, d, c64, d.state == kRest, table);
-    auto value = [&](int t) { return of(t, of.x[t], of.probs ? of.probs[t] : 0.0f); };
-    const int per = (blocks + kThreads - 1) / kThreads;
-    double target = 0.0, upto, none;
-    const int b = first_above<kDrawWaves>([&](int k) { return sums[k]; }, 0, blocks, per, 0.0,
-                                          [&](double all) { return target = r * all; }, upto);
-    if (b >= 0) {
-      token = first_above<kDrawWaves>(value, b * kBlock, min((b + 1) * kBlock, a.vocab), kBlock / kThreads, upto,
-                                      [&](double) { return target; }, none);
-    } else {                             // nothing is left of p: from p itself
-      of = weights_of(a, d, c64, false, table);
-      token = first_above<kDrawWaves>(value, 0, a.vocab, (a.vocab + kThreads - 1) / kThreads, 0.0,
-                                      [&](double) { return r * d.z; }, none);
+  const double c64 = units_of(a, req);
+  fill_table(table);
+  const Decision d = decide<kRestWaves>(a, q, c64, [&](int row) {
+    const RowPart p = reinterpret_cast<const RowPart*>(a.work)[(size_t)row * parts + min(lane, parts - 1)];
+    return lane < parts ? p : RowPart{0.0, -INFINITY, 0x7fffffff, 0, 0};
+  });
+  if (d.state != kTarget && d.state != kRest) {
+    if (cut == 0) write_request<kRestWaves>(a, q, d, d.state == kGreedy ? d.best : -1);
+    return;
+  }
+  Weights of = weights_of(a, d, c64, d.state == kRest, table);
+  double* const sums = sums_at(a, parts) + (size_t)req * blocks;
+  const int b0 = (int)((long long)blocks * cut / cuts), b1 = (int)((long long)blocks * (cut + 1) / cuts);
+  auto place = [&](int b, int k) { return b * kBlock + 256 * (k >> 2) + 4 * lane + (k & 3); };
+  const float* probs = of.probs ? of.probs : of.x;                 // (loaded whatever)
+  auto load = [&](int b, float (&x)[16], float (&p)[16]) {
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) {
+      *reinterpret_cast<f32x4u*>(&x[k]) = *reinterpret_cast<const f32x4u*>(of.x + place(b, k));
+      if (PROBS) *reinterpret_cast<f32x4u*>(&p[k]) = *reinterpret_cast<const f32x4u*>(probs + place(b, k));
+    }
+  };
+  auto take = [&](const float (&x)[16], const float (&p)[16], int b) {
+    double s[4] = {};
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s[k & 3] += of(place(b, k), x[k], PROBS ? p[k] : 0.0f);
+    const double all = wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
+    if (lane == 0) __hip_atomic_store(sums + b, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  float x[16], p[16], nx[16], np[16];
+  const int whole = min(b1, a.vocab / kBlock);
+  int b = b0 + w;
+  if (b < whole) load(b, x, p);
+  for (; b < whole; b += kRestWaves) {
+    load(b + kRestWaves < whole ? b + kRestWaves : b, nx, np);
+    take(x, p, b);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      x[k] = nx[k];
+      if (PROBS) p[k] = np[k];
     }
   }
-  write_request<kDrawWaves>(a, q, d, token);
+  if (b < b1) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int t = min(place(b, k), a.vocab - 1);
+      const float y = of.x[t];
+      x[k] = place(b, k) < a.vocab ? y : -INFINITY;
+      if (PROBS) p[k] = probs[t];
+    }
+    take(x, p, b);
+  }
+  if (cuts > 1) {
+    // The sums go to and come from memory that all workgroups see by atomic stores and loads, and a wave's have arrived before
+    // its workgroup counts itself done. (A fence for all that a wave has written writes the whole L2 back: 104 us instead of
+    // 17 for 64 requests.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+      last = __hip_atomic_fetch_add(done_at(a, parts) + req, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == cuts - 1;
+    __syncthreads();
+    if (!last) return;
+  } else {
+    __syncthreads();
+  }
+  const double r = (double)a.sample_u[req];
+  auto value = [&](int t) { return of(t, of.x[t], of.probs ? of.probs[t] : 0.0f); };
+  double target = 0.0, upto, none;
+  const int found = first_above<kRestWaves>([&](int k) { return __hip_atomic_load(sums + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
+                                            0, blocks, (blocks + kThreads - 1) / kThreads, 0.0, [&](double all) { return target = r * all; }, upto);
+  int token;
+  if (found >= 0) {
+    token = first_above<kRestWaves>(value, found * kBlock, min((found + 1) * kBlock, a.vocab), kBlock / kThreads, upto,
+                                    [&](double) { return target; }, none);
+  } else {                               // nothing is left of p: from p itself
+    of = weights_of(a, d, c64, false, table);
+    token = first_above<kRestWaves>(value, 0, a.vocab, (a.vocab + kThreads - 1) / kThreads, 0.0,
+                                    [&](double) { return r * d.z; }, none);
+  }
+  write_request<kRestWaves>(a, q, d, token);
 }
 
-// Small vocabularies: all of a request in one workgroup, a wave for each row, then the weights from the row again. One launch
-// instead of three.
-constexpr int kSmallWaves = 8, kSmallVocab = 4096;
+// Small vocabularies: all of a request in one workgroup, a wave for each row, then the weights from the row again.
+constexpr int kSmallWaves = 8, kSmallVocab = 2048;
 __global__ __launch_bounds__(64 * kSmallWaves) void verify_small_kernel(VerifyArgs a) {
   constexpr int kThreads = 64 * kSmallWaves, kStep = 64 * kVerBatch;
   __shared__ double table[kVerTable];
@@ -515,13 +519,13 @@ static int verify_parts(int rows, int vocab) {
 static int verify_blocks(int vocab) { return (vocab + kBlock - 1) / kBlock; }
 
 size_t verify_work_bytes(int rows, int requests, int vocab) {
-  return (size_t)rows * verify_parts(rows, vocab) * sizeof(RowPart) + (size_t)requests * sizeof(Decision) +
+  return (size_t)rows * verify_parts(rows, vocab) * sizeof(RowPart) + (size_t)((requests + 1) & ~1) * sizeof(int) +
          (size_t)requests * verify_blocks(vocab) * sizeof(double);
 }
 
 hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
-  // (us of one / three launches: one request of 500 tokens 9.2 / 13.2, of 4000 12.2 / 14.0, of 8000 16.0 / 13.6; 64 of 4000 18.2 /
-  // 19.0, of 8000 29.8 / 20.8)
+  // (us of one / two launches, 4 drafts each: one request of 500 tokens 8.8 / 11.6, of 2000 8.8 / 12.3, of 4000 12.0 / 12.6; 64 of 500
+  // 8.7 / 15.8, of 2000 11.3 / 16.6, of 4000 18.2 / 16.9; 32 of 2000, 16 drafts 16.2 / 18.6)
   if (a.vocab <= kSmallVocab) {
     hipLaunchKernelGGL(verify_small_kernel, dim3((unsigned)a.requests), dim3(64 * kSmallWaves), 0, s, a);
     return hipGetLastError();
@@ -533,9 +537,6 @@ hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(a.probs ? verify_rest_kernel<true> : verify_rest_kernel<false>, dim3((unsigned)(a.requests * cuts)), dim3(64 * kRestWaves), 0, s, a, parts, cuts,
                      blocks);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)a.requests), dim3(64 * kDrawWaves), 0, s, a, parts, blocks);
   return hipGetLastError();
 }
 
