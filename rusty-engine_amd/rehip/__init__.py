@@ -663,48 +663,55 @@ def logprobs_dev(logits, ld, rows, vocab, targets, top_k, logprob, entropy, top_
                                  _p(top_ids), _p(top_logprobs), _p(work), work_bytes, _stream_ptr(stream)))
 
 
+def _call(fn, *args) -> None:
+    """An entry point with addresses as integers, buffers and streams (which pass themselves on), or objects that have a
+    `ptr` or a `handle`."""
+    try:
+        rc = fn(*args)
+    except C.ArgumentError:
+        rc = fn(*(int(a.ptr) if hasattr(a, "ptr") else int(a.handle) if hasattr(a, "handle") else a for a in args))
+    _check(rc)
+
+
 def attention_kv8_sinks_dev(q, ldq, rows, requests, row_start, row_count, kv_len, table, table_ld, page, n_pages, kcodes,
                             vcodes, kscale, vscale, max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window,
                             sinks, ctx, lse=None, work=None, work_bytes=0, stream=None):
     """attention_kv8_dev with `sinks` first tokens that stay visible behind the window, and the log of each row and
     head's sum of exponentials (re_attention_kv8_sinks_dev); the workspace is attention_kv8_work_bytes' too."""
-    _check(lib().re_attention_kv8_sinks_dev(_p(q), ldq, rows, requests, _p(row_start), _p(row_count), _p(kv_len),
-                                            _p(table), table_ld, page, n_pages, _p(kcodes), _p(vcodes), _p(kscale),
-                                            _p(vscale), max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window,
-                                            sinks, _p(ctx), _p(lse), _p(work), work_bytes, _stream_ptr(stream)))
+    _call(lib().re_attention_kv8_sinks_dev, q, ldq, rows, requests, row_start, row_count, kv_len, table, table_ld,
+          page, n_pages, kcodes, vcodes, kscale, vscale, max_rows, max_len, n_heads, n_kv_heads, head_dim, scale,
+          window, sinks, ctx, lse, work, work_bytes, stream)
 
 
 def kv8_mass_dev(q, ldq, lse, rows, requests, row_start, row_count, kv_len, table, table_ld, page, n_pages, kcodes,
                  kscale, max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window, sinks, mass, stream=None):
     """Adds the weight that a step's attention gives each cached token to `mass` (n_pages x n_kv_heads x page f32),
     with attention's lse (re_kv8_mass_dev)."""
-    _check(lib().re_kv8_mass_dev(_p(q), ldq, _p(lse), rows, requests, _p(row_start), _p(row_count), _p(kv_len), _p(table),
-                                 table_ld, page, n_pages, _p(kcodes), _p(kscale), max_rows, max_len, n_heads, n_kv_heads,
-                                 head_dim, scale, window, sinks, _p(mass), _stream_ptr(stream)))
+    _call(lib().re_kv8_mass_dev, q, ldq, lse, rows, requests, row_start, row_count, kv_len, table, table_ld, page,
+          n_pages, kcodes, kscale, max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window, sinks, mass,
+          stream)
 
 
 def kv_evict_plan_dev(requests, page, limit, keep, kv_len, table, table_ld, free, n_pages, n_free, kv_len_out, table_out,
                       free_out, n_free_out, from_len, from_table, dropped, status, stream=None):
     """Requests of more than `limit` tokens are cut to `keep` in fresh pages: lengths, tables and the stack, for all
     layers (re_kv_evict_plan_dev). The outputs may be the inputs; from_table is never table_out; dropped may be None."""
-    _check(lib().re_kv_evict_plan_dev(requests, page, limit, keep, _p(kv_len), _p(table), table_ld, _p(free), n_pages,
-                                      _p(n_free), _p(kv_len_out), _p(table_out), _p(free_out), _p(n_free_out),
-                                      _p(from_len), _p(from_table), _p(dropped), _p(status), _stream_ptr(stream)))
+    _call(lib().re_kv_evict_plan_dev, requests, page, limit, keep, kv_len, table, table_ld, free, n_pages, n_free,
+          kv_len_out, table_out, free_out, n_free_out, from_len, from_table, dropped, status, stream)
 
 
 def kv8_evict_dev(requests, from_len, from_table, table, table_ld, page, n_pages, kcodes, vcodes, kscale, vscale, mass,
                   n_kv_heads, head_dim, keep, first, recent, max_len, kept, stream=None):
     """One layer's tokens that stay move to the new pages: the first, the last and the heaviest ones
     (re_kv8_evict_dev); mass may be None if first + recent = keep."""
-    _check(lib().re_kv8_evict_dev(requests, _p(from_len), _p(from_table), _p(table), table_ld, page, n_pages, _p(kcodes),
-                                  _p(vcodes), _p(kscale), _p(vscale), _p(mass), n_kv_heads, head_dim, keep, first, recent,
-                                  max_len, _p(kept), _stream_ptr(stream)))
+    _call(lib().re_kv8_evict_dev, requests, from_len, from_table, table, table_ld, page, n_pages, kcodes, vcodes,
+          kscale, vscale, mass, n_kv_heads, head_dim, keep, first, recent, max_len, kept, stream)
 
 
 def kv_positions_dev(rows, row_seq, row_pos, requests, dropped, out, stream=None):
     """Rotary positions of a step's rows after evictions: what the plan counts and what the requests have lost
     (re_kv_positions_dev); `out` may be `row_pos`."""
-    _check(lib().re_kv_positions_dev(rows, _p(row_seq), _p(row_pos), requests, _p(dropped), _p(out), _stream_ptr(stream)))
+    _call(lib().re_kv_positions_dev, rows, row_seq, row_pos, requests, dropped, out, stream)
 
 
 def draft_verify_work_bytes(rows, requests, vocab) -> int:
@@ -715,16 +722,15 @@ def draft_verify_dev(logits, ld, rows, vocab, requests, row_start, row_count, to
                      sample_u, accepted, back, out_tokens, work=None, work_bytes=0, stream=None):
     """Drafted tokens against the target's probabilities, from given random numbers: how many are accepted, how many go
     back, and the tokens with the one behind them (re_draft_verify_dev); probs and temperature may be None."""
-    _check(lib().re_draft_verify_dev(_p(logits), ld, rows, vocab, requests, _p(row_start), _p(row_count), _p(tokens),
-                                     _p(probs), ldp, _p(temperature), _p(accept_u), _p(sample_u), _p(accepted), _p(back),
-                                     _p(out_tokens), _p(work), work_bytes, _stream_ptr(stream)))
+    _call(lib().re_draft_verify_dev, logits, ld, rows, vocab, requests, row_start, row_count, tokens, probs, ldp,
+          temperature, accept_u, sample_u, accepted, back, out_tokens, work, work_bytes, stream)
 
 
 def kv_rewind_dev(requests, page, back, kv_len, table, table_ld, free, n_pages, n_free, kv_len_out, n_free_out,
                   stream=None):
     """Takes back[b] tokens off the requests' ends and their pages back to the stack (re_kv_rewind_dev)."""
-    _check(lib().re_kv_rewind_dev(requests, page, _p(back), _p(kv_len), _p(table), table_ld, _p(free), n_pages,
-                                  _p(n_free), _p(kv_len_out), _p(n_free_out), _stream_ptr(stream)))
+    _call(lib().re_kv_rewind_dev, requests, page, back, kv_len, table, table_ld, free, n_pages, n_free, kv_len_out,
+          n_free_out, stream)
 
 
 # ---- int8 activations (src/kernel.rs:70-166) ---------------------------------------------------

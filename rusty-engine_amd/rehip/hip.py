@@ -90,6 +90,11 @@ class DeviceBuffer:
         check(hip().hipMemcpy(out.ctypes.data, C.c_void_p(self.ptr), n * itemsize, D2H))
         return out
 
+    @property
+    def _as_parameter_(self):
+        """What a call of the library gets for this buffer."""
+        return self.ptr
+
     def zero(self) -> None:
         check(hip().hipMemset(C.c_void_p(self.ptr), 0, self.nbytes))
 
@@ -110,6 +115,10 @@ class Stream:
         s = C.c_void_p()
         check(hip().hipStreamCreate(C.byref(s)))
         self.handle = s.value
+
+    @property
+    def _as_parameter_(self):
+        return self.handle
 
     def synchronize(self) -> None:
         check(hip().hipStreamSynchronize(C.c_void_p(self.handle)))

@@ -967,4 +967,4 @@ class _Offset:
     """A device address inside a buffer (for passing a row of a larger buffer)."""
 
     def __init__(self, buf, byte_offset: int):
-        self.ptr = buf.ptr + byte_offset
+        self.ptr = self._as_parameter_ = buf.ptr + byte_offset

@@ -1,5 +1,6 @@
 """The entry points for long conversations and drafted tokens without a GPU: refusals come before any launch; the plain
 restatements that the GPU is held to agree with what they restate."""
+import ctypes
 import math
 
 import numpy as np
@@ -126,6 +127,20 @@ def test_no_rows_is_no_work():
     rehip.kv8_mass_dev(**{**MASS, "rows": 0})
     rehip.draft_verify_dev(**{**VERIFY, "requests": 0, "rows": 0})
     assert rehip.draft_verify_work_bytes(0, 1, 100) == 0 and rehip.draft_verify_work_bytes(1, 0, 100) == 0
+
+
+class View:
+    """What else may stand for an address or a stream."""
+    def __init__(self, **k):
+        self.__dict__.update(k)
+
+
+def test_views_and_streams():
+    change = {k: View(ptr=A) for k in ("kv_len", "table", "free", "n_free", "back", "kv_len_out")}
+    refused(SIZE, rehip.kv_rewind_dev, **{**REWIND, **change, "stream": View(handle=0), "page": 0})
+    refused(SIZE, rehip.kv_rewind_dev, **{**REWIND, "page": 0, "stream": 0})
+    with pytest.raises(ctypes.ArgumentError):
+        rehip.kv_rewind_dev(**{**REWIND, "table": 1.5, "page": 0})
 
 
 # ---- the plain restatements ----------------------------------------------------------------------
