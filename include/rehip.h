@@ -434,7 +434,8 @@ int re_kv8_mass_dev(const float *d_q, size_t ldq, const float *d_lse, size_t row
  * pages are -1); d_from_len: a cut request's old length, 0 for the others; d_from_table (requests x table_ld): a cut
  * request's old entries (may be d_table if d_table_out is another buffer; never d_table_out); d_dropped: NULL, or per
  * request += the tokens it lost, 0 where it holds none (re_kv_positions_dev adds them to its rows' positions);
- * d_status[0] requests over the limit that were left, d_status[1] cut ones. Up to 4096 requests.
+ * d_status[0] requests over the limit that were left, d_status[1] cut ones. d_from_len is neither of the lengths' buffers. Not
+ * for requests that share pages: a cut one gives all of its pages back. Up to 4096 requests.
  *
  * re_kv8_evict_dev, for each layer: of a cut request's tokens the first `first`, the last `recent` and the heaviest of
  * those between them stay, `keep` in all, KV head by KV head (ties to the earlier token; a NaN counts as -inf, a token

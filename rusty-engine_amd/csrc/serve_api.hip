@@ -289,6 +289,8 @@ int re_kv_evict_plan_dev(size_t requests, size_t page, size_t limit, size_t keep
     return report_error(RE_ERR_SIZE, "%zu of %zu tokens to keep (1 .. that, up to 2^30)", keep, limit);
   if (d_table_out == d_from_table)
     return report_error(RE_ERR_ARG, "the old table and the new one must be two buffers");
+  if (d_from_len == d_kv_len || d_from_len == d_kv_len_out)
+    return report_error(RE_ERR_ARG, "the cut requests' old lengths must be a buffer of their own");
   const EvictPlanArgs a{d_kv_len, d_table, d_free, d_n_free, d_kv_len_out, d_table_out, d_free_out, d_n_free_out,
                         d_from_len, d_from_table, d_dropped, d_status, (int)requests, (int)page, (int)table_ld,
                         (int)n_pages, (int)(limit < (1u << 30) ? limit : (1u << 30)), (int)keep};

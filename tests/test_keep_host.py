@@ -73,6 +73,11 @@ def test_evict_plan_refusals(code, change):
     refused(code, rehip.kv_evict_plan_dev, **{**PLAN, **change})
 
 
+@pytest.mark.parametrize("same", ["kv_len", "kv_len_out"])
+def test_evict_plan_keeps_old_lengths_apart(same):
+    refused(ARG, rehip.kv_evict_plan_dev, **{**PLAN, "kv_len": A + 64, "kv_len_out": A + 128, same: A})
+
+
 EVICT = dict(requests=4, from_len=A, from_table=A, table=B, table_ld=8, page=64, n_pages=16, kcodes=A, vcodes=A, kscale=A,
              vscale=A, mass=A, n_kv_heads=2, head_dim=64, keep=100, first=4, recent=50, max_len=300, kept=A)
 
