@@ -573,6 +573,7 @@ class DeviceDecoder:
             self.rope = B(max_seq * hd * 4)
             rope_table_dev(g.rope_freq_base, hd, max_seq, self.rope, self.stream)
         self.graph = None
+        self._drafted = None
         self._seq_len = 0
         self._whole = True                 # no call ended on its way since the last one that came through
 
@@ -806,12 +807,12 @@ class DeviceDecoder:
     def step_drafted(self, drafts, temperature: float = 0.0, probs=None, accept_u=None, sample_u=None) -> list:
         """Decodes the token in `tok` and the drafted ones behind it in one pass; returns the drafts that the model
         accepts and the token that it puts behind them, 1 to len(drafts) + 1 tokens (`draft_verify_dev`). Greedy at
-        temperature 0: the tokens that as many `step` calls would give. Else drafts (drawn from the rows of `probs`, or
+        temperature 0: the tokens that as many `step` calls would give, where products of several rows and of one round
+        alike enough to leave the largest logit the same. Else drafts (drawn from the rows of `probs`, or
         certain without them) are accepted with the random numbers `accept_u`, one each, and the token behind is drawn
         with `sample_u`, all from [0, 1): the tokens are then distributed as the model's own. Rejected drafts are
         taken back as by setting seq_len."""
-        from . import draft_verify_dev, draft_verify_work_bytes, hip, rmsnorm_dev
-        B = hip.DeviceBuffer
+        from . import draft_verify_dev, hip, rmsnorm_dev
         g, s, v, n0 = self.g, self.stream, self.mb.n_vocab, self.seq_len
         drafts = np.asarray(drafts, np.int32).reshape(-1)
         n, rows = drafts.size, drafts.size + 1
@@ -820,35 +821,38 @@ class DeviceDecoder:
         u, r = np.zeros(rows, np.float32), np.float32(sample_u or 0)
         if accept_u is not None:
             u[:n] = np.asarray(accept_u, np.float32).reshape(n)
-        q = None
         if probs is not None:
-            q = B.from_array(np.concatenate([np.asarray(probs, np.float32).reshape(n, v), np.zeros((1, v), np.float32)]))
+            probs = np.asarray(probs, np.float32).reshape(n, v)
         s.synchronize()
         tokens = np.concatenate([self.tok.download(np.int32, 1), drafts])
         self._forward_rows(tokens)                             # (checks the tokens and the room)
+        if self._drafted is None or self._drafted.rows < rows:
+            self._drafted = _DraftedRows(rows, v)
+        b = self._drafted
         rmsnorm_dev(self.x, self.output_norm, rows, g.d_model, g.rms_eps, self.n, s)
-        logits = B(rows * v * 4)
-        self.output.matmul_dev(self.n, rows, logits, self.mode, stream=s)
-        i32 = lambda a: B.from_array(np.asarray(a, np.int32))   # noqa: E731
-        accepted, back, out = i32([0]), i32([0]), i32(np.full(rows, -1))
-        nbytes = draft_verify_work_bytes(rows, 1, v)
-        args = [i32([0]), i32([rows]), i32(tokens), B.from_array(np.array([temperature], np.float32)), B.from_array(u),
-                B.from_array(np.array([r], np.float32)), B(nbytes)]
-        draft_verify_dev(logits, v, rows, v, 1, *args[:3], q, v, *args[3:6], accepted, back, out, args[6], nbytes, s)
+        self.output.matmul_dev(self.n, rows, b.logits, self.mode, stream=s)
+        b.row_count.upload(np.array([rows], np.int32))
+        b.tokens.upload(tokens)
+        b.random.upload(np.concatenate([u, np.array([r, temperature], np.float32)]))
+        q = None
+        if probs is not None and n:
+            q = b.probs = b.probs or hip.DeviceBuffer(b.rows * v * 4)
+            q.upload(probs)                                    # (the last row has no draft)
+        draft_verify_dev(b.logits, v, rows, v, 1, b.row_start, b.row_count, b.tokens, q, v, _Offset(b.random, 4 * (rows + 1)),
+                         b.random, _Offset(b.random, 4 * rows), b.found, _Offset(b.found, 4), b.out, b.work, b.work_bytes, s)
         s.synchronize()
-        k = int(accepted.download(np.int32, 1)[0])
-        got = out.download(np.int32, rows)[:k + 1]
+        k = int(b.found.download(np.int32, 1)[0])
+        got = b.out.download(np.int32, rows)[:k + 1]
         self._done(rows)
         if got[k] < 0:
             self.seq_len = n0
             raise ValueError("step_drafted: the model's logits are not finite")
         self.seq_len = n0 + 1 + k
-        hip.copy_device(self.logits_buf.ptr, logits.ptr + 4 * k * v, 4 * v)
-        self.tok.upload(got[k:])
-        hist = self.hist.download(np.int32, self.max_seq)
-        places = np.arange(n0 + 1, min(n0 + 2 + k, self.max_seq))
-        hist[places] = got[:places.size]
-        self.hist.upload(hist)
+        hip.copy_device(self.logits_buf.ptr, b.logits.ptr + 4 * k * v, 4 * v)
+        hip.copy_device(self.tok.ptr, b.out.ptr + 4 * k, 4)
+        known = min(k + 1, self.max_seq - n0 - 1)
+        if known > 0:
+            hip.copy_device(self.hist.ptr + 4 * (n0 + 1), b.out.ptr, 4 * known)
         return [int(t) for t in got]
 
     def generate_drafted(self, prompt, max_new: int, most: int = 4, ngram: int = 2):
@@ -961,6 +965,21 @@ def lookup_drafts(tokens, most: int, ngram: int = 2) -> list:
         if tokens[at:at + ngram] == last:
             return list(tokens[at + ngram:at + ngram + most])
     return []
+
+
+class _DraftedRows:
+    """The buffers of a step of up to `rows` tokens, the drafted ones and the one before them."""
+
+    def __init__(self, rows: int, vocab: int):
+        from . import draft_verify_work_bytes
+        from .hip import DeviceBuffer as B
+        self.rows = rows
+        self.logits, self.probs = B(rows * vocab * 4), None
+        self.row_start, self.row_count = B.from_array(np.zeros(1, np.int32)), B(4)
+        self.tokens, self.out, self.found = B(rows * 4), B(rows * 4), B(8)
+        self.random = B((rows + 2) * 4)                        # a number for each row, the drawn token's, the temperature
+        self.work_bytes = max(draft_verify_work_bytes(n, 1, vocab) for n in range(1, rows + 1))
+        self.work = B(self.work_bytes)
 
 
 class _Offset:

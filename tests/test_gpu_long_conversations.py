@@ -401,6 +401,25 @@ def test_drafted_steps(tiny, kv_cache):
     plain.close()
 
 
+def test_drafted_steps_of_growing_length(tiny):
+    """The buffers of a step grow with its drafts and serve shorter ones afterwards; a sequence that is full ends them."""
+    prompt = np.random.default_rng(4).integers(0, 1000, 20)
+    plain = qwen.DeviceDecoder(tiny, max_seq=50, prefill_rows=32, kv_cache="int8")
+    want = [plain.prefill(prompt)] + [plain.step() for _ in range(30)]
+    plain.close()
+    dd = qwen.DeviceDecoder(tiny, max_seq=50, prefill_rows=32, kv_cache="int8")
+    assert dd.prefill(prompt) == want[0]
+    at = 0
+    for n in (1, 6, 2, 0, 9):
+        assert dd.step_drafted(want[at + 1:at + 1 + n]) == want[at + 1:at + 2 + n]
+        at += n + 1
+    with pytest.raises(ValueError):
+        dd.step_drafted(want[:7])                               # (seven drafts and the token before them: one place too few)
+    assert dd.step_drafted(want[at + 1:at + 7]) == want[at + 1:at + 8] and dd.seq_len == 50
+    assert dd.history(20, 30) == want[:30]                       # (the token behind the last place is in no history)
+    dd.close()
+
+
 def test_lookup_drafts():
     assert qwen.lookup_drafts([1, 2, 3, 4, 1, 2], 4) == [3, 4, 1, 2]
     assert qwen.lookup_drafts([1, 2, 3, 1, 2, 5, 1, 2], 1) == [5]
