@@ -280,8 +280,8 @@ __device__ __forceinline__ int piece_key(const MassPlace& o, int ch, int keys) {
 
 // W = 1: a wave for each piece. Else a workgroup for each, whose W waves take every W-th tile.
 // Steps of a piece: as many as leave a SIMD two waves (us of 1 / 2 for a wave alone: 64 requests of up to 8192 tokens, 4 heads of
-// 128 20.9 / 16.8; of 2 / 4 for prompts of 8 heads of 64 62 / 52).
-constexpr int mass_steps(int nb, int w) { return w > 1 && nb <= 2 ? 4 : nb <= 4 ? 2 : 1; }
+// 128 20.9 / 16.8; of 2 / 4 for prompts of 8 heads of 64 62 / 48).
+constexpr int mass_steps(int nb, int w) { return w >= 4 && nb <= 2 ? 4 : nb <= 4 ? 2 : 1; }
 template <int NB, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 2) void kv8_mass_kernel(PagedBatch b, Kv8Cache c, MassArgs a, MassCut t) {
   constexpr int KS = mass_steps(NB, W), kKeys = 32 * KS, kLeft = MassKeys<NB, KS>::kLeft;
@@ -350,19 +350,35 @@ static MassCut mass_cut(const PagedBatch& b, const MassArgs& a, int keys) {
 }
 
 template <int NB, int W>
-static void launch_mass_as(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
-  const MassCut t = mass_cut(b, a, 32 * mass_steps(NB, W));
-  const long pieces = (long)b.requests * c.kv_heads * t.chunks;
-  const long groups = std::min(W == 1 ? (pieces + 3) / 4 : pieces, W == 4 ? 1024L : 512L);
-  hipLaunchKernelGGL((kv8_mass_kernel<NB, W>), dim3((unsigned)groups), dim3(W == 1 ? 256 : 64 * W), 0, s, b, c, a, t);
+static long mass_count(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a) {
+  return (long)b.requests * c.kv_heads * mass_cut(b, a, 32 * mass_steps(NB, W)).chunks;
 }
+template <int NB, int W>
+static void launch_mass_as(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
+  const long pieces = mass_count<NB, W>(b, c, a);
+  const long groups = W == 1 ? std::min((pieces + 3) / 4, 512L) : std::min(pieces, 4096L / W);
+  hipLaunchKernelGGL((kv8_mass_kernel<NB, W>), dim3((unsigned)groups), dim3(W == 1 ? 256 : 64 * W), 0, s, b, c, a,
+                     mass_cut(b, a, 32 * mass_steps(NB, W)));
+}
+// Waves of a piece, us of each:
+//   one up to four tiles of vectors (1 / 2 / 4: 64 vectors of one request of 1000 tokens, 2 heads of 64 7.5 / 8.7 / 8.5, of 64 of up to 2000,
+//     8 of 64 13.6 / 15.8 / 20.2; but 128 of one of 1000 10.4 / 8.7 / 8.5), of heads beyond 128 up to one tile unless their pieces are many
+//     (1 / 2: 64 vectors of one of 1000, 4 of 256 14.2 / 7.7, of 16 of up to 500 13.4 / 9.4; of one of 8000 14.3 / 15.8);
+//   two for a few more vectors of so many pieces that they fill the card by themselves (2 / 4: 128 vectors of 64 requests of up to
+//     2000, 8 of 64 21.4 / 26.8, of 128 31.1 / 38.5, 256 vectors 49.4 / 57.4, 4 of 256 79 / 94; but 512, 8 of 64 72 / 66, and 256, 2 of
+//     64 15.9 / 14.4);
+//   eight for long prompts of few pieces (4 / 8: 2048 vectors of two requests of up to 5000, a window of 1000, 8 of 64 50 / 39, 4000, 8 of
+//     128 82 / 64, 2048 of one of 8000, 2 of 64 36.6 / 30.3, but 8 of 64 53 / 59);
+//   else four.
 template <int NB>
 static void launch_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
-  // eight waves for the heads whose pieces are shorter (us of 4 / 8: prompts of 8 heads of 64 47 / 52, of 128 with a window of 1000
-  // 82 / 64)
-  constexpr int W = NB <= 2 ? 4 : 8;
-  if ((long)a.max_rows * (a.heads / c.kv_heads) > 64) launch_mass_as<NB, W>(b, c, a, s);
-  else launch_mass_as<NB, 1>(b, c, a, s);
+  const long vectors = (long)a.max_rows * (a.heads / c.kv_heads);
+  const bool alone = NB <= 4 || vectors <= 16 || mass_count<NB, 1>(b, c, a) > 1024;
+  if (vectors <= 64 && alone) launch_mass_as<NB, 1>(b, c, a, s);
+  else if (vectors <= 64) launch_mass_as<NB, 2>(b, c, a, s);
+  else if (vectors <= 256 && mass_count<NB, 2>(b, c, a) > 4096) launch_mass_as<NB, 2>(b, c, a, s);
+  else if (vectors >= 1024 && mass_count<NB, 8>(b, c, a) <= (NB <= 2 ? 448 : 576)) launch_mass_as<NB, 8>(b, c, a, s);
+  else launch_mass_as<NB, 4>(b, c, a, s);
 }
 
 hipError_t launch_kv8_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
@@ -385,6 +401,11 @@ hipError_t launch_kv8_mass(const PagedBatch& b, const Kv8Cache& c, const MassArg
 // below that). The M-th largest key is found by its digits, 11, 11 and 10 bits from the top: a histogram of those whose
 // higher digits are the ones found so far, and a scan of it from the top. Then a token stays if its key is larger, or equal
 // and among the first of those.
+//
+// 32 requests of 8 heads and up to 8192 tokens, 8 MB of masses: 13.7 us (2101 tokens, two heads: 10.2), not bandwidth but a chain:
+// lengths, table, masses (held in registers after that), then for each digit zeros, counts in LDS, a scan, four barriers, and a last
+// scan for the places. A search that ends with the first digit whose bin stays whole; scans by every wave for itself with one
+// barrier for each digit took 14.4 (10.9).
 constexpr int kPickMost = 16;            // tokens of a thread at a time
 constexpr int kPickBins = 2048;
 
@@ -507,6 +528,11 @@ __global__ __launch_bounds__(THREADS) void kv8_evict_pick_kernel(EvictArgs a, in
 // One workgroup for each new page and head, K or V. A lane makes 16 bytes of a block of 32 tokens x 32 dimensions: K's are
 // two tokens' 8 dimensions, two loads of 8 bytes; V's are 8 tokens' 2 dimensions, and of each of them the 16 old bytes
 // that hold them with 7 neighbours are loaded. Where a lane's tokens lie is found once for all blocks of dimensions.
+//
+// 28 requests cut to 2048 tokens, 8 heads of 128: 96 us. 236 MB are read and written, but a token's codes lie in 8 and 16 byte
+// pieces among its neighbours': with every fourth token kept or more nearly every line of the old pages is fetched, 417 MB,
+// 4.3 TB/s. Blocks taken whole to LDS and scattered from there, each line fetched once for sure: 167 us (the scatter writes
+// single bytes).
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 // the code in byte i of x, rounded to another scale: q + 1.5 2^23 rounds q to an integer, whose low byte is the code (q is a
@@ -630,7 +656,8 @@ __global__ __launch_bounds__(256) void kv8_evict_move_kernel(EvictArgs a, Kv8Cac
 
 hipError_t launch_kv8_evict(const EvictArgs& a, const Kv8Cache& c, hipStream_t s) {
   const dim3 picks((unsigned)(a.requests * c.kv_heads));
-  // the fewest waves that hold a request's tokens at once: their barriers are shorter
+  // the fewest waves that hold a request's tokens at once: their barriers are shorter (us of the kernel with 1024 threads / these: one
+  // request of 2101 tokens 14.8 / 10.4, 32 of up to 8192 17.2 / 13.6)
   if (a.max_len <= 256 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<256>, picks, dim3(256), 0, s, a, c.kv_heads);
   else if (a.max_len <= 512 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<512>, picks, dim3(512), 0, s, a, c.kv_heads);
   else hipLaunchKernelGGL(kv8_evict_pick_kernel<1024>, picks, dim3(1024), 0, s, a, c.kv_heads);

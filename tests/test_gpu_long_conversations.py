@@ -302,6 +302,21 @@ def test_masses_of_prompts_of_many_requests():
     check_mass(cache, bt, q, 0.2, 0, 0)
 
 
+@pytest.mark.parametrize("hd,kv_heads,page", [(32, 4, 32), (64, 2, 64), (96, 2, 32), (128, 3, 96), (160, 1, 32), (256, 2, 64)])
+@pytest.mark.parametrize("requests,window,sinks", [(2, 0, 0), (2, 37, 5), (60, 0, 0), (60, 37, 5), (130, 20, 2)])
+def test_masses_by_shares_of_waves(hd, kv_heads, page, requests, window, sinks):
+    """Steps whose pieces are shared by two waves (many requests of a few rows), four and eight (long prompts of few)."""
+    rng = np.random.default_rng(hd + requests)
+    few, grp = requests == 2, 8
+    rows = [150, 97] if few else rng.integers(0, 14, requests)
+    len_of = np.array([400, 97]) if few else np.minimum(rng.integers(0, 120, requests) + rows, 120)
+    bt, cache, q = make(rng, rows, len_of, page, grp * kv_heads, kv_heads, hd)
+    most = int(np.max(rows))
+    assert (grp * most >= 1024) if few else 64 < grp * most <= 256
+    for max_len in (400, 8000):                                    # (four waves at the second)
+        check_mass(cache, bt, q, hd ** -0.5, window, sinks, max_rows=most, max_len=max_len if few else 40 * max_len // 2)
+
+
 def test_starts_that_do_not_ascend_stay_in_bounds():
     """Rubbish in the batch arrays: nothing is read or written out of place (what comes out is not looked at)."""
     rng = np.random.default_rng(3)
