@@ -366,7 +366,10 @@ hipError_t launch_kv8_append(const PagedBatch& b, const Kv8Cache& c, const float
 // requests of 1 .. 16384 tokens (4 heads of 128, 135 MB) 34.4 us, 30 of them here: HBM behind the first three trips to
 // memory; one row of 14 heads, 211 tokens 9.6 us, 6.7 in the kernel: those trips. Prompts of 1000 rows behind up to 5000
 // tokens (four, 32 heads of 128) 189 .. 194 us, 465 .. 475 TFLOP/s of products and as many again of low parts: 0.9 of the rate of a large
-// f16 matrix product (1.06 PFLOP/s) on the matrix cores.
+// f16 matrix product (1.06 PFLOP/s) on the matrix cores. With a window and sinks: 64 requests of up to 65536 tokens, a window of
+// 4096 (32 heads in 4 of 128, 82 MB) 25.1 us, 22 + 4.5 in the two launches; up to five rows of 32 requests, 2048 (8 heads of
+// 128, 58 MB) 29.4, 25 + 6; 3400 rows behind up to 12000 tokens, 2048 (32 heads in 4 of 128) 295 .. 301 us, 420 TFLOP/s and as many of
+// low parts: as without sinks (290): the last of equally long tiles, 3.3 for each place on the card, leave some idle.
 constexpr float kTermBits = 10.0f, kSlack = 5.0f;     // 2^(10 + 5) stays below f16's 65504
 
 // How a launch cuts the batch: a tile holds up to vecs query vectors of one request and KV head, rows_per rows of its
