@@ -16,18 +16,18 @@ namespace rehip {
 // f16, q in two f16 parts, f32 sums. A key belongs to one wave or workgroup, so its sum is taken in one order.
 //
 // A piece is 32 KS keys of one request and head, held as f16 operands in registers; tiles of 16 query vectors that see some of
-// them go past, each split by the wave that multiplies it (the matrix operand's lanes are those that load it), the next one
-// on its way meanwhile. Sums over a tile's vectors stay in the lanes until the end, and are then taken by halves, so that
-// every lane ends with a key or two of its own. Steps of few vectors: a wave takes a piece alone (W = 1). Prompts: a
-// workgroup's W waves share a piece and take every W-th tile. The launch has about as many workgroups as run at once, and each
-// takes every so-manieth piece of the whole batch, found from the lengths: with a piece for each of the longest request's, most
-// workgroups of a ragged batch would find nothing (64 requests of up to 8192 tokens 32 us instead of 17).
+// them go past, each split by the wave that multiplies it, the next one on its way meanwhile. Sums over a tile's vectors stay in
+// the lanes until the end, and are then taken by halves, so that every lane ends with a key or two of its own. Steps of few vectors:
+// a wave takes a piece alone (W = 1). Prompts: a workgroup's W waves share a piece and take every W-th tile. The launch has about
+// as many workgroups as run at once, and each takes every so-manieth piece of the whole batch, found from the lengths: with a piece
+// for each of the longest request's, most workgroups of a ragged batch would find nothing (64 requests of up to 8192 tokens 32 us
+// instead of 17).
 //
-// 64 requests of up to 8192 tokens, 32 heads in 4 of 128, 36 MB: 16.8 us, 2.1 TB/s: two pieces a wave, one after the other, four
+// 64 requests of up to 8192 tokens, 32 heads in 4 of 128, 36 MB: 14.6 us, 2.4 TB/s: two pieces a wave, one after the other, four
 // trips to memory each. Two prompts of up to 1000 rows behind up to 5000 tokens, 16 heads in 8 of 64, 9.7 GFLOP and as many of low
 // parts: 47 us: exponentials, the split of q (each vector for every 128 keys) and few pieces of unequal length (the first keys
-// are seen by every row), two waves on a SIMD half of the time waiting. Passing split tiles on in LDS between waves of
-// different keys did not pay (57; 32 heads in 4 of 128 268 us instead of 117: then a quarter of the pieces).
+// are seen by every row), two waves on a SIMD half of the time waiting. One prompt of 961 rows, 32 heads in 4 of 128: 71 us, the
+// workgroups of the first keys, which every row sees, with the split of q for each 32.
 struct MassCut {
   int chunks;                            // pieces of a request and head, of the longest planned
   int mode;                              // how a piece is found: below
@@ -112,41 +112,51 @@ __device__ __forceinline__ void mass_pieces(const PagedBatch& b, const MassArgs&
   }
 }
 
-// A vector as its lanes load it: vector `lane % 16` of a tile, dimensions 32 k + 8 (lane / 16) ..
-template <int NB>
+// A tile of 16 vectors. The matrix operand's lane m + 16 g has vector m, dimensions 32 k + 8 g .. . Loaded by those lanes (DIRECT) every
+// lane of an instruction meets a line of its own, and the CU's load unit, a line a clock, bounds pieces of few keys whatever the
+// waves: so four lanes next to one another load 128 bytes of one vector (lane l: vector l / 4, dimensions 32 k + 8 (l % 4) ..) and split
+// them, and what a lane then holds, 16 bytes of each part, is what one lane of the operand needs: they change places in the
+// wave's own LDS (us of direct / this: a step of 64 requests, 4 heads of 128 16.0 / 14.8, 4000 vectors of two requests of up to 5000, 4 of
+// 256 291 / 182; but pieces of 128 keys of 64, 16 heads in 8, 46.5 / 51.6).
+constexpr int kMassSlots = 68;           // 64 lanes' 16 bytes and a slot behind every 16, so that both orders meet all banks
+__device__ __forceinline__ int mass_slot(int i) { return i + (i >> 4); }
+template <int NB, bool DIRECT>
 struct MassVector {
   float x[NB][8], lse;
-  int row;
+  int row;                               // of the operand's vector
   __device__ __forceinline__ void load(const MassArgs& a, const MassPlace& o, int row0, int grp, int head, int tile) {
-    const int vec = 16 * tile + (threadIdx.x & 15);
+    const int lane = threadIdx.x & 63, vec = 16 * tile + (lane & 15), from = DIRECT ? vec : 16 * tile + (lane >> 2);
+    const int at = from / grp, part = DIRECT ? lane >> 4 : lane & 3;
     row = vec / grp;
-    const int r = row0 + min(row, o.n - 1), hq = head * grp + vec - row * grp;
-    const float* p = a.q + (size_t)r * a.ldq + (size_t)hq * (32 * NB) + 8 * ((threadIdx.x & 63) >> 4);
-    lse = a.lse[(size_t)r * a.heads + hq];
+    const float* p = a.q + (size_t)(row0 + min(at, o.n - 1)) * a.ldq + (size_t)(head * grp + from - at * grp) * (32 * NB) + 8 * part;
+    lse = a.lse[(size_t)(row0 + min(row, o.n - 1)) * a.heads + head * grp + vec - row * grp];
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
       *reinterpret_cast<float4*>(&x[k][0]) = *reinterpret_cast<const float4*>(p + 32 * k);
       *reinterpret_cast<float4*>(&x[k][4]) = *reinterpret_cast<const float4*>(p + 32 * k + 4);
     }
   }
-  // its two f16 parts, scaled by the power of two that takes the largest element to 2^13 .. 2^14; the factor of its products and
-  // its lse, in powers of 2. A row that is not there, sees nothing or is not finite gives no weight: q = 0, lse = inf
-  __device__ __forceinline__ float2 split(const MassArgs& a, const MassPlace& o, float minus_one, h8 (&hi)[NB], h8 (&lo)[NB]) {
+  // the operand's two f16 parts, scaled by the power of two that takes the largest element to 2^13 .. 2^14; the factor of its
+  // products and its lse, in powers of 2. A row that is not there, sees nothing or is not finite gives no weight: lse = inf, and q = 0
+  // if it is not finite. `swap`: the wave's LDS
+  __device__ __forceinline__ float2 split(const MassArgs& a, const MassPlace& o, float minus_one, h8* swap, h8 (&hi)[NB], h8 (&lo)[NB]) {
+    const int lane = threadIdx.x & 63;
     unsigned top = 0;
 #pragma unroll
     for (int k = 0; k < NB; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
-    top = max(top, lane_xor_u32<16>(top));
-    top = max(top, lane_xor_u32<32>(top));
-    const int e = (int)(top >> 23), f = min(267 - e, 253);
-    const bool ok = e != 255 && row < o.n && fabsf(lse) < INFINITY;
+    top = max(top, lane_xor_u32<DIRECT ? 16 : 1>(top));
+    top = max(top, lane_xor_u32<DIRECT ? 32 : 2>(top));
+    const int e = (int)(top >> 23);
+    int f = min(267 - e, 253);
     const float up = copysignf(__uint_as_float((unsigned)f << 23), a.scale);
-    if (__ballot(!ok) != 0) {
+    if (e == 255) f = -1;
+    if (__ballot(f < 0) != 0) {
 #pragma unroll
       for (int k = 0; k < NB; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[k][j] = ok ? x[k][j] : 0.0f;
+        for (int j = 0; j < 8; ++j) x[k][j] = f < 0 ? 0.0f : x[k][j];
     }
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
@@ -154,6 +164,23 @@ struct MassVector {
       for (int j = 0; j < 8; ++j) x[k][j] *= up;
       split8(x[k], minus_one, hi[k], lo[k]);
     }
+    if constexpr (!DIRECT) {
+      const int to = mass_slot(lane), from = mass_slot(4 * (lane & 15) + (lane >> 4));
+      wave_sync();                       // (the tile before has been read)
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        swap[2 * k * kMassSlots + to] = hi[k];
+        swap[(2 * k + 1) * kMassSlots + to] = lo[k];
+      }
+      f = __shfl(f, 4 * (lane & 15), 64);
+      wave_sync();
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        hi[k] = swap[2 * k * kMassSlots + from];
+        lo[k] = swap[(2 * k + 1) * kMassSlots + from];
+      }
+    }
+    const bool ok = f >= 0 && row < o.n && fabsf(lse) < INFINITY;
     return ok ? make_float2(__uint_as_float((unsigned)(254 - f) << 23) * (fabsf(a.scale) * 1.4426950408889634f),
                             lse * 1.4426950408889634f)
               : make_float2(0.0f, INFINITY);
@@ -281,12 +308,14 @@ __device__ __forceinline__ int piece_key(const MassPlace& o, int ch, int keys) {
 // W = 1: a wave for each piece. Else a workgroup for each, whose W waves take every W-th tile.
 // Steps of a piece: as many as leave a SIMD two waves (us of 1 / 2 for a wave alone: 64 requests of up to 8192 tokens, 4 heads of
 // 128 20.9 / 16.8; of 2 / 4 for prompts of 8 heads of 64 62 / 48).
-constexpr int mass_steps(int nb, int w) { return w >= 4 && nb <= 2 ? 4 : nb <= 4 ? 2 : 1; }
+constexpr int mass_steps(int nb, int w) { return w == 4 && nb <= 2 ? 4 : nb <= 4 && w < 16 ? 2 : 1; }
 template <int NB, int W>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 2) void kv8_mass_kernel(PagedBatch b, Kv8Cache c, MassArgs a, MassCut t) {
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, W < 16 ? 2 : 4) void kv8_mass_kernel(PagedBatch b, Kv8Cache c, MassArgs a, MassCut t) {
   constexpr int KS = mass_steps(NB, W), kKeys = 32 * KS, kLeft = MassKeys<NB, KS>::kLeft;
+  constexpr bool kDirect = KS == 4;
   __shared__ float red[W > 1 ? W - 1 : 1][kLeft][64];
   __shared__ int at[kMassList];
+  __shared__ h8 swap[kDirect ? 1 : W == 1 ? 4 : W][2 * NB * kMassSlots];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = a.heads / c.kv_heads;
   float minus_one = -1.0f;
   asm volatile("" : "+v"(minus_one));
@@ -297,7 +326,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 2) void kv8_mass_kernel(Page
     keys.load(b, c, a, o, req, head, k0);
     const int2 tiles = mass_tiles(a, o, grp, k0, kKeys);
     int tile = tiles.x + (W == 1 ? 0 : w);
-    MassVector<NB> q;
+    MassVector<NB, kDirect> q;
     if (tile < tiles.y) q.load(a, o, row0, grp, head, tile);
     h8 kf[KS][NB][2];
 #pragma unroll
@@ -309,7 +338,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, 2) void kv8_mass_kernel(Page
       }
     for (; tile < tiles.y; tile += W) {
       h8 hi[NB], lo[NB];
-      const float2 v = q.split(a, o, minus_one, hi, lo);
+      const float2 v = q.split(a, o, minus_one, swap[kDirect ? 0 : w], hi, lo);
       const int pos = o.p0 + q.row;
       q.load(a, o, row0, grp, head, tile + W < tiles.y ? tile + W : tile);          // (on its way meanwhile)
       f32x4 st[KS][2] = {};
@@ -360,24 +389,34 @@ static void launch_mass_as(const PagedBatch& b, const Kv8Cache& c, const MassArg
   hipLaunchKernelGGL((kv8_mass_kernel<NB, W>), dim3((unsigned)groups), dim3(W == 1 ? 256 : 64 * W), 0, s, b, c, a,
                      mass_cut(b, a, 32 * mass_steps(NB, W)));
 }
+// Eight and sixteen waves of a piece have a CU each, so they pay if the launch's work is no more than a round of 256: the pieces of
+// all keys by how much of the rows they see on average (the first keys are seen by every row, the last by one), of several requests
+// of which about half are that long.
+template <int NB, int W>
+static bool one_round(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a) {
+  const long keys = 32 * mass_steps(NB, W), rows = std::min(a.max_rows, a.max_len);
+  long span = a.max_len - rows / 2;
+  if (a.window > 0) span = std::min(span, (long)std::max(a.max_rows, a.window) + a.sinks);
+  return (span + keys - 1) / keys * c.kv_heads * ((b.requests + 1) / 2) <= 256;
+}
 // Waves of a piece, us of each:
 //   one up to four tiles of vectors (1 / 2 / 4: 64 vectors of one request of 1000 tokens, 2 heads of 64 7.5 / 8.7 / 8.5, of 64 of up to 2000,
-//     8 of 64 13.6 / 15.8 / 20.2; but 128 of one of 1000 10.4 / 8.7 / 8.5), of heads beyond 128 up to one tile unless their pieces are many
-//     (1 / 2: 64 vectors of one of 1000, 4 of 256 14.2 / 7.7, of 16 of up to 500 13.4 / 9.4; of one of 8000 14.3 / 15.8);
+//     8 of 64 13.6 / 15.8 / 20.2; but 128 of one of 1000 10.4 / 8.7 / 8.5), of heads beyond 128 up to one tile unless their pieces are many;
 //   two for a few more vectors of so many pieces that they fill the card by themselves (2 / 4: 128 vectors of 64 requests of up to
-//     2000, 8 of 64 21.4 / 26.8, of 128 31.1 / 38.5, 256 vectors 49.4 / 57.4, 4 of 256 79 / 94; but 512, 8 of 64 72 / 66, and 256, 2 of
-//     64 15.9 / 14.4);
-//   eight for long prompts of few pieces (4 / 8: 2048 vectors of two requests of up to 5000, a window of 1000, 8 of 64 50 / 39, 4000, 8 of
-//     128 82 / 64, 2048 of one of 8000, 2 of 64 36.6 / 30.3, but 8 of 64 53 / 59);
-//   else four.
+//     2000, 8 of 64 21.4 / 26.8, of 128 31.1 / 38.5, 256 vectors 49.4 / 57.4; but 512, 8 of 64 72 / 66, and 256, 2 of 64 15.9 / 14.4);
+//   sixteen of 32 keys for prompts of so few that all have a CU (4 / 8 / 16: 1000 tokens, 4000 vectors, 2 of 64 62 / 38 / 28, 4 of 128
+//     75 / 55 / 41; but three of 475, 8 of 128 32 / 31 / 35);
+//   eight of 64 (32 of heads beyond 128) if one round does (4 / 8: 2048 vectors of two requests of up to 5000, a window of 1000, 8
+//     of 64 52 / 30, of 128 49 / 36; 500 rows of one of 2500, 8 of 128 53 / 57, 1000 78 / 68);
+//   else four, of 128 keys of heads up to 64.
 template <int NB>
 static void launch_mass(const PagedBatch& b, const Kv8Cache& c, const MassArgs& a, hipStream_t s) {
   const long vectors = (long)a.max_rows * (a.heads / c.kv_heads);
   const bool alone = NB <= 4 || vectors <= 16 || mass_count<NB, 1>(b, c, a) > 1024;
   if (vectors <= 64 && alone) launch_mass_as<NB, 1>(b, c, a, s);
-  else if (vectors <= 64) launch_mass_as<NB, 2>(b, c, a, s);
-  else if (vectors <= 256 && mass_count<NB, 2>(b, c, a) > 4096) launch_mass_as<NB, 2>(b, c, a, s);
-  else if (vectors >= 1024 && mass_count<NB, 8>(b, c, a) <= (NB <= 2 ? 448 : 576)) launch_mass_as<NB, 8>(b, c, a, s);
+  else if (vectors <= 64 || (vectors <= 256 && mass_count<NB, 2>(b, c, a) > 4096)) launch_mass_as<NB, 2>(b, c, a, s);
+  else if (NB <= 4 && vectors > 128 && mass_count<NB, 16>(b, c, a) <= 256) launch_mass_as<NB, NB <= 4 ? 16 : 8>(b, c, a, s);
+  else if (vectors > 128 && one_round<NB, 8>(b, c, a)) launch_mass_as<NB, 8>(b, c, a, s);
   else launch_mass_as<NB, 4>(b, c, a, s);
 }
 
