@@ -568,7 +568,7 @@ __global__ __launch_bounds__(THREADS) void kv8_evict_pick_kernel(EvictArgs a, in
 // two tokens' 8 dimensions, two loads of 8 bytes; V's are 8 tokens' 2 dimensions, and of each of them the 16 old bytes
 // that hold them with 7 neighbours are loaded. Where a lane's tokens lie is found once for all blocks of dimensions.
 //
-// 28 requests cut to 2048 tokens, 8 heads of 128: 96 us. 236 MB are read and written, but a token's codes lie in 8 and 16 byte
+// 27 requests cut to 2048 tokens, 8 heads of 128: 96 us. 236 MB are read and written, but a token's codes lie in 8 and 16 byte
 // pieces among its neighbours': with every fourth token kept or more nearly every line of the old pages is fetched, 417 MB,
 // 4.3 TB/s. Blocks taken whole to LDS and scattered from there, each line fetched once for sure: 167 us (the scatter writes
 // single bytes).
