@@ -465,10 +465,9 @@ __global__ __launch_bounds__(THREADS) void kv8_evict_pick_kernel(EvictArgs a, in
   if (T <= a.keep || T > a.table_ld * a.page) return;
   int* const kept = a.kept + (size_t)blockIdx.x * a.keep;
   const int* const table = a.from_table + (size_t)req * a.table_ld;
-  const int M = a.keep - a.first - a.recent, end = T - a.recent;   // M of the tokens first .. end - 1
+  const int M = a.keep - a.first - a.recent, end = T - a.recent;   // M > 0 of the tokens first .. end - 1
   for (int i = tid; i < a.first; i += THREADS) kept[i] = i;
   for (int i = tid; i < a.recent; i += THREADS) kept[a.keep - a.recent + i] = end + i;
-  if (M == 0) return;
   const int per = min(kPickMost, ((end + THREADS - 1) / THREADS + 3) & ~3), block = THREADS * per;
   // tokens at .. at + per - 1 (those behind the middle: some of its own)
   auto load = [&](int at, unsigned (&key)[kPickMost]) {
@@ -565,6 +564,10 @@ __global__ __launch_bounds__(THREADS) void kv8_evict_pick_kernel(EvictArgs a, in
 // from, so that no code grows, a code round(c * (s_old / s_new)), ties to even. Places behind the last token get code 0 and
 // mass 0.
 //
+// Where the first and the last tokens are all that stay, which they are is plain: no launch has picked any, and K's workgroups
+// write them down (one request of 2101 tokens 12.4 us of both calls, 15.4 with a launch that picks nothing; another kernel, since the
+// picked tokens' moves lose 5 % by the condition).
+//
 // One workgroup for each new page and head, K or V. A lane makes 16 bytes of a block of 32 tokens x 32 dimensions: K's are
 // two tokens' 8 dimensions, two loads of 8 bytes; V's are 8 tokens' 2 dimensions, and of each of them the 16 old bytes
 // that hold them with 7 neighbours are loaded. Where a lane's tokens lie is found once for all blocks of dimensions.
@@ -587,7 +590,10 @@ __device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c
   return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
-template <bool IS_V>
+// token i of those that stay where the first and the last are all of them
+__device__ __forceinline__ int end_token(const EvictArgs& a, int T, int i) { return i < a.first ? i : T - a.keep + i; }
+
+template <bool IS_V, bool ENDS>
 __device__ __forceinline__ void move_page(const EvictArgs& a, const Kv8Cache& c, int req, int p, int pid, int head) {
   __shared__ const int8_t* src[256];     // the old page's first block of the token's 32
   __shared__ int place[256];             // .. and the token's place in it
@@ -601,7 +607,7 @@ __device__ __forceinline__ void move_page(const EvictArgs& a, const Kv8Cache& c,
   int from = -1, at = 0;
   float s = 0.0f;
   if (tid < count) {
-    const int t = a.kept[((size_t)req * c.kv_heads + head) * a.keep + p * a.page + tid];
+    const int t = ENDS ? end_token(a, T, p * a.page + tid) : a.kept[((size_t)req * c.kv_heads + head) * a.keep + p * a.page + tid];
     if (t >= 0 && t < T) {
       const int pg = t / a.page, id = a.from_table[(size_t)req * a.table_ld + pg];
       at = t - pg * a.page;
@@ -679,6 +685,7 @@ __device__ __forceinline__ void move_page(const EvictArgs& a, const Kv8Cache& c,
   }
 }
 
+template <bool ENDS>
 __global__ __launch_bounds__(256) void kv8_evict_move_kernel(EvictArgs a, Kv8Cache c, long units) {
   const int fresh = (a.keep + a.page - 1) / a.page;
   for (long u = blockIdx.x; u < units; u += gridDim.x) {
@@ -686,25 +693,32 @@ __global__ __launch_bounds__(256) void kv8_evict_move_kernel(EvictArgs a, Kv8Cac
     const int head = (int)(page % c.kv_heads), p = (int)(page / c.kv_heads % fresh), req = (int)(page / c.kv_heads / fresh);
     const int T = a.from_len[req];
     if (T <= a.keep || T > a.table_ld * a.page) continue;
+    if (ENDS && (u & 1) == 0) {
+      const int i = p * a.page + threadIdx.x;
+      if ((int)threadIdx.x < a.page && i < a.keep) a.kept[((size_t)req * c.kv_heads + head) * a.keep + i] = end_token(a, T, i);
+    }
     const int pid = a.table[(size_t)req * a.table_ld + p];
     if (pid < 0 || pid >= a.n_pages) continue;
-    if (u & 1) move_page<true>(a, c, req, p, pid, head);
-    else move_page<false>(a, c, req, p, pid, head);
+    if (u & 1) move_page<true, ENDS>(a, c, req, p, pid, head);
+    else move_page<false, ENDS>(a, c, req, p, pid, head);
     __syncthreads();
   }
 }
 
 hipError_t launch_kv8_evict(const EvictArgs& a, const Kv8Cache& c, hipStream_t s) {
   const dim3 picks((unsigned)(a.requests * c.kv_heads));
-  // the fewest waves that hold a request's tokens at once: their barriers are shorter (us of the kernel with 1024 threads / these: one
-  // request of 2101 tokens 14.8 / 10.4, 32 of up to 8192 17.2 / 13.6)
-  if (a.max_len <= 256 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<256>, picks, dim3(256), 0, s, a, c.kv_heads);
-  else if (a.max_len <= 512 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<512>, picks, dim3(512), 0, s, a, c.kv_heads);
-  else hipLaunchKernelGGL(kv8_evict_pick_kernel<1024>, picks, dim3(1024), 0, s, a, c.kv_heads);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  const bool ends = a.first + a.recent == a.keep;
+  if (!ends) {
+    // the fewest waves that hold a request's tokens at once: their barriers are shorter (us of the kernel with 1024 threads / these:
+    // one request of 2101 tokens 14.8 / 10.4, 32 of up to 8192 17.2 / 13.6)
+    if (a.max_len <= 256 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<256>, picks, dim3(256), 0, s, a, c.kv_heads);
+    else if (a.max_len <= 512 * kPickMost) hipLaunchKernelGGL(kv8_evict_pick_kernel<512>, picks, dim3(512), 0, s, a, c.kv_heads);
+    else hipLaunchKernelGGL(kv8_evict_pick_kernel<1024>, picks, dim3(1024), 0, s, a, c.kv_heads);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   const long units = 2L * a.requests * c.kv_heads * ((a.keep + a.page - 1) / a.page);
-  hipLaunchKernelGGL(kv8_evict_move_kernel, dim3((unsigned)std::min(units, 1L << 22)), dim3(256), 0, s, a, c, units);
+  hipLaunchKernelGGL(ends ? kv8_evict_move_kernel<true> : kv8_evict_move_kernel<false>, dim3((unsigned)std::min(units, 1L << 22)), dim3(256), 0, s, a, c, units);
   return hipGetLastError();
 }
 

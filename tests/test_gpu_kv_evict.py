@@ -172,6 +172,15 @@ def test_evict_of_long_requests(len_of, keep, first, recent, max_len):
     check_evict(rng, len_of, 64, 1, 32, keep, keep, first, recent, spare=700, masses="fine", max_len=max_len)
 
 
+@pytest.mark.parametrize("keep,first,recent", [(90, 40, 50), (90, 90, 0), (90, 0, 90), (33, 1, 32)])
+def test_evict_to_the_ends(keep, first, recent):
+    """Nothing to pick: absent pages among the old ones, lengths that nothing is cut of, masses that move along."""
+    def spoil(p):
+        p.table[0, 1], p.table[0, 3], p.table[1] = -1, p.n_pages + 3, -1
+        p.len[2] = p.ld * p.page + 1
+    check_evict(np.random.default_rng(keep + first), [300, 200, 250, 500, 20, 100, 101], 32, 2, 64, 100, keep, first, recent, spoil=spoil)
+
+
 def test_evict_with_absent_pages():
     """Tokens without a page are the first to go; those that stay have code, scale and mass 0."""
     def spoil(p):
