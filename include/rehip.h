@@ -462,7 +462,8 @@ int re_kv_positions_dev(size_t rows, const int *d_row_seq, const int *d_row_pos,
  * (ranges ascending and disjoint, as above; 0: none): row i is the target's after token d_tokens[row i], d_tokens[row i + 1] the
  * token drafted there, and the last row has no draft behind it, so that a request of one row just draws a token. p =
  * softmax(logits / T), T = d_temperature[b] (NULL: 1). d_probs (stride ldp), or NULL: the distributions q that the drafts were
- * drawn from, row by row; finite, not negative. A draft d is accepted if d_accept_u[row] * q(d) < p(d) (without d_probs:
+ * drawn from, row by row; finite, not negative. Of d_probs and d_accept_u a request's last row is not read, of d_tokens its first:
+ * buffers may end before them. A draft d is accepted if d_accept_u[row] * q(d) < p(d) (without d_probs:
  * q(d) = 1). In the place of the first that is not, a token is drawn from max(0, p - q) over its sum (without d_probs: from
  * p without d; where nothing is left, from p), behind the last from p. Drawn: the lowest token t with sum over j <= t
  * of the weights > d_sample_u[b] * their sum; both random numbers from [0, 1). T <= 0 or NaN: greedy, a draft is accepted

@@ -241,10 +241,11 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, const RequestRow
   for (int i0 = 0; i0 < q.count; i0 += WAVES) {
     const int i = i0 + w, row = q.row0 + min(i, q.count - 1);
     const bool drafted = i < q.count - 1;
-    // (the draft's logit and probability are on their way with the row's parts)
+    // (the draft's logit and probability are on their way with the row's parts; the last row has no draft, and no more than its
+    // logits need be there)
     const int t = drafted ? a.tokens[row + 1] : 0, at = min(max(t, 0), a.vocab - 1);
-    const float x = a.x[(size_t)row * a.ld + at], share = a.probs ? a.probs[(size_t)row * a.ldp + at] : 1.0f;
-    const float u = a.accept_u[row];
+    const float x = a.x[(size_t)row * a.ld + at];
+    const float share = drafted && a.probs ? a.probs[(size_t)row * a.ldp + at] : 1.0f, u = drafted ? a.accept_u[row] : 0.0f;
     const RowPart p = joined_wave(part(row), c64);
     const bool none = p.bad || p.m == -INFINITY;
     bool accepted = false;

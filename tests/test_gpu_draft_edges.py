@@ -1,0 +1,33 @@
+"""Verified drafts at the edges of their buffers, against keep_ref.py in 64 bits."""
+import numpy as np
+import pytest
+
+import keep_ref as ref
+import rehip
+from rehip import hip
+from test_gpu_draft_verify import drafts, get
+from test_gpu_kv8 import i32
+
+pytestmark = pytest.mark.gpu
+B = hip.DeviceBuffer
+
+
+def f32(a):
+    return B.from_array(np.ascontiguousarray(a, np.float32))
+
+
+@pytest.mark.parametrize("vocab,count", [(2048, [2] * 120 + [17]), (8192, [5] * 13), (8192, [65])])
+def test_buffers_that_end_with_the_last_draft(vocab, count):
+    """The last row of all has no draft, so neither probabilities nor a random number: 2 MiB of probabilities end before it."""
+    rng = np.random.default_rng(vocab + len(count))
+    x, start, count, tokens, q, u, r = drafts(rng, count, vocab)
+    rows, n = len(x), len(count)
+    assert (rows - 1) * vocab * 4 == 1 << 21
+    out = np.full(rows, -5, np.int32)
+    acc, back = ref.verify(x, start, count, tokens, q, None, u, r, out)
+    nb = rehip.draft_verify_work_bytes(rows, n, vocab)
+    got = [i32(np.full(n, -5)), i32(np.full(n, -5)), i32(np.full(rows, -5))]
+    rehip.draft_verify_dev(f32(x), vocab, rows, vocab, n, i32(start), i32(count), i32(tokens), f32(q[:-1]), vocab, None, f32(u[:-1]),
+                           f32(r), *got, B(nb), nb)
+    for g, w in zip(got, (acc, back, out)):
+        np.testing.assert_array_equal(get(g, len(w)), w)
