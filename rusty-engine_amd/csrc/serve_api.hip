@@ -371,6 +371,8 @@ int re_draft_verify_dev(const float* d_logits, size_t ld, size_t rows, size_t vo
   const size_t need = re_draft_verify_work_bytes(rows, requests, vocab);
   if (!d_work) return report_error(RE_ERR_ARG, "null workspace, need %zu bytes", need);
   if (work_bytes < need) return report_error(RE_ERR_SIZE, "draft workspace of %zu bytes, need %zu", work_bytes, need);
+  if (d_out_tokens < d_tokens + rows && d_tokens < d_out_tokens + rows)
+    return report_error(RE_ERR_ARG, "the tokens that come out must be a buffer apart from the drafted ones");
   const VerifyArgs a{d_logits, d_row_start, d_row_count, d_tokens, d_probs, d_temperature, d_accept_u, d_sample_u,
                      d_accepted, d_back, d_out_tokens, d_work, ld, ldp, (int)rows, (int)vocab, (int)requests};
   HIP_TRY(launch_verify(a, (hipStream_t)stream));
