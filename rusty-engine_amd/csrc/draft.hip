@@ -517,13 +517,16 @@ __global__ __launch_bounds__(64 * kSmallWaves) void verify_small_kernel(VerifyAr
 
 // about four workgroups for each CU (us of 768 / 1024 / 1536 / 2048: 200 requests of up to 3 drafts, 32000 tokens 38.5 / 38.3 / 40.1 / 41.1, 32 of
 // up to 4, 64000 24.0 / 23.8 / 24.7 / 24.4, 8 of up to 4, 151936 21.2 / 20.7 / 20.5 / 20.2)
+constexpr int kVerGroups = 1024;
 static int verify_parts(int rows, int vocab) {
-  return std::max(1, std::min({(vocab + kVerStep - 1) / kVerStep, kVerParts, 1024 / std::max(rows, 1)}));
+  return std::max(1, std::min({(vocab + kVerStep - 1) / kVerStep, kVerParts, kVerGroups / std::max(rows, 1)}));
 }
 static int verify_blocks(int vocab) { return (vocab + kBlock - 1) / kBlock; }
 
+// (at least what fewer rows, requests or tokens take, so that a program's largest step may size it for all)
 size_t verify_work_bytes(int rows, int requests, int vocab) {
-  return (size_t)rows * verify_parts(rows, vocab) * sizeof(RowPart) + (size_t)((requests + 1) & ~1) * sizeof(int) +
+  const size_t parts = std::max((size_t)rows, std::min((size_t)kVerGroups, (size_t)rows * verify_parts(1, vocab)));
+  return parts * sizeof(RowPart) + (size_t)((requests + 1) & ~1) * sizeof(int) +
          (size_t)requests * verify_blocks(vocab) * sizeof(double);
 }
 

@@ -715,6 +715,7 @@ def kv_positions_dev(rows, row_seq, row_pos, requests, dropped, out, stream=None
 
 
 def draft_verify_work_bytes(rows, requests, vocab) -> int:
+    """Bytes of the workspace of draft_verify_dev; those of the largest step serve smaller ones too."""
     return int(lib().re_draft_verify_work_bytes(rows, requests, vocab))
 
 

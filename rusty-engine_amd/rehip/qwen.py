@@ -978,7 +978,7 @@ class _DraftedRows:
         self.row_start, self.row_count = B.from_array(np.zeros(1, np.int32)), B(4)
         self.tokens, self.out, self.found = B(rows * 4), B(rows * 4), B(8)
         self.random = B((rows + 2) * 4)                        # a number for each row, the drawn token's, the temperature
-        self.work_bytes = max(draft_verify_work_bytes(n, 1, vocab) for n in range(1, rows + 1))
+        self.work_bytes = draft_verify_work_bytes(rows, 1, vocab)
         self.work = B(self.work_bytes)
 
 

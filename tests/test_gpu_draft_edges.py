@@ -31,3 +31,19 @@ def test_buffers_that_end_with_the_last_draft(vocab, count):
                            f32(r), *got, B(nb), nb)
     for g, w in zip(got, (acc, back, out)):
         np.testing.assert_array_equal(get(g, len(w)), w)
+
+
+def test_a_workspace_for_the_largest_step_serves_smaller_ones():
+    """Sized once for 1025 rows, which are not cut into parts; fewer rows are cut into two and more."""
+    rng, vocab, n = np.random.default_rng(11), 9000, 41
+    nb = rehip.draft_verify_work_bytes(1025, n, vocab)
+    work = B(nb)
+    for per in (25, 12, 6, 1):
+        x, start, count, tokens, q, u, r = drafts(rng, [per] * n, vocab, probs=False)
+        out = np.full(len(x), -5, np.int32)
+        acc, back = ref.verify(x, start, count, tokens, None, None, u, r, out)
+        got = [i32(np.full(n, -5)), i32(np.full(n, -5)), i32(np.full(len(x), -5))]
+        rehip.draft_verify_dev(f32(x), vocab, len(x), vocab, n, i32(start), i32(count), i32(tokens), None, 0, None, f32(u), f32(r), *got,
+                               work, nb)
+        for g, w in zip(got, (acc, back, out)):
+            np.testing.assert_array_equal(get(g, len(w)), w)
