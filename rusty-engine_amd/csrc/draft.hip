@@ -26,7 +26,7 @@ namespace rehip {
 // 64 requests of up to 4 drafts, 189 rows of 151936 and the drafts' probabilities, 153 MB: 52 us, 32 + 22 in the two
 // kernels. The rows: 115 MB, 3.6 TB/s; without the exponentials they take 23, with them the vector units' 64-bit rate bounds (5 clocks
 // for each of 15 operations; a table of 32 and one term more: 34.5). One request of 4 drafts 13 us: two launches of latency,
-// 5.2 + 11. (With the token drawn by a launch of its own 54 and 14.5.)
+// 5.2 + 11.
 constexpr int kVerWaves = 4;
 constexpr int kVerBatch = 16;            // logits of a lane at a time
 constexpr int kVerStep = 64 * kVerBatch * kVerWaves;
@@ -193,7 +193,9 @@ __device__ __forceinline__ RowPart row_part(const float* x, int vocab, int s0, i
   return mine;
 }
 
-// behind the rows' parts: of each request the workgroups that are done with it, then the sums of its blocks
+// behind the rows' parts: of each request the workgroups that are done with it, then the sums of its blocks (never negative, and
+// kNotYet until they are there)
+constexpr double kNotYet = -1.0;
 __device__ __forceinline__ int* done_at(const VerifyArgs& a, int parts) {
   return reinterpret_cast<int*>(reinterpret_cast<RowPart*>(a.work) + (size_t)a.rows * parts);
 }
@@ -202,7 +204,7 @@ __device__ __forceinline__ double* sums_at(const VerifyArgs& a, int parts) {
 }
 
 // One workgroup per (row, part).
-__global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs a, int parts) {
+__global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs a, int parts, int blocks) {
   __shared__ double table[kVerTable];
   __shared__ RowPart ws[kVerWaves];
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -216,7 +218,11 @@ __global__ __launch_bounds__(64 * kVerWaves) void verify_rows_kernel(VerifyArgs 
     counts = q.req >= 0 && r < q.row0 + q.count;
     if (!counts) return false;
     c64 = units_of(a, q.req);
-    if (r == q.row0 && part == 0 && threadIdx.x == 0) done_at(a, parts)[q.req] = 0;
+    if (r == q.row0 && part == 0) {
+      if (threadIdx.x == 0) done_at(a, parts)[q.req] = 0;
+      double* const sums = sums_at(a, parts) + (size_t)q.req * blocks;
+      for (int k = threadIdx.x; k < blocks; k += 64 * kVerWaves) sums[k] = kNotYet;
+    }
     fill_table(table);
     return true;
   });
@@ -389,6 +395,7 @@ constexpr int kRestWaves = 8;
 constexpr int kBlock = 1024;             // tokens of a block
 constexpr int kRestMost = 512;           // workgroups, about (us of 256 / 512 / 1024: 64 requests of 151936 tokens 51.8 / 49.6 / 57.0, 200 of
                                          // 32000 40.3 / 40.1 / 45.1)
+constexpr int kMostWaits = 1 << 16;      // loads, about a microsecond each
 template <bool PROBS>
 __global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs a, int parts, int cuts, int blocks) {
   constexpr int kThreads = 64 * kRestWaves;
@@ -453,10 +460,6 @@ __global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs
     take(x, p, b);
   }
   if (cuts > 1) {
-    // The sums go to and come from memory that all workgroups see by atomic stores and loads, and a wave's have arrived before
-    // its workgroup counts itself done. (A fence for all that a wave has written writes the whole L2 back: 104 us instead of
-    // 17 for 64 requests.)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0)
       last = __hip_atomic_fetch_add(done_at(a, parts) + req, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == cuts - 1;
@@ -465,11 +468,20 @@ __global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs
   } else {
     __syncthreads();
   }
+  // The counter orders nothing: a sum that is not here yet is waited for, by itself. (With a counter that releases and acquires, which
+  // writes the L2 back in every workgroup, 55.5 us instead of 52 for 64 requests; with a launch of its own for what follows 53.5, one
+  // request 14 instead of 12.) All that it waits for have been stored, so it takes a trip to memory or none; the wait's end does
+  // not depend on that.
+  auto sum = [&](int k) {
+    double v = kNotYet;
+    for (int i = 0; i < kMostWaits && v == kNotYet; ++i) v = __hip_atomic_load(sums + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return v;
+  };
   const double r = (double)a.sample_u[req];
   auto value = [&](int t) { return of(t, of.x[t], of.probs ? of.probs[t] : 0.0f); };
   double target = 0.0, upto, none;
-  const int found = first_above<kRestWaves>([&](int k) { return __hip_atomic_load(sums + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
-                                            0, blocks, (blocks + kThreads - 1) / kThreads, 0.0, [&](double all) { return target = r * all; }, upto);
+  const int found = first_above<kRestWaves>(sum, 0, blocks, (blocks + kThreads - 1) / kThreads, 0.0,
+                                            [&](double all) { return target = r * all; }, upto);
   int token;
   if (found >= 0) {
     token = first_above<kRestWaves>(value, found * kBlock, min((found + 1) * kBlock, a.vocab), kBlock / kThreads, upto,
@@ -539,7 +551,7 @@ hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
   }
   const int parts = verify_parts(a.rows, a.vocab), blocks = verify_blocks(a.vocab);
   const int cuts = std::max(1, std::min((blocks + kRestWaves - 1) / kRestWaves, kRestMost / a.requests));
-  hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(a.rows * parts)), dim3(64 * kVerWaves), 0, s, a, parts);
+  hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(a.rows * parts)), dim3(64 * kVerWaves), 0, s, a, parts, blocks);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(a.probs ? verify_rest_kernel<true> : verify_rest_kernel<false>, dim3((unsigned)(a.requests * cuts)),

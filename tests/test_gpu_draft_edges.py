@@ -47,3 +47,26 @@ def test_a_workspace_for_the_largest_step_serves_smaller_ones():
                                work, nb)
         for g, w in zip(got, (acc, back, out)):
             np.testing.assert_array_equal(get(g, len(w)), w)
+
+
+def test_calls_back_to_back_see_their_own_sums():
+    """Many calls in one workspace with nothing waited for between them, alternating inputs: a request's last workgroup takes
+    the sums of this call, not those that the call before left in the same places."""
+    vocab, count = 40000, [4, 1, 3, 5, 2]
+    n, rows = len(count), sum(count)
+    nb = rehip.draft_verify_work_bytes(rows, n, vocab)
+    work, sets = B(nb), []
+    for seed in (21, 22):
+        rng = np.random.default_rng(seed)
+        x, start, count, tokens, q, u, r = drafts(rng, count, vocab, sharp=-20, likely=0.3)
+        out = np.full(rows, -5, np.int32)
+        want = (*ref.verify(x, start, count, tokens, q, None, u, r, out), out)
+        sets.append(((f32(x), i32(start), i32(count), i32(tokens), f32(q), f32(u), f32(r)), want))
+    got = [[i32(np.full(n, -5)), i32(np.full(n, -5)), i32(np.full(rows, -5))] for _ in range(60)]
+    hip.synchronize()
+    for i, o in enumerate(got):
+        x, start, count, tokens, q, u, r = sets[i % 2][0]
+        rehip.draft_verify_dev(x, vocab, rows, vocab, n, start, count, tokens, q, vocab, None, u, r, *o, work, nb)
+    for i, o in enumerate(got):
+        for g, w in zip(o, sets[i % 2][1]):
+            np.testing.assert_array_equal(get(g, len(w)), w)
