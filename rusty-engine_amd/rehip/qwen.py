@@ -808,7 +808,7 @@ class DeviceDecoder:
         """Decodes the token in `tok` and the drafted ones behind it in one pass; returns the drafts that the model
         accepts and the token that it puts behind them, 1 to len(drafts) + 1 tokens (`draft_verify_dev`). Greedy at
         temperature 0: the tokens that as many `step` calls would give, where products of several rows and of one round
-        alike enough to leave the largest logit the same. Else drafts (drawn from the rows of `probs`, or
+        alike enough to leave the largest logit the same (of logits that are equal the lowest id, where `step` takes the highest). Else drafts (drawn from the rows of `probs`, or
         certain without them) are accepted with the random numbers `accept_u`, one each, and the token behind is drawn
         with `sample_u`, all from [0, 1): the tokens are then distributed as the model's own. Rejected drafts are
         taken back as by setting seq_len."""
@@ -856,8 +856,11 @@ class DeviceDecoder:
         return [int(t) for t in got]
 
     def generate_drafted(self, prompt, max_new: int, most: int = 4, ngram: int = 2):
-        """`generate` with up to `most` tokens a step drafted by looking up the last `ngram` tokens earlier in the
-        sequence (`lookup_drafts`): the same greedy tokens in fewer steps where the text repeats itself."""
+        """`generate` with up to `most` tokens a step drafted by looking up the last `ngram` tokens earlier in the prompt and
+        in what it has generated (`lookup_drafts`): fewer steps where the text repeats itself, and the same greedy tokens, as far
+        as `step_drafted` gives them. Where nothing is found it is `step`. A drafted step takes longer (its kernels are
+        launched one by one), so it pays where a few drafts of it are accepted; and every step looks through all of the tokens
+        on the host, 0.2 us for each."""
         p0 = self.seq_len
         prompt = [int(t) for t in np.asarray(prompt).reshape(-1)]
         if p0 + len(prompt) + max_new > self.max_seq:
@@ -865,7 +868,8 @@ class DeviceDecoder:
         out = [self.prefill(prompt)][:max_new]
         while len(out) < max_new:
             room = min(most, max_new - len(out) - 1, self.cap - 1)
-            out += self.step_drafted(lookup_drafts(prompt + out, room, ngram))
+            drafts = lookup_drafts(prompt + out, room, ngram)
+            out += self.step_drafted(drafts) if drafts else [self.step()]
         return out
 
     def replay(self, steps: int) -> None:
