@@ -262,10 +262,10 @@ int re_kv8_mass_dev(const float* d_q, size_t ldq, const float* d_lse, size_t row
   if (!a16(d_q) || !a16(d_mass)) return report_error(RE_ERR_ARG, "q and masses must be 16-byte aligned");
   if (rows == 0 || requests == 0) return RE_OK;
   if (max_rows == 0) return report_error(RE_ERR_SIZE, "max_rows 0 for %zu rows", rows);
-  if (max_rows * (n_heads / n_kv_heads) > (1u << 30) || requests * n_kv_heads > kMassMaxWorkgroups)
+  const size_t ml = max_len < (1u << 30) ? max_len : (1u << 30), mr = max_rows < rows ? max_rows : rows;
+  if (mr * (n_heads / n_kv_heads) > (1u << 30) || requests * n_kv_heads > kMassMaxWorkgroups)
     return report_error(RE_ERR_SIZE, "weights of %zu rows and %zu requests with %zu heads are too many for one call", rows,
                         requests, n_heads);
-  const size_t ml = max_len < (1u << 30) ? max_len : (1u << 30), mr = max_rows < rows ? max_rows : rows;
   const PagedBatch b{d_row_start, d_row_count, d_kv_len, d_table, (int)requests, (int)rows, (int)table_ld, (int)page,
                      (int)n_pages};
   const Kv8Cache c{const_cast<int8_t*>(d_kcodes), nullptr, const_cast<float*>(d_kscale), nullptr, (int)n_kv_heads,
