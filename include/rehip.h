@@ -418,7 +418,10 @@ int re_attention_kv8_sinks_dev(const float *d_q, size_t ldq, size_t rows, size_t
  * page f32, d_mass[page][head][place] += the sum over the request's rows that see the token and over the query heads of that
  * KV head of exp(scale * q . k - lse), with the q, window and sinks of the attention call and the d_lse that it gave. A
  * token that the step brought starts from 0, so pages need no preparation. A row whose q or lse is not finite adds
- * nothing. Accurate to about 2^-23 |lse| of a weight. Here a page belongs to one request. No workspace; d_q and d_mass
+ * nothing. Every row of the batch adds its weights: made right behind attention, before drafts are verified, those of drafts that are
+ * rejected stay in the masses of the tokens before them, and eviction ranks by them. To count only the rows that stay, keep each
+ * layer's q and lse and make the call behind re_kv_rewind_dev, with row_count - back in row_count's place and the lengths that it
+ * left: rows then have the positions that they had. Accurate to about 2^-23 |lse| of a weight. Here a page belongs to one request. No workspace; d_q and d_mass
  * 16-byte aligned. */
 int re_kv8_mass_dev(const float *d_q, size_t ldq, const float *d_lse, size_t rows, size_t requests,
                     const int *d_row_start, const int *d_row_count, const int *d_kv_len, const int *d_table,
@@ -482,7 +485,8 @@ int re_draft_verify_dev(const float *d_logits, size_t ld, size_t rows, size_t vo
 /* Takes d_back[b] tokens (negative: none; more than there are: all) off the ends of the requests' lengths; pages that hold
  * none of the rest go back to the stack, behind the free ones in request order. d_kv_len_out and d_n_free_out may be
  * d_kv_len and d_n_free; the table is left. Lengths outside 0 .. table_ld * page stay. Such pages belong to one request. A
- * part-filled page keeps the scale that the tokens behind had raised. Up to 4096 requests. */
+ * part-filled page keeps the scale that the tokens behind had raised, and the tokens that are left keep the weights that
+ * the rows taken back had added to their masses (re_kv8_mass_dev says how to leave those out). Up to 4096 requests. */
 int re_kv_rewind_dev(size_t requests, size_t page, const int *d_back, const int *d_kv_len, const int *d_table,
                      size_t table_ld, int *d_free, size_t n_pages, const int *d_n_free, int *d_kv_len_out,
                      int *d_n_free_out, void *stream);

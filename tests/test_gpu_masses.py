@@ -1,9 +1,14 @@
 """A step's weights (kv8_mass_dev) against keep_ref.py in 64 bits: calls that attention takes, and what drafted steps leave."""
+import copy
+
 import numpy as np
 import pytest
 
-from test_gpu_attention_sinks import check_mass
-from test_gpu_kv8 import make
+import keep_ref as ref
+import rehip
+from rehip import hip
+from test_gpu_attention_sinks import attend_sinks, check_mass, weigh
+from test_gpu_kv8 import i32, make
 
 pytestmark = pytest.mark.gpu
 
@@ -14,3 +19,38 @@ def test_any_bound_of_the_rows(max_rows):
     rng = np.random.default_rng(1)
     bt, cache, q = make(rng, [3, 0, 20], [50, 7, 90], 32, 8, 2, 64)
     check_mass(cache, bt, q, 0.125, 30, 4, max_rows=max_rows, max_len=90)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
+@pytest.mark.parametrize("requests", [1, 6, 90])
+def test_weights_behind_the_rewind_count_the_rows_that_stay(requests, window, sinks):
+    """Behind kv_rewind_dev, with the counts less what went back and the lengths that it left, the weights are those of a step that
+    had brought only the rows that stay; the places behind them keep what they had."""
+    rng = np.random.default_rng(requests + window)
+    page, heads, kv, hd = 32, 8, 2, 64
+    rows_of = rng.integers(1, 6, requests)
+    bt, cache, q = make(rng, rows_of, rows_of + rng.integers(0, 100, requests), page, heads, kv, hd)
+    back = rng.integers(0, rows_of)                               # (the first row stays)
+    back[0] = rows_of[0] - 1
+    _, lse = attend_sinks(cache, bt, q, 0.125, window, sinks)     # of all rows
+    length, free, n_free = i32(bt.len), i32(np.zeros(bt.n_pages)), i32([0])
+    rehip.kv_rewind_dev(requests, page, i32(back), length, i32(bt.table), bt.ld, free, bt.n_pages, n_free, length, n_free)
+    hip.synchronize()
+    stay = copy.copy(bt)
+    stay.count, stay.len = (bt.count - back).astype(np.int32), length.download(np.int32, requests)
+    np.testing.assert_array_equal(stay.len, bt.len - back)
+    start = rng.random(cache.shape[:3]).astype(np.float32)
+    want = start.astype(np.float64)
+    tol = ref.mass(q, lse, stay.plain(), cache.k, cache.ks, 0.125, window, sinks, want)
+    got = weigh(cache, stay, q, lse, 0.125, window, sinks, start, max_rows=5)
+    assert np.all(np.abs(got - want) <= tol)
+    # rejected rows are not looked at: NaN in their place changes nothing, in weights (to the last bit) and in attention
+    q2 = q.copy()
+    for b in range(requests):
+        q2[bt.start[b] + stay.count[b]:bt.start[b] + bt.count[b]] = np.nan
+    _, lse2 = attend_sinks(cache, stay, q2, 0.125, window, sinks, max_rows=5)
+    np.testing.assert_array_equal(got, weigh(cache, stay, q2, lse, 0.125, window, sinks, start, max_rows=5))
+    live = np.concatenate([np.arange(s, s + c) for s, c in zip(stay.start, stay.count)])
+    off = np.abs(lse2[live] - lse[live])
+    assert np.all(off <= 2 * ref.attention(q, stay.plain(), (cache.k, cache.v, cache.ks, cache.vs), 0.125, window, sinks,
+                                                  np.zeros(q.shape), np.zeros(lse.shape))[1][live])
