@@ -436,7 +436,8 @@ int re_kv8_mass_dev(const float *d_q, size_t ldq, const float *d_lse, size_t row
  * (d_kv_len_out, d_table_out, d_free_out, d_n_free_out may be the inputs; entries of d_table_out behind a cut request's
  * pages are -1); d_from_len: a cut request's old length, 0 for the others; d_from_table (requests x table_ld): a cut
  * request's old entries (may be d_table if d_table_out is another buffer; never d_table_out); d_dropped: NULL, or per
- * request += the tokens it lost, 0 where it holds none (re_kv_positions_dev adds them to its rows' positions);
+ * request += the tokens it lost, 0 where it holds none (re_kv_positions_dev adds them to its rows' positions; a request number that
+ * passes to another conversation with no such call between keeps the old one's, and is set to 0 by the caller);
  * d_status[0] requests over the limit that were left, d_status[1] cut ones. d_from_len is neither of the lengths' buffers. Not
  * for requests that share pages: a cut one gives all of its pages back. Up to 4096 requests.
  *
@@ -457,7 +458,9 @@ int re_kv8_evict_dev(size_t requests, const int *d_from_len, const int *d_from_t
                      size_t recent, size_t max_len, int *d_kept, void *stream);
 
 /* Rotary positions of a step's rows after evictions: d_out[r] = d_row_pos[r] + d_dropped[d_row_seq[r]], -1 for rows without a
- * request (of the plan's d_row_seq and d_row_pos, which count what the cache holds). d_out may be d_row_pos. */
+ * request (of the plan's d_row_seq and d_row_pos, which count what the cache holds). d_out may be d_row_pos. Positions go on with the conversation, and
+ * tokens that stay keep the rotation of theirs: what an eviction bounds is memory, not the range of positions, so a conversation
+ * longer than the trained one needs frequencies scaled for it (re_rope_freqs). */
 int re_kv_positions_dev(size_t rows, const int *d_row_seq, const int *d_row_pos, size_t requests, const int *d_dropped,
                         int *d_out, void *stream);
 
@@ -470,7 +473,8 @@ int re_kv_positions_dev(size_t rows, const int *d_row_seq, const int *d_row_pos,
  * q(d) = 1). In the place of the first that is not, a token is drawn from max(0, p - q) over its sum (without d_probs: from
  * p without d; where nothing is left, from p), behind the last from p. Drawn: the lowest token t with sum over j <= t
  * of the weights > d_sample_u[b] * their sum; both random numbers from [0, 1). T <= 0 or NaN: greedy, a draft is accepted
- * if it is the largest logit (ties to the lower id), and the token behind is the largest. Sums are taken in 64 bits. A
+ * if it is the largest logit (ties to the lower id), and the token behind is the largest. Exponentials are good to
+ * 3.6e-11 of their value and sums are taken in 64 bits: a random number that close to a token's border may draw its neighbour. A
  * draft outside 0 .. vocab - 1 is not accepted. A row with NaN or +inf among its logits, or nothing above -inf, has no
  * distribution: its draft is not accepted, and the token in its place is -1. Outputs: d_accepted[b] drafts, d_back[b] = the
  * others (for re_kv_rewind_dev), d_out_tokens[row i]: the accepted drafts, the token behind them, -1 after that; rows

@@ -686,7 +686,7 @@ def attention_kv8_sinks_dev(q, ldq, rows, requests, row_start, row_count, kv_len
 def kv8_mass_dev(q, ldq, lse, rows, requests, row_start, row_count, kv_len, table, table_ld, page, n_pages, kcodes,
                  kscale, max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window, sinks, mass, stream=None):
     """Adds the weight that a step's attention gives each cached token to `mass` (n_pages x n_kv_heads x page f32),
-    with attention's lse (re_kv8_mass_dev)."""
+    with attention's lse (re_kv8_mass_dev, which says how to leave out rejected drafts' rows)."""
     _call(lib().re_kv8_mass_dev, q, ldq, lse, rows, requests, row_start, row_count, kv_len, table, table_ld, page,
           n_pages, kcodes, kscale, max_rows, max_len, n_heads, n_kv_heads, head_dim, scale, window, sinks, mass,
           stream)
@@ -710,7 +710,7 @@ def kv8_evict_dev(requests, from_len, from_table, table, table_ld, page, n_pages
 
 def kv_positions_dev(rows, row_seq, row_pos, requests, dropped, out, stream=None):
     """Rotary positions of a step's rows after evictions: what the plan counts and what the requests have lost
-    (re_kv_positions_dev); `out` may be `row_pos`."""
+    (re_kv_positions_dev), so that they go on with the conversation, without bound; `out` may be `row_pos`."""
     _call(lib().re_kv_positions_dev, rows, row_seq, row_pos, requests, dropped, out, stream)
 
 
