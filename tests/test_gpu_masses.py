@@ -54,3 +54,27 @@ def test_weights_behind_the_rewind_count_the_rows_that_stay(requests, window, si
     off = np.abs(lse2[live] - lse[live])
     assert np.all(off <= 2 * ref.attention(q, stay.plain(), (cache.k, cache.v, cache.ks, cache.vs), 0.125, window, sinks,
                                                   np.zeros(q.shape), np.zeros(lse.shape))[1][live])
+
+
+# (KV heads, rows of the longest, max_len planned for), with 8 query heads of a KV head: a wave for each piece, two (heads beyond 128),
+# four waves (many pieces), eight (so many that each has a CU, more than that of half the size) and sixteen
+SHARED = {"few rows": (2, 5, 400), "many pieces": (2, 40, 18000), "a round": (2, 40, 4500), "few pieces": (1, 40, 400)}
+
+
+@pytest.mark.parametrize("name", SHARED)
+@pytest.mark.parametrize("hd,page", [(32, 64), (64, 32), (96, 128), (128, 64), (160, 32), (192, 96), (224, 32), (256, 64)])
+def test_shares_of_waves_of_every_head_size(name, hd, page):
+    kv, rows, max_len = SHARED[name]
+    rng = np.random.default_rng(hd + rows)
+    bt, cache, q = make(rng, [rows, rows - 3], [300, 77], page, 8 * kv, kv, hd)
+    for window, sinks in ((0, 0), (50, 9)):
+        check_mass(cache, bt, q, hd ** -0.5, window, sinks, max_rows=rows, max_len=max_len)
+
+
+@pytest.mark.parametrize("requests", [70, 1030])
+@pytest.mark.parametrize("hd,rows", [(64, 3), (128, 1), (192, 1), (256, 2)])
+def test_many_requests_of_larger_heads(requests, hd, rows):
+    rng = np.random.default_rng(requests + hd)
+    rows_of = rng.integers(0, rows + 1, requests)
+    bt, cache, q = make(rng, rows_of, rows_of + rng.integers(0, 70, requests), 32, 4, 2, hd)
+    check_mass(cache, bt, q, hd ** -0.5, 30, 3)
