@@ -458,9 +458,9 @@ int re_kv8_evict_dev(size_t requests, const int *d_from_len, const int *d_from_t
                      size_t recent, size_t max_len, int *d_kept, void *stream);
 
 /* Rotary positions of a step's rows after evictions: d_out[r] = d_row_pos[r] + d_dropped[d_row_seq[r]], -1 for rows without a
- * request (of the plan's d_row_seq and d_row_pos, which count what the cache holds). d_out may be d_row_pos. Positions go on with the conversation, and
- * tokens that stay keep the rotation of theirs: what an eviction bounds is memory, not the range of positions, so a conversation
- * longer than the trained one needs frequencies scaled for it (re_rope_freqs). */
+ * request (of the plan's d_row_seq and d_row_pos, which count what the cache holds). d_out may be d_row_pos. Positions go on with
+ * the conversation, and tokens that stay keep the rotation of theirs: what an eviction bounds is memory, not the range of
+ * positions, so a conversation longer than the trained one needs frequencies scaled for it (re_rope_freqs). */
 int re_kv_positions_dev(size_t rows, const int *d_row_seq, const int *d_row_pos, size_t requests, const int *d_dropped,
                         int *d_out, void *stream);
 
@@ -478,8 +478,9 @@ int re_kv_positions_dev(size_t rows, const int *d_row_seq, const int *d_row_pos,
  * draft outside 0 .. vocab - 1 is not accepted. A row with NaN or +inf among its logits, or nothing above -inf, has no
  * distribution: its draft is not accepted, and the token in its place is -1. Outputs: d_accepted[b] drafts, d_back[b] = the
  * others (for re_kv_rewind_dev), d_out_tokens[row i]: the accepted drafts, the token behind them, -1 after that; rows
- * outside the requests' are left. The outputs are buffers of their own (d_out_tokens over d_tokens is refused). d_work: re_draft_verify_work_bytes bytes (never fewer for more
- * rows, requests or tokens: the largest step's serve all), 16-byte aligned; as above. */
+ * outside the requests' are left. The outputs are buffers of their own (d_out_tokens over d_tokens is refused).
+ * d_work: re_draft_verify_work_bytes bytes (never fewer for more rows, requests or tokens: the largest step's serve all), 16-byte
+ * aligned; as above. */
 size_t re_draft_verify_work_bytes(size_t rows, size_t requests, size_t vocab);
 int re_draft_verify_dev(const float *d_logits, size_t ld, size_t rows, size_t vocab, size_t requests,
                         const int *d_row_start, const int *d_row_count, const int *d_tokens, const float *d_probs,

@@ -23,10 +23,10 @@ namespace rehip {
 // the sums of its weights by blocks of the vocabulary, of which the last workgroup finds the one where r falls, and the token in
 // it.
 //
-// 64 requests of up to 4 drafts, 189 rows of 151936 and the drafts' probabilities, 153 MB: 52 us, 32 + 22 in the two
-// kernels. The rows: 115 MB, 3.6 TB/s; without the exponentials they take 23, with them the vector units' 64-bit rate bounds (5 clocks
-// for each of 15 operations; a table of 32 and one term more: 34.5). One request of 4 drafts 13 us: two launches of latency,
-// 5.2 + 11.
+// 64 requests of up to 4 drafts, 189 rows of 151936 and the drafts' probabilities, 153 MB: 52 us, 32 + 23 in the two
+// kernels. The rows: 115 MB, 3.6 TB/s. Without the exponentials they take 23; the 64-bit operations, 15 of 5 clocks for each logit, are
+// 14 on all SIMDs: neither bounds by itself, the two run mostly one after the other (a table of 32 and one term more: 34.5). One
+// request of 4 drafts 10.5 .. 13 us: two launches of latency, 5 + 9.
 constexpr int kVerWaves = 4;
 constexpr int kVerBatch = 16;            // logits of a lane at a time
 constexpr int kVerStep = 64 * kVerBatch * kVerWaves;
@@ -468,10 +468,10 @@ __global__ __launch_bounds__(64 * kRestWaves) void verify_rest_kernel(VerifyArgs
   } else {
     __syncthreads();
   }
-  // The counter orders nothing: a sum that is not here yet is waited for, by itself. (With a counter that releases and acquires, which
-  // writes the L2 back in every workgroup, 55.5 us instead of 52 for 64 requests; with a launch of its own for what follows 53.5, one
-  // request 14 instead of 12.) All that it waits for have been stored, so it takes a trip to memory or none; the wait's end does
-  // not depend on that.
+  // The counter orders nothing: a sum that is not here yet is waited for, by itself. (us of 64 requests and of one: so 52.4 and 11.8, with
+  // a counter that releases and acquires, which writes the L2 back in every workgroup, 55.5 and 12, with a launch of its own for
+  // what follows 53.5 and 14.) All sums have been stored by then, so it takes a trip to memory more or none; that the wait
+  // ends does not depend on it.
   auto sum = [&](int k) {
     double v = kNotYet;
     for (int i = 0; i < kMostWaits && v == kNotYet; ++i) v = __hip_atomic_load(sums + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
