@@ -420,8 +420,8 @@ int re_attention_kv8_sinks_dev(const float *d_q, size_t ldq, size_t rows, size_t
  * token that the step brought starts from 0, so pages need no preparation. A row whose q or lse is not finite adds
  * nothing. Every row of the batch adds its weights: made right behind attention, before drafts are verified, those of drafts that are
  * rejected stay in the masses of the tokens before them, and eviction ranks by them. To count only the rows that stay, keep each
- * layer's q and lse and make the call behind re_kv_rewind_dev, with row_count - back in row_count's place and the lengths that it
- * left: rows then have the positions that they had. Accurate to about 2^-23 |lse| of a weight. Here a page belongs to one request. No workspace; d_q and d_mass
+ * layer's q and lse and make the call behind re_kv_rewind_dev and before re_kv_evict_plan_dev, with row_count - back in row_count's
+ * place and the lengths that the rewind left: rows then have the positions that they had. Accurate to about 2^-23 |lse| of a weight. Here a page belongs to one request. No workspace; d_q and d_mass
  * 16-byte aligned. */
 int re_kv8_mass_dev(const float *d_q, size_t ldq, const float *d_lse, size_t rows, size_t requests,
                     const int *d_row_start, const int *d_row_count, const int *d_kv_len, const int *d_table,
